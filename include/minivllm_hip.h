@@ -62,8 +62,8 @@ const char* mgi_last_error(void);
  * 1.02 the prefill key split (mgi_paged_prefill's workspace arguments and
  * mgi_paged_prefill_workspace_bytes); 1.03 mgi_paged_decode_noalloc; 1.04
  * mgi_paged_decode_append. mgi_decode_linear, mgi_decode_linear_norm, their
- * queries and mgi_paged_decode_workgroup_waves came later without a change to
- * the others. */
+ * queries, mgi_paged_decode_workgroup_waves, mgi_qk_norm_rope and
+ * mgi_kv_append_rope came later without a change to the others. */
 int mgi_abi_version(void);
 
 /*
@@ -342,6 +342,59 @@ int mgi_decode_linear_norm_pays(int64_t B, int64_t N, int64_t K);
 
 /* Workspace bytes mgi_decode_linear_norm needs for these sizes. */
 size_t mgi_decode_linear_norm_workspace_bytes(int64_t B, int64_t N, int64_t K);
+
+/*
+ * RMS norms of query and key heads with the position rotation, in one pass. No
+ * counterpart in the reference, whose models learn their position embeddings.
+ * For t < T, every head row x of D elements of q [T, Hq, D] and k [T, Hk, D]:
+ *   y = x * rsqrt(mean_d x_d^2 + eps) * weight      (y = x without weights)
+ *   out_i = y_i c_p - y_j s_p,  out_j = y_j c_p + y_i s_p   for pairs p < R/2
+ * with c_p = cos_sin[positions[t], p], s_p = cos_sin[positions[t], R/2 + p], and
+ * (i, j) = (p, p + R/2), or (2p, 2p + 1) with interleaved != 0. Dims past R =
+ * rotary_dim (even, 2 .. D) are not rotated. Arithmetic is f32, rounded once.
+ * cos_sin: f32 [table_rows, R], rows contiguous, table_stride apart. A row whose
+ * position is outside the table has no angles: its rotated dims come out NaN.
+ * q_weight, k_weight: [D] contiguous, of weight_dtype (dtype or MGI_F32), or both
+ * null. q, k, q_out, k_out share one dtype and have any strides; the outputs must
+ * not overlap the inputs. D <= 512.
+ */
+int mgi_qk_norm_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
+                     void* k_out, const int64_t* k_out_strides, /* [3] */
+                     const void* q, const int64_t* q_strides, /* [3] */
+                     const void* k, const int64_t* k_strides, /* [3] */
+                     int dtype,
+                     const void* positions, int64_t pos_stride, int pos_itype,
+                     const float* cos_sin, int64_t table_stride, int64_t table_rows, int64_t rotary_dim,
+                     const void* q_weight, const void* k_weight, int weight_dtype,
+                     float eps, int interleaved,
+                     int64_t T, int64_t Hq, int64_t Hk, int64_t D, void* stream);
+
+/*
+ * KV append with the same norms and rotation on the way: keys are normed, rotated
+ * and written to the pool's slots, values copied there, as mgi_kv_append writes
+ * rows k_new, v_new of Hk heads (skipped rows, conversions and repeated slots as
+ * there; values are bit-exact where the dtypes agree), and the normed, rotated
+ * queries go to q_out, which has the pool's dtype, as the attention that
+ * follows takes them. q, k and v share one dtype. A row whose position is outside
+ * the table is not written to the pool, and its query comes out NaN in the
+ * rotated dims.
+ */
+int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
+                       void* k_pool, void* v_pool,
+                       const int64_t* k_pool_strides, /* [5] */
+                       const int64_t* v_pool_strides, /* [5] */
+                       int pool_dtype,
+                       const void* q, const int64_t* q_strides, /* [3] */
+                       const void* k_new, const int64_t* k_new_strides, /* [3] */
+                       const void* v_new, const int64_t* v_new_strides, /* [3] */
+                       int new_dtype,
+                       const void* slot_mapping, int64_t slot_stride, int slot_itype,
+                       const void* positions, int64_t pos_stride, int pos_itype,
+                       const float* cos_sin, int64_t table_stride, int64_t table_rows, int64_t rotary_dim,
+                       const void* q_weight, const void* k_weight, int weight_dtype,
+                       float eps, int interleaved,
+                       int64_t T, int64_t Hq, int64_t Hk, int64_t D,
+                       int64_t S, int64_t N, int64_t L, int64_t layer_idx, void* stream);
 
 #ifdef __cplusplus
 }

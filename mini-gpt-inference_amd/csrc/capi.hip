@@ -681,6 +681,106 @@ int launch_append(const AppendSpec& ap, const int64_t* k_pool_strides, const int
   return MGI_OK;
 }
 
+// The arguments mgi_qk_norm_rope and mgi_kv_append_rope share.
+struct RopeSpec {
+  void* q_out;
+  const int64_t* qo;  // strides [3]
+  const void* q;
+  const int64_t* qs;
+  const void* k;
+  const int64_t* ks;
+  int dtype, out_dtype;
+  const void* positions;
+  int64_t pos_stride;
+  int pos_itype;
+  const float* cos_sin;
+  int64_t table_stride, table_rows, rotary_dim;
+  const void* q_weight;
+  const void* k_weight;
+  int weight_dtype;
+  float eps;
+  int interleaved;
+  int64_t T, Hq, Hk, D;
+};
+
+// Checks them (T > 0) and fills the kernel's arguments but for where keys and
+// values go.
+int rope_args(const RopeSpec& r, mgi::RopeArgs* a) {
+  if (!r.q_out || !r.q || !r.k || !r.positions || !r.cos_sin) return fail(MGI_EINVAL, "null tensor pointer");
+  if (!r.qo || !r.qs || !r.ks) return fail(MGI_EINVAL, "null stride array");
+  if (r.Hq <= 0 || r.Hk <= 0 || r.D <= 0) return fail(MGI_EINVAL, "q and k dimensions must be nonzero");
+  if (!valid_dtype(r.dtype) || !valid_dtype(r.out_dtype)) return fail(MGI_EINVAL, "unknown dtype code");
+  if (!valid_itype(r.pos_itype)) return fail(MGI_EINVAL, "positions must be int32 or int64");
+  if (!nonneg(r.qo, 3) || !nonneg(r.qs, 3) || !nonneg(r.ks, 3) || r.pos_stride < 0 || r.table_stride < 0)
+    return fail(MGI_EINVAL, "strides must be non-negative");
+  if (r.rotary_dim < 2 || r.rotary_dim % 2 != 0 || r.rotary_dim > r.D)
+    return fail(MGI_EINVAL, "rotary_dim must be even, from 2 to head_dim");
+  if (r.table_rows < 1) return fail(MGI_EINVAL, "cos_sin needs at least one position");
+  if (!r.q_weight != !r.k_weight) return fail(MGI_EINVAL, "q_weight and k_weight come together");
+  if (r.q_weight && r.weight_dtype != MGI_F32 && r.weight_dtype != r.dtype)
+    return fail(MGI_EINVAL, "norm weights must have q's dtype or f32");
+  if (!std::isfinite(r.eps) || r.eps < 0.f) return fail(MGI_EINVAL, "eps must be finite and non-negative");
+  if (r.D > 512) return fail(MGI_EUNSUPPORTED, "head_dim larger than 512");
+  // One launch's threads, 64 to a head row at most, are counted in 32 bits.
+  if (r.Hq > kMaxGridYZ || r.Hk > kMaxGridYZ || r.T >= (int64_t(1) << 24) || r.T * (r.Hq + 2 * r.Hk) >= (int64_t(1) << 26))
+    return fail(MGI_EUNSUPPORTED, "rows x heads too large for one launch");
+  a->q = r.q;
+  a->q_st = r.qs[0], a->q_sh = r.qs[1], a->q_sd = r.qs[2];
+  a->k = r.k;
+  a->k_st = r.ks[0], a->k_sh = r.ks[1], a->k_sd = r.ks[2];
+  a->q_out = r.q_out;
+  a->qo_st = r.qo[0], a->qo_sh = r.qo[1], a->qo_sd = r.qo[2];
+  a->positions = r.positions;
+  a->pos_s = r.pos_stride;
+  a->pos_i64 = r.pos_itype == MGI_I64;
+  a->table = r.cos_sin;
+  a->table_s = r.table_stride;
+  a->P = r.table_rows;
+  a->qw = r.q_weight;
+  a->kw = r.k_weight;
+  a->w_f32 = r.weight_dtype == MGI_F32;
+  a->dtype = r.dtype;
+  a->eps = r.eps;
+  a->inv_d = 1.0f / (float)r.D;
+  a->T = (int)r.T;
+  a->Hq = (int)r.Hq;
+  a->Hk = (int)r.Hk;
+  a->D = (int)r.D;
+  a->R = (int)r.rotary_dim;
+  a->interleaved = r.interleaved != 0;
+  a->cus = device_cus();
+  return MGI_OK;
+}
+
+// Picks the chunk of the vector kernel (0: the one for any strides) and launches.
+// A lane's two chunks must not straddle the halves they lie in, and every chunk
+// of every row must be aligned to its size, up to 16 bytes.
+int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
+  const int64_t eb = dtype_bytes(a.dtype), ob = dtype_bytes(out_dtype);
+  auto fits = [](int64_t bytes, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides, int64_t e) {
+    const int64_t al = std::min<int64_t>(16, bytes);
+    for (const void* p : ptrs)
+      if (reinterpret_cast<uintptr_t>(p) % (uintptr_t)al) return false;
+    for (int64_t s : strides)
+      if (s * e % al) return false;
+    return true;
+  };
+  const bool unit = a.q_sd == 1 && a.k_sd == 1 && a.qo_sd == 1 && a.ko_sd == 1 && (!a.Hv || (a.v_sd == 1 && a.vo_sd == 1));
+  a.chunk = 0;
+  for (int c : {8, 4}) {
+    if (c * eb > 16 || !unit || (a.R / 2) % c || (a.D - a.R) % (2 * c)) continue;
+    if (fits(c * eb, {a.q, a.k, a.v}, {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh}, eb) &&
+        fits(c * ob, {a.q_out, a.k_out, a.v_out},
+             {a.qo_st, a.qo_sh, a.ko_sn, a.ko_st, a.ko_sh, a.vo_sn, a.vo_st, a.vo_sh}, ob)) {
+      a.chunk = c;
+      break;
+    }
+  }
+  const hipError_t e = mgi::launch_rope(a, a.dtype, out_dtype, stream);
+  if (e != hipSuccess) return fail(MGI_ELAUNCH, std::string("launch failed: ") + hipGetErrorString(e));
+  return MGI_OK;
+}
+
 // Checks the two decode-step linear calls share.
 int check_linear(std::initializer_list<const void*> tensors, int dtype, int64_t B, int64_t N, int64_t K) {
   using namespace mgi;
@@ -973,6 +1073,72 @@ int mgi_kv_append(void* k_pool, void* v_pool, const int64_t* k_pool_strides,
   if (rc != MGI_OK) return rc;
   return launch_append(ap, k_pool_strides, v_pool_strides, pool_dtype, T, H, D, S, N, layer_idx,
                        static_cast<hipStream_t>(stream));
+}
+
+int mgi_qk_norm_rope(void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
+                     const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                     const void* positions, int64_t pos_stride, int pos_itype, const float* cos_sin,
+                     int64_t table_stride, int64_t table_rows, int64_t rotary_dim, const void* q_weight,
+                     const void* k_weight, int weight_dtype, float eps, int interleaved, int64_t T, int64_t Hq,
+                     int64_t Hk, int64_t D, void* stream) {
+  g_err.clear();
+  if (T < 0) return fail(MGI_EINVAL, "row count must be non-negative");
+  if (T == 0) return MGI_OK;
+  mgi::RopeArgs a{};
+  const int rc = rope_args({q_out, q_out_strides, q, q_strides, k, k_strides, dtype, dtype, positions, pos_stride,
+                            pos_itype, cos_sin, table_stride, table_rows, rotary_dim, q_weight, k_weight,
+                            weight_dtype, eps, interleaved, T, Hq, Hk, D}, &a);
+  if (rc != MGI_OK) return rc;
+  if (!k_out) return fail(MGI_EINVAL, "null tensor pointer");
+  if (!k_out_strides) return fail(MGI_EINVAL, "null stride array");
+  if (!nonneg(k_out_strides, 3)) return fail(MGI_EINVAL, "strides must be non-negative");
+  a.k_out = k_out;
+  a.ko_st = k_out_strides[0], a.ko_sh = k_out_strides[1], a.ko_sd = k_out_strides[2];
+  return launch_rope_checked(a, dtype, static_cast<hipStream_t>(stream));
+}
+
+int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, void* k_pool, void* v_pool,
+                       const int64_t* k_pool_strides, const int64_t* v_pool_strides, int pool_dtype, const void* q,
+                       const int64_t* q_strides, const void* k_new, const int64_t* k_new_strides, const void* v_new,
+                       const int64_t* v_new_strides, int new_dtype, const void* slot_mapping, int64_t slot_stride,
+                       int slot_itype, const void* positions, int64_t pos_stride, int pos_itype,
+                       const float* cos_sin, int64_t table_stride, int64_t table_rows, int64_t rotary_dim,
+                       const void* q_weight, const void* k_weight, int weight_dtype, float eps, int interleaved,
+                       int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t N, int64_t L,
+                       int64_t layer_idx, void* stream) {
+  g_err.clear();
+  if (T < 0) return fail(MGI_EINVAL, "row count must be non-negative");
+  if (T == 0) return MGI_OK;
+  if (!k_pool || !v_pool) return fail(MGI_EINVAL, "null tensor pointer");
+  if (!k_pool_strides || !v_pool_strides) return fail(MGI_EINVAL, "null stride array");
+  if (S <= 0 || N <= 0 || L <= 0) return fail(MGI_EINVAL, "pool dimensions must be nonzero");
+  if (layer_idx < 0 || layer_idx >= L) return fail(MGI_EINVAL, "layer_idx outside KV pool");
+  if (S >= (int64_t(1) << 31)) return fail(MGI_EUNSUPPORTED, "block size must be < 2^31");
+  if (!valid_dtype(pool_dtype)) return fail(MGI_EINVAL, "unknown dtype code");
+  if (!nonneg(k_pool_strides, 5) || !nonneg(v_pool_strides, 5)) return fail(MGI_EINVAL, "strides must be non-negative");
+  AppendSpec ap{k_pool, v_pool, k_new, v_new, k_new_strides, v_new_strides, new_dtype, slot_mapping, slot_stride,
+                slot_itype};
+  int rc = check_append(ap, pool_dtype, T);
+  if (rc != MGI_OK) return rc;
+  mgi::RopeArgs a{};
+  rc = rope_args({q_out, q_out_strides, q, q_strides, k_new, k_new_strides, new_dtype, pool_dtype, positions,
+                  pos_stride, pos_itype, cos_sin, table_stride, table_rows, rotary_dim, q_weight, k_weight,
+                  weight_dtype, eps, interleaved, T, Hq, Hk, D}, &a);
+  if (rc != MGI_OK) return rc;
+  const int64_t pb = dtype_bytes(pool_dtype);
+  a.v = v_new;
+  a.v_st = v_new_strides[0], a.v_sh = v_new_strides[1], a.v_sd = v_new_strides[2];
+  a.k_out = static_cast<char*>(k_pool) + layer_idx * k_pool_strides[0] * pb;
+  a.ko_sn = k_pool_strides[1], a.ko_st = k_pool_strides[2], a.ko_sh = k_pool_strides[3], a.ko_sd = k_pool_strides[4];
+  a.v_out = static_cast<char*>(v_pool) + layer_idx * v_pool_strides[0] * pb;
+  a.vo_sn = v_pool_strides[1], a.vo_st = v_pool_strides[2], a.vo_sh = v_pool_strides[3], a.vo_sd = v_pool_strides[4];
+  a.slots = slot_mapping;
+  a.sl_s = slot_stride;
+  a.sl_i64 = slot_itype == MGI_I64;
+  a.Hv = (int)Hk;
+  a.S = (int)S;
+  a.N = N;
+  return launch_rope_checked(a, pool_dtype, static_cast<hipStream_t>(stream));
 }
 
 int mgi_decode_linear(void* out, const void* x, const void* weight, const void* bias, int gelu, int dtype,

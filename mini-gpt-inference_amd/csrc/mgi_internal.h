@@ -74,6 +74,43 @@ struct AppendArgs {
   int64_t N;
 };
 
+// Head norms and position rotation, with or without the append (see rope.hip).
+// Strides in elements; the pool pointers already point at layer layer_idx.
+struct RopeArgs {
+  const void* q;
+  const void* k;
+  const void* v;       // append only
+  int64_t q_st, q_sh, q_sd;
+  int64_t k_st, k_sh, k_sd;
+  int64_t v_st, v_sh, v_sd;
+  void* q_out;
+  int64_t qo_st, qo_sh, qo_sd;
+  void* k_out;         // [T, Hk, D], or the pool's keys: st is then the stride of a slot in its block
+  int64_t ko_sn, ko_st, ko_sh, ko_sd;
+  void* v_out;         // the pool's values
+  int64_t vo_sn, vo_st, vo_sh, vo_sd;
+  const void* slots;   // null: k_out is [T, Hk, D]
+  int64_t sl_s;
+  int sl_i64;
+  const void* positions;
+  int64_t pos_s;
+  int pos_i64;
+  const float* table;  // [P, R]: cos of the R/2 angles, then sin
+  int64_t table_s, P;
+  const void* qw;      // RMS norm weights [D], both or neither
+  const void* kw;
+  int w_f32;           // weights are f32 (else of q's type)
+  int dtype;           // of q, k, v
+  float eps, inv_d;
+  int T, Hq, Hk, Hv, D, R, S;
+  int64_t N;
+  int interleaved;
+  int chunk;           // elements of a lane's chunk (8 or 4), 0: the kernel for any strides
+  int gp_shift;        // log2(lanes per head row), set by the launcher
+  int cus;
+};
+hipError_t launch_rope(const RopeArgs& a, int in_dtype, int out_dtype, hipStream_t stream);
+
 // Paged prefill attention of one chunk: query row i (absolute position
 // start + i) attends keys 0 .. start + i through one block-table row. Pool
 // pointers already point at layer layer_idx; strides are in elements and the

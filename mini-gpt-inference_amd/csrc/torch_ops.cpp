@@ -11,6 +11,7 @@
 // marshalling of 20-30 arguments per call; the kernels and their launch
 // decisions are the library's, unchanged. Nothing here computes attention.
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -204,6 +205,106 @@ at::Tensor paged_prefill(const at::Tensor& q, const at::Tensor& kp, const at::Te
   return out;
 }
 
+void* ptr(const c10::optional<at::Tensor>& t) { return t ? t->data_ptr() : nullptr; }
+
+// Refuses what the pointers of t would not show (lazy negation), and gradients.
+void check_plain(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors) {
+    if (t->is_neg() || t->layout() != at::kStrided) value_error("tensors must be dense and not lazily negated");
+    if (at::GradMode::is_enabled() && t->requires_grad())
+      throw std::runtime_error("hip is inference-only; run under torch.inference_mode()");
+  }
+}
+
+// Checks the rotary calls share; q and k are [T,Hq,D] and [T,Hk,D].
+void check_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions, const at::Tensor& cos_sin,
+                const c10::optional<at::Tensor>& qw, const c10::optional<at::Tensor>& kw, double eps) {
+  if (!q.is_cuda()) value_error("q must be on a GPU device for the HIP backend");
+  if (q.dim() != 3 || k.dim() != 3) value_error("q and k must have shapes [T,Hq,D] and [T,Hk,D]");
+  const int64_t T = q.size(0), D = q.size(2);
+  if (k.size(0) != T || k.size(2) != D) value_error("k must have q's rows and head dimension");
+  if (q.size(1) == 0 || k.size(1) == 0 || D == 0) value_error("q and k dimensions must be nonzero");
+  if (D > 512) value_error("HIP backend supports head_dim <= 512");
+  if (dtype_code(q.scalar_type()) < 0) value_error("q must be float32, bfloat16 or float16");
+  if (k.scalar_type() != q.scalar_type()) value_error("q and k must share a float dtype");
+  if (positions.dim() != 1 || positions.size(0) != T) value_error("positions must have shape [T]");
+  if (index_code(positions.scalar_type()) < 0) value_error("positions must be integer");
+  if (cos_sin.dim() != 2 || cos_sin.scalar_type() != at::kFloat || cos_sin.stride(1) != 1)
+    value_error("cos_sin must be a float32 table [positions, rotary_dim] with contiguous rows");
+  if (cos_sin.size(1) < 2 || cos_sin.size(1) % 2 != 0 || cos_sin.size(1) > D)
+    value_error("rotary_dim must be even, from 2 to head_dim");
+  if (cos_sin.size(0) < 1) value_error("cos_sin needs at least one position");
+  if (qw.has_value() != kw.has_value()) value_error("q_weight and k_weight come together");
+  const auto dev = q.device();
+  if (k.device() != dev || positions.device() != dev || cos_sin.device() != dev)
+    value_error("all inputs must reside on same GPU device");
+  check_plain({&q, &k, &positions, &cos_sin});
+  if (qw) {
+    for (const at::Tensor* w : {&*qw, &*kw}) {
+      if (w->dim() != 1 || w->size(0) != D || !w->is_contiguous() || w->scalar_type() != qw->scalar_type() ||
+          (w->scalar_type() != at::kFloat && w->scalar_type() != q.scalar_type()))
+        value_error("q_weight and k_weight must be contiguous [head_dim] tensors of q's dtype or float32");
+      if (w->device() != dev) value_error("all inputs must reside on same GPU device");
+    }
+    check_plain({&*qw, &*kw});
+  }
+  if (!std::isfinite((float)eps) || eps < 0) value_error("eps must be finite and non-negative");
+}
+
+// qk_norm_rope(q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved) ->
+// (q_out, k_out), fresh contiguous tensors.
+py::tuple qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                       const at::Tensor& cos_sin, const c10::optional<at::Tensor>& qw,
+                       const c10::optional<at::Tensor>& kw, double eps, bool interleaved) {
+  check_rope(q, k, positions, cos_sin, qw, kw, eps);
+  const c10::DeviceGuard guard(q.device());
+  at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  check_status(mgi_qk_norm_rope(
+      qo.data_ptr(), qo.strides().data(), ko.data_ptr(), ko.strides().data(), q.data_ptr(), q.strides().data(),
+      k.data_ptr(), k.strides().data(), dtype_code(q.scalar_type()), positions.data_ptr(), positions.stride(0),
+      index_code(positions.scalar_type()), cos_sin.data_ptr<float>(), cos_sin.stride(0), cos_sin.size(0),
+      cos_sin.size(1), ptr(qw), ptr(kw), qw ? dtype_code(qw->scalar_type()) : MGI_F32, (float)eps, interleaved,
+      q.size(0), q.size(1), k.size(1), q.size(2), stream_of(q)));
+  return py::make_tuple(qo, ko);
+}
+
+// kv_append_rope(k_pool, v_pool, layer_idx, q, k, v, slot_mapping, positions,
+// cos_sin, q_weight, k_weight, eps, interleaved) -> q_out in the pool's dtype.
+at::Tensor kv_append_rope(const at::Tensor& kp, const at::Tensor& vp, int64_t layer_idx, const at::Tensor& q,
+                          const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots,
+                          const at::Tensor& positions, const at::Tensor& cos_sin,
+                          const c10::optional<at::Tensor>& qw, const c10::optional<at::Tensor>& kw, double eps,
+                          bool interleaved) {
+  if (!kp.is_cuda()) value_error("KV pool must be on a GPU device for the HIP backend");
+  if (k.dim() != 3 || v.sizes() != k.sizes()) value_error("k and v must have matching shape [T,H,D]");
+  check_pool(kp, vp);
+  const int64_t T = k.size(0), L = kp.size(0), N = kp.size(1), S = kp.size(2), H = kp.size(3), D = kp.size(4);
+  if (S <= 0) value_error("block_size must be positive");
+  if (k.size(1) != H || k.size(2) != D) value_error("k/v head dimensions do not match the KV pool");
+  const int pd = dtype_code(kp.scalar_type());
+  if (pd < 0 || vp.scalar_type() != kp.scalar_type()) value_error("KV pool must be float32, bfloat16 or float16");
+  if (v.scalar_type() != k.scalar_type()) value_error("k and v must share a float dtype");
+  if (slots.dim() != 1 || slots.size(0) != T) value_error("slot_mapping must have shape [T]");
+  const int st = index_code(slots.scalar_type());
+  if (st < 0) value_error("slot_mapping must contain integer slots");
+  if (layer_idx < 0 || layer_idx >= L) value_error("layer_idx outside KV pool");
+  check_rope(q, k, positions, cos_sin, qw, kw, eps);
+  const auto dev = q.device();
+  if (kp.device() != dev || vp.device() != dev || v.device() != dev || slots.device() != dev)
+    value_error("all inputs must reside on same GPU device");
+  check_plain({&kp, &vp, &v, &slots});
+  const c10::DeviceGuard guard(dev);
+  at::Tensor qo = at::empty(q.sizes(), kp.options());
+  check_status(mgi_kv_append_rope(
+      qo.data_ptr(), qo.strides().data(), kp.data_ptr(), vp.data_ptr(), kp.strides().data(), vp.strides().data(), pd,
+      q.data_ptr(), q.strides().data(), k.data_ptr(), k.strides().data(), v.data_ptr(), v.strides().data(),
+      dtype_code(q.scalar_type()), slots.data_ptr(), slots.stride(0), st, positions.data_ptr(), positions.stride(0),
+      index_code(positions.scalar_type()), cos_sin.data_ptr<float>(), cos_sin.stride(0), cos_sin.size(0),
+      cos_sin.size(1), ptr(qw), ptr(kw), qw ? dtype_code(qw->scalar_type()) : MGI_F32, (float)eps, interleaved, T,
+      q.size(1), H, D, S, N, L, layer_idx, stream_of(q)));
+  return qo;
+}
+
 // Whether t is a plain contiguous, 16-byte aligned tensor of x's dtype and
 // (current) device with `numel` elements: what the decode-step linear kernels
 // take.
@@ -216,7 +317,6 @@ bool linear_ok(const at::Tensor& t, const at::Tensor& x, int64_t numel) {
 bool linear_ok(const c10::optional<at::Tensor>& t, const at::Tensor& x, int64_t numel) {
   return !t || linear_ok(*t, x, numel);
 }
-void* ptr(const c10::optional<at::Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 
 // decode_linear(x, weight, bias, gelu): act(x W^T + bias) for x [B, 1, K] -> [B,
 // 1, N]; None when the kernel does not take the call, or PyTorch's calls are the
@@ -274,11 +374,14 @@ py::object decode_linear_norm(const c10::optional<at::Tensor>& x, const c10::opt
 }  // namespace
 
 PYBIND11_MODULE(_hip_ops, m) {
-  m.doc() = "PyTorch binding of libminivllm_hip.so (kv_append, paged_decode, paged_decode_append, paged_prefill)";
+  m.doc() = "PyTorch binding of libminivllm_hip.so (kv_append, kv_append_rope, qk_norm_rope, paged_decode, "
+            "paged_decode_append, paged_prefill, decode_linear, decode_linear_norm)";
   m.def("kv_append", &kv_append);
   m.def("paged_decode", &paged_decode);
   m.def("paged_decode_append", &paged_decode_append);
   m.def("paged_prefill", &paged_prefill);
+  m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("kv_append_rope", &kv_append_rope);
   m.def("decode_linear", &decode_linear);
   m.def("decode_linear_norm", &decode_linear_norm);
 }

@@ -207,6 +207,123 @@ def paged_prefill(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, bt: torch
     return out
 
 
+def _check_plain(*tensors: torch.Tensor) -> None:
+    """Refuses what a tensor's pointer would not show (lazy negation), and gradients."""
+    for t in tensors:
+        if t.is_neg() or t.layout != torch.strided:
+            raise ValueError("tensors must be dense and not lazily negated")
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError("hip is inference-only; run under torch.inference_mode()")
+
+
+def _check_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                qw: torch.Tensor | None, kw: torch.Tensor | None, eps: float) -> None:
+    if not q.is_cuda:
+        raise ValueError("q must be on a GPU device for the HIP backend")
+    if q.ndim != 3 or k.ndim != 3:
+        raise ValueError("q and k must have shapes [T,Hq,D] and [T,Hk,D]")
+    t, h, d = q.shape
+    if k.shape[0] != t or k.shape[2] != d:
+        raise ValueError("k must have q's rows and head dimension")
+    if h == 0 or k.shape[1] == 0 or d == 0:
+        raise ValueError("q and k dimensions must be nonzero")
+    if d > 512:
+        raise ValueError("HIP backend supports head_dim <= 512")
+    if q.dtype not in _FLOATS:
+        raise ValueError("q must be float32, bfloat16 or float16")
+    if k.dtype != q.dtype:
+        raise ValueError("q and k must share a float dtype")
+    if positions.ndim != 1 or positions.shape[0] != t:
+        raise ValueError("positions must have shape [T]")
+    if positions.dtype not in _INDEX:
+        raise ValueError("positions must be integer")
+    if cos_sin.ndim != 2 or cos_sin.dtype != torch.float32 or cos_sin.stride(1) != 1:
+        raise ValueError("cos_sin must be a float32 table [positions, rotary_dim] with contiguous rows")
+    if cos_sin.shape[1] < 2 or cos_sin.shape[1] % 2 != 0 or cos_sin.shape[1] > d:
+        raise ValueError("rotary_dim must be even, from 2 to head_dim")
+    if cos_sin.shape[0] < 1:
+        raise ValueError("cos_sin needs at least one position")
+    if (qw is None) != (kw is None):
+        raise ValueError("q_weight and k_weight come together")
+    if any(x.device != q.device for x in (k, positions, cos_sin)):
+        raise ValueError("all inputs must reside on same GPU device")
+    _check_plain(q, k, positions, cos_sin)
+    if qw is not None:
+        for w in (qw, kw):
+            if w.ndim != 1 or w.shape[0] != d or not w.is_contiguous() or w.dtype != qw.dtype \
+                    or w.dtype not in (torch.float32, q.dtype):
+                raise ValueError("q_weight and k_weight must be contiguous [head_dim] tensors of q's dtype or float32")
+            if w.device != q.device:
+                raise ValueError("all inputs must reside on same GPU device")
+        _check_plain(qw, kw)
+    if not math.isfinite(eps) or eps > 3.4028234e38 or eps < 0:
+        raise ValueError("eps must be finite and non-negative")
+
+
+def _rope_tail(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+               qw: torch.Tensor | None, kw: torch.Tensor | None, eps: float, interleaved: bool) -> list:
+    return [positions.data_ptr(), positions.stride(0), _native.ITYPE_CODES[positions.dtype], cos_sin.data_ptr(),
+            cos_sin.stride(0), *cos_sin.shape, _ptr(qw), _ptr(kw),
+            _native.DTYPE_CODES[torch.float32 if qw is None else qw.dtype], float(eps), int(interleaved),
+            q.shape[0], q.shape[1], k.shape[1], q.shape[2]]
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                 qw: torch.Tensor | None, kw: torch.Tensor | None, eps: float, interleaved: bool):
+    """(q_out, k_out): head norms and position rotation."""
+    _check_rope(q, k, positions, cos_sin, qw, kw, eps)
+    lib = _native.lib()
+    with torch.cuda.device(q.device):
+        qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _native.check(lib.mgi_qk_norm_rope(
+            qo.data_ptr(), _native.strides(qo), ko.data_ptr(), _native.strides(ko), q.data_ptr(), _native.strides(q),
+            k.data_ptr(), _native.strides(k), _native.DTYPE_CODES[q.dtype],
+            *_rope_tail(q, k, positions, cos_sin, qw, kw, eps, interleaved), _native.stream_handle(q.device)))
+    return qo, ko
+
+
+def kv_append_rope(kp: torch.Tensor, vp: torch.Tensor, layer_idx: int, q: torch.Tensor, k: torch.Tensor,
+                   v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                   qw: torch.Tensor | None, kw: torch.Tensor | None, eps: float, interleaved: bool) -> torch.Tensor:
+    """kv_append with head norms and rotation on the way; the queries' in the pool's dtype."""
+    if not kp.is_cuda:
+        raise ValueError("KV pool must be on a GPU device for the HIP backend")
+    if k.ndim != 3 or v.shape != k.shape:
+        raise ValueError("k and v must have matching shape [T,H,D]")
+    _check_pool(kp, vp)
+    L, N, S, H, D = kp.shape
+    T = k.shape[0]
+    if S <= 0:
+        raise ValueError("block_size must be positive")
+    if k.shape[1] != H or k.shape[2] != D:
+        raise ValueError("k/v head dimensions do not match the KV pool")
+    if kp.dtype not in _FLOATS or vp.dtype != kp.dtype:
+        raise ValueError("KV pool must be float32, bfloat16 or float16")
+    if v.dtype != k.dtype:
+        raise ValueError("k and v must share a float dtype")
+    if slots.ndim != 1 or slots.shape[0] != T:
+        raise ValueError("slot_mapping must have shape [T]")
+    if slots.dtype not in _INDEX:
+        raise ValueError("slot_mapping must contain integer slots")
+    if not 0 <= layer_idx < L:
+        raise ValueError("layer_idx outside KV pool")
+    _check_rope(q, k, positions, cos_sin, qw, kw, eps)
+    if any(x.device != q.device for x in (kp, vp, v, slots)):
+        raise ValueError("all inputs must reside on same GPU device")
+    _check_plain(kp, vp, v, slots)
+    lib = _native.lib()
+    with torch.cuda.device(q.device):
+        qo = torch.empty(q.shape, dtype=kp.dtype, device=q.device)
+        _native.check(lib.mgi_kv_append_rope(
+            qo.data_ptr(), _native.strides(qo), kp.data_ptr(), vp.data_ptr(), _native.strides(kp),
+            _native.strides(vp), _native.DTYPE_CODES[kp.dtype], q.data_ptr(), _native.strides(q),
+            k.data_ptr(), _native.strides(k), v.data_ptr(), _native.strides(v), _native.DTYPE_CODES[q.dtype],
+            slots.data_ptr(), slots.stride(0), _native.ITYPE_CODES[slots.dtype],
+            *_rope_tail(q, k, positions, cos_sin, qw, kw, eps, interleaved), S, N, L, int(layer_idx),
+            _native.stream_handle(q.device)))
+    return qo
+
+
 def _linear_ok(t: torch.Tensor | None, x: torch.Tensor, numel: int) -> bool:
     """Whether t (or no tensor) is plain, contiguous and 16-byte aligned, of x's
     dtype and (current) device, with numel elements."""

@@ -45,6 +45,8 @@ EXPORTED_SYMBOLS = (
     "mgi_decode_linear_norm",
     "mgi_decode_linear_norm_pays",
     "mgi_decode_linear_norm_workspace_bytes",
+    "mgi_qk_norm_rope",
+    "mgi_kv_append_rope",
 )
 
 _lock = threading.Lock()
@@ -138,6 +140,29 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mgi_decode_linear_norm_pays.argtypes = [_i64, _i64, _i64]
     lib.mgi_decode_linear_norm_workspace_bytes.restype = ctypes.c_size_t
     lib.mgi_decode_linear_norm_workspace_bytes.argtypes = [_i64, _i64, _i64]
+    rope = [
+        _p, _i64, _i,                      # positions, stride, itype
+        _p, _i64, _i64, _i64,              # cos_sin, row stride, rows, rotary_dim
+        _p, _p, _i,                        # q and k norm weights, dtype
+        ctypes.c_float, _i,                # eps, interleaved
+        _i64, _i64, _i64, _i64,            # T Hq Hk D
+    ]
+    lib.mgi_qk_norm_rope.restype = _i
+    lib.mgi_qk_norm_rope.argtypes = [
+        _p, _pi64, _p, _pi64,              # q_out, k_out, strides
+        _p, _pi64, _p, _pi64, _i,          # q, k, strides, dtype
+        *rope, _p,                         # stream
+    ]
+    lib.mgi_kv_append_rope.restype = _i
+    lib.mgi_kv_append_rope.argtypes = [
+        _p, _pi64,                         # q_out, strides
+        _p, _p, _pi64, _pi64, _i,          # pools, strides, pool dtype
+        _p, _pi64, _p, _pi64, _p, _pi64, _i,  # q, new k/v, strides, dtype
+        _p, _i64, _i,                      # slot mapping, stride, itype
+        *rope,
+        _i64, _i64, _i64, _i64,            # S N L layer
+        _p,                                # stream
+    ]
 
 
 def lib() -> ctypes.CDLL:
@@ -167,7 +192,8 @@ def lib() -> ctypes.CDLL:
 
 def ops():
     """The eager path's binding: kv_append, paged_decode, paged_decode_append,
-    paged_prefill, decode_linear and decode_linear_norm on tensors, validated,
+    paged_prefill, decode_linear, decode_linear_norm, qk_norm_rope and
+    kv_append_rope on tensors, validated,
     calling the C ABI on the current stream.
 
     Normally the PyTorch extension _hip_ops (csrc/torch_ops.cpp). When the

@@ -26,6 +26,11 @@ paged_prefill_hip is the prefill counterpart (the reference's per-token
 loop, minivllm/attention.py:269-299, and its sdpa_v2 gather,
 minivllm/attention.py:229-267): causal attention of one chunk's queries over
 the sequence's cached prefix and the chunk itself, read from the pool.
+
+qk_norm_rope_hip and kv_append_rope_hip norm and rotate query and key heads by
+their positions, the latter on the way into the pool. They are inference-only
+(RuntimeError for tensors that require gradients while grad mode is on) and run
+on their tensors' device, current or not.
 """
 from __future__ import annotations
 
@@ -81,6 +86,50 @@ def kv_append(pool: KVBlockPool, layer_idx: int, k: torch.Tensor, v: torch.Tenso
     with a negative slot are skipped. Bit-exact when k/v share the pool dtype.
     """
     _native.ops().kv_append(pool.k, pool.v, int(layer_idx), k, v, slot_mapping)
+
+
+def rope_table(positions: int, rotary_dim: int, *, base: float = 10000.0, device=None) -> torch.Tensor:
+    """The cos_sin table of the rotary calls: [positions, rotary_dim] float32, row p
+    holding the cosines of p * base ** (-2 i / rotary_dim), i < rotary_dim / 2, then
+    the sines. The angles are computed in 64 bits, as 32 lose far positions."""
+    if positions < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rope_table needs positions >= 1 and an even rotary_dim")
+    half = rotary_dim // 2
+    freq = base ** (-torch.arange(half, dtype=torch.float64, device=device) / half)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat((angle.cos(), angle.sin()), dim=1).float()
+
+
+def qk_norm_rope_hip(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                     q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, *,
+                     eps: float = 1e-6, interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head (with the weights, [D]) and the
+    rotation by its row's position, in one pass.
+
+    q: [T, Hq, D], k: [T, Hk, D], any strides; positions: [T] integers; cos_sin: a
+    rope_table of rotary_dim <= D. Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1)
+    when ``interleaved``; dims past rotary_dim are normed only. Arithmetic is
+    float32, rounded once. A position outside the table gives NaN in the rotated
+    dims. Returns fresh contiguous (q_out, k_out).
+    """
+    return _native.ops().qk_norm_rope(q, k, positions, cos_sin, q_weight, k_weight, float(eps), bool(interleaved))
+
+
+def kv_append_rope_hip(pool: KVBlockPool, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       slot_mapping: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                       q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, *,
+                       eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
+    """kv_append of the rotated keys and the values, and the rotated queries, in
+    one launch: qk_norm_rope_hip's norms (with weights) and rotation, the keys
+    and values written to the pool's slots under kv_append's rules.
+
+    q: [T, Hq, D]; k, v: [T, H, D] of the pool's H heads; a chunk's T rows or a decode
+    batch's. Returns the queries, [T, Hq, D] in the pool's dtype, for the attention
+    that follows. Rows with a negative slot, or a position outside the table,
+    leave the pool as it was.
+    """
+    return _native.ops().kv_append_rope(pool.k, pool.v, int(layer_idx), q, k, v, slot_mapping, positions, cos_sin,
+                                        q_weight, k_weight, float(eps), bool(interleaved))
 
 
 def paged_prefill_hip(q: torch.Tensor, pool: KVBlockPool, block_table: torch.Tensor,
