@@ -62,8 +62,9 @@ const char* mgi_last_error(void);
  * 1.02 the prefill key split (mgi_paged_prefill's workspace arguments and
  * mgi_paged_prefill_workspace_bytes); 1.03 mgi_paged_decode_noalloc; 1.04
  * mgi_paged_decode_append. mgi_decode_linear, mgi_decode_linear_norm, their
- * queries, mgi_paged_decode_workgroup_waves, mgi_qk_norm_rope and
- * mgi_kv_append_rope came later without a change to the others. */
+ * queries, mgi_paged_decode_workgroup_waves, mgi_qk_norm_rope,
+ * mgi_kv_append_rope and mgi_paged_decode_shared came later without a change to
+ * the others. */
 int mgi_abi_version(void);
 
 /*
@@ -395,6 +396,43 @@ int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
                        float eps, int interleaved,
                        int64_t T, int64_t Hq, int64_t Hk, int64_t D,
                        int64_t S, int64_t N, int64_t L, int64_t layer_idx, void* stream);
+
+/*
+ * Decode attention of a batch whose sequences begin with the same cached blocks:
+ * mgi_paged_decode's result (one query token per sequence), with the first
+ * shared_blocks entries of every row of block_tables taken from row 0, and those
+ * blocks read once for all rows. No counterpart in the reference.
+ *
+ * q and out are [B, Hq, D] with Hq a multiple of the pool's Hk heads: query head h
+ * reads KV head h / (Hq / Hk). Context lengths count all tokens, the shared ones
+ * included; a sequence shorter than shared_blocks * S reads its first tokens from
+ * row 0's blocks all the same, by itself. Lengths are clamped to [0, M*S], a table
+ * entry outside [0, N) masks its block, a row without keys gives 0, and only the
+ * tokens of some row's context enter any result. Arithmetic is f32, but that 2-byte types round
+ * the softmax weights to their type for the second product (as mgi_paged_prefill).
+ * 0 <= shared_blocks <= M. B <= 65535, B*Hq < 2^25, M*S < 2^30, D <= 512.
+ *
+ * workspace: mgi_paged_decode_shared_workspace_bytes(...) bytes for the same sizes,
+ * 16-byte aligned; may be NULL when that is 0. Contents need no initialisation;
+ * calls that overlap in time need separate workspaces. Same inputs, same bits.
+ */
+int mgi_paged_decode_shared(void* out, const int64_t* out_strides, /* [3] */
+                            const void* q, const int64_t* q_strides, /* [3] */
+                            const void* k_pool, const void* v_pool,
+                            const int64_t* k_pool_strides, /* [5] */
+                            const int64_t* v_pool_strides, /* [5] */
+                            int dtype,
+                            const void* block_tables, const int64_t* bt_strides, /* [2] */
+                            int bt_itype,
+                            const void* context_lens, int64_t cl_stride, int cl_itype,
+                            int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t N,
+                            int64_t M, int64_t L, int64_t layer_idx, int64_t shared_blocks,
+                            float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes mgi_paged_decode_shared needs for these sizes on the current
+ * device (0 if none). */
+size_t mgi_paged_decode_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S,
+                                               int64_t M, int64_t shared_blocks, int dtype);
 
 #ifdef __cplusplus
 }

@@ -781,6 +781,53 @@ int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
   return MGI_OK;
 }
 
+// How mgi_paged_decode_shared runs a call of these sizes on the matrix-core kernels.
+struct SharedPlan {
+  int one_launch, gsets, vheads, row_tiles, row_sets, chunks, chunk_tiles, prefix_wgs, own_waves, own_min_tiles;
+  int64_t own_slot, cont_slot, slots;
+  size_t ml_offset, cum_offset, total;
+};
+
+SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M, int64_t shared, int dtype) {
+  SharedPlan p{};
+  const int64_t G = Hq / Hk, cus = device_cus(), keys = dtype == MGI_F32 ? 16 : 32;
+  p.gsets = (int)((G + 15) / 16);
+  p.vheads = (int)(Hk * p.gsets);
+  const int64_t tiles = (shared * S + keys - 1) / keys;
+  const int64_t own_bound = B * ((M * S + keys - 1) / keys) * p.vheads;
+  const int forced = env_int("MINIVLLM_HIP_SHARED_SPLIT", -1);
+  p.one_launch = B > mgi::kSharedMaxB || own_bound >= (int64_t(1) << 30) || forced == 0;
+  if (p.one_launch) return p;
+  const int64_t rows = B * G;
+  p.row_tiles = rows <= 16 ? 1 : rows <= 32 || D > 128 ? 2 : 4;
+  p.row_tiles = std::min(p.row_tiles, env_int("MINIVLLM_HIP_SHARED_TILES", 4));
+  p.row_sets = (int)((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
+  if (tiles) {
+    const int64_t target = std::max<int64_t>(1, env_int("MINIVLLM_HIP_SHARED_WGS", 2) * cus / (Hk * p.row_sets));
+    p.chunk_tiles = (int)std::max<int64_t>((tiles + target - 1) / target, env_int("MINIVLLM_HIP_SHARED_CHUNK", 8));
+    p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
+    p.prefix_wgs = (int)(p.chunks * Hk * p.row_sets);
+  }
+  p.own_waves = (int)(4 * env_int("MINIVLLM_HIP_SHARED_OWN", 2) * cus);
+  p.own_min_tiles = 2;
+  p.own_slot = B * Hq * p.chunks;
+  p.cont_slot = p.own_slot + B * Hq;
+  p.slots = p.cont_slot + (int64_t)p.own_waves * 16;
+  p.ml_offset = (size_t)round_up(p.slots * D * 4, kWorkspaceAlign);
+  p.cum_offset = (size_t)round_up((int64_t)p.ml_offset + p.slots * 8, kWorkspaceAlign);
+  p.total = p.cum_offset + (size_t)(B * 4);
+  return p;
+}
+
+// n / d = umulhi(n, mul) >> shift for 0 <= n < 2^31 and d >= 2: with 2^(s-1) < d <=
+// 2^s, mul = ceil(2^(31+s) / d) exceeds the quotient by less than 2^s / d.
+void magic_of(int64_t d, uint32_t* mul, int* shift) {
+  int s = 1;
+  while ((int64_t(1) << s) < d) ++s;
+  *mul = d < 2 ? 0 : (uint32_t)(((uint64_t(1) << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d);
+  *shift = s - 1;
+}
+
 // Checks the two decode-step linear calls share.
 int check_linear(std::initializer_list<const void*> tensors, int dtype, int64_t B, int64_t N, int64_t K) {
   using namespace mgi;
@@ -1139,6 +1186,102 @@ int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, void* k_pool, 
   a.S = (int)S;
   a.N = N;
   return launch_rope_checked(a, pool_dtype, static_cast<hipStream_t>(stream));
+}
+
+size_t mgi_paged_decode_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M,
+                                               int64_t shared_blocks, int dtype) {
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk != 0 || D <= 0 || S <= 0 || M <= 0 || M >= (int64_t(1) << 30) / S ||
+      shared_blocks < 0 || shared_blocks > M || B > kMaxGridYZ || Hq > kMaxGridYZ || !valid_dtype(dtype))
+    return 0;
+  return D % 8 == 0 && D <= 256 ? shared_plan(B, Hq, Hk, D, S, M, shared_blocks, dtype).total : 0;
+}
+
+int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides,
+                            const void* k_pool, const void* v_pool, const int64_t* k_pool_strides,
+                            const int64_t* v_pool_strides, int dtype, const void* block_tables,
+                            const int64_t* bt_strides, int bt_itype, const void* context_lens, int64_t cl_stride,
+                            int cl_itype, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t N,
+                            int64_t M, int64_t L, int64_t layer_idx, int64_t shared_blocks, float scale,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mgi;
+  g_err.clear();
+  if (!out || !q || !k_pool || !v_pool || !block_tables || !context_lens) return fail(MGI_EINVAL, "null tensor pointer");
+  if (!out_strides || !q_strides || !k_pool_strides || !v_pool_strides || !bt_strides)
+    return fail(MGI_EINVAL, "null stride array");
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || D <= 0) return fail(MGI_EINVAL, "q dimensions must be nonzero");
+  if (Hq % Hk != 0) return fail(MGI_EINVAL, "query heads must be a multiple of the pool's heads");
+  if (S <= 0 || N <= 0 || L <= 0) return fail(MGI_EINVAL, "pool dimensions must be nonzero");
+  if (M < 1) return fail(MGI_EINVAL, "block_tables need at least one block column");
+  if (shared_blocks < 0 || shared_blocks > M) return fail(MGI_EINVAL, "shared_blocks outside the block tables");
+  if (layer_idx < 0 || layer_idx >= L) return fail(MGI_EINVAL, "layer_idx outside KV pool");
+  if (!valid_dtype(dtype)) return fail(MGI_EINVAL, "unknown dtype code");
+  if (!valid_itype(bt_itype) || !valid_itype(cl_itype)) return fail(MGI_EINVAL, "index arrays must be int32 or int64");
+  if (!std::isfinite(scale)) return fail(MGI_EINVAL, "scale must be finite");
+  if (!nonneg(out_strides, 3) || !nonneg(q_strides, 3) || !nonneg(k_pool_strides, 5) || !nonneg(v_pool_strides, 5) ||
+      !nonneg(bt_strides, 2) || cl_stride < 0)
+    return fail(MGI_EINVAL, "strides must be non-negative");
+  if (B > kMaxGridYZ || Hq > kMaxGridYZ) return fail(MGI_EUNSUPPORTED, "batch or heads larger than 65535");
+  if (B * Hq >= (int64_t(1) << 25)) return fail(MGI_EUNSUPPORTED, "rows x heads too large for one launch");
+  if (M >= (int64_t(1) << 30) / S) return fail(MGI_EUNSUPPORTED, "M*S must be < 2^30");
+  if (D > 512) return fail(MGI_EUNSUPPORTED, "head_dim larger than 512");
+
+  const int64_t eb = dtype_bytes(dtype);
+  SharedArgs a{};
+  a.k = static_cast<const char*>(k_pool) + layer_idx * k_pool_strides[0] * eb;
+  a.v = static_cast<const char*>(v_pool) + layer_idx * v_pool_strides[0] * eb;
+  a.out = out;
+  a.o_sb = out_strides[0], a.o_sh = out_strides[1], a.o_sd = out_strides[2];
+  a.q = q;
+  a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_sd = q_strides[2];
+  a.k_sn = k_pool_strides[1], a.k_ss = k_pool_strides[2], a.k_sh = k_pool_strides[3], a.k_sd = k_pool_strides[4];
+  a.v_sn = v_pool_strides[1], a.v_ss = v_pool_strides[2], a.v_sh = v_pool_strides[3], a.v_sd = v_pool_strides[4];
+  a.bt = block_tables;
+  a.bt_sb = bt_strides[0], a.bt_sm = bt_strides[1];
+  a.bt_i64 = bt_itype == MGI_I64;
+  a.cl = context_lens;
+  a.cl_s = cl_stride;
+  a.cl_i64 = cl_itype == MGI_I64;
+  a.B = (int)B, a.Hq = (int)Hq, a.G = (int)(Hq / Hk), a.D = (int)D, a.S = (int)S, a.M = (int)M;
+  a.N = N;
+  a.shared = (int)shared_blocks;
+  a.P = (int)(shared_blocks * S);
+  a.scale_log2 = scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f;
+  a.lazy = 6.f / a.scale_log2;
+  a.q_flip = scale < 0.f ? (dtype == MGI_F32 ? 0x80000000u : 0x80008000u) : 0u;
+  a.q_zero = scale == 0.f;
+  magic_of(S, &a.s_mul, &a.s_shift);
+  magic_of(a.G, &a.g_mul, &a.g_shift);
+  // The matrix-core kernels: 16-byte pieces of head rows, contiguous and aligned,
+  // a 16-token run within 32-bit offsets.
+  a.tiles = D % 8 == 0 && D <= 256 && q_strides[2] == 1 && out_strides[2] == 1 && k_pool_strides[4] == 1 &&
+            v_pool_strides[4] == 1 && aligned16(q) && aligned16(out) && aligned16(a.k) && aligned16(a.v) &&
+            mult16(q_strides[0], eb) && mult16(q_strides[1], eb) && mult16(out_strides[0], eb) &&
+            mult16(out_strides[1], eb) && mult16(a.k_sn, eb) && mult16(a.k_ss, eb) && mult16(a.k_sh, eb) &&
+            mult16(a.v_sn, eb) && mult16(a.v_ss, eb) && mult16(a.v_sh, eb) &&
+            std::max(a.k_ss, a.v_ss) * eb < (int64_t(1) << 27);
+  if (a.tiles) {
+    const SharedPlan p = shared_plan(B, Hq, Hk, D, S, M, shared_blocks, dtype);
+    a.one_launch = p.one_launch;
+    a.gsets = p.gsets, a.vheads = p.vheads, a.row_tiles = p.row_tiles, a.row_sets = p.row_sets;
+    a.chunks = p.chunks, a.chunk_tiles = p.chunk_tiles, a.prefix_wgs = p.prefix_wgs;
+    a.own_waves = p.own_waves, a.own_min_tiles = p.own_min_tiles;
+    a.own_slot = p.own_slot, a.cont_slot = p.cont_slot;
+    if (!p.one_launch) {
+      if (!workspace) return fail(MGI_EWORKSPACE, "workspace required for the split pass");
+      if (workspace_bytes < p.total)
+        return fail(MGI_EWORKSPACE, "workspace smaller than mgi_paged_decode_shared_workspace_bytes()");
+      if (!aligned16(workspace)) return fail(MGI_EINVAL, "workspace must be 16-byte aligned");
+      a.ws_acc = static_cast<float*>(workspace);
+      a.ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.ml_offset);
+      a.ws_cum = reinterpret_cast<int*>(static_cast<char*>(workspace) + p.cum_offset);
+    }
+  }
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const hipError_t e = dtype == MGI_F32    ? launch_paged_shared_f32(a, st)
+                       : dtype == MGI_BF16 ? launch_paged_shared_bf16(a, st)
+                                           : launch_paged_shared_f16(a, st);
+  if (e != hipSuccess) return fail(MGI_ELAUNCH, std::string("launch failed: ") + hipGetErrorString(e));
+  return MGI_OK;
 }
 
 int mgi_decode_linear(void* out, const void* x, const void* weight, const void* bias, int gelu, int dtype,

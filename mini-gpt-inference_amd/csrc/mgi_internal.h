@@ -111,6 +111,50 @@ struct RopeArgs {
 };
 hipError_t launch_rope(const RopeArgs& a, int in_dtype, int out_dtype, hipStream_t stream);
 
+// Decode attention of a batch with shared leading blocks (see paged_shared.h).
+// Strides in elements; the pool pointers already point at layer layer_idx.
+struct SharedArgs {
+  void* out;
+  int64_t o_sb, o_sh, o_sd;
+  const void* q;
+  int64_t q_sb, q_sh, q_sd;
+  const void* k;
+  const void* v;
+  int64_t k_sn, k_ss, k_sh, k_sd;
+  int64_t v_sn, v_ss, v_sh, v_sd;
+  const void* bt;
+  int64_t bt_sb, bt_sm;
+  const void* cl;
+  int64_t cl_s;
+  int bt_i64, cl_i64;
+  int B, Hq, G, D, S, M;   // G query heads per KV head
+  int64_t N;
+  int shared, P;           // shared blocks, and their tokens
+  float scale_log2, lazy;  // |scale| * log2(e) (1 for a scale of 0); the maximum's slack in raw scores
+  uint32_t q_flip;         // sign bits of a word of q, for a negative scale
+  int q_zero;              // scale is 0
+  uint32_t s_mul, g_mul;   // divisions by S and G (magic_of)
+  int s_shift, g_shift;
+  int tiles;               // the matrix-core kernels (else the one for any strides)
+  int one_launch;          // one workgroup per (row, virtual head)
+  int gsets, vheads;       // sets of 16 query heads per KV head; KV heads times sets
+  int row_tiles, row_sets; // shared piece: 16-row query tiles per wavefront, and sets of those
+  int chunks, chunk_tiles; // shared piece: ranges of tokens, key tiles in each
+  int prefix_wgs;          // row_sets * chunks * KV heads
+  int own_waves;           // wavefronts for the rows' own tokens
+  int own_min_tiles;       // least tiles of one of their segments
+  // Partials: [B, Hq, chunks] of the shared piece, [B, Hq] of the first own
+  // pieces, 16 for each own wavefront's continued one.
+  int64_t own_slot, cont_slot;
+  float* ws_acc;           // [slots, D]
+  float2* ws_ml;           // [slots] (maximum in log2 units, sum)
+  int* ws_cum;             // [B] prefix sums of the rows' own tiles
+};
+constexpr int kSharedMaxB = 4096;      // rows of the split form (their prefix sums live in LDS)
+hipError_t launch_paged_shared_f32(const SharedArgs& a, hipStream_t stream);
+hipError_t launch_paged_shared_bf16(const SharedArgs& a, hipStream_t stream);
+hipError_t launch_paged_shared_f16(const SharedArgs& a, hipStream_t stream);
+
 // Paged prefill attention of one chunk: query row i (absolute position
 // start + i) attends keys 0 .. start + i through one block-table row. Pool
 // pointers already point at layer layer_idx; strides are in elements and the

@@ -305,6 +305,49 @@ at::Tensor kv_append_rope(const at::Tensor& kp, const at::Tensor& vp, int64_t la
   return qo;
 }
 
+// paged_decode_shared(q, k_pool, v_pool, block_tables, context_lengths, layer_idx,
+// shared_blocks) -> [B, Hq, D] of q's dtype: paged_decode with the first
+// shared_blocks blocks of all rows those of row 0, read once.
+at::Tensor paged_decode_shared(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& bt,
+                               const at::Tensor& cl, int64_t layer_idx, int64_t shared_blocks) {
+  if (!q.is_cuda()) value_error("q must be on a GPU device for the HIP backend");
+  if (q.dim() != 3) value_error("q must have shape [B,H,D]");
+  const int64_t b = q.size(0), h = q.size(1), d = q.size(2);
+  if (b == 0 || h == 0 || d == 0) value_error("q dimensions must be nonzero");
+  if (d > 512) value_error("HIP backend supports head_dim <= 512");
+  const int qd = dtype_code(q.scalar_type());
+  if (qd < 0) value_error("q must be float32, bfloat16 or float16");
+  if (kp.scalar_type() != q.scalar_type() || vp.scalar_type() != q.scalar_type())
+    value_error("KV pool dtype must match q dtype");
+  check_pool(kp, vp);
+  const int64_t L = kp.size(0), N = kp.size(1), S = kp.size(2), hk = kp.size(3);
+  if (S <= 0) value_error("block_size must be positive");
+  if (hk <= 0 || h % hk != 0 || kp.size(4) != d)
+    value_error("q heads must be a multiple of the KV pool's, of its head dimension");
+  if (bt.dim() != 2 || bt.size(0) != b) value_error("block_tables must have shape [B,M]");
+  if (cl.dim() != 1 || cl.size(0) != b) value_error("context_lengths must have shape [B]");
+  if (index_code(bt.scalar_type()) < 0) value_error("block_tables must contain integer indices");
+  if (index_code(cl.scalar_type()) < 0) value_error("context_lengths must be integer");
+  if (layer_idx < 0 || layer_idx >= L) value_error("layer_idx outside KV pool");
+  const auto dev = q.device();
+  if (kp.device() != dev || vp.device() != dev || bt.device() != dev || cl.device() != dev)
+    value_error("all inputs must reside on same GPU device");
+  const int64_t M = bt.size(1);
+  if (M < 1) value_error("block_tables need at least one block column");
+  if (shared_blocks < 0 || shared_blocks > M) value_error("shared_blocks outside the block tables");
+  check_plain({&q, &kp, &vp, &bt, &cl});
+  const c10::DeviceGuard guard(dev);
+  at::Tensor out = at::empty({b, h, d}, q.options()), ws;
+  const size_t ws_bytes = mgi_paged_decode_shared_workspace_bytes(b, h, hk, d, S, M, shared_blocks, qd);
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte));
+  check_status(mgi_paged_decode_shared(
+      out.data_ptr(), out.strides().data(), q.data_ptr(), q.strides().data(), kp.data_ptr(), vp.data_ptr(),
+      kp.strides().data(), vp.strides().data(), qd, bt.data_ptr(), bt.strides().data(), index_code(bt.scalar_type()),
+      cl.data_ptr(), cl.stride(0), index_code(cl.scalar_type()), b, h, hk, d, S, N, M, L, layer_idx, shared_blocks,
+      (float)(1.0 / std::sqrt((double)d)), ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q)));
+  return out;
+}
+
 // Whether t is a plain contiguous, 16-byte aligned tensor of x's dtype and
 // (current) device with `numel` elements: what the decode-step linear kernels
 // take.
@@ -375,11 +418,12 @@ py::object decode_linear_norm(const c10::optional<at::Tensor>& x, const c10::opt
 
 PYBIND11_MODULE(_hip_ops, m) {
   m.doc() = "PyTorch binding of libminivllm_hip.so (kv_append, kv_append_rope, qk_norm_rope, paged_decode, "
-            "paged_decode_append, paged_prefill, decode_linear, decode_linear_norm)";
+            "paged_decode_append, paged_decode_shared, paged_prefill, decode_linear, decode_linear_norm)";
   m.def("kv_append", &kv_append);
   m.def("paged_decode", &paged_decode);
   m.def("paged_decode_append", &paged_decode_append);
   m.def("paged_prefill", &paged_prefill);
+  m.def("paged_decode_shared", &paged_decode_shared);
   m.def("qk_norm_rope", &qk_norm_rope);
   m.def("kv_append_rope", &kv_append_rope);
   m.def("decode_linear", &decode_linear);

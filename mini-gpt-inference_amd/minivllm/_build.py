@@ -43,7 +43,8 @@ HIP_FLAGS = [
 # the prefill kernel's MFMA results in AGPRs and copies them back and forth
 # for the softmax (64 v_accvgpr moves per key tile).
 MFMA_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-MFMA_SOURCES = {"decode_linear.hip", "paged_prefill.hip"}
+MFMA_SOURCES = {"decode_linear.hip", "paged_prefill.hip", "paged_shared_f32.hip", "paged_shared_bf16.hip",
+                "paged_shared_f16.hip"}
 
 
 def library_path() -> Path:

@@ -324,6 +324,62 @@ def kv_append_rope(kp: torch.Tensor, vp: torch.Tensor, layer_idx: int, q: torch.
     return qo
 
 
+def paged_decode_shared(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, bt: torch.Tensor, cl: torch.Tensor,
+                        layer_idx: int, shared_blocks: int) -> torch.Tensor:
+    """paged_decode with the first shared_blocks blocks of all rows those of row 0, read once."""
+    if not q.is_cuda:
+        raise ValueError("q must be on a GPU device for the HIP backend")
+    if q.ndim != 3:
+        raise ValueError("q must have shape [B,H,D]")
+    b, h, d = q.shape
+    if b == 0 or h == 0 or d == 0:
+        raise ValueError("q dimensions must be nonzero")
+    if d > 512:
+        raise ValueError("HIP backend supports head_dim <= 512")
+    if q.dtype not in _FLOATS:
+        raise ValueError("q must be float32, bfloat16 or float16")
+    if kp.dtype != q.dtype or vp.dtype != q.dtype:
+        raise ValueError("KV pool dtype must match q dtype")
+    _check_pool(kp, vp)
+    L, N, S, hk = kp.shape[:4]
+    if S <= 0:
+        raise ValueError("block_size must be positive")
+    if hk <= 0 or h % hk != 0 or kp.shape[4] != d:
+        raise ValueError("q heads must be a multiple of the KV pool's, of its head dimension")
+    if bt.ndim != 2 or bt.shape[0] != b:
+        raise ValueError("block_tables must have shape [B,M]")
+    if cl.ndim != 1 or cl.shape[0] != b:
+        raise ValueError("context_lengths must have shape [B]")
+    if bt.dtype not in _INDEX:
+        raise ValueError("block_tables must contain integer indices")
+    if cl.dtype not in _INDEX:
+        raise ValueError("context_lengths must be integer")
+    if not 0 <= layer_idx < L:
+        raise ValueError("layer_idx outside KV pool")
+    if any(x.device != q.device for x in (kp, vp, bt, cl)):
+        raise ValueError("all inputs must reside on same GPU device")
+    M = bt.shape[1]
+    if M < 1:
+        raise ValueError("block_tables need at least one block column")
+    if not 0 <= shared_blocks <= M:
+        raise ValueError("shared_blocks outside the block tables")
+    _check_plain(q, kp, vp, bt, cl)
+    lib = _native.lib()
+    code = _native.DTYPE_CODES[q.dtype]
+    with torch.cuda.device(q.device):
+        out = torch.empty((b, h, d), dtype=q.dtype, device=q.device)
+        ws_bytes = int(lib.mgi_paged_decode_shared_workspace_bytes(b, h, hk, d, S, M, int(shared_blocks), code))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        _native.check(lib.mgi_paged_decode_shared(
+            out.data_ptr(), _native.strides(out), q.data_ptr(), _native.strides(q),
+            kp.data_ptr(), vp.data_ptr(), _native.strides(kp), _native.strides(vp), code,
+            bt.data_ptr(), _native.strides(bt), _native.ITYPE_CODES[bt.dtype],
+            cl.data_ptr(), cl.stride(0), _native.ITYPE_CODES[cl.dtype],
+            b, h, hk, d, S, N, M, L, int(layer_idx), int(shared_blocks), 1.0 / math.sqrt(d),
+            _ptr(ws), ws_bytes, _native.stream_handle(q.device)))
+    return out
+
+
 def _linear_ok(t: torch.Tensor | None, x: torch.Tensor, numel: int) -> bool:
     """Whether t (or no tensor) is plain, contiguous and 16-byte aligned, of x's
     dtype and (current) device, with numel elements."""

@@ -47,6 +47,8 @@ EXPORTED_SYMBOLS = (
     "mgi_decode_linear_norm_workspace_bytes",
     "mgi_qk_norm_rope",
     "mgi_kv_append_rope",
+    "mgi_paged_decode_shared",
+    "mgi_paged_decode_shared_workspace_bytes",
 )
 
 _lock = threading.Lock()
@@ -163,6 +165,20 @@ def _declare(lib: ctypes.CDLL) -> None:
         _i64, _i64, _i64, _i64,            # S N L layer
         _p,                                # stream
     ]
+    lib.mgi_paged_decode_shared.restype = _i
+    lib.mgi_paged_decode_shared.argtypes = [
+        _p, _pi64,                         # out, strides
+        _p, _pi64,                         # q, strides
+        _p, _p, _pi64, _pi64, _i,          # pools, strides, dtype
+        _p, _pi64, _i,                     # block tables, strides, itype
+        _p, _i64, _i,                      # context lengths, stride, itype
+        _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,  # B Hq Hk D S N M L layer
+        _i64, ctypes.c_float,              # shared blocks, scale
+        _p, ctypes.c_size_t,               # workspace, bytes
+        _p,                                # stream
+    ]
+    lib.mgi_paged_decode_shared_workspace_bytes.restype = ctypes.c_size_t
+    lib.mgi_paged_decode_shared_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i]
 
 
 def lib() -> ctypes.CDLL:
@@ -192,8 +208,8 @@ def lib() -> ctypes.CDLL:
 
 def ops():
     """The eager path's binding: kv_append, paged_decode, paged_decode_append,
-    paged_prefill, decode_linear, decode_linear_norm, qk_norm_rope and
-    kv_append_rope on tensors, validated,
+    paged_prefill, decode_linear, decode_linear_norm, qk_norm_rope,
+    kv_append_rope and paged_decode_shared on tensors, validated,
     calling the C ABI on the current stream.
 
     Normally the PyTorch extension _hip_ops (csrc/torch_ops.cpp). When the

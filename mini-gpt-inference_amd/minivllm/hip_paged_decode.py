@@ -78,6 +78,26 @@ def paged_attention_batch_append_hip(q: torch.Tensor, pool: KVBlockPool, block_t
                                              k, v, slot_mapping, int(split_tokens))
 
 
+def paged_attention_shared_prefix_hip(q: torch.Tensor, pool: KVBlockPool, block_tables: torch.Tensor,
+                                      context_lengths: torch.Tensor, layer_idx: int, *,
+                                      shared_blocks: int) -> torch.Tensor:
+    """paged_attention_batch_hip for sequences that begin with the same cached
+    blocks: the first ``shared_blocks`` entries of every row of block_tables are
+    taken from row 0 (the others' are not read), and those blocks' keys and
+    values are read once for all rows, on the matrix cores.
+
+    q: [B, Hq, D] with Hq a multiple of the pool's heads H; query head h reads KV
+    head h // (Hq // H). context_lengths count a sequence's tokens, the shared ones
+    included; a sequence shorter than the shared blocks (a padding row of
+    length 0, say) is attended by itself. shared_blocks = 0 is plain decode
+    attention with grouped query heads. Returns a fresh [B, Hq, D] tensor of
+    q.dtype. 2-byte types round the softmax weights to their type for the product
+    with the values, as paged_prefill_hip does; sums are float32.
+    """
+    return _native.ops().paged_decode_shared(q, pool.k, pool.v, block_tables, context_lengths, int(layer_idx),
+                                             int(shared_blocks))
+
+
 def kv_append(pool: KVBlockPool, layer_idx: int, k: torch.Tensor, v: torch.Tensor,
               slot_mapping: torch.Tensor) -> None:
     """Scatters rows k[t], v[t] ([T, H, D], any strides) into pool slots slot_mapping[t].

@@ -1,0 +1,352 @@
+"""paged_attention_shared_prefix_hip against the softmax in 64 bits: the split form
+and the one-launch form, grouped heads, rows shorter than the shared blocks, NaN
+in every slot no row holds, masked entries, odd block sizes and strides, scores of
+-inf, graphs and streams, and a rotary decode step through the pool.
+
+Tolerance. With A = sum_t w_t |V_t| (w the softmax weights), u = 2^-24 and n keys:
+ - a score is a chain of D fused terms: off by at most D u X, X = scale sum_d
+   |q_d k_d|; scaling, the exponent's difference and exp2 add 4 u (1 + X); a weight
+   and the sum that divides it are each off by that: 2 (D + 4) u max_t X + 8 u;
+ - n fused additions into output and sum, joined over pieces: 2 (n + 32) u;
+ - 2-byte types: every weight rounded, at most eps / 2 of it: eps / 2 of A;
+ - the output's rounding: eps / 2 of itself (f32: u)."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from minivllm import _ctypes_ops, _native
+from minivllm import hip_paged_decode as hpd
+from minivllm.kv_block_pool import KVBlockPool
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DTYPES = pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+ROUTES = pytest.mark.parametrize("route", ["split", "one"])
+
+
+@pytest.fixture(autouse=True)
+def _route(request, monkeypatch):
+    route = request.node.callspec.params.get("route") if hasattr(request.node, "callspec") else None
+    if route:
+        monkeypatch.setenv("MINIVLLM_HIP_SHARED_SPLIT", "1" if route == "split" else "0")
+
+
+def make(B, Hq, Hk, D, S, shared, ctx, dtype, seed=0, layers=2, layer=1, itype=torch.int64):
+    """q, pool, tables, lengths over a permuted pool with NaN in every slot that no row holds."""
+    g = torch.Generator().manual_seed(seed)
+    M = max(1, shared, max(-(-max(0, c) // S) for c in ctx))
+    need = [max(0, -(-c // S) - shared) for c in ctx]
+    N = shared + sum(need) + 3
+    perm = torch.randperm(N, generator=g)
+    tables = torch.full((B, M), -1, dtype=torch.int64)
+    tables[0, :shared] = perm[:shared]  # the other rows' shared entries stay -1: they are not read
+    at = shared
+    used = torch.zeros((N, S), dtype=torch.bool)
+    longest = max(ctx)
+    for i in range(shared):
+        used[perm[i], :max(0, min(S, longest - i * S))] = True
+    for b in range(B):
+        for i in range(need[b]):
+            tables[b, shared + i] = perm[at]
+            used[perm[at], :max(0, min(S, ctx[b] - (shared + i) * S))] = True
+            at += 1
+    pool = KVBlockPool(layers, N, S, Hk, D, device=DEV, dtype=dtype)
+    for t in (pool.k, pool.v):
+        t.fill_(float("nan"))
+        x = torch.randn((N, S, Hk, D), generator=g)
+        x[~used] = float("nan")
+        t[layer] = x.to(dtype).to(DEV)
+    q = torch.randn((B, Hq, D), generator=g).to(dtype).to(DEV)
+    return q, pool, tables.to(itype).to(DEV), torch.tensor(ctx, dtype=itype, device=DEV), layer
+
+
+def reference(q, pool, tables, ctx, layer, shared, scale=None):
+    """(out, A, X, n) in 64 bits; a row without keys gives 0."""
+    B, Hq, D = q.shape
+    _, N, S, Hk, _ = pool.k.shape
+    G, M = Hq // Hk, tables.shape[1]
+    scale = 1 / math.sqrt(D) if scale is None else scale
+    out = torch.zeros((B, Hq, D), dtype=torch.float64, device=DEV)
+    A, X, most = torch.zeros_like(out), torch.zeros((B, Hq, 1), dtype=torch.float64, device=DEV), 0
+    for b in range(B):
+        c = min(max(int(ctx[b]), 0), M * S)
+        t = torch.arange(c, device=DEV)
+        blk = t // S
+        row = torch.where(blk < shared, tables[0, blk], tables[b, blk]).long()
+        ok = (row >= 0) & (row < N)
+        row, off = row[ok], (t % S)[ok]
+        if row.numel() == 0:
+            continue
+        most = max(most, row.numel())
+        k = pool.k[layer, row, off].double().repeat_interleave(G, 1)  # [n, Hq, D]
+        v = pool.v[layer, row, off].double().repeat_interleave(G, 1)
+        s = (k * q[b].double()).sum(-1) * scale
+        w = torch.softmax(s, 0)[..., None]
+        out[b], A[b] = (w * v).sum(0), (w * v.abs()).sum(0)
+        X[b, :, 0] = (k * q[b].double()).abs().sum(-1).amax(0) * abs(scale)
+    return out, A, X, most
+
+
+def check(got, want, dtype, what=""):
+    out, A, X, n = want
+    D = got.shape[-1]
+    half = 0.5 * torch.finfo(dtype).eps
+    bound = (2 * (D + 4) * U * X + 8 * U + 2 * (n + 32) * U) * A + half * out.abs()
+    if dtype != F32:
+        bound = bound + half * A
+    bound = bound * 1.01 + torch.finfo(dtype).tiny * half
+    assert torch.isfinite(got).all(), f"{what}: {int((~torch.isfinite(got)).sum())} not finite"
+    worst = ((got.double() - out).abs() / bound).max().item()
+    assert worst <= 1.0, f"{what}: {worst:.3g} of the bound"
+
+
+# (B, Hq, Hk, D, S, shared blocks, lengths): the shared tokens are shared * S.
+CASES = {
+    "one row one token": (1, 1, 1, 64, 16, 0, [1]),
+    "one row shared only": (1, 4, 4, 64, 16, 1, [16]),
+    "two short": (2, 2, 1, 128, 16, 2, [33, 40]),
+    "lengths around the shared blocks": (9, 4, 4, 128, 16, 3, [48, 0, 1, 47, 49, 63, 64, 65, 200]),
+    "all shorter than the shared blocks": (4, 6, 2, 64, 16, 4, [63, 5, 0, 40]),
+    "no shared blocks": (5, 8, 2, 128, 16, 0, [1, 17, 300, 64, 0]),
+    "grouped 8, tile ends inside": (7, 16, 2, 128, 16, 5, [81, 90, 100, 80, 333, 97, 112]),
+    "many rows": (40, 6, 3, 64, 32, 9, [288 + 7 * i for i in range(40)]),
+    "rows past one set": (70, 4, 2, 128, 16, 11, [176 + (i * 37) % 130 for i in range(70)]),
+    "wide groups": (3, 40, 2, 64, 16, 6, [96, 130, 211]),
+    "padded head dim": (6, 4, 2, 80, 16, 7, [112, 113, 150, 128, 90, 300]),
+    "narrow heads": (4, 8, 8, 32, 16, 8, [200, 256, 131, 222]),
+    "head dim 8": (3, 2, 2, 8, 16, 2, [40, 33, 32]),
+    "wide heads": (5, 4, 2, 256, 16, 4, [64, 70, 100, 64, 150]),
+    "wide padded heads": (20, 6, 3, 200, 32, 3, [96 + 9 * i for i in range(20)]),
+    "block size 3": (4, 4, 2, 64, 3, 31, [93, 94, 120, 50]),
+    "block size 1": (3, 2, 2, 128, 1, 70, [70, 71, 139]),
+    "block size 24": (4, 6, 2, 128, 24, 3, [72, 80, 173, 96]),
+    "block size 48": (4, 6, 6, 96, 48, 2, [96, 97, 250, 110]),
+    "odd head dim": (4, 4, 2, 20, 16, 3, [48, 50, 64, 30]),
+    "head dim 512": (3, 2, 1, 512, 16, 2, [32, 40, 33]),
+    "long": (3, 4, 2, 128, 16, 130, [2080, 2500, 5000]),
+}
+
+
+@DTYPES
+@ROUTES
+@pytest.mark.parametrize("name", CASES)
+def test_against_64_bits(name, dtype, route):
+    B, Hq, Hk, D, S, shared, ctx = CASES[name]
+    q, pool, tables, lens, layer = make(B, Hq, Hk, D, S, shared, ctx, dtype, seed=len(name))
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=shared)
+    again = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=shared)
+    assert got.shape == q.shape and got.dtype == dtype and got.is_contiguous()
+    check(got, reference(q, pool, tables, lens, layer, shared), dtype, name)
+    assert torch.equal(got, again)
+    for b, c in enumerate(ctx):
+        assert c > 0 or not got[b].any()
+
+
+@DTYPES
+@ROUTES
+def test_masked_entries_and_clamped_lengths(dtype, route):
+    """Entries outside the pool mask their blocks, in the shared and in a row's own
+    part; a row whose every entry is masked gives 0; lengths past the table and
+    below 0 are clamped."""
+    ctx = [160, 161, 320, 200, 175, 100]
+    q, pool, tables, lens, layer = make(6, 6, 2, 128, 16, 10, ctx, dtype, seed=3, itype=torch.int32)
+    N = pool.k.shape[1]
+    tables[0, 3], tables[0, 9] = -1, N
+    tables[2, 15], tables[3, 10] = N + 5, -7
+    tables[2, 19] = -1
+    lens[2], lens[5] = 100000, -4
+    # The slots this row now reaches must be finite, where its blocks are.
+    pool.k.nan_to_num_(0.25), pool.v.nan_to_num_(0.25)
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=10)
+    check(got, reference(q, pool, tables, lens, layer, 10), dtype)
+    assert not got[5].any()
+    tables.fill_(-1)
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=10)
+    assert not got.any()
+
+
+@DTYPES
+@ROUTES
+def test_infinite_scores_and_values_in_unused_slots(dtype, route):
+    """A score of -inf is a weight of 0, a row of nothing else NaN, as softmax has
+    it; NaN or infinite keys and values past a length do not show (make() puts NaN
+    there; infinities here)."""
+    ctx = [64, 70, 33, 1, 96]
+    q, pool, tables, lens, layer = make(5, 4, 4, 64, 16, 2, ctx, dtype, seed=9)
+    pool.k.copy_(torch.where(pool.k.isnan(), torch.inf, pool.k)), pool.v.copy_(torch.where(pool.v.isnan(), -torch.inf, pool.v))
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k = pool.k[layer]
+    k[tables[0, 0].long(), 3, :, 0] = -torch.inf
+    k[tables[1, 4].long(), 2, :, 0] = -torch.inf
+    k[tables[4, 5].long(), :, :, 0] = -torch.inf
+    k[tables[0, 0].long(), 0, :, 0] = -torch.inf  # all that row 3 holds
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=2)
+    out, A, X, n = reference(q, pool, tables, lens, layer, 2)
+    assert torch.isnan(got[3]).all() and torch.isnan(out[3]).all()
+    rest = [0, 1, 2, 4]
+    X = torch.full_like(X, 16.0)  # more than the finite keys have: 64 products of unit normals over 8
+    check(got[rest], (out[rest], A[rest], X[rest], n), dtype)
+
+
+@ROUTES
+def test_large_scores(route):
+    """Scores that differ by hundreds: late maxima rescale what came before."""
+    ctx = [400, 321, 500]
+    for dtype in (BF16, F32):
+        q, pool, tables, lens, layer = make(3, 4, 2, 128, 16, 20, ctx, dtype, seed=4)
+        ramp = torch.linspace(0.1, 30, 500, device=DEV)
+        for b in range(3):
+            for t in range(ctx[b]):
+                e = tables[0 if t < 320 else b, t // 16].long()
+                if t >= 320 or b == 0:
+                    pool.k[layer, e, t % 16] *= ramp[t].to(dtype)
+        got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=20)
+        check(got, reference(q, pool, tables, lens, layer, 20), dtype, str(dtype))
+
+
+@ROUTES
+def test_strides_and_layouts(route):
+    """q as a slice of a fused projection, transposed q, a pool whose heads come
+    first or whose head dim is strided, tables and lengths strided: the same values."""
+    ctx = [80, 90, 300, 64]
+    q, pool, tables, lens, layer = make(4, 8, 2, 64, 16, 4, ctx, BF16, seed=5)
+    want = reference(q, pool, tables, lens, layer, 4)
+    wide = torch.full((4, 14, 64), float("nan"), dtype=BF16, device=DEV)
+    wide[:, 3:11] = q
+    wide_t = torch.stack((tables, tables * 0 - 1), -1)[..., 0]
+    wide_l = torch.stack((lens, lens * 0), -1)[..., 0]
+    heads_first = KVBlockPool(1, 1, 1, 1, 1, device=DEV, dtype=BF16)
+    heads_first.k, heads_first.v = (t.transpose(2, 3).contiguous().transpose(2, 3) for t in (pool.k, pool.v))
+    apart = KVBlockPool(1, 1, 1, 1, 1, device=DEV, dtype=BF16)
+    apart.k, apart.v = (torch.stack((t, t), -1)[..., 1] for t in (pool.k, pool.v))
+    call = lambda *x: hpd.paged_attention_shared_prefix_hip(*x, layer, shared_blocks=4)
+    for name, args in {"slice": (wide[:, 3:11], pool, wide_t, wide_l),
+                       "transposed": (q.transpose(0, 1).contiguous().transpose(0, 1), pool, tables, lens),
+                       "dims apart": (q.transpose(1, 2).contiguous().transpose(1, 2), pool, tables, lens),
+                       "heads first": (q, heads_first, tables, lens), "strided pool": (q, apart, tables, lens)}.items():
+        check(call(*args), want, BF16, name)
+
+
+@ROUTES
+def test_any_finite_scale_through_the_c_entry(route):
+    lib = _native.lib()
+    ctx = [50, 49, 80, 20]
+    for dtype in (F32, F16):
+        q, pool, tables, lens, layer = make(4, 4, 2, 64, 16, 3, ctx, dtype, seed=6)
+        L, N, S, H, D = pool.k.shape
+        for scale in (0.3, -0.2, 0.0):
+            out = torch.full_like(q, float("nan"))
+            n = lib.mgi_paged_decode_shared_workspace_bytes(4, 4, 2, 64, S, tables.shape[1], 3, _native.DTYPE_CODES[dtype])
+            ws = torch.full((max(n, 16),), 255, dtype=torch.uint8, device=DEV)
+            _native.check(lib.mgi_paged_decode_shared(
+                out.data_ptr(), _native.strides(out), q.data_ptr(), _native.strides(q), pool.k.data_ptr(), pool.v.data_ptr(),
+                _native.strides(pool.k), _native.strides(pool.v), _native.DTYPE_CODES[dtype], tables.data_ptr(),
+                _native.strides(tables), 1, lens.data_ptr(), 1, 1, 4, 4, 2, 64, S, N, tables.shape[1], L, layer, 3, scale,
+                ws.data_ptr(), n, _native.stream_handle(DEV)))
+            check(out, reference(q, pool, tables, lens, layer, 3, scale), dtype, f"{dtype} {scale}")
+
+
+@ROUTES
+def test_graph_replays_beside_eager_calls(route):
+    """A captured call replayed on new inputs between eager ones: equal bits."""
+    ctx = [100, 64, 150, 70, 99]
+    q, pool, tables, lens, layer = make(5, 8, 4, 128, 16, 4, ctx, BF16, seed=7)
+    pool.k.nan_to_num_(0.5), pool.v.nan_to_num_(0.5)
+    call = lambda: hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(i)).to(BF16).to(DEV))
+        lens[2], lens[1] = 150 - 9 * i, 64 - 20 * i
+        graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        check(out, reference(q, pool, tables, lens, layer, 4), BF16, f"replay {i}")
+
+
+@ROUTES
+def test_two_streams_at_once(route):
+    ctx = [200 + 3 * i for i in range(30)]
+    q, pool, tables, lens, layer = make(30, 8, 4, 128, 16, 10, ctx, F16, seed=8)
+    call = lambda: hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=10)
+    want = call()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i in range(10):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_decode_steps_through_the_pool(interleaved):
+    """A common prompt appended by kv_append_rope_hip, then decode steps of six
+    sequences: rotary append and shared-prefix attention against the formulas in 64
+    bits on the pool's own values, and against paged_attention_batch_hip."""
+    B, H, D, S, P = 6, 4, 64, 16, 48
+    table = hpd.rope_table(256, D, device=DEV)
+    g = torch.Generator().manual_seed(21)
+    rand = lambda *s: torch.randn(s, generator=g).to(BF16).to(DEV)
+    pool = KVBlockPool(1, 40, S, H, D, device=DEV, dtype=BF16)
+    pool.k.fill_(float("nan")), pool.v.fill_(float("nan"))
+    perm = torch.randperm(40, generator=g)
+    tables = torch.full((B, 6), -1)
+    tables[:, :3] = perm[:3]
+    tables[:, 3:] = perm[3:3 + 3 * B].view(B, 3)
+    w = rand(D), rand(D)
+    at = lambda b, t: int(tables[b, t // S]) * S + t % S
+    x = rand(P, 3, H, D)
+    hpd.kv_append_rope_hip(pool, 0, x[:, 0], x[:, 1], x[:, 2], torch.tensor([at(0, t) for t in range(P)], device=DEV),
+                           torch.arange(P, device=DEV), table, *w, interleaved=interleaved)
+    own = [0, 3, 15, 16, 1, 30]
+    for step in range(35):
+        length = [P + min(o, step) + 1 for o in own]
+        pos = torch.tensor(length, device=DEV) - 1
+        slots = torch.tensor([at(b, n - 1) for b, n in enumerate(length)], device=DEV)
+        x = rand(B, 3, H, D)
+        q = hpd.kv_append_rope_hip(pool, 0, x[:, 0], x[:, 1], x[:, 2], slots, pos, table, *w, interleaved=interleaved)
+        lens, tab = pos + 1, tables.to(DEV)
+        out = hpd.paged_attention_shared_prefix_hip(q, pool, tab, lens, 0, shared_blocks=3)
+        if step % 7 == 0:
+            check(out, reference(q, pool, tab, lens, 0, 3), BF16, f"step {step}")
+            plain = hpd.paged_attention_batch_hip(q, pool, tab, lens, 0)
+            assert (out.float() - plain.float()).abs().max() <= 2.0 ** -6 * (1 + plain.float().abs().max())
+
+
+def test_ctypes_path_is_bit_identical_and_refuses_alike():
+    ext = _native._load_extension()
+    q, pool, tables, lens, layer = make(4, 8, 2, 64, 16, 4, [80, 64, 90, 10], BF16, seed=10)
+    a, b = (o.paged_decode_shared(q, pool.k, pool.v, tables, lens, layer, 4) for o in (ext, _ctypes_ops))
+    assert torch.equal(a, b)
+    zero = KVBlockPool(1, 4, 0, 2, 64, device=DEV, dtype=BF16)
+    grad = q.float().requires_grad_()
+    bad = {"rank": (q[0], pool.k, pool.v, tables, lens, 1, 4), "heads": (q[:, :7], pool.k, pool.v, tables, lens, 1, 4),
+           "dtype": (q.float(), pool.k, pool.v, tables, lens, 1, 4), "int": (q.int(), pool.k, pool.v, tables, lens, 1, 4),
+           "head dim": (q[..., :32], pool.k, pool.v, tables, lens, 1, 4), "tables": (q, pool.k, pool.v, tables[:3], lens, 1, 4),
+           "lengths": (q, pool.k, pool.v, tables, lens[:3], 1, 4), "table type": (q, pool.k, pool.v, tables.float(), lens, 1, 4),
+           "length type": (q, pool.k, pool.v, tables, lens.float(), 1, 4), "layer": (q, pool.k, pool.v, tables, lens, 2, 4),
+           "shared": (q, pool.k, pool.v, tables, lens, 1, 99), "negative": (q, pool.k, pool.v, tables, lens, 1, -1),
+           "no columns": (q, pool.k, pool.v, tables[:, :0], lens, 1, 0), "empty": (q[:0], pool.k, pool.v, tables[:0], lens[:0], 1, 0),
+           "block size": (q, zero.k, zero.v, tables, lens, 0, 0), "cpu": (q, pool.k, pool.v, tables.cpu(), lens, 1, 4),
+           "pool": (q, pool.k, pool.v[:, :2], tables, lens, 1, 4),
+           "gradient": (grad, pool.k.float(), pool.v.float(), tables, lens, 1, 4)}
+    for name, args in bad.items():
+        kind = RuntimeError if name == "gradient" else ValueError
+        with pytest.raises(kind) as x:
+            ext.paged_decode_shared(*args)
+        with pytest.raises(kind) as y:
+            _ctypes_ops.paged_decode_shared(*args)
+        assert str(x.value) == str(y.value), name
