@@ -783,36 +783,36 @@ int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
 
 // How mgi_paged_decode_shared runs a call of these sizes on the matrix-core kernels.
 struct SharedPlan {
-  int one_launch, gsets, vheads, row_tiles, row_sets, chunks, chunk_tiles, prefix_wgs, own_waves, own_min_tiles;
-  int64_t own_slot, cont_slot, slots;
+  int one_launch, gsets, vheads, wgs, lds_tiles, row_tiles, set_rows, row_sets, s_units, s_tiles, s_cost, s_min, own_min;
+  int64_t s_cont, own_slot, own_cont, slots;
   size_t ml_offset, cum_offset, total;
 };
 
 SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M, int64_t shared, int dtype) {
   SharedPlan p{};
-  const int64_t G = Hq / Hk, cus = device_cus(), keys = dtype == MGI_F32 ? 16 : 32;
+  const int64_t G = Hq / Hk, rows = B * G, keys = dtype == MGI_F32 ? 16 : 32;
   p.gsets = (int)((G + 15) / 16);
   p.vheads = (int)(Hk * p.gsets);
-  const int64_t tiles = (shared * S + keys - 1) / keys;
-  const int64_t own_bound = B * ((M * S + keys - 1) / keys) * p.vheads;
   const int forced = env_int("MINIVLLM_HIP_SHARED_SPLIT", -1);
-  p.one_launch = B > mgi::kSharedMaxB || own_bound >= (int64_t(1) << 30) || forced == 0;
+  p.lds_tiles = dtype != MGI_F32 && D <= 128 && S % 16 == 0 && rows > env_int("MINIVLLM_HIP_SHARED_LDS", 32);
+  p.row_tiles = rows > (p.lds_tiles ? 64 : 16) && D <= 128 ? 2 : 1;
+  p.set_rows = (p.lds_tiles ? 64 : 16) * p.row_tiles;
+  p.row_sets = (int)((rows + p.set_rows - 1) / p.set_rows);
+  const int64_t step = p.lds_tiles ? 64 : 4 * keys, tiles = (shared * S + step - 1) / step;
+  // Tile numbers are 32-bit, and the rows' prefix sums live in LDS.
+  p.one_launch = forced == 0 || B > mgi::kSharedMaxB || Hk * p.row_sets * tiles >= (int64_t(1) << 30) ||
+                 B * ((M * S + keys - 1) / keys) * p.vheads >= (int64_t(1) << 30);
   if (p.one_launch) return p;
-  const int64_t rows = B * G;
-  p.row_tiles = rows <= 16 ? 1 : rows <= 32 || D > 128 ? 2 : 4;
-  p.row_tiles = std::min(p.row_tiles, env_int("MINIVLLM_HIP_SHARED_TILES", 4));
-  p.row_sets = (int)((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
-  if (tiles) {
-    const int64_t target = std::max<int64_t>(1, env_int("MINIVLLM_HIP_SHARED_WGS", 2) * cus / (Hk * p.row_sets));
-    p.chunk_tiles = (int)std::max<int64_t>((tiles + target - 1) / target, env_int("MINIVLLM_HIP_SHARED_CHUNK", 8));
-    p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
-    p.prefix_wgs = (int)(p.chunks * Hk * p.row_sets);
-  }
-  p.own_waves = (int)(4 * env_int("MINIVLLM_HIP_SHARED_OWN", 2) * cus);
-  p.own_min_tiles = 2;
-  p.own_slot = B * Hq * p.chunks;
-  p.cont_slot = p.own_slot + B * Hq;
-  p.slots = p.cont_slot + (int64_t)p.own_waves * 16;
+  p.s_tiles = (int)tiles;
+  p.s_units = (int)(Hk * p.row_sets);
+  p.s_cost = env_int("MINIVLLM_HIP_SHARED_COST", (int)(step / keys));
+  p.s_min = env_int("MINIVLLM_HIP_SHARED_SMIN", 2);
+  p.own_min = env_int("MINIVLLM_HIP_SHARED_OMIN", 4);
+  p.wgs = (int)round_up(env_int("MINIVLLM_HIP_SHARED_WGS", 2) * device_cus(), 8);
+  p.s_cont = B * Hq;
+  p.own_slot = p.s_cont + (tiles ? (int64_t)p.wgs * p.set_rows : 0);
+  p.own_cont = p.own_slot + B * Hq;
+  p.slots = p.own_cont + (int64_t)p.wgs * 4 * 16;
   p.ml_offset = (size_t)round_up(p.slots * D * 4, kWorkspaceAlign);
   p.cum_offset = (size_t)round_up((int64_t)p.ml_offset + p.slots * 8, kWorkspaceAlign);
   p.total = p.cum_offset + (size_t)(B * 4);
@@ -1258,14 +1258,14 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
             mult16(q_strides[0], eb) && mult16(q_strides[1], eb) && mult16(out_strides[0], eb) &&
             mult16(out_strides[1], eb) && mult16(a.k_sn, eb) && mult16(a.k_ss, eb) && mult16(a.k_sh, eb) &&
             mult16(a.v_sn, eb) && mult16(a.v_ss, eb) && mult16(a.v_sh, eb) &&
-            std::max(a.k_ss, a.v_ss) * eb < (int64_t(1) << 27);
+            std::max(a.k_ss, a.v_ss) * eb < (int64_t(1) << 27) && N < (int64_t(1) << 31);
   if (a.tiles) {
     const SharedPlan p = shared_plan(B, Hq, Hk, D, S, M, shared_blocks, dtype);
     a.one_launch = p.one_launch;
-    a.gsets = p.gsets, a.vheads = p.vheads, a.row_tiles = p.row_tiles, a.row_sets = p.row_sets;
-    a.chunks = p.chunks, a.chunk_tiles = p.chunk_tiles, a.prefix_wgs = p.prefix_wgs;
-    a.own_waves = p.own_waves, a.own_min_tiles = p.own_min_tiles;
-    a.own_slot = p.own_slot, a.cont_slot = p.cont_slot;
+    a.gsets = p.gsets, a.vheads = p.vheads, a.wgs = p.wgs, a.lds_tiles = p.lds_tiles, a.row_tiles = p.row_tiles;
+    a.set_rows = p.set_rows, a.row_sets = p.row_sets, a.s_units = p.s_units, a.s_tiles = p.s_tiles, a.s_cost = p.s_cost;
+    a.s_min = p.s_min, a.own_min = p.own_min;
+    a.s_cont = p.s_cont, a.own_slot = p.own_slot, a.own_cont = p.own_cont;
     if (!p.one_launch) {
       if (!workspace) return fail(MGI_EWORKSPACE, "workspace required for the split pass");
       if (workspace_bytes < p.total)

@@ -138,14 +138,17 @@ struct SharedArgs {
   int tiles;               // the matrix-core kernels (else the one for any strides)
   int one_launch;          // one workgroup per (row, virtual head)
   int gsets, vheads;       // sets of 16 query heads per KV head; KV heads times sets
-  int row_tiles, row_sets; // shared piece: 16-row query tiles per wavefront, and sets of those
-  int chunks, chunk_tiles; // shared piece: ranges of tokens, key tiles in each
-  int prefix_wgs;          // row_sets * chunks * KV heads
-  int own_waves;           // wavefronts for the rows' own tokens
-  int own_min_tiles;       // least tiles of one of their segments
-  // Partials: [B, Hq, chunks] of the shared piece, [B, Hq] of the first own
-  // pieces, 16 for each own wavefront's continued one.
-  int64_t own_slot, cont_slot;
+  int wgs;                 // workgroups of the split launch (a multiple of 8)
+  int lds_tiles;           // shared tiles go through LDS
+  int row_tiles;           // 16-row query tiles per wavefront of the shared part
+  int set_rows, row_sets;  // query rows per workgroup of it, and such sets per KV head
+  int s_units, s_tiles;    // its list: KV heads x sets, key tiles of each
+  int s_cost;              // cost of one of its tiles, an own tile being 1
+  int s_min, own_min;      // least tiles of a segment
+  // Partials: [B, Hq] of the pieces that begin a row's shared run and, from own_slot,
+  // of those that begin its own; set_rows per workgroup (s_cont) and 16 per
+  // wavefront (own_cont) for continued ones.
+  int64_t s_cont, own_slot, own_cont;
   float* ws_acc;           // [slots, D]
   float2* ws_ml;           // [slots] (maximum in log2 units, sum)
   int* ws_cum;             // [B] prefix sums of the rows' own tiles

@@ -35,6 +35,7 @@
 
 #include <type_traits>
 
+#include "lds_tiles.h"
 #include "mgi_common.h"
 #include "mgi_internal.h"
 #include "minivllm_hip.h"
@@ -94,7 +95,8 @@ struct Tile {
   uint4 k[kGroups][kKS];
   VVec v[kRows][kHF];
   bool full;       // every key counts
-  uint32_t mask;   // bit j: value row j's key counts
+  int n[kGroups];  // S a multiple of 16: keys of each group that count
+  uint32_t mask;   // other S: bit j, the lane's value row j counts
 };
 
 // Running softmax of NQ x 16 query rows; lane l holds row l & 15 of each.
@@ -127,106 +129,124 @@ __device__ __forceinline__ int64_t table_entry(const SharedArgs& a, int b, int j
   return load_index(a.bt, a.bt_i64, (int64_t)(j < a.shared ? 0 : b) * a.bt_sb + (int64_t)j * a.bt_sm);
 }
 
-// The pool block ids of a tile's groups, one per 16 keys (S a multiple of 16).
-template <int GROUPS>
-struct Ids {
-  int64_t id[GROUPS];
+// Where the 16-key groups of a wavefront's next tiles lie (S a multiple of 16, so
+// each lies in one block): lane i holds group i % GR of tile i / GR, as byte offsets
+// into the pool, and how many of its keys count. One table load serves 64 / GR tiles,
+// and the next window's is issued a window ahead: read where it is used, an entry
+// costs a wait for every load in flight (the document case, 128 x 32 heads over
+// 65 536 tokens: 351 us so, see the table in the documentation for now).
+struct Window {
+  uint32_t k_lo, k_hi, v_lo, v_hi;
+  int n;
 };
-template <int GROUPS>
-__device__ __forceinline__ Ids<GROUPS> load_ids(const SharedArgs& a, int b, int t0, int end) {
-  Ids<GROUPS> r;
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    const int tok = t0 + 16 * g;
-    r.id[g] = tok < end ? table_entry(a, b, fast_div(tok, a.s_mul, a.s_shift, a.S)) : -1;
-  }
-  return r;
+
+// The lane's table entry (-1: none, or outside the pool) for its group, whose first
+// token is tok.
+__device__ __forceinline__ int window_entry(const SharedArgs& a, int b, int tok, int end) {
+  if (tok >= end) return -1;
+  const int64_t id = table_entry(a, b, fast_div(tok, a.s_mul, a.s_shift, a.S));
+  return id >= 0 && id < a.N ? (int)id : -1;
+}
+template <typename T>
+__device__ __forceinline__ Window make_window(const SharedArgs& a, int id, int tok, int end) {
+  const int64_t at = max(id, 0), off = id < 0 ? 0 : tok - fast_div(tok, a.s_mul, a.s_shift, a.S) * a.S;
+  const uint64_t k = (uint64_t)(at * a.k_sn + off * a.k_ss) * sizeof(T), v = (uint64_t)(at * a.v_sn + off * a.v_ss) * sizeof(T);
+  return {(uint32_t)k, (uint32_t)(k >> 32), (uint32_t)v, (uint32_t)(v >> 32), id < 0 ? 0 : min(16, end - tok)};
+}
+__device__ __forceinline__ int64_t lane_offset(uint32_t lo, uint32_t hi, int i) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)lo, i) |
+                   ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, i) << 32));
 }
 
-// Loads the tile of keys t0 .. of one KV head. UNI: S is a multiple of 16, so a
-// 16-key group lies in one block and its addresses are a scalar base and a lane
-// offset; otherwise every lane looks its keys up. FULL: D == DP.
-template <typename T, int DP, bool UNI, bool FULL>
-__device__ __forceinline__ void load_tile(const SharedArgs& a, int b, int kvh, int t0, int end,
-                                          const Ids<Tile<T, DP>::kGroups>& ids, Tile<T, DP>& f) {
+// Loads the keys, and the values, of the tile whose groups are lanes at .. of the
+// window, of the KV head at kp, vp. Rows past a group's last key read that one again.
+// FULL: D == DP.
+template <typename T, int DP, bool FULL>
+__device__ __forceinline__ void load_keys(const SharedArgs& a, const char* kp, const Window& w, int at, Tile<T, DP>& f) {
   using L = Tile<T, DP>;
   const int lane = (int)threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
-  const char* kp = (const char*)a.k + (int64_t)kvh * a.k_sh * (int)sizeof(T);
-  const char* vp = (const char*)a.v + (int64_t)kvh * a.v_sh * (int)sizeof(T);
-  const uint32_t k_ss = (uint32_t)a.k_ss * sizeof(T), v_ss = (uint32_t)a.v_ss * sizeof(T);
-  const uint32_t vcol = (uint32_t)(row * L::kEV) * sizeof(T);
+  const uint32_t ss = (uint32_t)a.k_ss * sizeof(T);
+#pragma unroll
+  for (int g = 0; g < L::kGroups; ++g) {
+    const int n = __builtin_amdgcn_readlane(w.n, at + g);
+    const char* base = kp + lane_offset(w.k_lo, w.k_hi, at + g);
+    const uint32_t off = (uint32_t)min(row, max(n, 1) - 1) * ss + (uint32_t)kg * 16;
+#pragma unroll
+    for (int s = 0; s < L::kKS; ++s)
+      f.k[g][s] = FULL || (kg + 4 * s) * L::kCE < a.D ? *(const uint4*)(base + off + 64 * s) : make_uint4(0, 0, 0, 0);
+  }
+}
+template <typename T, int DP, bool FULL>
+__device__ __forceinline__ void load_values(const SharedArgs& a, const char* vp, const Window& w, int at, Tile<T, DP>& f) {
+  using L = Tile<T, DP>;
   using V = typename L::VVec;
-  auto chunk_ok = [&](int s) { return FULL || (kg + 4 * s) * L::kCE < a.D; };
-  auto col_ok = [&](int h) { return FULL || 16 * L::kEV * h + row * L::kEV < a.D; };
-  if constexpr (UNI) {
-    bool full = t0 + L::kKeys <= end;
-    uint32_t mask = 0;
+  const int lane = (int)threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
+  const uint32_t ss = (uint32_t)a.v_ss * sizeof(T), col = (uint32_t)(row * L::kEV) * sizeof(T);
+  f.full = true;
 #pragma unroll
-    for (int g = 0; g < L::kGroups; ++g) {
-      const int tok = t0 + 16 * g;
-      int64_t id = ids.id[g];
-      const bool ok = id >= 0 && id < a.N;
-      full &= ok;
-      id = ok ? id : 0;
-      // Rows past the end read the last valid one again; its values are cleared.
-      const int n = ok ? min(16, max(0, end - tok)) : 0;
-      const int blk = fast_div(tok, a.s_mul, a.s_shift, a.S), off = ok ? tok - blk * a.S : 0;
-      const char* kb = kp + (id * a.k_sn + (int64_t)off * a.k_ss) * (int)sizeof(T);
-      const char* vb = vp + (id * a.v_sn + (int64_t)off * a.v_ss) * (int)sizeof(T);
-      const int last = max(n, 1) - 1;
-      const uint32_t kr = (uint32_t)min(row, last) * k_ss + (uint32_t)kg * 16;
+  for (int g = 0; g < L::kGroups; ++g) {
+    const int n = __builtin_amdgcn_readlane(w.n, at + g);
+    const char* base = vp + lane_offset(w.v_lo, w.v_hi, at + g);
+    f.n[g] = n;
+    f.full &= n == 16;
 #pragma unroll
-      for (int s = 0; s < L::kKS; ++s)
-        f.k[g][s] = chunk_ok(s) ? *(const uint4*)(kb + (kr + 64 * s)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = 4 * kg + j;
-        mask |= (key < n ? 1u : 0u) << (4 * g + j);
-        const uint32_t vr = (uint32_t)min(key, last) * v_ss + vcol;
-#pragma unroll
-        for (int h = 0; h < L::kHF; ++h)
-          f.v[4 * g + j][h] = col_ok(h) ? *(const V*)(vb + (vr + 16 * L::kEV * (int)sizeof(T) * h)) : V{};
-      }
-    }
-    f.full = full;
-    f.mask = mask;
-  } else {
-    auto find = [&](int key, bool* ok) {
-      const int k = min(key, end - 1), blk = fast_div(k, a.s_mul, a.s_shift, a.S);
-      const int64_t id = table_entry(a, b, blk);
-      *ok = key < end && id >= 0 && id < a.N;
-      return *ok ? make_longlong2(id, k - blk * a.S) : make_longlong2(0, 0);
-    };
-#pragma unroll
-    for (int g = 0; g < L::kGroups; ++g) {
-      bool ok;
-      const longlong2 at = find(t0 + 16 * g + row, &ok);
-      const char* p = kp + (at.x * a.k_sn + at.y * a.k_ss) * (int)sizeof(T) + kg * 16;
-#pragma unroll
-      for (int s = 0; s < L::kKS; ++s) f.k[g][s] = chunk_ok(s) ? *(const uint4*)(p + 64 * s) : make_uint4(0, 0, 0, 0);
-    }
-    uint32_t mask = 0;
-#pragma unroll
-    for (int j = 0; j < L::kRows; ++j) {
-      bool ok;
-      const longlong2 at = find(t0 + 16 * (j / 4) + 4 * kg + j % 4, &ok);
-      mask |= (ok ? 1u : 0u) << j;
-      const char* p = vp + (at.x * a.v_sn + at.y * a.v_ss) * (int)sizeof(T) + vcol;
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t off = (uint32_t)min(4 * kg + j, max(n, 1) - 1) * ss + col;
 #pragma unroll
       for (int h = 0; h < L::kHF; ++h)
-        f.v[j][h] = col_ok(h) ? *(const V*)(p + 16 * L::kEV * (int)sizeof(T) * h) : V{};
+        f.v[4 * g + j][h] = FULL || 16 * L::kEV * h + row * L::kEV < a.D ? *(const V*)(base + off + 16 * L::kEV * (int)sizeof(T) * h) : V{};
     }
-    f.mask = mask;
-    f.full = __all(mask == (1u << L::kRows) - 1);
   }
 }
 
-// One tile's scores, weights and products for NQ x 16 query rows.
-template <typename T, int DP, int NQ>
-__device__ __forceinline__ void attend_tile(const SharedArgs& a, Tile<T, DP>& f, const uint4 (&qf)[NQ][Tile<T, DP>::kKS],
-                                            State<DP, NQ>& st) {
+// The same for any S: every lane looks its keys up. Keys t0 .. below end.
+struct Found {
+  int64_t block;
+  int off;
+  bool ok;
+};
+__device__ __forceinline__ Found find_key(const SharedArgs& a, int b, int key, int end) {
+  const int k = min(key, end - 1), blk = fast_div(k, a.s_mul, a.s_shift, a.S);
+  const int64_t id = table_entry(a, b, blk);
+  const bool ok = key < end && id >= 0 && id < a.N;
+  return {ok ? id : 0, ok ? k - blk * a.S : 0, ok};
+}
+template <typename T, int DP>
+__device__ __forceinline__ void load_keys_any(const SharedArgs& a, const char* kp, int b, int t0, int end, Tile<T, DP>& f) {
   using L = Tile<T, DP>;
-  f32x4 s[NQ][L::kGroups];
+  const int lane = (int)threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
+#pragma unroll
+  for (int g = 0; g < L::kGroups; ++g) {
+    const Found at = find_key(a, b, t0 + 16 * g + row, end);
+    const char* p = kp + (at.block * a.k_sn + at.off * a.k_ss) * (int)sizeof(T) + kg * 16;
+#pragma unroll
+    for (int s = 0; s < L::kKS; ++s)
+      f.k[g][s] = (kg + 4 * s) * L::kCE < a.D ? *(const uint4*)(p + 64 * s) : make_uint4(0, 0, 0, 0);
+  }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void load_values_any(const SharedArgs& a, const char* vp, int b, int t0, int end, Tile<T, DP>& f) {
+  using L = Tile<T, DP>;
+  using V = typename L::VVec;
+  const int lane = (int)threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
+  f.mask = 0;
+#pragma unroll
+  for (int j = 0; j < L::kRows; ++j) {
+    const Found at = find_key(a, b, t0 + 16 * (j / 4) + 4 * kg + j % 4, end);
+    f.mask |= (at.ok ? 1u : 0u) << j;
+    const char* p = vp + (at.block * a.v_sn + at.off * a.v_ss) * (int)sizeof(T) + row * L::kEV * (int)sizeof(T);
+#pragma unroll
+    for (int h = 0; h < L::kHF; ++h)
+      f.v[j][h] = 16 * L::kEV * h + row * L::kEV < a.D ? *(const V*)(p + 16 * L::kEV * (int)sizeof(T) * h) : V{};
+  }
+  f.full = __all(f.mask == (1u << L::kRows) - 1);
+}
+
+// Scores of a tile for NQ x 16 query rows.
+template <typename T, int DP, int NQ>
+__device__ __forceinline__ void score_tile(const Tile<T, DP>& f, const uint4 (&qf)[NQ][Tile<T, DP>::kKS],
+                                           f32x4 (&s)[NQ][Tile<T, DP>::kGroups]) {
+  using L = Tile<T, DP>;
 #pragma unroll
   for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -245,17 +265,27 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, Tile<T, DP>& f,
             s[q][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(fword(f.k[g][c], e), fword(qf[q][c], e), s[q][g], 0, 0, 0);
         }
       }
+}
+
+// Their weights, and the products with the values.
+template <typename T, int DP, int NQ, bool UNI>
+__device__ __forceinline__ void attend_tile(const SharedArgs& a, Tile<T, DP>& f, f32x4 (&s)[NQ][Tile<T, DP>::kGroups],
+                                            State<DP, NQ>& st) {
+  using L = Tile<T, DP>;
   if (!f.full) {
+    const int kg = ((int)threadIdx.x & 63) >> 4;
+    bool some = false;
 #pragma unroll
     for (int j = 0; j < L::kRows; ++j) {
-      const bool ok = (f.mask >> j) & 1;
+      const bool ok = UNI ? 4 * kg + j % 4 < f.n[j / 4] : (f.mask >> j) & 1;
+      some |= ok;
 #pragma unroll
       for (int q = 0; q < NQ; ++q) s[q][j / 4][j % 4] = ok ? s[q][j / 4][j % 4] : kNegInf;
       // A weight of 0 times an infinity or NaN in an unused slot is no 0.
 #pragma unroll
       for (int h = 0; h < L::kHF; ++h) f.v[j][h] = ok ? f.v[j][h] : typename L::VVec{};
     }
-    st.any |= __any(f.mask != 0);
+    st.any |= __any(some);
   } else {
     st.any = true;
   }
@@ -330,49 +360,65 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, Tile<T, DP>& f,
   }
 }
 
-// Attends the tiles first, first + step, ... below end, the next one loading
-// while one is computed.
+// Attends the tiles first, first + step, ... below end of row b's table. A tile's
+// keys are loaded into the registers the one before has given its scores from, and
+// its values where that one's products have been taken: half a tile is always on
+// its way, without a second set of registers (with one, two wavefronts fit a SIMD
+// and spilled; so, three do).
 template <typename T, int DP, int NQ, bool UNI, bool FULL>
 __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh, int first, int step, int end,
                                              const uint4 (&qf)[NQ][Tile<T, DP>::kKS], State<DP, NQ>& st) {
   using L = Tile<T, DP>;
   if (first >= end) return;
-  L f0, f1;
-  Ids<L::kGroups> ids{};
-  if constexpr (UNI) ids = load_ids<L::kGroups>(a, b, first, end);
-  load_tile<T, DP, UNI, FULL>(a, b, kvh, first, end, ids, f0);
-  int t = first + step;
-  if constexpr (UNI) ids = load_ids<L::kGroups>(a, b, t, end);
-  while (true) {
-    Ids<L::kGroups> next{};
-    if (t < end) {
-      if constexpr (UNI) next = load_ids<L::kGroups>(a, b, t + step, end);
-      load_tile<T, DP, UNI, FULL>(a, b, kvh, t, end, ids, f1);
+  const char* kp = (const char*)a.k + (int64_t)kvh * a.k_sh * (int)sizeof(T);
+  const char* vp = (const char*)a.v + (int64_t)kvh * a.v_sh * (int)sizeof(T);
+  constexpr int kSpan = 64 / L::kGroups;  // tiles of a window
+  const int lane = (int)threadIdx.x & 63;
+  int tok = 0, entry = -1;                // the lane's group of the next window
+  Window win{};
+  if constexpr (UNI) {
+    tok = first + lane / L::kGroups * step + 16 * (lane % L::kGroups);
+    entry = window_entry(a, b, tok, end);
+  }
+  L f;
+  auto keys = [&](int i) {
+    if constexpr (UNI) {
+      if (i % kSpan == 0) {
+        win = make_window<T>(a, entry, tok, end);
+        tok += kSpan * step;
+        entry = window_entry(a, b, tok, end);
+      }
+      load_keys<T, DP, FULL>(a, kp, win, i % kSpan * L::kGroups, f);
+    } else {
+      load_keys_any<T, DP>(a, kp, b, first + i * step, end, f);
     }
-    attend_tile<T, DP, NQ>(a, f0, qf, st);
-    if (t >= end) break;
-    t += step;
-    if (t < end) {
-      if constexpr (UNI) ids = load_ids<L::kGroups>(a, b, t + step, end);
-      load_tile<T, DP, UNI, FULL>(a, b, kvh, t, end, next, f0);
-    }
-    attend_tile<T, DP, NQ>(a, f1, qf, st);
-    if (t >= end) break;
-    t += step;
+  };
+  auto values = [&](int i) {
+    if constexpr (UNI) load_values<T, DP, FULL>(a, vp, win, i % kSpan * L::kGroups, f);
+    else load_values_any<T, DP>(a, vp, b, first + i * step, end, f);
+  };
+  const int n = (end - first + step - 1) / step;
+  keys(0);
+  values(0);
+  for (int i = 0; i < n; ++i) {
+    f32x4 s[NQ][L::kGroups];
+    score_tile<T, DP, NQ>(f, qf, s);
+    if (i + 1 < n) keys(i + 1);
+    attend_tile<T, DP, NQ, UNI>(a, f, s, st);
+    if (i + 1 < n) values(i + 1);
   }
 }
 
 // Query fragments of NQ x 16 rows of one KV head's query heads: row r is sequence
 // r / G's head r % G, from row r0 on; rows past `rows` are zero.
 template <typename T, int DP, int NQ, bool FULL>
-__device__ __forceinline__ void load_queries(const SharedArgs& a, int kvh, int64_t r0, int64_t rows,
+__device__ __forceinline__ void load_queries(const SharedArgs& a, int kvh, int r0, int rows,
                                              uint4 (&qf)[NQ][Tile<T, DP>::kKS]) {
   using L = Tile<T, DP>;
   const int lane = (int)threadIdx.x & 63, kg = lane >> 4;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    const int64_t r = r0 + 16 * q + (lane & 15);
-    const int bb = fast_div((int)r, a.g_mul, a.g_shift, a.G), g = (int)r - bb * a.G;
+    const int r = r0 + 16 * q + (lane & 15), bb = fast_div(r, a.g_mul, a.g_shift, a.G), g = r - bb * a.G;
     const T* p = (const T*)a.q + (int64_t)bb * a.q_sb + (int64_t)(kvh * a.G + g) * a.q_sh + kg * L::kCE;
 #pragma unroll
     for (int s = 0; s < L::kKS; ++s) {
@@ -479,122 +525,61 @@ __device__ __forceinline__ int clamped_ctx(const SharedArgs& a, int b) {
 struct Own {
   int first, end;
 };
+constexpr int kSplitWaves = 4;
 __device__ __forceinline__ Own own_range(const SharedArgs& a, int b) {
   const int c = clamped_ctx(a, b);
   return {c < a.P ? 0 : a.P, c};
 }
 
-// The list of all rows' own tiles, (b, virtual head, tile) in that order, cut into
-// equal segments, one per wavefront. A virtual head is a KV head and a set of at
-// most 16 of its query heads.
-__device__ __forceinline__ int segment_tiles(const SharedArgs& a, int total) {
-  return max(a.own_min_tiles, (int)(((int64_t)total + a.own_waves - 1) / a.own_waves));
+// The work is two lists: the shared tokens' tiles, (KV head, set of query rows, tile)
+// in that order, and the rows' own, (row, virtual head, tile), a virtual head
+// being a KV head and a set of at most 16 of its query heads. The launch's
+// workgroups are dealt out between the lists by cost, and each list is cut into
+// equal segments: one per workgroup of the first list, one per wavefront of the
+// second. A segment's first piece may continue a run that another began: it leaves
+// its partial in the segment's slots, a piece that begins a run in the rows' own.
+struct Split {
+  int shared_wgs;  // workgroups of the first list
+  int seg_shared;  // tiles of their segments
+  int seg_own;
+};
+__device__ __forceinline__ Split make_split(const SharedArgs& a, int own_total) {
+  const int total = a.s_units * a.s_tiles;
+  const int64_t cs = (int64_t)total * a.s_cost, co = own_total;
+  Split r{};
+  r.shared_wgs = total == 0 ? 0 : own_total == 0 ? a.wgs : (int)min((int64_t)a.wgs - 1, max((int64_t)1, (a.wgs * cs + (cs + co) / 2) / (cs + co)));
+  if (r.shared_wgs) r.seg_shared = max(a.s_min, (total + r.shared_wgs - 1) / r.shared_wgs);
+  const int waves = (a.wgs - r.shared_wgs) * kSplitWaves;
+  if (waves) r.seg_own = max(a.own_min, (own_total + waves - 1) / waves);
+  return r;
 }
 
-template <typename T, int DP, bool UNI, bool FULL>
-__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int* cum) {
-  using L = Tile<T, DP>;
-  const int lane = (int)threadIdx.x & 63;
-  // cum[b]: tiles of rows 0 .. b, of one virtual head.
-  const int total = uniform(cum[a.B - 1]) * a.vheads, seg = segment_tiles(a, total);
-  const int64_t lo64 = (int64_t)wave_index * seg;
-  if (lo64 >= total) return;
-  int u = (int)lo64;
-  const int stop = (int)min((int64_t)total, lo64 + seg);
-  int b = 0;
-  {  // the row of tile u: the first with cum[b] * vheads > u
-    int lo = 0, hi = a.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (cum[mid] * a.vheads > u) hi = mid;
-      else lo = mid + 1;
-    }
-    b = lo;
-  }
-  uint4 qf[1][L::kKS];
-  State<DP, 1> st;
-  while (u < stop) {
-    b = uniform(b);
-    const int before = b ? uniform(cum[b - 1]) : 0, tiles = uniform(cum[b]) - before;
-    if (tiles == 0) {
-      ++b;
-      continue;
-    }
-    const int rem = u - before * a.vheads;
-    const int vh = rem / tiles, tile = rem - vh * tiles;
-    const int n = min(tiles - tile, stop - u);
-    const int kvh = vh / a.gsets, g0 = (vh - kvh * a.gsets) * 16;
-    const Own own = own_range(a, b);
-    load_queries<T, DP, 1, FULL>(a, kvh, (int64_t)b * a.G + g0, (int64_t)(b + 1) * a.G, qf);
-    st.reset();
-    const int first = own.first + tile * L::kKeys;
-    stream_tiles<T, DP, 1, UNI, FULL>(a, b, kvh, first, L::kKeys, min(own.end, first + n * L::kKeys), qf, st);
-    const int g = g0 + (lane & 15);
-    const float l = coded_sum(across_groups_sum(st.l[0]), st.any);
-    // A piece that begins its row's tiles has the row's slot, another the segment's.
-    const int64_t slot = tile == 0 ? a.own_slot + (int64_t)b * a.Hq + kvh * a.G + g
-                                   : a.cont_slot + (int64_t)wave_index * 16 + (lane & 15);
-    if (g < a.G) store_partial<T>(a, st, 0, slot, st.m[0] == kNegInf ? kNegInf : st.mc[0], l);
-    u += n;
-    if (vh == a.vheads - 1 && tile + n == tiles) ++b;
-  }
+// Workgroup blockIdx.x's place: XCD blockIdx.x % 8 takes a contiguous run of each
+// list (sets of rows that read the same keys then share its L2), and starts with
+// its part of the first.
+struct Place {
+  bool shared;
+  int index;  // in its list's workgroups
+};
+__device__ __forceinline__ Place make_place(const SharedArgs& a, const Split& sp) {
+  const int x = (int)blockIdx.x & 7, j = (int)blockIdx.x >> 3;
+  const int mine = sp.shared_wgs / 8 + (x < sp.shared_wgs % 8), before = x * (sp.shared_wgs / 8) + min(x, sp.shared_wgs % 8);
+  if (j < mine) return {true, before + j};
+  return {false, x * (a.wgs / 8) - before + j - mine};
 }
 
-constexpr int kSplitWaves = 4;
-
-// The pieces: workgroups 0 .. prefix_wgs - 1 take the shared tokens, (KV head,
-// query rows, range of tokens) each; the wavefronts of the others the rows' own.
-template <typename T, int DP, int NQ, bool UNI, bool FULL>
-__global__ void __launch_bounds__(64 * kSplitWaves) paged_shared_split(const SharedArgs a) {
-  using L = Tile<T, DP>;
-  __shared__ __align__(16) char lds[kSplitWaves / 2 * (DP / 16) * 64 * 16 > kSharedMaxB * 4
-                                        ? kSplitWaves / 2 * (DP / 16) * 64 * 16 : kSharedMaxB * 4];
-  __shared__ float ml[kSplitWaves][2][NQ * 16];
-  __shared__ int part[kSplitWaves];
+// Prefix sums of the rows' own tiles into cum[0 .. B); returns the total.
+template <int KEYS>
+__device__ __forceinline__ int scan_own(const SharedArgs& a, int* cum, int* part) {
   const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-  if ((int)blockIdx.x < a.prefix_wgs) {
-    const int i = (int)blockIdx.x, rest = i / a.row_sets, set = i - rest * a.row_sets;
-    const int kvh = rest / a.chunks, chunk = rest - kvh * a.chunks;
-    const int64_t rows = (int64_t)a.B * a.G, r0 = (int64_t)set * 16 * NQ;
-    int slot_b[NQ], slot_g[NQ];
-    bool takes[NQ], some = false;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int r = (int)r0 + 16 * q + (lane & 15);
-      slot_b[q] = fast_div(r, a.g_mul, a.g_shift, a.G);
-      slot_g[q] = r - slot_b[q] * a.G;
-      takes[q] = r < rows && clamped_ctx(a, slot_b[q]) >= a.P;
-      some |= takes[q];
-    }
-    if (!__any(some)) return;  // the same in every wavefront of the workgroup
-    uint4 qf[NQ][L::kKS];
-    State<DP, NQ> st;
-    load_queries<T, DP, NQ, FULL>(a, kvh, r0, rows, qf);
-    st.reset();
-    const int first = chunk * a.chunk_tiles * L::kKeys, end = min(a.P, first + a.chunk_tiles * L::kKeys);
-    stream_tiles<T, DP, NQ, UNI, FULL>(a, 0, kvh, first + wave * L::kKeys, kSplitWaves * L::kKeys, end, qf, st);
-    join_waves<DP, NQ, kSplitWaves>(st, wave, ml, (f32x4*)lds);
-    if (wave == 0) {
-#pragma unroll
-      for (int q = 0; q < NQ; ++q)
-        if (takes[q])
-          store_partial<T>(a, st, q, ((int64_t)slot_b[q] * a.Hq + kvh * a.G + slot_g[q]) * a.chunks + chunk, st.mc[q], st.l[q]);
-    }
-    return;
-  }
-  // Prefix sums of the rows' own tiles, in LDS; the first of these workgroups
-  // leaves them for the joining launch.
-  int* cum = (int*)lds;
   const int per = (a.B + 64 * kSplitWaves - 1) / (64 * kSplitWaves), b0 = (int)threadIdx.x * per;
   int sum = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = b0 + i;
-    if (b < a.B) {
-      const Own own = own_range(a, b);
-      sum += (own.end - own.first + L::kKeys - 1) / L::kKeys;
-      cum[b] = sum;
+  for (int i = 0; i < per; ++i)
+    if (b0 + i < a.B) {
+      const Own own = own_range(a, b0 + i);
+      sum += (own.end - own.first + KEYS - 1) / KEYS;
+      cum[b0 + i] = sum;
     }
-  }
   int incl = sum;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -603,62 +588,423 @@ __global__ void __launch_bounds__(64 * kSplitWaves) paged_shared_split(const Sha
   }
   if (lane == 63) part[wave] = incl;
   __syncthreads();
-  int base = incl - sum;
-  for (int w = 0; w < wave; ++w) base += part[w];
+  int base = incl - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < kSplitWaves; ++w) {
+    if (w < wave) base += part[w];
+    total += part[w];
+  }
   for (int i = 0; i < per; ++i)
     if (b0 + i < a.B) {
       const int v = cum[b0 + i] + base;
       cum[b0 + i] = v;
-      if ((int)blockIdx.x == a.prefix_wgs) a.ws_cum[b0 + i] = v;
+      if (blockIdx.x == 0) a.ws_cum[b0 + i] = v;  // for the joining launch
     }
   __syncthreads();
-  const int wave_index = ((int)blockIdx.x - a.prefix_wgs) * kSplitWaves + wave;
-  attend_own<T, DP, UNI, FULL>(a, wave_index, cum);
+  return uniform(total);
 }
 
-// Joins the partials of one (row, query head) per wavefront.
-template <typename T>
-__global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
+template <typename T, int DP, bool UNI, bool FULL>
+__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum) {
+  using L = Tile<T, DP>;
   const int lane = (int)threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + uniform((int)threadIdx.x >> 6);
-  if (unit >= (int64_t)a.B * a.Hq) return;
-  const int b = (int)(unit / a.Hq), hq = (int)(unit - (int64_t)b * a.Hq);
-  const int kvh = hq / a.G, g = hq - kvh * a.G, set = g / 16;
-  const int before = b ? a.ws_cum[b - 1] : 0, tiles = a.ws_cum[b] - before;
-  const int seg = segment_tiles(a, a.ws_cum[a.B - 1] * a.vheads);
-  const int u = before * a.vheads + (kvh * a.gsets + set) * tiles;
-  const int w0 = u / seg, pieces = tiles ? (u + tiles - 1) / seg - w0 + 1 : 0;
-  const int shared = clamped_ctx(a, b) >= a.P ? a.chunks : 0, n = shared + pieces;
-  auto slot = [&](int i) -> int64_t {
-    if (i < shared) return unit * a.chunks + i;
-    if (i == shared) return a.own_slot + unit;
-    return a.cont_slot + (int64_t)(w0 + i - shared) * 16 + (g - set * 16);
-  };
-  float top = kNegInf;
-  for (int i = lane; i < n; i += 64) {
-    const float2 x = a.ws_ml[slot(i)];
-    if (!(x.y <= 0.f)) top = fmaxf(top, x.x);
+  if ((int64_t)wave_index * seg >= total) return;
+  int u = wave_index * seg, b = 0;
+  const int stop = min(total, u + seg);
+  for (int hi = a.B - 1; b < hi;) {  // the row of tile u: the first with cum[b] * vheads > u
+    const int mid = (b + hi) >> 1;
+    if (uniform(cum[mid]) * a.vheads > u) hi = mid;
+    else b = mid + 1;
   }
-  top = wave_max(top);
-  float sum = 0.f;
-  bool dead = false;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < n; ++i) {
-    const int64_t s = slot(i);
-    const float2 x = a.ws_ml[s];
-    if (x.y <= 0.f) {
-      dead |= x.y < 0.f;
+  uint4 qf[1][L::kKS];
+  State<DP, 1> st;
+  while (u < stop) {
+    const int before = b ? uniform(cum[b - 1]) : 0, tiles = uniform(cum[b]) - before;
+    if (tiles == 0) {
+      ++b;
       continue;
     }
-    const float w = fast_exp2(x.x - top);
-    sum += x.y * w;
-    if (4 * lane < a.D) acc += w * *(const f32x4*)(a.ws_acc + s * a.D + 4 * lane);
+    const int rem = u - before * a.vheads;
+    const int vh = rem / tiles, tile = rem - vh * tiles, n = min(tiles - tile, stop - u);
+    const int kvh = vh / a.gsets, g0 = (vh - kvh * a.gsets) * 16, g = g0 + (lane & 15);
+    const Own own = own_range(a, b);
+    load_queries<T, DP, 1, FULL>(a, kvh, b * a.G + g0, (b + 1) * a.G, qf);
+    st.reset();
+    const int first = uniform(own.first) + tile * L::kKeys;
+    stream_tiles<T, DP, 1, UNI, FULL>(a, b, kvh, first, L::kKeys, min(uniform(own.end), first + n * L::kKeys), qf, st);
+    const float l = coded_sum(across_groups_sum(st.l[0]), st.any);
+    const int64_t slot = tile == 0 ? a.own_slot + (int64_t)b * a.Hq + kvh * a.G + g
+                                   : a.own_cont + (int64_t)wave_index * 16 + (lane & 15);
+    if (g < a.G) store_partial<T>(a, st, 0, slot, st.m[0] == kNegInf ? kNegInf : st.mc[0], l);
+    u += n;
+    if (vh == a.vheads - 1 && tile + n == tiles) ++b;
   }
-  const float r = sum == 0.f ? (dead ? __builtin_nanf("") : 0.f) : 1.f / sum;
-  if (4 * lane < a.D) {
-    T* o = (T*)a.out + (int64_t)b * a.o_sb + (int64_t)hq * a.o_sh + 4 * lane;
+}
+
+// The slot of the lane's query row r (of a shared piece that begins its run or
+// continues it), or -1 where the row takes no part.
+__device__ __forceinline__ int64_t shared_slot(const SharedArgs& a, int kvh, int r, int r0, bool begins, int wg) {
+  if (r >= a.B * a.G) return -1;
+  const int b = fast_div(r, a.g_mul, a.g_shift, a.G), g = r - b * a.G;
+  if (clamped_ctx(a, b) < a.P) return -1;
+  return begins ? (int64_t)b * a.Hq + kvh * a.G + g : a.s_cont + (int64_t)wg * a.set_rows + (r - r0);
+}
+
+// Shared pieces from registers, for up to 32 query rows a set and for what the tiles
+// in LDS do not take: the workgroup's wavefronts take every fourth tile of a piece
+// (a tile of the list is four of theirs) and join in LDS.
+template <typename T, int DP, int NQ, bool UNI, bool FULL>
+__device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int seg, f32x4* buf, float (*ml)[2][NQ * 16]) {
+  using L = Tile<T, DP>;
+  const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const int total = a.s_units * a.s_tiles, step = kSplitWaves * L::kKeys;
+  if ((int64_t)wg * seg >= total) return;
+  const int stop = min(total, wg * seg + seg);
+  uint4 qf[NQ][L::kKS];
+  State<DP, NQ> st;
+  for (int u = wg * seg, n; u < stop; u += n) {
+    const int unit = u / a.s_tiles, tile = u - unit * a.s_tiles, kvh = unit / a.row_sets, r0 = (unit - kvh * a.row_sets) * 16 * NQ;
+    n = min(a.s_tiles - tile, stop - u);
+    load_queries<T, DP, NQ, FULL>(a, kvh, r0, a.B * a.G, qf);
+    st.reset();
+    stream_tiles<T, DP, NQ, UNI, FULL>(a, 0, kvh, tile * step + wave * L::kKeys, step, min(a.P, (tile + n) * step), qf, st);
+    join_waves<DP, NQ, kSplitWaves>(st, wave, ml, buf);
+    if (wave == 0) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) Elem<T>::store(o + e, acc[e] * r);
+      for (int q = 0; q < NQ; ++q) {
+        const int64_t slot = shared_slot(a, kvh, r0 + 16 * q + (lane & 15), r0, tile == 0, wg);
+        if (slot >= 0) store_partial<T>(a, st, q, slot, st.mc[q], st.l[q]);
+      }
+    }
+  }
+}
+
+template <typename T, int DP, int NQ, bool UNI, bool FULL>
+__global__ void __launch_bounds__(64 * kSplitWaves, DP > 128 ? 1 : 2) paged_shared_split(const SharedArgs a) {
+  constexpr int kBuf = kSplitWaves / 2 * (DP / 16) * 64 * 16, kCum = kSharedMaxB * 4;
+  __shared__ __align__(16) char lds[kBuf > kCum ? kBuf : kCum];
+  __shared__ float ml[kSplitWaves][2][NQ * 16];
+  __shared__ int part[kSplitWaves];
+  const int total = scan_own<Tile<T, DP>::kKeys>(a, (int*)lds, part) * a.vheads;
+  const Split sp = make_split(a, total);
+  const Place at = make_place(a, sp);
+  if (at.shared) {
+    attend_shared<T, DP, NQ, UNI, FULL>(a, at.index, sp.seg_shared, (f32x4*)lds, ml);
+  } else {
+    attend_own<T, DP, UNI, FULL>(a, at.index * kSplitWaves + uniform((int)threadIdx.x >> 6), sp.seg_own, total, (const int*)lds);
+  }
+}
+
+// ------------------------------------------------- shared tiles in LDS
+// More than 32 query rows: the workgroup's four wavefronts hold 16 QB rows each and
+// read the same 64-key tiles from LDS, copied there straight from memory one tile
+// ahead, so a key is read from L2 once per 64 QB rows. Each wavefront copies 16 of
+// a tile's rows: one group of the block table's, at a scalar base. As in
+// paged_prefill_tr, S^T's rows are the keys 32 c + 8 (r / 4) + 4 h + r % 4 for block
+// 2 c + h, which puts 8 consecutive keys of its column into a lane, and V^T comes
+// out of ds_read_b64_tr_b16; the weights' sums are one more product, with ones.
+template <typename T, int DP, int QB>
+struct LdsState {
+  f32x4 acc[QB][DP / 16], sum[QB];
+  float m[QB], mc[QB];
+};
+
+template <typename T, int DP, int QB>
+__device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char* kl, uint32_t vl, uint32_t counts,
+                                                const uint4 (&qf)[QB][DP / 32], LdsState<T, DP, QB>& st) {
+  constexpr int kRowB = DP * 2, kCPR = DP / 8;
+  const int lane = (int)threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int kr = 8 * (col >> 2) + (col & 3);
+  f32x4 s[QB][4];
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+    for (int q = 0; q < QB; ++q) s[q][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int f = 0; f < DP / 32; ++f) {
+      const uint4 kv = *(const uint4*)(kl + (kr + 32 * (kb >> 1) + 4 * (kb & 1)) * kRowB + (((4 * f + g) ^ k_swz<kCPR>(kr)) << 4));
+#pragma unroll
+      for (int q = 0; q < QB; ++q) s[q][kb] = mfma16<T>(kv, qf[q][f], s[q][kb]);
+    }
+  }
+  if (counts != 0x10101010u) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const int j = 2 * (kb >> 1) + (g >> 1), first = 8 * (g & 1) + 4 * (kb & 1), n = (int)(counts >> (8 * j)) & 255;
+#pragma unroll
+      for (int q = 0; q < QB; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[q][kb][i] = first + i < n ? s[q][kb][i] : kNegInf;
+    }
+  }
+  const float c = a.scale_log2;
+  uint4 pf[QB][2];
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    float top = kNegInf;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[q][kb][i]);
+    if (__any(top > st.m[q] + a.lazy)) {
+      const float mn = fmaxf(st.m[q], across_groups_max(top)), mcn = mn == kNegInf ? 0.f : mn * c;
+      const float alpha = st.m[q] == kNegInf ? 0.f : fast_exp2(st.mc[q] - mcn);
+      st.m[q] = mn;
+      st.mc[q] = mcn;
+      st.sum[q] *= alpha;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) st.acc[q][t] *= alpha;
+    }
+    float p[16];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[4 * kb + i] = fast_exp2(fmaf(s[q][kb][i], c, -st.mc[q]));
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      pf[q][h] = make_uint4(pack2<T>(p[8 * h], p[8 * h + 1]), pack2<T>(p[8 * h + 2], p[8 * h + 3]),
+                            pack2<T>(p[8 * h + 4], p[8 * h + 5]), pack2<T>(p[8 * h + 6], p[8 * h + 7]));
+  }
+  const uint32_t one2 = pack2<T>(1.f, 1.f);
+  const uint4 ones = make_uint4(one2, one2, one2, one2);
+  const int vrow = 8 * g + (col >> 2), vq = lane & 3;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+      const uint32_t at = vl + vrow * kRowB + ((vq & 1) << 3) + (((2 * t + (vq >> 1)) ^ v_swz<kCPR>(vrow)) << 4) + 32 * h * kRowB;
+      const uint2 lo = TrRead<T>::at(at), hi = TrRead<T>::at(at + 4 * kRowB);
+#pragma unroll
+      for (int q = 0; q < QB; ++q) st.acc[q][t] = mfma16<T>(make_uint4(lo.x, lo.y, hi.x, hi.y), pf[q][h], st.acc[q][t]);
+    }
+#pragma unroll
+    for (int q = 0; q < QB; ++q) st.sum[q] = mfma16<T>(ones, pf[q][h], st.sum[q]);
+  }
+}
+
+template <typename T, int DP, int QB>
+__device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, int seg, char* lds) {
+  constexpr int kRowB = DP * 2, kCPR = DP / 8, kTileB = 64 * kRowB, kRPC = 1024 / kRowB, kCopies = 16 / kRPC;
+  const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int total = a.s_units * a.s_tiles;
+  if ((int64_t)wg * seg >= total) return;
+  const int stop = min(total, wg * seg + seg);
+  // The lane's part of the wavefront's copies: rows and chunks as the swizzles place them.
+  uint32_t ko[kCopies], vo[kCopies];
+  int row[kCopies], kc[kCopies], vc[kCopies];
+#pragma unroll
+  for (int c = 0; c < kCopies; ++c) {
+    row[c] = c * kRPC + lane / kCPR;
+    kc[c] = (lane % kCPR) ^ k_swz<kCPR>(16 * wave + row[c]);
+    vc[c] = (lane % kCPR) ^ v_swz<kCPR>(16 * wave + row[c]);
+    ko[c] = (uint32_t)row[c] * (uint32_t)a.k_ss * 2 + (uint32_t)kc[c] * 16;
+    vo[c] = (uint32_t)row[c] * (uint32_t)a.v_ss * 2 + (uint32_t)vc[c] * 16;
+  }
+  const uint32_t dst0 = lds_addr(lds) + (uint32_t)wave * 16 * kRowB;
+  const bool all_dims = a.D == DP;
+  uint4 qf[QB][DP / 32];
+  LdsState<T, DP, QB> st;
+  for (int u = wg * seg, n; u < stop; u += n) {
+    const int unit = u / a.s_tiles, tile0 = u - unit * a.s_tiles, kvh = unit / a.row_sets;
+    const int r0 = (unit - kvh * a.row_sets) * 64 * QB, mine = r0 + wave * 16 * QB;
+    n = min(a.s_tiles - tile0, stop - u);
+    const char* kp = (const char*)a.k + (int64_t)kvh * a.k_sh * 2;
+    const char* vp = (const char*)a.v + (int64_t)kvh * a.v_sh * 2;
+    // A window of 64 tiles: lane i holds tile i's four groups' key counts and the
+    // place of the wavefront's own.
+    int tok = (tile0 + lane) * 64, entry[4];
+    auto look = [&]() {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) entry[j] = window_entry(a, 0, tok + 16 * j, a.P);
+    };
+    Window win{};
+    uint32_t counts = 0;
+    uint32_t now = 0, next = 0;  // key counts of the tile computed and of the one copied
+    auto copy = [&](int i, int stage) {
+      if (i % 64 == 0) {
+        counts = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) counts |= (uint32_t)(entry[j] < 0 ? 0 : min(16, a.P - tok - 16 * j)) << (8 * j);
+        const int e = wave == 0 ? entry[0] : wave == 1 ? entry[1] : wave == 2 ? entry[2] : entry[3];
+        win = make_window<T>(a, e, tok + 16 * wave, a.P);
+        tok += 64 * 64;
+        look();
+      }
+      const int at = i % 64;
+      next = (uint32_t)__builtin_amdgcn_readlane((int)counts, at);
+      const char* kb = kp + lane_offset(win.k_lo, win.k_hi, at);
+      const char* vb = vp + lane_offset(win.v_lo, win.v_hi, at);
+      uint32_t kd = dst0 + stage * 2 * kTileB, vd = kd + kTileB;
+      if (all_dims && next == 0x10101010u) {
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+          copy16_to_lds(kb, ko[c], kd + 1024 * c);
+          copy16_to_lds(vb, vo[c], vd + 1024 * c);
+        }
+      } else {  // what does not count is zeros
+        const int m = (int)(next >> (8 * wave)) & 255;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+          const void* ks = row[c] < m && kc[c] * 8 < a.D ? (const void*)(kb + ko[c]) : (const void*)(kZeroRow + kc[c] * 16);
+          const void* vs = row[c] < m && vc[c] * 8 < a.D ? (const void*)(vb + vo[c]) : (const void*)(kZeroRow + vc[c] * 16);
+          copy16_to_lds(ks, kd + 1024 * c);
+          copy16_to_lds(vs, vd + 1024 * c);
+        }
+      }
+    };
+    look();
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+      const int r = mine + 16 * q + col, bb = fast_div(r, a.g_mul, a.g_shift, a.G);
+      const T* p = (const T*)a.q + (int64_t)bb * a.q_sb + (int64_t)(kvh * a.G + r - bb * a.G) * a.q_sh + 8 * g;
+#pragma unroll
+      for (int f = 0; f < DP / 32; ++f) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < a.B * a.G && 32 * f + 8 * g < a.D && !a.q_zero) {
+          x = *(const uint4*)(p + 32 * f);
+          x = make_uint4(x.x ^ a.q_flip, x.y ^ a.q_flip, x.z ^ a.q_flip, x.w ^ a.q_flip);
+        }
+        qf[q][f] = x;
+      }
+      st.sum[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+      st.m[q] = kNegInf;
+      st.mc[q] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) st.acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    bool any = false;
+    const bool active = mine < a.B * a.G;
+    __syncthreads();  // the tiles of the piece before, and the scan's sums, are done with
+    copy(0, 0);
+    auto turn = [&](int i, auto stage) {
+      constexpr int S = decltype(stage)::value;
+      now = next;
+      wait_and_barrier<0>();  // tile i has landed, and tile i - 1 is done with
+      if (i + 1 < n) copy(i + 1, S ^ 1);
+      any |= now != 0;
+      if (active) attend_lds_tile<T, DP, QB>(a, lds + S * 2 * kTileB, lds_addr(lds) + S * 2 * kTileB + kTileB, now, qf, st);
+    };
+    for (int i = 0; i < n; i += 2) {
+      turn(i, Stage<0>{});
+      if (i + 1 < n) turn(i + 1, Stage<1>{});
+    }
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+      const int64_t slot = shared_slot(a, kvh, mine + 16 * q + col, r0, tile0 == 0, wg);
+      if (slot < 0) continue;
+      if (lane < 16) a.ws_ml[slot] = make_float2(st.m[q] == kNegInf ? kNegInf : st.mc[q], coded_sum(st.sum[q][0], any));
+      float* out = a.ws_acc + slot * a.D + 4 * g;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t)
+        if (16 * t + 4 * g < a.D) *(f32x4*)(out + 16 * t) = st.acc[q][t];
+    }
+  }
+}
+
+template <typename T, int DP, int QB, bool FULL>
+__global__ void __launch_bounds__(64 * kSplitWaves, 2) paged_shared_split_lds(const SharedArgs a) {
+  __shared__ __align__(1024) char lds[4 * 64 * DP * 2];
+  __shared__ int part[kSplitWaves];
+  static_assert(sizeof(lds) >= kSharedMaxB * 4, "the rows' prefix sums fit the tiles' place");
+  const int total = scan_own<Tile<T, DP>::kKeys>(a, (int*)lds, part) * a.vheads;
+  const Split sp = make_split(a, total);
+  const Place at = make_place(a, sp);
+  if (at.shared) {
+    attend_shared_lds<T, DP, QB>(a, at.index, sp.seg_shared, lds);
+  } else {
+    attend_own<T, DP, true, FULL>(a, at.index * kSplitWaves + uniform((int)threadIdx.x >> 6), sp.seg_own, total, (const int*)lds);
+  }
+}
+
+// Joins the partials of one (row, query head) per JW wavefronts: lanes over the
+// pieces for their weights, then D / 4 lanes to a piece's row.
+template <typename T, int JW>
+__global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
+  __shared__ f32x4 part[4][64];
+  __shared__ float ml[4][2];
+  const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * (4 / JW) + wave / JW;
+  const bool live = unit < (int64_t)a.B * a.Hq;
+  const int b = live ? (int)(unit / a.Hq) : 0, hq = live ? (int)(unit - (int64_t)b * a.Hq) : 0;
+  const int kvh = hq / a.G, g = hq - kvh * a.G, set = g / 16, r = b * a.G + g;
+  const int before = b ? a.ws_cum[b - 1] : 0, tiles = a.ws_cum[b] - before;
+  const Split sp = make_split(a, a.ws_cum[a.B - 1] * a.vheads);
+  int shared = 0, s0 = 0, pieces = 0, w0 = 0;
+  if (a.s_tiles && clamped_ctx(a, b) >= a.P) {
+    const int u = (kvh * a.row_sets + r / a.set_rows) * a.s_tiles;
+    s0 = u / sp.seg_shared;
+    shared = (u + a.s_tiles - 1) / sp.seg_shared - s0 + 1;
+  }
+  if (tiles) {
+    const int u = before * a.vheads + (kvh * a.gsets + set) * tiles;
+    w0 = u / sp.seg_own;
+    pieces = (u + tiles - 1) / sp.seg_own - w0 + 1;
+  }
+  const int n = live ? shared + pieces : 0;
+  auto slot = [&](int i) -> int64_t {
+    if (i < shared) return i == 0 ? unit : a.s_cont + (int64_t)(s0 + i) * a.set_rows + r % a.set_rows;
+    i -= shared;
+    return i == 0 ? a.own_slot + unit : a.own_cont + (int64_t)(w0 + i) * 16 + (g - set * 16);
+  };
+  const int lpr = a.D <= 64 ? 16 : a.D <= 128 ? 32 : 64, at = lane / lpr, d = 4 * (lane % lpr), per = 64 / lpr;
+  float top = kNegInf, sum = 0.f;
+  bool dead = false;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 64 * (wave % JW); i0 < n; i0 += 64 * JW) {
+    const float2 x = i0 + lane < n ? a.ws_ml[slot(i0 + lane)] : make_float2(kNegInf, 0.f);
+    const bool counts = !(x.y <= 0.f);
+    dead |= x.y < 0.f;
+    const float mn = fmaxf(top, wave_max(counts ? x.x : kNegInf));
+    const float alpha = top == kNegInf ? 0.f : fast_exp2(top - mn);
+    const float w = counts ? fast_exp2(x.x - mn) : 0.f;
+    sum = sum * alpha + wave_sum(counts ? x.y * w : 0.f);
+    acc *= alpha;
+    top = mn;
+    const int m = min(64, n - i0);
+#pragma unroll 4
+    for (int i = 0; i < m; i += per) {
+      // Every lane takes part in the exchange: a lane reads one that is switched off as 0.
+      const float wi = __shfl(w, i + at, 64);
+      const int use = __shfl((int)counts, i + at, 64);
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (use && i + at < m && d < a.D) v = *(const f32x4*)(a.ws_acc + slot(i0 + i + at) * a.D + d);
+      acc += wi * v;
+    }
+  }
+#pragma unroll
+  for (int m = 32; m >= 16; m >>= 1)
+    if (lpr <= m) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], m, 64);
+    }
+  dead = __any(dead);
+  if constexpr (JW > 1) {
+    if (lane == 0) ml[wave][0] = top, ml[wave][1] = sum == 0.f && dead ? -1.f : sum;
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave % JW) return;
+    float tn = kNegInf, sn = 0.f;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    dead = false;
+#pragma unroll
+    for (int w = 0; w < JW; ++w)
+      if (!(ml[wave + w][1] <= 0.f)) tn = fmaxf(tn, ml[wave + w][0]);
+#pragma unroll
+    for (int w = 0; w < JW; ++w) {
+      const float l = ml[wave + w][1];
+      dead |= l < 0.f;
+      if (l <= 0.f) continue;
+      const float f = fast_exp2(ml[wave + w][0] - tn);
+      sn += l * f;
+      acc += f * part[wave + w][lane];
+    }
+    sum = sn;
+  }
+  const float inv = sum == 0.f ? (dead ? __builtin_nanf("") : 0.f) : 1.f / sum;
+  if (live && at == 0 && d < a.D) {
+    T* o = (T*)a.out + (int64_t)b * a.o_sb + (int64_t)hq * a.o_sh + d;
+    if constexpr (sizeof(T) == 4) *(f32x4*)o = acc * inv;
+    else *(uint2*)o = make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
   }
 }
 
@@ -675,7 +1021,7 @@ __global__ void __launch_bounds__(64 * kOneWaves<DP>) paged_shared_one(const Sha
   const int end = clamped_ctx(a, b);
   uint4 qf[1][L::kKS];
   State<DP, 1> st;
-  load_queries<T, DP, 1, FULL>(a, kvh, (int64_t)b * a.G + g0, (int64_t)(b + 1) * a.G, qf);
+  load_queries<T, DP, 1, FULL>(a, kvh, b * a.G + g0, (b + 1) * a.G, qf);
   st.reset();
   stream_tiles<T, DP, 1, UNI, FULL>(a, b, kvh, wave * L::kKeys, kOneWaves<DP> * L::kKeys, end, qf, st);
   join_waves<DP, 1, kOneWaves<DP>>(st, wave, ml, buf);
@@ -747,14 +1093,19 @@ hipError_t launch_tiles(const SharedArgs& a, hipStream_t stream) {
     return hipLaunchKernel((const void*)&paged_shared_one<T, DP, UNI, FULL>, dim3((unsigned)a.vheads, (unsigned)a.B),
                            dim3(64 * kOneWaves<DP>), kargs, 0, stream);
   const void* fn = (const void*)&paged_shared_split<T, DP, 1, UNI, FULL>;
-  if (a.row_tiles == 2) fn = (const void*)&paged_shared_split<T, DP, 2, UNI, FULL>;
-  if constexpr (DP < 256)
-    if (a.row_tiles == 4) fn = (const void*)&paged_shared_split<T, DP, 4, UNI, FULL>;
-  const unsigned wgs = (unsigned)(a.prefix_wgs + a.own_waves / kSplitWaves);
-  const hipError_t e = hipLaunchKernel(fn, dim3(wgs), dim3(64 * kSplitWaves), kargs, 0, stream);
+  if constexpr (DP <= 128)
+    if (a.row_tiles == 2) fn = (const void*)&paged_shared_split<T, DP, 2, UNI, FULL>;
+  if constexpr (sizeof(T) == 2 && DP <= 128 && UNI) {
+    if (a.lds_tiles)
+      fn = a.row_tiles == 2 ? (const void*)&paged_shared_split_lds<T, DP, 2, FULL> : (const void*)&paged_shared_split_lds<T, DP, 1, FULL>;
+  }
+  const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)a.wgs), dim3(64 * kSplitWaves), kargs, 0, stream);
   if (e != hipSuccess) return e;
+  // Few rows leave many pieces to each: four wavefronts join them.
   const int64_t units = (int64_t)a.B * a.Hq;
-  return hipLaunchKernel((const void*)&paged_shared_join<T>, dim3((unsigned)((units + 3) / 4)), dim3(256), kargs, 0, stream);
+  if (units <= 4 * a.wgs)
+    return hipLaunchKernel((const void*)&paged_shared_join<T, 4>, dim3((unsigned)units), dim3(256), kargs, 0, stream);
+  return hipLaunchKernel((const void*)&paged_shared_join<T, 1>, dim3((unsigned)((units + 3) / 4)), dim3(256), kargs, 0, stream);
 }
 
 template <typename T, int DP>
