@@ -783,7 +783,7 @@ int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
 
 // How mgi_paged_decode_shared runs a call of these sizes on the matrix-core kernels.
 struct SharedPlan {
-  int one_launch, gsets, vheads, wgs, lds_tiles, row_tiles, set_rows, row_sets, s_units, s_tiles, s_cost, s_min, own_min;
+  int one_launch, gsets, vheads, wgs, lds_tiles, row_tiles, set_rows, team, set_blocks, s_units, s_tiles, s_cost, s_min, own_min;
   int64_t s_cont, own_slot, own_cont, slots;
   size_t ml_offset, cum_offset, total;
 };
@@ -797,17 +797,20 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   p.lds_tiles = dtype != MGI_F32 && D <= 128 && S % 16 == 0 && rows > env_int("MINIVLLM_HIP_SHARED_LDS", 32);
   p.row_tiles = rows > (p.lds_tiles ? 64 : 16) && D <= 128 ? 2 : 1;
   p.set_rows = (p.lds_tiles ? 64 : 16) * p.row_tiles;
-  p.row_sets = (int)((rows + p.set_rows - 1) / p.set_rows);
+  // Sets of rows a team takes together: as many of up to 16 as fill their blocks evenly.
+  const int64_t sets = (rows + p.set_rows - 1) / p.set_rows;
+  p.set_blocks = (int)((sets + 15) / 16);
+  p.team = (int)((sets + p.set_blocks - 1) / p.set_blocks);
   const int64_t step = p.lds_tiles ? 64 : 4 * keys, tiles = (shared * S + step - 1) / step;
   // Tile numbers are 32-bit, and the rows' prefix sums live in LDS.
-  p.one_launch = forced == 0 || B > mgi::kSharedMaxB || Hk * p.row_sets * tiles >= (int64_t(1) << 30) ||
+  p.one_launch = forced == 0 || B > mgi::kSharedMaxB || Hk * p.set_blocks * tiles >= (int64_t(1) << 30) ||
                  B * ((M * S + keys - 1) / keys) * p.vheads >= (int64_t(1) << 30);
   if (p.one_launch) return p;
   p.s_tiles = (int)tiles;
-  p.s_units = (int)(Hk * p.row_sets);
+  p.s_units = (int)(Hk * p.set_blocks);
   p.s_cost = env_int("MINIVLLM_HIP_SHARED_COST", (int)(step / keys));
-  p.s_min = env_int("MINIVLLM_HIP_SHARED_SMIN", 2);
-  p.own_min = env_int("MINIVLLM_HIP_SHARED_OMIN", 4);
+  p.s_min = env_int("MINIVLLM_HIP_SHARED_SMIN", 1);
+  p.own_min = env_int("MINIVLLM_HIP_SHARED_OMIN", 1);
   p.wgs = (int)round_up(env_int("MINIVLLM_HIP_SHARED_WGS", 2) * device_cus(), 8);
   p.s_cont = B * Hq;
   p.own_slot = p.s_cont + (tiles ? (int64_t)p.wgs * p.set_rows : 0);
@@ -815,7 +818,7 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   p.slots = p.own_cont + (int64_t)p.wgs * 4 * 16;
   p.ml_offset = (size_t)round_up(p.slots * D * 4, kWorkspaceAlign);
   p.cum_offset = (size_t)round_up((int64_t)p.ml_offset + p.slots * 8, kWorkspaceAlign);
-  p.total = p.cum_offset + (size_t)(B * 4);
+  p.total = p.cum_offset + (size_t)(B * 4 + 8);
   return p;
 }
 
@@ -1263,7 +1266,7 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
     const SharedPlan p = shared_plan(B, Hq, Hk, D, S, M, shared_blocks, dtype);
     a.one_launch = p.one_launch;
     a.gsets = p.gsets, a.vheads = p.vheads, a.wgs = p.wgs, a.lds_tiles = p.lds_tiles, a.row_tiles = p.row_tiles;
-    a.set_rows = p.set_rows, a.row_sets = p.row_sets, a.s_units = p.s_units, a.s_tiles = p.s_tiles, a.s_cost = p.s_cost;
+    a.set_rows = p.set_rows, a.team = p.team, a.set_blocks = p.set_blocks, a.s_units = p.s_units, a.s_tiles = p.s_tiles, a.s_cost = p.s_cost;
     a.s_min = p.s_min, a.own_min = p.own_min;
     a.s_cont = p.s_cont, a.own_slot = p.own_slot, a.own_cont = p.own_cont;
     if (!p.one_launch) {
@@ -1273,7 +1276,8 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
       if (!aligned16(workspace)) return fail(MGI_EINVAL, "workspace must be 16-byte aligned");
       a.ws_acc = static_cast<float*>(workspace);
       a.ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.ml_offset);
-      a.ws_cum = reinterpret_cast<int*>(static_cast<char*>(workspace) + p.cum_offset);
+      a.ws_split = reinterpret_cast<int*>(static_cast<char*>(workspace) + p.cum_offset);
+      a.ws_cum = a.ws_split + 2;
     }
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -141,8 +141,9 @@ struct SharedArgs {
   int wgs;                 // workgroups of the split launch (a multiple of 8)
   int lds_tiles;           // shared tiles go through LDS
   int row_tiles;           // 16-row query tiles per wavefront of the shared part
-  int set_rows, row_sets;  // query rows per workgroup of it, and such sets per KV head
-  int s_units, s_tiles;    // its list: KV heads x sets, key tiles of each
+  int set_rows;            // query rows per workgroup of it
+  int team, set_blocks;    // sets that workgroups of a team take together, and blocks of those per KV head
+  int s_units, s_tiles;    // its list: KV heads x blocks, key tiles of each
   int s_cost;              // cost of one of its tiles, an own tile being 1
   int s_min, own_min;      // least tiles of a segment
   // Partials: [B, Hq] of the pieces that begin a row's shared run and, from own_slot,
@@ -152,6 +153,7 @@ struct SharedArgs {
   float* ws_acc;           // [slots, D]
   float2* ws_ml;           // [slots] (maximum in log2 units, sum)
   int* ws_cum;             // [B] prefix sums of the rows' own tiles
+  int* ws_split;           // the two lists' segment lengths
 };
 constexpr int kSharedMaxB = 4096;      // rows of the split form (their prefix sums live in LDS)
 hipError_t launch_paged_shared_f32(const SharedArgs& a, hipStream_t stream);

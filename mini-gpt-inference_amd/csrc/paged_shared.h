@@ -148,9 +148,10 @@ __device__ __forceinline__ int window_entry(const SharedArgs& a, int b, int tok,
   return id >= 0 && id < a.N ? (int)id : -1;
 }
 template <typename T>
-__device__ __forceinline__ Window make_window(const SharedArgs& a, int id, int tok, int end) {
+__device__ __forceinline__ Window make_window(const SharedArgs& a, int id, int tok, int end, int kvh) {
   const int64_t at = max(id, 0), off = id < 0 ? 0 : tok - fast_div(tok, a.s_mul, a.s_shift, a.S) * a.S;
-  const uint64_t k = (uint64_t)(at * a.k_sn + off * a.k_ss) * sizeof(T), v = (uint64_t)(at * a.v_sn + off * a.v_ss) * sizeof(T);
+  const uint64_t k = (uint64_t)(at * a.k_sn + off * a.k_ss + kvh * a.k_sh) * sizeof(T);
+  const uint64_t v = (uint64_t)(at * a.v_sn + off * a.v_ss + kvh * a.v_sh) * sizeof(T);
   return {(uint32_t)k, (uint32_t)(k >> 32), (uint32_t)v, (uint32_t)(v >> 32), id < 0 ? 0 : min(16, end - tok)};
 }
 __device__ __forceinline__ int64_t lane_offset(uint32_t lo, uint32_t hi, int i) {
@@ -159,7 +160,7 @@ __device__ __forceinline__ int64_t lane_offset(uint32_t lo, uint32_t hi, int i) 
 }
 
 // Loads the keys, and the values, of the tile whose groups are lanes at .. of the
-// window, of the KV head at kp, vp. Rows past a group's last key read that one again.
+// window (kp, vp: the pools). Rows past a group's last key read that one again.
 // FULL: D == DP.
 template <typename T, int DP, bool FULL>
 __device__ __forceinline__ void load_keys(const SharedArgs& a, const char* kp, const Window& w, int at, Tile<T, DP>& f) {
@@ -363,8 +364,8 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, Tile<T, DP>& f,
 // Attends the tiles first, first + step, ... below end of row b's table. A tile's
 // keys are loaded into the registers the one before has given its scores from, and
 // its values where that one's products have been taken: half a tile is always on
-// its way, without a second set of registers (with one, two wavefronts fit a SIMD
-// and spilled; so, three do).
+// its way. (A second set of registers, a whole tile ahead, changed nothing: 133 us
+// either way for 64 x 32 heads.)
 template <typename T, int DP, int NQ, bool UNI, bool FULL>
 __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh, int first, int step, int end,
                                              const uint4 (&qf)[NQ][Tile<T, DP>::kKS], State<DP, NQ>& st) {
@@ -384,24 +385,24 @@ __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh
   auto keys = [&](int i) {
     if constexpr (UNI) {
       if (i % kSpan == 0) {
-        win = make_window<T>(a, entry, tok, end);
+        win = make_window<T>(a, entry, tok, end, kvh);
         tok += kSpan * step;
         entry = window_entry(a, b, tok, end);
       }
-      load_keys<T, DP, FULL>(a, kp, win, i % kSpan * L::kGroups, f);
+      load_keys<T, DP, FULL>(a, (const char*)a.k, win, i % kSpan * L::kGroups, f);
     } else {
       load_keys_any<T, DP>(a, kp, b, first + i * step, end, f);
     }
   };
   auto values = [&](int i) {
-    if constexpr (UNI) load_values<T, DP, FULL>(a, vp, win, i % kSpan * L::kGroups, f);
+    if constexpr (UNI) load_values<T, DP, FULL>(a, (const char*)a.v, win, i % kSpan * L::kGroups, f);
     else load_values_any<T, DP>(a, vp, b, first + i * step, end, f);
   };
   const int n = (end - first + step - 1) / step;
+  f32x4 s[NQ][L::kGroups];
   keys(0);
   values(0);
   for (int i = 0; i < n; ++i) {
-    f32x4 s[NQ][L::kGroups];
     score_tile<T, DP, NQ>(f, qf, s);
     if (i + 1 < n) keys(i + 1);
     attend_tile<T, DP, NQ, UNI>(a, f, s, st);
@@ -521,34 +522,31 @@ __device__ __forceinline__ int clamped_ctx(const SharedArgs& a, int b) {
   return (int)(c < 0 ? 0 : c > top ? top : c);
 }
 
-// Row b's own tokens are first .. end - 1.
-struct Own {
-  int first, end;
-};
 constexpr int kSplitWaves = 4;
-__device__ __forceinline__ Own own_range(const SharedArgs& a, int b) {
-  const int c = clamped_ctx(a, b);
-  return {c < a.P ? 0 : a.P, c};
-}
-
-// The work is two lists: the shared tokens' tiles, (KV head, set of query rows, tile)
-// in that order, and the rows' own, (row, virtual head, tile), a virtual head
+// The work is two lists: the shared tokens' tiles, (KV head, block of row sets, tile)
+// in that order, each for a team of workgroups, one to a set of query rows, that
+// walk the same keys together and find them in their XCD's L2 (8 sets of 128 rows
+// over 65 536 tokens: 197 us with a list per set); and the rows' own, (row, virtual head, tile), a virtual head
 // being a KV head and a set of at most 16 of its query heads. The launch's
 // workgroups are dealt out between the lists by cost, and each list is cut into
-// equal segments: one per workgroup of the first list, one per wavefront of the
-// second. A segment's first piece may continue a run that another began: it leaves
+// equal segments: one per team of the first list, one per wavefront of the second. A segment's first piece may continue a run that another began: it leaves
 // its partial in the segment's slots, a piece that begins a run in the rows' own.
 struct Split {
-  int shared_wgs;  // workgroups of the first list
-  int seg_shared;  // tiles of their segments
+  int shared_wgs;  // workgroups of the first list, whole teams
+  int seg_shared;  // tiles of a team's segment
   int seg_own;
 };
 __device__ __forceinline__ Split make_split(const SharedArgs& a, int own_total) {
   const int total = a.s_units * a.s_tiles;
-  const int64_t cs = (int64_t)total * a.s_cost, co = own_total;
+  const int64_t cs = (int64_t)total * a.team * a.s_cost, co = own_total;
   Split r{};
-  r.shared_wgs = total == 0 ? 0 : own_total == 0 ? a.wgs : (int)min((int64_t)a.wgs - 1, max((int64_t)1, (a.wgs * cs + (cs + co) / 2) / (cs + co)));
-  if (r.shared_wgs) r.seg_shared = max(a.s_min, (total + r.shared_wgs - 1) / r.shared_wgs);
+  int teams = 0;
+  if (total) {
+    const int64_t fair = (a.wgs * cs + (cs + co) * a.team / 2) / ((cs + co) * a.team);
+    teams = (int)max((int64_t)1, min(fair, (int64_t)(a.wgs - (own_total > 0)) / a.team));
+    r.seg_shared = max(a.s_min, (total + teams - 1) / teams);
+  }
+  r.shared_wgs = teams * a.team;
   const int waves = (a.wgs - r.shared_wgs) * kSplitWaves;
   if (waves) r.seg_own = max(a.own_min, (own_total + waves - 1) / waves);
   return r;
@@ -568,17 +566,19 @@ __device__ __forceinline__ Place make_place(const SharedArgs& a, const Split& sp
   return {false, x * (a.wgs / 8) - before + j - mine};
 }
 
-// Prefix sums of the rows' own tiles into cum[0 .. B); returns the total.
+// Prefix sums of the rows' own tiles into cum[0 .. B), their lengths into ctx; returns
+// the total.
 template <int KEYS>
-__device__ __forceinline__ int scan_own(const SharedArgs& a, int* cum, int* part) {
+__device__ __forceinline__ int scan_own(const SharedArgs& a, int* cum, int* ctx, int* part) {
   const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int per = (a.B + 64 * kSplitWaves - 1) / (64 * kSplitWaves), b0 = (int)threadIdx.x * per;
   int sum = 0;
   for (int i = 0; i < per; ++i)
     if (b0 + i < a.B) {
-      const Own own = own_range(a, b0 + i);
-      sum += (own.end - own.first + KEYS - 1) / KEYS;
+      const int c = clamped_ctx(a, b0 + i);
+      sum += (c - (c < a.P ? 0 : a.P) + KEYS - 1) / KEYS;
       cum[b0 + i] = sum;
+      ctx[b0 + i] = c;
     }
   int incl = sum;
 #pragma unroll
@@ -604,40 +604,111 @@ __device__ __forceinline__ int scan_own(const SharedArgs& a, int* cum, int* part
   return uniform(total);
 }
 
-template <typename T, int DP, bool UNI, bool FULL>
-__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum) {
-  using L = Tile<T, DP>;
-  const int lane = (int)threadIdx.x & 63;
-  if ((int64_t)wave_index * seg >= total) return;
-  int u = wave_index * seg, b = 0;
-  const int stop = min(total, u + seg);
-  for (int hi = a.B - 1; b < hi;) {  // the row of tile u: the first with cum[b] * vheads > u
+// Where tile u of the rows' own lies.
+struct OwnTile {
+  int b, vh, tile, tiles;  // row, virtual head, tile of its run, the run's tiles
+};
+__device__ __forceinline__ OwnTile find_own(const SharedArgs& a, const int* cum, int u) {
+  int b = 0;
+  for (int hi = a.B - 1; b < hi;) {  // the first row with cum[b] * vheads > u
     const int mid = (b + hi) >> 1;
-    if (uniform(cum[mid]) * a.vheads > u) hi = mid;
+    if (cum[mid] * a.vheads > u) hi = mid;
     else b = mid + 1;
   }
+  const int before = b ? cum[b - 1] : 0, tiles = cum[b] - before, rem = u - before * a.vheads, vh = rem / tiles;
+  return {b, vh, rem - vh * tiles, tiles};
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_own(const SharedArgs& a, const State<DP, 1>& st, int wave_index, int b, int vh, bool begins) {
+  const int lane = (int)threadIdx.x & 63, kvh = vh / a.gsets, g = (vh - kvh * a.gsets) * 16 + (lane & 15);
+  const float l = coded_sum(across_groups_sum(st.l[0]), st.any);
+  const int64_t slot = begins ? a.own_slot + (int64_t)b * a.Hq + kvh * a.G + g : a.own_cont + (int64_t)wave_index * 16 + (lane & 15);
+  if (g < a.G) store_partial<T>(a, st, 0, slot, st.m[0] == kNegInf ? kNegInf : st.mc[0], l);
+}
+template <typename T, int DP, bool FULL>
+__device__ __forceinline__ void load_own_queries(const SharedArgs& a, int b, int vh, uint4 (&qf)[1][Tile<T, DP>::kKS]) {
+  const int kvh = vh / a.gsets;
+  load_queries<T, DP, 1, FULL>(a, kvh, b * a.G + (vh - kvh * a.gsets) * 16, (b + 1) * a.G, qf);
+}
+
+// A wavefront's segment of the rows' own tiles, as one stream over rows and heads:
+// the window's lanes find their own tiles, so a run's end costs no new chain of
+// loads (length, table, queries, keys), only its partial. With a loop over runs
+// instead each cost about 4 us: 13 x 16 heads, 14.9 us where a wavefront had one
+// tile and 19.0 where it had two.
+template <typename T, int DP, bool FULL>
+__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum, const int* ctx) {
+  using L = Tile<T, DP>;
+  constexpr int kSpan = 64 / L::kGroups;
+  const int lane = (int)threadIdx.x & 63;
+  if ((int64_t)wave_index * seg >= total) return;
+  const int u0 = wave_index * seg, n = min(total - u0, seg);
+  Window win{};
+  int row = 0, head = 0;  // of the lane's tile; head: virtual head, and whether the tile begins its run
+  auto fill = [&](int t) {
+    const int u = u0 + t + lane / L::kGroups;
+    if (u < u0 + n) {
+      const OwnTile o = find_own(a, cum, u);
+      const int c = ctx[o.b], tok = (c < a.P ? 0 : a.P) + o.tile * L::kKeys + 16 * (lane % L::kGroups), kvh = o.vh / a.gsets;
+      win = make_window<T>(a, window_entry(a, o.b, tok, c), tok, c, kvh);
+      row = o.b;
+      head = 2 * o.vh + (o.tile == 0);
+    }
+  };
+  const char* kp = (const char*)a.k;
+  const char* vp = (const char*)a.v;
   uint4 qf[1][L::kKS];
   State<DP, 1> st;
-  while (u < stop) {
-    const int before = b ? uniform(cum[b - 1]) : 0, tiles = uniform(cum[b]) - before;
-    if (tiles == 0) {
-      ++b;
-      continue;
+  L f;
+  f32x4 s[1][L::kGroups];
+  fill(0);
+  int b = __builtin_amdgcn_readlane(row, 0), h = __builtin_amdgcn_readlane(head, 0);
+  load_own_queries<T, DP, FULL>(a, b, h >> 1, qf);
+  load_keys<T, DP, FULL>(a, kp, win, 0, f);
+  load_values<T, DP, FULL>(a, vp, win, 0, f);
+  st.reset();
+  for (int t = 0; t < n; ++t) {
+    score_tile<T, DP, 1>(f, qf, s);
+    const bool more = t + 1 < n;
+    const int at = (t + 1) % kSpan * L::kGroups;
+    int nb = b, nh = h;
+    if (more) {
+      if (at == 0) fill(t + 1);
+      nb = __builtin_amdgcn_readlane(row, at);
+      nh = __builtin_amdgcn_readlane(head, at);
+      load_keys<T, DP, FULL>(a, kp, win, at, f);
     }
-    const int rem = u - before * a.vheads;
-    const int vh = rem / tiles, tile = rem - vh * tiles, n = min(tiles - tile, stop - u);
-    const int kvh = vh / a.gsets, g0 = (vh - kvh * a.gsets) * 16, g = g0 + (lane & 15);
-    const Own own = own_range(a, b);
-    load_queries<T, DP, 1, FULL>(a, kvh, b * a.G + g0, (b + 1) * a.G, qf);
+    const bool ends = !more || nb != b || (nh >> 1) != (h >> 1);
+    if (more && ends) load_own_queries<T, DP, FULL>(a, nb, nh >> 1, qf);
+    attend_tile<T, DP, 1, true>(a, f, s, st);
+    if (more) load_values<T, DP, FULL>(a, vp, win, at, f);
+    if (ends) {
+      store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
+      st.reset();
+      b = nb;
+      h = nh;
+    }
+  }
+}
+
+// The same for any S, a run at a time.
+template <typename T, int DP>
+__device__ __forceinline__ void attend_own_any(const SharedArgs& a, int wave_index, int seg, int total, const int* cum, const int* ctx) {
+  using L = Tile<T, DP>;
+  if ((int64_t)wave_index * seg >= total) return;
+  const int stop = min(total, wave_index * seg + seg);
+  uint4 qf[1][L::kKS];
+  State<DP, 1> st;
+  for (int u = wave_index * seg, n; u < stop; u += n) {
+    const OwnTile o = find_own(a, cum, u);
+    const int b = uniform(o.b), vh = uniform(o.vh), tile = uniform(o.tile), c = uniform(ctx[b]);
+    n = min(uniform(o.tiles) - tile, stop - u);
+    load_own_queries<T, DP, false>(a, b, vh, qf);
     st.reset();
-    const int first = uniform(own.first) + tile * L::kKeys;
-    stream_tiles<T, DP, 1, UNI, FULL>(a, b, kvh, first, L::kKeys, min(uniform(own.end), first + n * L::kKeys), qf, st);
-    const float l = coded_sum(across_groups_sum(st.l[0]), st.any);
-    const int64_t slot = tile == 0 ? a.own_slot + (int64_t)b * a.Hq + kvh * a.G + g
-                                   : a.own_cont + (int64_t)wave_index * 16 + (lane & 15);
-    if (g < a.G) store_partial<T>(a, st, 0, slot, st.m[0] == kNegInf ? kNegInf : st.mc[0], l);
-    u += n;
-    if (vh == a.vheads - 1 && tile + n == tiles) ++b;
+    const int first = (c < a.P ? 0 : a.P) + tile * L::kKeys;
+    stream_tiles<T, DP, 1, false, false>(a, b, vh / a.gsets, first, L::kKeys, min(c, first + n * L::kKeys), qf, st);
+    store_own<T>(a, st, wave_index, b, vh, tile == 0);
   }
 }
 
@@ -658,13 +729,16 @@ __device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int s
   using L = Tile<T, DP>;
   const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int total = a.s_units * a.s_tiles, step = kSplitWaves * L::kKeys;
-  if ((int64_t)wg * seg >= total) return;
-  const int stop = min(total, wg * seg + seg);
+  const int team = wg / a.team, member = wg - team * a.team;
+  if ((int64_t)team * seg >= total) return;
+  const int stop = min(total, team * seg + seg);
   uint4 qf[NQ][L::kKS];
   State<DP, NQ> st;
-  for (int u = wg * seg, n; u < stop; u += n) {
-    const int unit = u / a.s_tiles, tile = u - unit * a.s_tiles, kvh = unit / a.row_sets, r0 = (unit - kvh * a.row_sets) * 16 * NQ;
+  for (int u = team * seg, n; u < stop; u += n) {
+    const int unit = u / a.s_tiles, tile = u - unit * a.s_tiles, kvh = unit / a.set_blocks;
+    const int r0 = ((unit - kvh * a.set_blocks) * a.team + member) * 16 * NQ;
     n = min(a.s_tiles - tile, stop - u);
+    if (r0 >= a.B * a.G) continue;
     load_queries<T, DP, NQ, FULL>(a, kvh, r0, a.B * a.G, qf);
     st.reset();
     stream_tiles<T, DP, NQ, UNI, FULL>(a, 0, kvh, tile * step + wave * L::kKeys, step, min(a.P, (tile + n) * step), qf, st);
@@ -681,17 +755,21 @@ __device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int s
 
 template <typename T, int DP, int NQ, bool UNI, bool FULL>
 __global__ void __launch_bounds__(64 * kSplitWaves, DP > 128 ? 1 : 2) paged_shared_split(const SharedArgs a) {
-  constexpr int kBuf = kSplitWaves / 2 * (DP / 16) * 64 * 16, kCum = kSharedMaxB * 4;
+  constexpr int kBuf = kSplitWaves / 2 * (DP / 16) * 64 * 16, kCum = kSharedMaxB * 8;
   __shared__ __align__(16) char lds[kBuf > kCum ? kBuf : kCum];
   __shared__ float ml[kSplitWaves][2][NQ * 16];
   __shared__ int part[kSplitWaves];
-  const int total = scan_own<Tile<T, DP>::kKeys>(a, (int*)lds, part) * a.vheads;
+  int *cum = (int*)lds, *ctx = cum + kSharedMaxB;
+  const int total = scan_own<Tile<T, DP>::kKeys>(a, cum, ctx, part) * a.vheads;
   const Split sp = make_split(a, total);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.ws_split[0] = sp.seg_shared, a.ws_split[1] = sp.seg_own;
   const Place at = make_place(a, sp);
   if (at.shared) {
     attend_shared<T, DP, NQ, UNI, FULL>(a, at.index, sp.seg_shared, (f32x4*)lds, ml);
   } else {
-    attend_own<T, DP, UNI, FULL>(a, at.index * kSplitWaves + uniform((int)threadIdx.x >> 6), sp.seg_own, total, (const int*)lds);
+    const int w = at.index * kSplitWaves + uniform((int)threadIdx.x >> 6);
+    if constexpr (UNI) attend_own<T, DP, FULL>(a, w, sp.seg_own, total, cum, ctx);
+    else attend_own_any<T, DP>(a, w, sp.seg_own, total, cum, ctx);
   }
 }
 
@@ -716,16 +794,25 @@ __device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char*
   const int lane = (int)threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int kr = 8 * (col >> 2) + (col & 3);
   f32x4 s[QB][4];
+  // The next block's keys are read before this one's products; left to itself the
+  // compiler waits for every read.
+  uint4 kv[2][DP / 32];
+  auto read = [&](int kb) {
+#pragma unroll
+    for (int f = 0; f < DP / 32; ++f)
+      kv[kb & 1][f] = *(const uint4*)(kl + (kr + 32 * (kb >> 1) + 4 * (kb & 1)) * kRowB + (((4 * f + g) ^ k_swz<kCPR>(kr)) << 4));
+  };
+  read(0);
 #pragma unroll
   for (int kb = 0; kb < 4; ++kb) {
+    if (kb < 3) read(kb + 1);
 #pragma unroll
     for (int q = 0; q < QB; ++q) s[q][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int f = 0; f < DP / 32; ++f) {
-      const uint4 kv = *(const uint4*)(kl + (kr + 32 * (kb >> 1) + 4 * (kb & 1)) * kRowB + (((4 * f + g) ^ k_swz<kCPR>(kr)) << 4));
+    for (int f = 0; f < DP / 32; ++f)
 #pragma unroll
-      for (int q = 0; q < QB; ++q) s[q][kb] = mfma16<T>(kv, qf[q][f], s[q][kb]);
-    }
+      for (int q = 0; q < QB; ++q) s[q][kb] = mfma16<T>(kv[kb & 1][f], qf[q][f], s[q][kb]);
+    __builtin_amdgcn_sched_barrier(0);
   }
   if (counts != 0x10101010u) {
 #pragma unroll
@@ -770,15 +857,20 @@ __device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char*
   const int vrow = 8 * g + (col >> 2), vq = lane & 3;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
+    uint4 vv[DP / 16];
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
       const uint32_t at = vl + vrow * kRowB + ((vq & 1) << 3) + (((2 * t + (vq >> 1)) ^ v_swz<kCPR>(vrow)) << 4) + 32 * h * kRowB;
       const uint2 lo = TrRead<T>::at(at), hi = TrRead<T>::at(at + 4 * kRowB);
-#pragma unroll
-      for (int q = 0; q < QB; ++q) st.acc[q][t] = mfma16<T>(make_uint4(lo.x, lo.y, hi.x, hi.y), pf[q][h], st.acc[q][t]);
+      vv[t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
 #pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+      for (int q = 0; q < QB; ++q) st.acc[q][t] = mfma16<T>(vv[t], pf[q][h], st.acc[q][t]);
+#pragma unroll
     for (int q = 0; q < QB; ++q) st.sum[q] = mfma16<T>(ones, pf[q][h], st.sum[q]);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -787,8 +879,9 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
   constexpr int kRowB = DP * 2, kCPR = DP / 8, kTileB = 64 * kRowB, kRPC = 1024 / kRowB, kCopies = 16 / kRPC;
   const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int total = a.s_units * a.s_tiles;
-  if ((int64_t)wg * seg >= total) return;
-  const int stop = min(total, wg * seg + seg);
+  const int team = wg / a.team, member = wg - team * a.team;
+  if ((int64_t)team * seg >= total) return;
+  const int stop = min(total, team * seg + seg);
   // The lane's part of the wavefront's copies: rows and chunks as the swizzles place them.
   uint32_t ko[kCopies], vo[kCopies];
   int row[kCopies], kc[kCopies], vc[kCopies];
@@ -804,12 +897,11 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
   const bool all_dims = a.D == DP;
   uint4 qf[QB][DP / 32];
   LdsState<T, DP, QB> st;
-  for (int u = wg * seg, n; u < stop; u += n) {
-    const int unit = u / a.s_tiles, tile0 = u - unit * a.s_tiles, kvh = unit / a.row_sets;
-    const int r0 = (unit - kvh * a.row_sets) * 64 * QB, mine = r0 + wave * 16 * QB;
+  for (int u = team * seg, n; u < stop; u += n) {
+    const int unit = u / a.s_tiles, tile0 = u - unit * a.s_tiles, kvh = unit / a.set_blocks;
+    const int r0 = ((unit - kvh * a.set_blocks) * a.team + member) * 64 * QB, mine = r0 + wave * 16 * QB;
     n = min(a.s_tiles - tile0, stop - u);
-    const char* kp = (const char*)a.k + (int64_t)kvh * a.k_sh * 2;
-    const char* vp = (const char*)a.v + (int64_t)kvh * a.v_sh * 2;
+    if (r0 >= a.B * a.G) continue;  // the last block's teams may be short
     // A window of 64 tiles: lane i holds tile i's four groups' key counts and the
     // place of the wavefront's own.
     int tok = (tile0 + lane) * 64, entry[4];
@@ -826,14 +918,14 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
 #pragma unroll
         for (int j = 0; j < 4; ++j) counts |= (uint32_t)(entry[j] < 0 ? 0 : min(16, a.P - tok - 16 * j)) << (8 * j);
         const int e = wave == 0 ? entry[0] : wave == 1 ? entry[1] : wave == 2 ? entry[2] : entry[3];
-        win = make_window<T>(a, e, tok + 16 * wave, a.P);
+        win = make_window<T>(a, e, tok + 16 * wave, a.P, kvh);
         tok += 64 * 64;
         look();
       }
       const int at = i % 64;
       next = (uint32_t)__builtin_amdgcn_readlane((int)counts, at);
-      const char* kb = kp + lane_offset(win.k_lo, win.k_hi, at);
-      const char* vb = vp + lane_offset(win.v_lo, win.v_hi, at);
+      const char* kb = (const char*)a.k + lane_offset(win.k_lo, win.k_hi, at);
+      const char* vb = (const char*)a.v + lane_offset(win.v_lo, win.v_hi, at);
       uint32_t kd = dst0 + stage * 2 * kTileB, vd = kd + kTileB;
       if (all_dims && next == 0x10101010u) {
 #pragma unroll
@@ -905,14 +997,16 @@ template <typename T, int DP, int QB, bool FULL>
 __global__ void __launch_bounds__(64 * kSplitWaves, 2) paged_shared_split_lds(const SharedArgs a) {
   __shared__ __align__(1024) char lds[4 * 64 * DP * 2];
   __shared__ int part[kSplitWaves];
-  static_assert(sizeof(lds) >= kSharedMaxB * 4, "the rows' prefix sums fit the tiles' place");
-  const int total = scan_own<Tile<T, DP>::kKeys>(a, (int*)lds, part) * a.vheads;
+  static_assert(sizeof(lds) >= kSharedMaxB * 8, "the rows' prefix sums and lengths fit the tiles' place");
+  int *cum = (int*)lds, *ctx = cum + kSharedMaxB;
+  const int total = scan_own<Tile<T, DP>::kKeys>(a, cum, ctx, part) * a.vheads;
   const Split sp = make_split(a, total);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.ws_split[0] = sp.seg_shared, a.ws_split[1] = sp.seg_own;
   const Place at = make_place(a, sp);
   if (at.shared) {
     attend_shared_lds<T, DP, QB>(a, at.index, sp.seg_shared, lds);
   } else {
-    attend_own<T, DP, true, FULL>(a, at.index * kSplitWaves + uniform((int)threadIdx.x >> 6), sp.seg_own, total, (const int*)lds);
+    attend_own<T, DP, FULL>(a, at.index * kSplitWaves + uniform((int)threadIdx.x >> 6), sp.seg_own, total, cum, ctx);
   }
 }
 
@@ -928,21 +1022,22 @@ __global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
   const int b = live ? (int)(unit / a.Hq) : 0, hq = live ? (int)(unit - (int64_t)b * a.Hq) : 0;
   const int kvh = hq / a.G, g = hq - kvh * a.G, set = g / 16, r = b * a.G + g;
   const int before = b ? a.ws_cum[b - 1] : 0, tiles = a.ws_cum[b] - before;
-  const Split sp = make_split(a, a.ws_cum[a.B - 1] * a.vheads);
-  int shared = 0, s0 = 0, pieces = 0, w0 = 0;
+  const int seg_shared = a.ws_split[0], seg_own = a.ws_split[1];
+  int shared = 0, s0 = 0, member = 0, pieces = 0, w0 = 0;
   if (a.s_tiles && clamped_ctx(a, b) >= a.P) {
-    const int u = (kvh * a.row_sets + r / a.set_rows) * a.s_tiles;
-    s0 = u / sp.seg_shared;
-    shared = (u + a.s_tiles - 1) / sp.seg_shared - s0 + 1;
+    const int rs = r / a.set_rows, u = (kvh * a.set_blocks + rs / a.team) * a.s_tiles;
+    member = rs % a.team;
+    s0 = u / seg_shared;
+    shared = (u + a.s_tiles - 1) / seg_shared - s0 + 1;
   }
   if (tiles) {
     const int u = before * a.vheads + (kvh * a.gsets + set) * tiles;
-    w0 = u / sp.seg_own;
-    pieces = (u + tiles - 1) / sp.seg_own - w0 + 1;
+    w0 = u / seg_own;
+    pieces = (u + tiles - 1) / seg_own - w0 + 1;
   }
   const int n = live ? shared + pieces : 0;
   auto slot = [&](int i) -> int64_t {
-    if (i < shared) return i == 0 ? unit : a.s_cont + (int64_t)(s0 + i) * a.set_rows + r % a.set_rows;
+    if (i < shared) return i == 0 ? unit : a.s_cont + ((int64_t)(s0 + i) * a.team + member) * a.set_rows + r % a.set_rows;
     i -= shared;
     return i == 0 ? a.own_slot + unit : a.own_cont + (int64_t)(w0 + i) * 16 + (g - set * 16);
   };
@@ -950,8 +1045,10 @@ __global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
   float top = kNegInf, sum = 0.f;
   bool dead = false;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 64 * (wave % JW); i0 < n; i0 += 64 * JW) {
-    const float2 x = i0 + lane < n ? a.ws_ml[slot(i0 + lane)] : make_float2(kNegInf, 0.f);
+  const int share = (n + JW - 1) / JW, stop = min(n, (wave % JW + 1) * share);  // the wavefront's pieces
+  for (int i0 = wave % JW * share; i0 < stop; i0 += 64) {
+    const int m = min(64, stop - i0);
+    const float2 x = lane < m ? a.ws_ml[slot(i0 + lane)] : make_float2(kNegInf, 0.f);
     const bool counts = !(x.y <= 0.f);
     dead |= x.y < 0.f;
     const float mn = fmaxf(top, wave_max(counts ? x.x : kNegInf));
@@ -960,8 +1057,7 @@ __global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
     sum = sum * alpha + wave_sum(counts ? x.y * w : 0.f);
     acc *= alpha;
     top = mn;
-    const int m = min(64, n - i0);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < m; i += per) {
       // Every lane takes part in the exchange: a lane reads one that is switched off as 0.
       const float wi = __shfl(w, i + at, 64);
@@ -1101,9 +1197,10 @@ hipError_t launch_tiles(const SharedArgs& a, hipStream_t stream) {
   }
   const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)a.wgs), dim3(64 * kSplitWaves), kargs, 0, stream);
   if (e != hipSuccess) return e;
-  // Few rows leave many pieces to each: four wavefronts join them.
+  // Four wavefronts join a row's pieces where there are many: at most so many of either kind.
   const int64_t units = (int64_t)a.B * a.Hq;
-  if (units <= 4 * a.wgs)
+  const int64_t most = 2 + (int64_t)a.wgs * kSplitWaves / ((int64_t)a.B * a.vheads) + (a.s_units ? a.wgs / (a.s_units * a.team) : 0);
+  if (most > 24)
     return hipLaunchKernel((const void*)&paged_shared_join<T, 4>, dim3((unsigned)units), dim3(256), kargs, 0, stream);
   return hipLaunchKernel((const void*)&paged_shared_join<T, 1>, dim3((unsigned)((units + 3) / 4)), dim3(256), kargs, 0, stream);
 }
