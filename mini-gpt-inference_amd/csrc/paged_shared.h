@@ -141,9 +141,10 @@ struct Window {
 };
 
 // The lane's table entry (-1: none, or outside the pool) for its group, whose first
-// token is tok.
-__device__ __forceinline__ int window_entry(const SharedArgs& a, int b, int tok, int end) {
-  if (tok >= end) return -1;
+// token is tok. Entries past a row's length are read too (and not used), so that the
+// load does not wait for the length.
+__device__ __forceinline__ int window_entry(const SharedArgs& a, int b, int tok) {
+  if (tok >= a.M * a.S) return -1;
   const int64_t id = table_entry(a, b, fast_div(tok, a.s_mul, a.s_shift, a.S));
   return id >= 0 && id < a.N ? (int)id : -1;
 }
@@ -152,7 +153,7 @@ __device__ __forceinline__ Window make_window(const SharedArgs& a, int id, int t
   const int64_t at = max(id, 0), off = id < 0 ? 0 : tok - fast_div(tok, a.s_mul, a.s_shift, a.S) * a.S;
   const uint64_t k = (uint64_t)(at * a.k_sn + off * a.k_ss + kvh * a.k_sh) * sizeof(T);
   const uint64_t v = (uint64_t)(at * a.v_sn + off * a.v_ss + kvh * a.v_sh) * sizeof(T);
-  return {(uint32_t)k, (uint32_t)(k >> 32), (uint32_t)v, (uint32_t)(v >> 32), id < 0 ? 0 : min(16, end - tok)};
+  return {(uint32_t)k, (uint32_t)(k >> 32), (uint32_t)v, (uint32_t)(v >> 32), id < 0 ? 0 : max(0, min(16, end - tok))};
 }
 __device__ __forceinline__ int64_t lane_offset(uint32_t lo, uint32_t hi, int i) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)lo, i) |
@@ -370,7 +371,6 @@ template <typename T, int DP, int NQ, bool UNI, bool FULL>
 __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh, int first, int step, int end,
                                              const uint4 (&qf)[NQ][Tile<T, DP>::kKS], State<DP, NQ>& st) {
   using L = Tile<T, DP>;
-  if (first >= end) return;
   const char* kp = (const char*)a.k + (int64_t)kvh * a.k_sh * (int)sizeof(T);
   const char* vp = (const char*)a.v + (int64_t)kvh * a.v_sh * (int)sizeof(T);
   constexpr int kSpan = 64 / L::kGroups;  // tiles of a window
@@ -379,15 +379,16 @@ __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh
   Window win{};
   if constexpr (UNI) {
     tok = first + lane / L::kGroups * step + 16 * (lane % L::kGroups);
-    entry = window_entry(a, b, tok, end);
+    entry = window_entry(a, b, tok);
   }
+  if (first >= end) return;
   L f;
   auto keys = [&](int i) {
     if constexpr (UNI) {
       if (i % kSpan == 0) {
         win = make_window<T>(a, entry, tok, end, kvh);
         tok += kSpan * step;
-        entry = window_entry(a, b, tok, end);
+        entry = window_entry(a, b, tok);
       }
       load_keys<T, DP, FULL>(a, (const char*)a.k, win, i % kSpan * L::kGroups, f);
     } else {
@@ -437,56 +438,6 @@ __device__ __forceinline__ void load_queries(const SharedArgs& a, int kvh, int r
 // key counted; -1 keys counted and every score was -inf.
 __device__ __forceinline__ float coded_sum(float l, bool any) { return l == 0.f && any ? -1.f : l; }
 
-// Joins the states of the workgroup's wavefronts into wavefront 0's: st.mc is then
-// the maximum (log2 units, kNegInf for none) and st.l the coded sum.
-template <int DP, int NQ, int WAVES>
-__device__ __forceinline__ void join_waves(State<DP, NQ>& st, int wave, float (*ml)[2][NQ * 16], f32x4* buf) {
-  const int lane = (int)threadIdx.x & 63, row = lane & 15;
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    st.l[q] = coded_sum(across_groups_sum(st.l[q]), st.any);
-    st.mc[q] = st.m[q] == kNegInf ? kNegInf : st.mc[q];
-    if (lane < 16) {
-      ml[wave][0][16 * q + row] = st.mc[q];
-      ml[wave][1][16 * q + row] = st.l[q];
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    float top = kNegInf, sum = 0.f;
-    bool dead = false;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ml[w][0][16 * q + row]);
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float m = ml[w][0][16 * q + row], l = ml[w][1][16 * q + row];
-      if (l <= 0.f) dead |= l < 0.f;
-      else sum += l * fast_exp2(m - top);
-    }
-    const float mine = st.l[q] <= 0.f ? 0.f : fast_exp2(st.mc[q] - top);
-#pragma unroll
-    for (int t = 0; t < DP / 16; ++t) st.acc[q][t] *= mine;
-    st.mc[q] = top;
-    st.l[q] = sum == 0.f && dead ? -1.f : sum;
-  }
-#pragma unroll
-  for (int q = 0; q < NQ; ++q)
-#pragma unroll
-    for (int half = WAVES / 2; half > 0; half >>= 1) {
-      if (wave >= half && wave < 2 * half) {
-#pragma unroll
-        for (int t = 0; t < DP / 16; ++t) buf[((wave - half) * (DP / 16) + t) * 64 + lane] = st.acc[q][t];
-      }
-      __syncthreads();
-      if (wave < half) {
-#pragma unroll
-        for (int t = 0; t < DP / 16; ++t) st.acc[q][t] += buf[(wave * (DP / 16) + t) * 64 + lane];
-      }
-      __syncthreads();
-    }
-}
-
 // Calls f(d, x) for the runs of kEV consecutive head dims d .. that the lane
 // holds of query tile q.
 template <typename T, int DP, int NQ, typename F>
@@ -503,6 +454,54 @@ __device__ __forceinline__ void each_run(const SharedArgs& a, const State<DP, NQ
       for (int t = 0; t < L::kEV; ++t) x[t] = st.acc[q][L::kEV * h + t][i];
       if (d < a.D) f(d, x);
     }
+}
+
+// Joins the states of the workgroup's wavefronts: each leaves its own in LDS, and after
+// one barrier every thread joins the pieces of some (row, 4 head dims) and calls
+// f(row, d, o, m, l) with the unscaled output, the maximum (log2 units, kNegInf for
+// none) and the coded sum. `rows` of the NQ x 16 are of interest.
+template <int DP, int NQ, int WAVES>
+struct JoinSpace {
+  float acc[WAVES][NQ * 16][DP + 4], m[WAVES][NQ * 16], l[WAVES][NQ * 16];
+};
+template <typename T, int DP, int NQ, int WAVES, typename F>
+__device__ __forceinline__ void join_waves(const SharedArgs& a, const State<DP, NQ>& st, int wave, int rows,
+                                           JoinSpace<DP, NQ, WAVES>& space, F f) {
+  const int lane = (int)threadIdx.x & 63;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int row = 16 * q + (lane & 15);
+    const float l = coded_sum(across_groups_sum(st.l[q]), st.any);
+    if (row >= rows) continue;
+    if (lane < 16) {
+      space.m[wave][row] = st.m[q] == kNegInf ? kNegInf : st.mc[q];
+      space.l[wave][row] = l;
+    }
+    each_run<T>(a, st, q, [&](int d, const float* x) {
+#pragma unroll
+      for (int e = 0; e < Tile<T, DP>::kEV; e += 4) *(f32x4*)&space.acc[wave][row][d + e] = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+    });
+  }
+  __syncthreads();
+  for (int i = (int)threadIdx.x; i < rows * (DP / 4); i += 64 * WAVES) {
+    const int row = i / (DP / 4), d = 4 * (i - row * (DP / 4));
+    if (d >= a.D) continue;
+    float top = kNegInf, sum = 0.f;
+    bool dead = false;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, space.m[w][row]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float l = space.l[w][row];
+      dead |= l < 0.f;
+      const float scale = l <= 0.f ? 0.f : fast_exp2(space.m[w][row] - top);
+      if (l <= 0.f) continue;
+      sum += l * scale;
+      o += scale * *(const f32x4*)&space.acc[w][row][d];
+    }
+    f(row, d, o, top, sum == 0.f && dead ? -1.f : sum);
+  }
 }
 
 // Writes the lane's row of query tile q as the partial of slot `slot`.
@@ -651,7 +650,7 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
     if (u < u0 + n) {
       const OwnTile o = find_own(a, cum, u);
       const int c = ctx[o.b], tok = (c < a.P ? 0 : a.P) + o.tile * L::kKeys + 16 * (lane % L::kGroups), kvh = o.vh / a.gsets;
-      win = make_window<T>(a, window_entry(a, o.b, tok, c), tok, c, kvh);
+      win = make_window<T>(a, window_entry(a, o.b, tok), tok, c, kvh);
       row = o.b;
       head = 2 * o.vh + (o.tile == 0);
     }
@@ -725,7 +724,7 @@ __device__ __forceinline__ int64_t shared_slot(const SharedArgs& a, int kvh, int
 // in LDS do not take: the workgroup's wavefronts take every fourth tile of a piece
 // (a tile of the list is four of theirs) and join in LDS.
 template <typename T, int DP, int NQ, bool UNI, bool FULL>
-__device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int seg, f32x4* buf, float (*ml)[2][NQ * 16]) {
+__device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int seg, JoinSpace<DP, NQ, kSplitWaves>& space) {
   using L = Tile<T, DP>;
   const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int total = a.s_units * a.s_tiles, step = kSplitWaves * L::kKeys;
@@ -742,22 +741,20 @@ __device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int s
     load_queries<T, DP, NQ, FULL>(a, kvh, r0, a.B * a.G, qf);
     st.reset();
     stream_tiles<T, DP, NQ, UNI, FULL>(a, 0, kvh, tile * step + wave * L::kKeys, step, min(a.P, (tile + n) * step), qf, st);
-    join_waves<DP, NQ, kSplitWaves>(st, wave, ml, buf);
-    if (wave == 0) {
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const int64_t slot = shared_slot(a, kvh, r0 + 16 * q + (lane & 15), r0, tile == 0, wg);
-        if (slot >= 0) store_partial<T>(a, st, q, slot, st.mc[q], st.l[q]);
-      }
-    }
+    __syncthreads();  // the joins before are done with the space
+    join_waves<T>(a, st, wave, 16 * NQ, space, [&](int row, int d, f32x4 o, float m, float l) {
+      const int64_t slot = shared_slot(a, kvh, r0 + row, r0, tile == 0, wg);
+      if (slot < 0) return;
+      *(f32x4*)(a.ws_acc + slot * a.D + d) = o;
+      if (d == 0) a.ws_ml[slot] = make_float2(m, l);
+    });
   }
 }
 
 template <typename T, int DP, int NQ, bool UNI, bool FULL>
 __global__ void __launch_bounds__(64 * kSplitWaves, DP > 128 ? 1 : 2) paged_shared_split(const SharedArgs a) {
-  constexpr int kBuf = kSplitWaves / 2 * (DP / 16) * 64 * 16, kCum = kSharedMaxB * 8;
-  __shared__ __align__(16) char lds[kBuf > kCum ? kBuf : kCum];
-  __shared__ float ml[kSplitWaves][2][NQ * 16];
+  using Space = JoinSpace<DP, NQ, kSplitWaves>;
+  __shared__ __align__(16) char lds[sizeof(Space) > kSharedMaxB * 8 ? sizeof(Space) : kSharedMaxB * 8];
   __shared__ int part[kSplitWaves];
   int *cum = (int*)lds, *ctx = cum + kSharedMaxB;
   const int total = scan_own<Tile<T, DP>::kKeys>(a, cum, ctx, part) * a.vheads;
@@ -765,7 +762,7 @@ __global__ void __launch_bounds__(64 * kSplitWaves, DP > 128 ? 1 : 2) paged_shar
   if (blockIdx.x == 0 && threadIdx.x == 0) a.ws_split[0] = sp.seg_shared, a.ws_split[1] = sp.seg_own;
   const Place at = make_place(a, sp);
   if (at.shared) {
-    attend_shared<T, DP, NQ, UNI, FULL>(a, at.index, sp.seg_shared, (f32x4*)lds, ml);
+    attend_shared<T, DP, NQ, UNI, FULL>(a, at.index, sp.seg_shared, *(Space*)lds);
   } else {
     const int w = at.index * kSplitWaves + uniform((int)threadIdx.x >> 6);
     if constexpr (UNI) attend_own<T, DP, FULL>(a, w, sp.seg_own, total, cum, ctx);
@@ -803,6 +800,7 @@ __device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char*
       kv[kb & 1][f] = *(const uint4*)(kl + (kr + 32 * (kb >> 1) + 4 * (kb & 1)) * kRowB + (((4 * f + g) ^ k_swz<kCPR>(kr)) << 4));
   };
   read(0);
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int kb = 0; kb < 4; ++kb) {
     if (kb < 3) read(kb + 1);
@@ -814,6 +812,19 @@ __device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char*
       for (int q = 0; q < QB; ++q) s[q][kb] = mfma16<T>(kv[kb & 1][f], qf[q][f], s[q][kb]);
     __builtin_amdgcn_sched_barrier(0);
   }
+  __builtin_amdgcn_s_setprio(0);
+  // The first half of V^T is read under the softmax, the second as the first's products
+  // let go of its registers.
+  const int vrow = 8 * g + (col >> 2), vq = lane & 3;
+  uint4 vv[DP / 16];
+  auto value = [&](int h, int t) {
+    const uint32_t at = vl + vrow * kRowB + ((vq & 1) << 3) + (((2 * t + (vq >> 1)) ^ v_swz<kCPR>(vrow)) << 4) + 32 * h * kRowB;
+    const uint2 lo = TrRead<T>::at(at), hi = TrRead<T>::at(at + 4 * kRowB);
+    vv[t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
+#pragma unroll
+  for (int t = 0; t < DP / 16; ++t) value(0, t);
+  __builtin_amdgcn_sched_barrier(0);
   if (counts != 0x10101010u) {
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
@@ -854,24 +865,20 @@ __device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char*
   }
   const uint32_t one2 = pack2<T>(1.f, 1.f);
   const uint4 ones = make_uint4(one2, one2, one2, one2);
-  const int vrow = 8 * g + (col >> 2), vq = lane & 3;
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint4 vv[DP / 16];
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
-      const uint32_t at = vl + vrow * kRowB + ((vq & 1) << 3) + (((2 * t + (vq >> 1)) ^ v_swz<kCPR>(vrow)) << 4) + 32 * h * kRowB;
-      const uint2 lo = TrRead<T>::at(at), hi = TrRead<T>::at(at + 4 * kRowB);
-      vv[t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-    }
-#pragma unroll
-    for (int t = 0; t < DP / 16; ++t)
 #pragma unroll
       for (int q = 0; q < QB; ++q) st.acc[q][t] = mfma16<T>(vv[t], pf[q][h], st.acc[q][t]);
+      if (h == 0) value(1, t);
+    }
 #pragma unroll
     for (int q = 0; q < QB; ++q) st.sum[q] = mfma16<T>(ones, pf[q][h], st.sum[q]);
     __builtin_amdgcn_sched_barrier(0);
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 
 template <typename T, int DP, int QB>
@@ -882,16 +889,16 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
   const int team = wg / a.team, member = wg - team * a.team;
   if ((int64_t)team * seg >= total) return;
   const int stop = min(total, team * seg + seg);
-  // The lane's part of the wavefront's copies: rows and chunks as the swizzles place them.
+  // The lane's part of the wavefront's copies: row c * kRPC + lane / kCPR of its 16, and
+  // the chunk of it that the swizzles place there.
+  auto copy_row = [&](int c, int l) { return c * kRPC + l / kCPR; };
+  auto k_chunk = [&](int c, int l) { return (l % kCPR) ^ k_swz<kCPR>(16 * wave + copy_row(c, l)); };
+  auto v_chunk = [&](int c, int l) { return (l % kCPR) ^ v_swz<kCPR>(16 * wave + copy_row(c, l)); };
   uint32_t ko[kCopies], vo[kCopies];
-  int row[kCopies], kc[kCopies], vc[kCopies];
 #pragma unroll
   for (int c = 0; c < kCopies; ++c) {
-    row[c] = c * kRPC + lane / kCPR;
-    kc[c] = (lane % kCPR) ^ k_swz<kCPR>(16 * wave + row[c]);
-    vc[c] = (lane % kCPR) ^ v_swz<kCPR>(16 * wave + row[c]);
-    ko[c] = (uint32_t)row[c] * (uint32_t)a.k_ss * 2 + (uint32_t)kc[c] * 16;
-    vo[c] = (uint32_t)row[c] * (uint32_t)a.v_ss * 2 + (uint32_t)vc[c] * 16;
+    ko[c] = (uint32_t)copy_row(c, lane) * (uint32_t)a.k_ss * 2 + (uint32_t)k_chunk(c, lane) * 16;
+    vo[c] = (uint32_t)copy_row(c, lane) * (uint32_t)a.v_ss * 2 + (uint32_t)v_chunk(c, lane) * 16;
   }
   const uint32_t dst0 = lds_addr(lds) + (uint32_t)wave * 16 * kRowB;
   const bool all_dims = a.D == DP;
@@ -907,7 +914,7 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
     int tok = (tile0 + lane) * 64, entry[4];
     auto look = [&]() {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) entry[j] = window_entry(a, 0, tok + 16 * j, a.P);
+      for (int j = 0; j < 4; ++j) entry[j] = window_entry(a, 0, tok + 16 * j);
     };
     Window win{};
     uint32_t counts = 0;
@@ -916,7 +923,7 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
       if (i % 64 == 0) {
         counts = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) counts |= (uint32_t)(entry[j] < 0 ? 0 : min(16, a.P - tok - 16 * j)) << (8 * j);
+        for (int j = 0; j < 4; ++j) counts |= (uint32_t)(entry[j] < 0 ? 0 : max(0, min(16, a.P - tok - 16 * j))) << (8 * j);
         const int e = wave == 0 ? entry[0] : wave == 1 ? entry[1] : wave == 2 ? entry[2] : entry[3];
         win = make_window<T>(a, e, tok + 16 * wave, a.P, kvh);
         tok += 64 * 64;
@@ -935,10 +942,14 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
         }
       } else {  // what does not count is zeros
         const int m = (int)(next >> (8 * wave)) & 255;
+        int l = lane;
+        asm volatile("" : "+v"(l));  // keeps this rare path's rows and chunks out of the loop's registers
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) {
-          const void* ks = row[c] < m && kc[c] * 8 < a.D ? (const void*)(kb + ko[c]) : (const void*)(kZeroRow + kc[c] * 16);
-          const void* vs = row[c] < m && vc[c] * 8 < a.D ? (const void*)(vb + vo[c]) : (const void*)(kZeroRow + vc[c] * 16);
+          const int kc = k_chunk(c, l), vc = v_chunk(c, l);
+          const bool ok = copy_row(c, l) < m;
+          const void* ks = ok && kc * 8 < a.D ? (const void*)(kb + ko[c]) : (const void*)(kZeroRow + kc * 16);
+          const void* vs = ok && vc * 8 < a.D ? (const void*)(vb + vo[c]) : (const void*)(kZeroRow + vc * 16);
           copy16_to_lds(ks, kd + 1024 * c);
           copy16_to_lds(vs, vd + 1024 * c);
         }
@@ -1110,24 +1121,19 @@ constexpr int kOneWaves = DP > 128 ? 4 : 8;
 template <typename T, int DP, bool UNI, bool FULL>
 __global__ void __launch_bounds__(64 * kOneWaves<DP>) paged_shared_one(const SharedArgs a) {
   using L = Tile<T, DP>;
-  __shared__ f32x4 buf[kOneWaves<DP> / 2 * (DP / 16) * 64];
-  __shared__ float ml[kOneWaves<DP>][2][16];
-  const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  __shared__ __align__(16) JoinSpace<DP, 1, kOneWaves<DP>> space;
+  const int wave = uniform((int)threadIdx.x >> 6);
   const int b = (int)blockIdx.y, vh = (int)blockIdx.x, kvh = vh / a.gsets, g0 = (vh - kvh * a.gsets) * 16;
-  const int end = clamped_ctx(a, b);
   uint4 qf[1][L::kKS];
   State<DP, 1> st;
   load_queries<T, DP, 1, FULL>(a, kvh, b * a.G + g0, (b + 1) * a.G, qf);
   st.reset();
-  stream_tiles<T, DP, 1, UNI, FULL>(a, b, kvh, wave * L::kKeys, kOneWaves<DP> * L::kKeys, end, qf, st);
-  join_waves<DP, 1, kOneWaves<DP>>(st, wave, ml, buf);
-  const int g = g0 + (lane & 15);
-  if (wave || g >= a.G) return;
-  const float r = st.l[0] == 0.f ? 0.f : st.l[0] < 0.f ? __builtin_nanf("") : 1.f / st.l[0];
-  T* o = (T*)a.out + (int64_t)b * a.o_sb + (int64_t)(kvh * a.G + g) * a.o_sh;
-  each_run<T>(a, st, 0, [&](int d, const float* x) {
-#pragma unroll
-    for (int e = 0; e < L::kEV; ++e) Elem<T>::store(o + d + e, x[e] * r);
+  stream_tiles<T, DP, 1, UNI, FULL>(a, b, kvh, wave * L::kKeys, kOneWaves<DP> * L::kKeys, clamped_ctx(a, b), qf, st);
+  join_waves<T>(a, st, wave, min(16, a.G - g0), space, [&](int row, int d, f32x4 o, float, float l) {
+    const f32x4 x = o * (l == 0.f ? 0.f : l < 0.f ? __builtin_nanf("") : 1.f / l);
+    T* p = (T*)a.out + (int64_t)b * a.o_sb + (int64_t)(kvh * a.G + g0 + row) * a.o_sh + d;
+    if constexpr (sizeof(T) == 4) *(f32x4*)p = x;
+    else *(uint2*)p = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
   });
 }
 
