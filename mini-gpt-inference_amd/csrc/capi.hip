@@ -722,7 +722,7 @@ int rope_args(const RopeSpec& r, mgi::RopeArgs* a) {
   if (!std::isfinite(r.eps) || r.eps < 0.f) return fail(MGI_EINVAL, "eps must be finite and non-negative");
   if (r.D > 512) return fail(MGI_EUNSUPPORTED, "head_dim larger than 512");
   // One launch's threads, 64 to a head row at most, are counted in 32 bits.
-  if (r.Hq > kMaxGridYZ || r.Hk > kMaxGridYZ || r.T >= (int64_t(1) << 24) || r.T * (r.Hq + 2 * r.Hk) >= (int64_t(1) << 26))
+  if (r.Hq > kMaxGridYZ || r.Hk > kMaxGridYZ || r.T >= (int64_t(1) << 24) || r.T * (r.Hq + 2 * r.Hk) >= (int64_t(1) << 25))
     return fail(MGI_EUNSUPPORTED, "rows x heads too large for one launch");
   a->q = r.q;
   a->q_st = r.qs[0], a->q_sh = r.qs[1], a->q_sd = r.qs[2];
@@ -769,7 +769,7 @@ int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
   a.chunk = 0;
   for (int c : {8, 4}) {
     if (c * eb > 16 || !unit || (a.R / 2) % c || (a.D - a.R) % (2 * c)) continue;
-    if (fits(c * eb, {a.q, a.k, a.v}, {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh}, eb) &&
+    if (fits(c * (a.w_f32 ? 4 : eb), {a.qw, a.kw}, {}, 1) && fits(c * eb, {a.q, a.k, a.v}, {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh}, eb) &&
         fits(c * ob, {a.q_out, a.k_out, a.v_out},
              {a.qo_st, a.qo_sh, a.ko_sn, a.ko_st, a.ko_sh, a.vo_sn, a.vo_st, a.vo_sh}, ob)) {
       a.chunk = c;

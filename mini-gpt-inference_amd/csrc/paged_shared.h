@@ -160,10 +160,18 @@ __device__ __forceinline__ int64_t lane_offset(uint32_t lo, uint32_t hi, int i) 
                    ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, i) << 32));
 }
 
+// 16 or 8 bytes.
+template <bool NT, typename V>
+__device__ __forceinline__ V load_piece(const char* p) {
+  if constexpr (!NT) return *(const V*)p;
+  typedef uint32_t u4 __attribute__((ext_vector_type(sizeof(V) / 4)));
+  return __builtin_bit_cast(V, __builtin_nontemporal_load((const u4*)p));
+}
+
 // Loads the keys, and the values, of the tile whose groups are lanes at .. of the
 // window (kp, vp: the pools). Rows past a group's last key read that one again.
 // FULL: D == DP.
-template <typename T, int DP, bool FULL>
+template <typename T, int DP, bool FULL, bool NT = false>
 __device__ __forceinline__ void load_keys(const SharedArgs& a, const char* kp, const Window& w, int at, Tile<T, DP>& f) {
   using L = Tile<T, DP>;
   const int lane = (int)threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
@@ -175,10 +183,10 @@ __device__ __forceinline__ void load_keys(const SharedArgs& a, const char* kp, c
     const uint32_t off = (uint32_t)min(row, max(n, 1) - 1) * ss + (uint32_t)kg * 16;
 #pragma unroll
     for (int s = 0; s < L::kKS; ++s)
-      f.k[g][s] = FULL || (kg + 4 * s) * L::kCE < a.D ? *(const uint4*)(base + off + 64 * s) : make_uint4(0, 0, 0, 0);
+      f.k[g][s] = FULL || (kg + 4 * s) * L::kCE < a.D ? load_piece<NT, uint4>(base + off + 64 * s) : make_uint4(0, 0, 0, 0);
   }
 }
-template <typename T, int DP, bool FULL>
+template <typename T, int DP, bool FULL, bool NT = false>
 __device__ __forceinline__ void load_values(const SharedArgs& a, const char* vp, const Window& w, int at, Tile<T, DP>& f) {
   using L = Tile<T, DP>;
   using V = typename L::VVec;
@@ -196,7 +204,7 @@ __device__ __forceinline__ void load_values(const SharedArgs& a, const char* vp,
       const uint32_t off = (uint32_t)min(4 * kg + j, max(n, 1) - 1) * ss + col;
 #pragma unroll
       for (int h = 0; h < L::kHF; ++h)
-        f.v[4 * g + j][h] = FULL || 16 * L::kEV * h + row * L::kEV < a.D ? *(const V*)(base + off + 16 * L::kEV * (int)sizeof(T) * h) : V{};
+        f.v[4 * g + j][h] = FULL || 16 * L::kEV * h + row * L::kEV < a.D ? load_piece<NT, V>(base + off + 16 * L::kEV * (int)sizeof(T) * h) : V{};
     }
   }
 }
@@ -636,7 +644,7 @@ __device__ __forceinline__ void load_own_queries(const SharedArgs& a, int b, int
 // loads (length, table, queries, keys), only its partial. With a loop over runs
 // instead each cost about 4 us: 13 x 16 heads, 14.9 us where a wavefront had one
 // tile and 19.0 where it had two.
-template <typename T, int DP, bool FULL>
+template <typename T, int DP, bool FULL, bool NT>
 __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum, const int* ctx) {
   using L = Tile<T, DP>;
   constexpr int kSpan = 64 / L::kGroups;
@@ -664,8 +672,8 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
   fill(0);
   int b = __builtin_amdgcn_readlane(row, 0), h = __builtin_amdgcn_readlane(head, 0);
   load_own_queries<T, DP, FULL>(a, b, h >> 1, qf);
-  load_keys<T, DP, FULL>(a, kp, win, 0, f);
-  load_values<T, DP, FULL>(a, vp, win, 0, f);
+  load_keys<T, DP, FULL, NT>(a, kp, win, 0, f);
+  load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
   st.reset();
   for (int t = 0; t < n; ++t) {
     score_tile<T, DP, 1>(f, qf, s);
@@ -676,12 +684,12 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
       if (at == 0) fill(t + 1);
       nb = __builtin_amdgcn_readlane(row, at);
       nh = __builtin_amdgcn_readlane(head, at);
-      load_keys<T, DP, FULL>(a, kp, win, at, f);
+      load_keys<T, DP, FULL, NT>(a, kp, win, at, f);
     }
     const bool ends = !more || nb != b || (nh >> 1) != (h >> 1);
     if (more && ends) load_own_queries<T, DP, FULL>(a, nb, nh >> 1, qf);
     attend_tile<T, DP, 1, true>(a, f, s, st);
-    if (more) load_values<T, DP, FULL>(a, vp, win, at, f);
+    if (more) load_values<T, DP, FULL, NT>(a, vp, win, at, f);
     if (ends) {
       store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
       st.reset();
@@ -689,6 +697,18 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
       h = nh;
     }
   }
+}
+
+// Own keys and values are read once a call: past what the 256 MB memory-side cache
+// may still hold of them they are loaded as non-temporal (64 x 32 heads, 582 MB of
+// own tokens: 133 us without, 115 with; 64 x 1, 50 MB, called again and again: 31.5
+// and 34.3).
+template <typename T, int DP, bool FULL>
+__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum, const int* ctx) {
+  if ((int64_t)total * Tile<T, DP>::kKeys * 2 * a.D * (int)sizeof(T) > (int64_t)192 << 20)
+    attend_own<T, DP, FULL, true>(a, wave_index, seg, total, cum, ctx);
+  else
+    attend_own<T, DP, FULL, false>(a, wave_index, seg, total, cum, ctx);
 }
 
 // The same for any S, a run at a time.

@@ -12,9 +12,12 @@
 // Bound by memory on long calls and by one launch on short ones, so nothing is
 // staged: a lane holds two chunks of a head row that a rotation needs together
 // (dims C p .. C p + C-1 and the same plus R/2), loads them with one instruction
-// each and shares only the sum of squares, over the lanes of the head (DPP).
-// A workgroup takes one row t and walks its heads (queries, keys, values), so
-// the row's cosines and sines are read once per workgroup and kept.
+// each and shares only the sum of squares, over the lanes of the head. Everything
+// but the angles loads at once, the angles once the position is there. One head row
+// to a lane: 8192 rows of 32 + 8 bf16 heads of 128 take 35.4 us, 4.9 TB/s, what a
+// large copy reaches; two rows 36.2, four 45.6 (more registers, fewer wavefronts),
+// and a workgroup per row walking its heads 62. 13 rows appended take 3.1 us replayed
+// from a graph (5.4 with the host's call).
 #include <type_traits>
 
 #include "mgi_common.h"
@@ -25,37 +28,8 @@ namespace mgi {
 
 constexpr int kRopeThreads = 256;
 
-// N consecutive elements as f32, and back with one rounding each. Pointers are
-// aligned to the chunk's bytes, 16 at most.
-template <int N>
-__device__ __forceinline__ void load_chunk(const float* p, float (&x)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p + i);
-    x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
-  }
-}
-template <int N, typename T>
-__device__ __forceinline__ void load_chunk(const T* p, float (&x)[N]) {
-  uint32_t w[N / 2];
-  if constexpr (N == 8) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1] = v.y;
-  }
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
-    if constexpr (std::is_same_v<T, bf16_t>) {
-      x[2 * i] = bf16_lo(w[i]);
-      x[2 * i + 1] = bf16_hi(w[i]);
-    } else {
-      x[2 * i] = f16_to_f32((uint16_t)(w[i] & 0xffffu));
-      x[2 * i + 1] = f16_to_f32((uint16_t)(w[i] >> 16));
-    }
-  }
-}
+// N consecutive elements from f32, with one rounding each. Pointers are aligned to the
+// chunk's bytes, 16 at most.
 template <int N>
 __device__ __forceinline__ void store_chunk(float* p, const float (&x)[N]) {
 #pragma unroll
@@ -74,11 +48,12 @@ __device__ __forceinline__ void store_chunk(T* p, const float (&x)[N]) {
   if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
-// N elements moved as they are.
-template <int N, typename T>
-__device__ __forceinline__ void copy_chunk(const T* s, T* d) {
-  if constexpr (N * sizeof(T) == 16) *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(s);
-  else *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(s);
+// Element i of an int32 or int64 array without a branch (whose end would wait for the
+// load): both words of an int64, the same word twice of an int32.
+__device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
+  const char* at = (const char*)p + i * (is64 ? 8 : 4);
+  const uint32_t lo = *(const uint32_t*)at, hi = *(const uint32_t*)(at + (is64 ? 4 : 0));
+  return is64 ? (int64_t)((uint64_t)lo | ((uint64_t)hi << 32)) : (int64_t)(int32_t)lo;
 }
 
 // Where row t's key and value go: the pool's slot, or row t of k_out (no v).
@@ -88,7 +63,7 @@ __device__ __forceinline__ bool rope_target(const RopeArgs& a, int64_t t, bool p
     *k_off = t * a.ko_st;
     return true;
   }
-  const int64_t slot = load_index(a.slots, a.sl_i64, t * a.sl_s);
+  const int64_t slot = index_at(a.slots, a.sl_i64, t * a.sl_s);
   if (!placed || slot < 0 || slot >= a.N * (int64_t)a.S) return false;
   const int64_t blk = slot / a.S, off = slot - blk * a.S;
   *k_off = blk * a.ko_sn + off * a.ko_st;
@@ -101,119 +76,146 @@ __device__ __forceinline__ float weight_at(const void* w, int f32, int dtype, in
   return dtype == MGI_BF16 ? bf16_to_f32(((const uint16_t*)w)[i]) : f16_to_f32(((const uint16_t*)w)[i]);
 }
 
+// A chunk as loaded, and as f32.
+template <typename T, int C>
+struct Raw {
+  uint32_t w[C * (int)sizeof(T) / 4];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (sizeof(w) == 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (sizeof(w) == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else if constexpr (std::is_same_v<T, bf16_t>) return i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
+    else return f16_to_f32((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+  }
+};
+
 // TI: q, k, v; TO: q_out and the keys' and values' target. C: elements per chunk.
 template <typename TI, typename TO, int C, bool INTER>
 __global__ void __launch_bounds__(kRopeThreads) rope_vec(const RopeArgs a) {
-  const int64_t t = blockIdx.x;
-  const int gp = 1 << a.gp_shift;                     // lanes per head row
-  const int sub = (int)threadIdx.x & (gp - 1);
-  const int heads = a.Hq + a.Hk + a.Hv;
-  const int step = ((int)blockDim.x >> a.gp_shift) * (int)gridDim.y;
-  int h = (int)blockIdx.y * ((int)blockDim.x >> a.gp_shift) + ((int)threadIdx.x >> a.gp_shift);
+  const int gp = 1 << a.gp_shift;  // lanes per head row
+  const int sub = (int)threadIdx.x & (gp - 1), slots = (int)blockDim.x >> a.gp_shift;
+  const int heads = a.Hq + a.Hk + a.Hv, total = a.T * heads;
   // The lane's two chunks: R / 2 apart inside the rotated dims, half of the
   // others apart past them.
   const int half = a.R >> 1, rot = half / C, rest = (a.D - a.R) >> 1;
   const bool live = sub < a.D / (2 * C), turns = sub < rot;
   const int d0 = turns ? sub * C : a.R + (sub - rot) * C, d1 = d0 + (turns ? half : rest);
 
-  const int64_t pos = load_index(a.positions, a.pos_i64, t * a.pos_s);
-  const bool placed = pos >= 0 && pos < a.P;
-  // Half-split: pairs (d0 + i, d1 + i) with cs[i]. Interleaved: pair i of the
-  // first chunk with cs[i], of the second with cs[C/2 + i].
-  float cs[C], sn[C], wq[2][C], wk[2][C];
-  const float nan = __builtin_nanf("");
-#pragma unroll
-  for (int i = 0; i < C; ++i) cs[i] = turns && !placed ? nan : 1.f, sn[i] = turns && !placed ? nan : 0.f;
-  if (turns && placed) {
-    const float* row = a.table + pos * a.table_s;
-    if constexpr (INTER) {
-      float lo[C / 2], hi[C / 2];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int i = 0; i < C / 2; ++i) lo[i] = row[(s ? d1 : d0) / 2 + i], hi[i] = row[half + (s ? d1 : d0) / 2 + i];
-#pragma unroll
-        for (int i = 0; i < C / 2; ++i) cs[s * C / 2 + i] = lo[i], sn[s * C / 2 + i] = hi[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) cs[i] = row[d0 + i], sn[i] = row[half + d0 + i];
-    }
-  }
-  if (a.qw && live) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        wq[s][i] = weight_at(a.qw, a.w_f32, a.dtype, (s ? d1 : d0) + i);
-        wk[s][i] = weight_at(a.kw, a.w_f32, a.dtype, (s ? d1 : d0) + i);
-      }
-  }
-  int64_t k_off = 0, v_off = 0;
-  const bool keeps = rope_target(a, t, placed, &k_off, &v_off);
-
-  for (; h < heads; h += step) {
-    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hk;
-    const int hh = is_q ? h : is_v ? h - a.Hq - a.Hk : h - a.Hq;
-    if (!live && !(a.qw && !is_v)) continue;  // an empty lane only helps its head's sum
+  const int64_t item = (int64_t)blockIdx.x * slots + ((int)threadIdx.x >> a.gp_shift);
+  const bool in = item < total;
+  const int t = in ? (int)((uint32_t)item / (uint32_t)heads) : 0, h = in ? (int)item - t * heads : 0;
+  const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hk;
+  const int hh = is_q ? h : is_v ? h - a.Hq - a.Hk : h - a.Hq;
+  const bool mine = in && live;
+  const int64_t pos = index_at(a.positions, a.pos_i64, t * a.pos_s);
+  Raw<TI, C> x[2];
+  if (mine) {
     const TI* src = is_q   ? (const TI*)a.q + t * a.q_st + (int64_t)hh * a.q_sh
                     : is_v ? (const TI*)a.v + t * a.v_st + (int64_t)hh * a.v_sh
                            : (const TI*)a.k + t * a.k_st + (int64_t)hh * a.k_sh;
-    TO* dst = is_q   ? (TO*)a.q_out + t * a.qo_st + (int64_t)hh * a.qo_sh
-              : is_v ? (TO*)a.v_out + v_off + (int64_t)hh * a.vo_sh
-                     : (TO*)a.k_out + k_off + (int64_t)hh * a.ko_sh;
-    if constexpr (std::is_same_v<TI, TO>) {
-      if (is_v) {  // a copy, bit for bit
-        if (keeps) copy_chunk<C>(src + d0, dst + d0), copy_chunk<C>(src + d1, dst + d1);
-        continue;
+    x[0].load(src + d0);
+    x[1].load(src + d1);
+  }
+  float w[2][C];  // the norm's weights
+  if (a.qw && mine && !is_v) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const void* p = is_q ? a.qw : a.kw;
+      const int d = s ? d1 : d0;
+      if (a.w_f32) {
+        Raw<float, 4> r[C / 4];
+#pragma unroll
+        for (int i = 0; i < C / 4; ++i) r[i].load((const float*)p + d + 4 * i);
+#pragma unroll
+        for (int i = 0; i < C; ++i) w[s][i] = r[i / 4][i % 4];
+      } else if constexpr (sizeof(TI) == 2) {
+        Raw<TI, C> r;
+        r.load((const TI*)p + d);
+#pragma unroll
+        for (int i = 0; i < C; ++i) w[s][i] = r[i];
       }
     }
-    float x[2][C];
-    if (live) {
-      load_chunk(src + d0, x[0]);
-      load_chunk(src + d1, x[1]);
+  }
+  const bool placed = pos >= 0 && pos < a.P;
+  int64_t k_off = 0, v_off = 0;
+  const bool keeps = is_q || (in && rope_target(a, t, placed, &k_off, &v_off));
+  TO* dst = is_q   ? (TO*)a.q_out + t * a.qo_st + (int64_t)hh * a.qo_sh
+            : is_v ? (TO*)a.v_out + v_off + (int64_t)hh * a.vo_sh
+                   : (TO*)a.k_out + k_off + (int64_t)hh * a.ko_sh;
+  float y[2][C];
+  if (is_v) {
+    if (!mine || !keeps) return;
+    if constexpr (std::is_same_v<TI, TO>) {  // a copy, bit for bit
+      x[0].store(dst + d0);
+      x[1].store(dst + d1);
+      return;
     }
-    if (a.qw && !is_v) {
-      float ss = 0.f;
-      if (live) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) ss = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], ss));
+    for (int i = 0; i < C; ++i) y[0][i] = x[0][i], y[1][i] = x[1][i];
+  } else {
+    // Half-split: pairs (d0 + i, d1 + i) with cs[i]. Interleaved: pair i of the
+    // first chunk with cs[i], of the second with cs[C/2 + i].
+    float z[2][C], cs[C], sn[C];
+    const float none = __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < C; ++i) z[0][i] = x[0][i], z[1][i] = x[1][i], cs[i] = sn[i] = none;
+    if (mine && turns && placed) {
+      const float* line = a.table + pos * a.table_s;
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const int p = INTER ? (i < C / 2 ? d0 / 2 + i : d1 / 2 + i - C / 2) : d0 + i;
+        cs[i] = line[p], sn[i] = line[half + p];
+      }
+    }
+    if (a.qw) {  // lanes without chunks only pass the others' sums on
+      float ss = 0.f;
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) ss = fmaf(z[0][i], z[0][i], fmaf(z[1][i], z[1][i], ss));
       }
       for (int m = gp >> 1; m > 0; m >>= 1) ss += __shfl_xor(ss, m, 64);
       const float r = 1.0f / sqrtf(ss * a.inv_d + a.eps);
+      if (mine) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int i = 0; i < C; ++i) x[s][i] = x[s][i] * r * (is_q ? wq[s][i] : wk[s][i]);
+          for (int i = 0; i < C; ++i) z[s][i] = z[s][i] * r * w[s][i];
+      }
     }
-    if (!live || (!is_q && !keeps)) continue;
-    float y[2][C];
-    if (is_v) {
+    if (!mine || !keeps) return;
+    if (!turns) {  // past the rotated dims: as it is (an infinity times 0 is no 0)
 #pragma unroll
-      for (int i = 0; i < C; ++i) y[0][i] = x[0][i], y[1][i] = x[1][i];
+      for (int i = 0; i < C; ++i) y[0][i] = z[0][i], y[1][i] = z[1][i];
     } else if constexpr (INTER) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int i = 0; i < C / 2; ++i) {
-          const float c = cs[s * C / 2 + i], n = sn[s * C / 2 + i], u = x[s][2 * i], w = x[s][2 * i + 1];
-          y[s][2 * i] = u * c - w * n;
-          y[s][2 * i + 1] = w * c + u * n;
+          const float c = cs[s * C / 2 + i], n = sn[s * C / 2 + i], p = z[s][2 * i], q = z[s][2 * i + 1];
+          y[s][2 * i] = p * c - q * n;
+          y[s][2 * i + 1] = q * c + p * n;
         }
     } else {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        y[0][i] = x[0][i] * cs[i] - x[1][i] * sn[i];
-        y[1][i] = x[1][i] * cs[i] + x[0][i] * sn[i];
+        y[0][i] = z[0][i] * cs[i] - z[1][i] * sn[i];
+        y[1][i] = z[1][i] * cs[i] + z[0][i] * sn[i];
       }
     }
-    if (!is_v && !turns) {  // past the rotated dims: x itself (an infinity times 0 is no 0)
-#pragma unroll
-      for (int i = 0; i < C; ++i) y[0][i] = x[0][i], y[1][i] = x[1][i];
-    }
-    store_chunk(dst + d0, y[0]);
-    store_chunk(dst + d1, y[1]);
   }
+  store_chunk(dst + d0, y[0]);
+  store_chunk(dst + d1, y[1]);
 }
 
 // Any strides and any even R: one wavefront per head row, lanes over the dims.
@@ -279,9 +281,8 @@ namespace {
 template <typename TI, typename TO>
 const void* rope_kernel(int chunk, int interleaved) {
   if (chunk == 0) return (const void*)&rope_any<TI, TO>;
-  if constexpr (sizeof(TI) == 2) {
+  if constexpr (sizeof(TI) == 2)
     if (chunk == 8) return interleaved ? (const void*)&rope_vec<TI, TO, 8, true> : (const void*)&rope_vec<TI, TO, 8, false>;
-  }
   return interleaved ? (const void*)&rope_vec<TI, TO, 4, true> : (const void*)&rope_vec<TI, TO, 4, false>;
 }
 
@@ -289,32 +290,30 @@ const void* rope_kernel(int chunk, int interleaved) {
 
 hipError_t launch_rope(const RopeArgs& args, int in_dtype, int out_dtype, hipStream_t stream) {
   RopeArgs a = args;
-  const int heads = a.Hq + a.Hk + a.Hv;
   const int c = a.chunk;
+  const int64_t total = (int64_t)a.T * (a.Hq + a.Hk + a.Hv);
+  if (c)
+    while ((1 << a.gp_shift) < a.D / (2 * c)) ++a.gp_shift;
+  // A wavefront to a workgroup where there are fewer than four per CU.
+  const int threads = (total << a.gp_shift) < 4 * 64 * (int64_t)a.cus ? 64 : kRopeThreads;
   const void* fn = nullptr;
   if (in_dtype == out_dtype)
     fn = in_dtype == MGI_F32    ? rope_kernel<float, float>(c, a.interleaved)
          : in_dtype == MGI_BF16 ? rope_kernel<bf16_t, bf16_t>(c, a.interleaved)
                                 : rope_kernel<f16_t, f16_t>(c, a.interleaved);
   else if (in_dtype == MGI_F32)
-    fn = out_dtype == MGI_BF16 ? rope_kernel<float, bf16_t>(c, a.interleaved) : rope_kernel<float, f16_t>(c, a.interleaved);
+    fn = out_dtype == MGI_BF16 ? rope_kernel<float, bf16_t>(c, a.interleaved)
+                               : rope_kernel<float, f16_t>(c, a.interleaved);
   else if (out_dtype == MGI_F32)
-    fn = in_dtype == MGI_BF16 ? rope_kernel<bf16_t, float>(c, a.interleaved) : rope_kernel<f16_t, float>(c, a.interleaved);
+    fn = in_dtype == MGI_BF16 ? rope_kernel<bf16_t, float>(c, a.interleaved)
+                              : rope_kernel<f16_t, float>(c, a.interleaved);
   else
     return hipErrorInvalidValue;
   void* kargs[] = {&a};
-  if (c == 0) {
-    const int64_t units = (int64_t)a.T * heads;
-    return hipLaunchKernel(fn, dim3((unsigned)((units + 3) / 4)), dim3(kRopeThreads), kargs, 0, stream);
-  }
-  while ((1 << a.gp_shift) < a.D / (2 * c)) ++a.gp_shift;
-  // A workgroup per row, as wide as its heads' lanes need, up to four wavefronts.
-  const int lanes = heads << a.gp_shift, threads = lanes >= kRopeThreads ? kRopeThreads : (lanes + 63) / 64 * 64;
-  // Rows too few to fill the CUs split their heads over workgroups.
-  const int per = threads >> a.gp_shift;
-  int split = 1;
-  if ((int64_t)a.T < 2 * a.cus) split = (heads + per - 1) / per;
-  return hipLaunchKernel(fn, dim3((unsigned)a.T, (unsigned)split), dim3(threads), kargs, 0, stream);
+  if (c == 0)
+    return hipLaunchKernel(fn, dim3((unsigned)((total + 3) / 4)), dim3(kRopeThreads), kargs, 0, stream);
+  const int64_t per = threads >> a.gp_shift;
+  return hipLaunchKernel(fn, dim3((unsigned)((total + per - 1) / per)), dim3(threads), kargs, 0, stream);
 }
 
 }  // namespace mgi
