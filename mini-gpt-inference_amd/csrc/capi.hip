@@ -783,18 +783,52 @@ int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
 
 // How mgi_paged_decode_shared runs a call of these sizes on the matrix-core kernels.
 struct SharedPlan {
-  int one_launch, gsets, vheads, wgs, lds_tiles, row_tiles, set_rows, team, set_blocks, s_units, s_tiles, s_cost, s_min, own_min;
+  int one_launch, gsets, vheads, wgs, lds_tiles, row_tiles, set_rows, team, set_blocks, s_units, s_tiles, s_cost, s_piece;
   int64_t s_cont, own_slot, own_cont, slots;
   size_t ml_offset, cum_offset, total;
 };
 
+// Whether one workgroup per (row, virtual head), each reading the shared tokens by
+// itself, is estimated faster than the split over all workgroups and its joining
+// launch. Only the table's width is known here: rows are taken to fill it in the
+// first estimate, whose longest row ends the call, and 0.6 of it in the second. In us,
+// fitted to 1500 shapes on MI355X (2-256 rows, 1-32 KV heads, 1-8 query heads each,
+// head_dim 32-128, 64 to 65 536 shared tokens, the three types); the slower one is
+// taken by more than 10 % in 1 of 27, the mean loss is 1 %. One launch / split:
+// 4 x 8 heads of 32, f32, 200-256 tokens, 128 shared: 7.1 / 12.2; 8 x 30, bf16,
+// 842: 17.8 / 25; 13 x 16, 820-1300, 800 shared: 15.3 / 15.0; 24 x 12, f32, 1520-1900,
+// 1504 shared: 40 / 21; 64 x 32, 4160-5120, 4096 shared: 409 / 115.
+bool shared_one_launch(int64_t B, int64_t Hk, int64_t vheads, int64_t rows, int64_t D, int64_t eb, int64_t keys,
+                       int64_t shared_tokens, int64_t tokens) {
+  const double width = D <= 64 ? 64 : D <= 128 ? 128 : 256, cus = (double)device_cus();
+  const double own = (double)(tokens - shared_tokens), row_mb = 2e-6 * (double)(D * eb);
+  // Eight wavefronts take a row's tiles in turn, 1.7 us a 16 KiB tile.
+  const double turns = (double)((tokens + keys - 1) / keys + 7) / 8, tile_us = 1.72 * std::pow(width * (double)eb / 256, 0.73);
+  const double wgs = (double)(B * vheads);
+  const double one_us = 4.5 + std::max(std::floor(turns) * tile_us * std::max(1.0, wgs / (0.83 * cus)),
+                                       wgs * (double)tokens * row_mb / 10.6);
+  const double mflop = 4e-6 * (double)(rows * Hk * shared_tokens * D);
+  const double split_us = 13.9 + (double)Hk * ((double)shared_tokens + 0.6 * (double)B * own) * row_mb / 5.0 +
+                          mflop / (eb == 2 ? 507.0 : 63.0);
+  return one_us <= split_us;
+}
+
+// MINIVLLM_HIP_SHARED_SPLIT = 0 or 1 takes one launch or the split, and
+// MINIVLLM_HIP_SHARED_LDS = 0 or 1 the shared tiles from registers or, where they can
+// be, from LDS (tuning and tests; read on every call).
 SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M, int64_t shared, int dtype) {
   SharedPlan p{};
-  const int64_t G = Hq / Hk, rows = B * G, keys = dtype == MGI_F32 ? 16 : 32;
+  const int64_t G = Hq / Hk, rows = B * G, eb = dtype_bytes(dtype), keys = eb == 2 ? 32 : 16;
   p.gsets = (int)((G + 15) / 16);
   p.vheads = (int)(Hk * p.gsets);
-  const int forced = env_int("MINIVLLM_HIP_SHARED_SPLIT", -1);
-  p.lds_tiles = dtype != MGI_F32 && D <= 128 && S % 16 == 0 && rows > env_int("MINIVLLM_HIP_SHARED_LDS", 32);
+  p.wgs = (int)round_up(2 * device_cus(), 8);  // two per CU, all resident
+  // Shared tiles through LDS: from 17 rows, whose registers the other form would
+  // leave half empty, to 64 they are up to 8 % faster, few or many; past that only
+  // with four tiles or more to a workgroup (65-128 rows: 15 % slower with fewer, 8-18
+  // % faster with more; 257 and up, 16 tiles: 31 % faster).
+  const int forced_lds = env_int("MINIVLLM_HIP_SHARED_LDS", -1);
+  const bool lds_pays = rows > 16 && (rows <= 64 || Hk * ((shared * S + 63) / 64) * ((rows + 127) / 128) >= 4 * p.wgs);
+  p.lds_tiles = eb == 2 && D <= 128 && S % 16 == 0 && (forced_lds >= 0 ? forced_lds != 0 : lds_pays);
   p.row_tiles = rows > (p.lds_tiles ? 64 : 16) && D <= 128 ? 2 : 1;
   p.set_rows = (p.lds_tiles ? 64 : 16) * p.row_tiles;
   // Sets of rows a team takes together: as many of up to 16 as fill their blocks evenly.
@@ -803,15 +837,19 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   p.team = (int)((sets + p.set_blocks - 1) / p.set_blocks);
   const int64_t step = p.lds_tiles ? 64 : 4 * keys, tiles = (shared * S + step - 1) / step;
   // Tile numbers are 32-bit, and the rows' prefix sums live in LDS.
-  p.one_launch = forced == 0 || B > mgi::kSharedMaxB || Hk * p.set_blocks * tiles >= (int64_t(1) << 30) ||
-                 B * ((M * S + keys - 1) / keys) * p.vheads >= (int64_t(1) << 30);
+  const int forced = env_int("MINIVLLM_HIP_SHARED_SPLIT", -1);
+  p.one_launch = B > mgi::kSharedMaxB || Hk * p.set_blocks * tiles >= (int64_t(1) << 30) ||
+                 B * ((M * S + keys - 1) / keys) * p.vheads >= (int64_t(1) << 30) ||
+                 (forced >= 0 ? forced == 0
+                              : shared_one_launch(B, Hk, p.vheads, rows, D, eb, keys, shared * S, M * S));
   if (p.one_launch) return p;
   p.s_tiles = (int)tiles;
   p.s_units = (int)(Hk * p.set_blocks);
-  p.s_cost = env_int("MINIVLLM_HIP_SHARED_COST", (int)(step / keys));
-  p.s_min = env_int("MINIVLLM_HIP_SHARED_SMIN", 1);
-  p.own_min = env_int("MINIVLLM_HIP_SHARED_OMIN", 1);
-  p.wgs = (int)round_up(env_int("MINIVLLM_HIP_SHARED_WGS", 2) * device_cus(), 8);
+  // By bytes; a piece costs two tiles more, its chain of loads (with none a list of
+  // two-tile pieces ended last: 130 x 13 heads, 128 shared tokens, 92 us, so 66; 100 x
+  // 4, D = 64, 3200: 26.5 and 22.3).
+  p.s_cost = (int)(step / keys);
+  p.s_piece = 8;
   p.s_cont = B * Hq;
   p.own_slot = p.s_cont + (tiles ? (int64_t)p.wgs * p.set_rows : 0);
   p.own_cont = p.own_slot + B * Hq;
@@ -1266,8 +1304,7 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
     const SharedPlan p = shared_plan(B, Hq, Hk, D, S, M, shared_blocks, dtype);
     a.one_launch = p.one_launch;
     a.gsets = p.gsets, a.vheads = p.vheads, a.wgs = p.wgs, a.lds_tiles = p.lds_tiles, a.row_tiles = p.row_tiles;
-    a.set_rows = p.set_rows, a.team = p.team, a.set_blocks = p.set_blocks, a.s_units = p.s_units, a.s_tiles = p.s_tiles, a.s_cost = p.s_cost;
-    a.s_min = p.s_min, a.own_min = p.own_min;
+    a.set_rows = p.set_rows, a.team = p.team, a.set_blocks = p.set_blocks, a.s_units = p.s_units, a.s_tiles = p.s_tiles, a.s_cost = p.s_cost, a.s_piece = p.s_piece;
     a.s_cont = p.s_cont, a.own_slot = p.own_slot, a.own_cont = p.own_cont;
     if (!p.one_launch) {
       if (!workspace) return fail(MGI_EWORKSPACE, "workspace required for the split pass");

@@ -144,8 +144,7 @@ struct SharedArgs {
   int set_rows;            // query rows per workgroup of it
   int team, set_blocks;    // sets that workgroups of a team take together, and blocks of those per KV head
   int s_units, s_tiles;    // its list: KV heads x blocks, key tiles of each
-  int s_cost;              // cost of one of its tiles, an own tile being 1
-  int s_min, own_min;      // least tiles of a segment
+  int s_cost, s_piece;     // cost of one of its tiles and of a piece, an own tile being 1
   // Partials: [B, Hq] of the pieces that begin a row's shared run and, from own_slot,
   // of those that begin its own; set_rows per workgroup (s_cont) and 16 per
   // wavefront (own_cont) for continued ones.

@@ -545,17 +545,17 @@ struct Split {
 };
 __device__ __forceinline__ Split make_split(const SharedArgs& a, int own_total) {
   const int total = a.s_units * a.s_tiles;
-  const int64_t cs = (int64_t)total * a.team * a.s_cost, co = own_total;
+  const int64_t cs = ((int64_t)total * a.s_cost + (int64_t)a.s_units * a.s_piece) * a.team, co = own_total;
   Split r{};
   int teams = 0;
   if (total) {
     const int64_t fair = (a.wgs * cs + (cs + co) * a.team / 2) / ((cs + co) * a.team);
     teams = (int)max((int64_t)1, min(fair, (int64_t)(a.wgs - (own_total > 0)) / a.team));
-    r.seg_shared = max(a.s_min, (total + teams - 1) / teams);
+    r.seg_shared = (total + teams - 1) / teams;
   }
   r.shared_wgs = teams * a.team;
   const int waves = (a.wgs - r.shared_wgs) * kSplitWaves;
-  if (waves) r.seg_own = max(a.own_min, (own_total + waves - 1) / waves);
+  if (waves) r.seg_own = max(1, (own_total + waves - 1) / waves);
   return r;
 }
 
@@ -667,16 +667,12 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
   const char* vp = (const char*)a.v;
   uint4 qf[1][L::kKS];
   State<DP, 1> st;
-  L f;
-  f32x4 s[1][L::kGroups];
   fill(0);
   int b = __builtin_amdgcn_readlane(row, 0), h = __builtin_amdgcn_readlane(head, 0);
   load_own_queries<T, DP, FULL>(a, b, h >> 1, qf);
-  load_keys<T, DP, FULL, NT>(a, kp, win, 0, f);
-  load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
   st.reset();
-  for (int t = 0; t < n; ++t) {
-    score_tile<T, DP, 1>(f, qf, s);
+  // Tile t, in f; the next one's loads go out first, into g.
+  auto turn = [&](int t, L& f, L& g) {
     const bool more = t + 1 < n;
     const int at = (t + 1) % kSpan * L::kGroups;
     int nb = b, nh = h;
@@ -684,17 +680,57 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
       if (at == 0) fill(t + 1);
       nb = __builtin_amdgcn_readlane(row, at);
       nh = __builtin_amdgcn_readlane(head, at);
-      load_keys<T, DP, FULL, NT>(a, kp, win, at, f);
+      load_keys<T, DP, FULL, NT>(a, kp, win, at, g);
+      load_values<T, DP, FULL, NT>(a, vp, win, at, g);
     }
     const bool ends = !more || nb != b || (nh >> 1) != (h >> 1);
+    f32x4 s[1][L::kGroups];
+    score_tile<T, DP, 1>(f, qf, s);
     if (more && ends) load_own_queries<T, DP, FULL>(a, nb, nh >> 1, qf);
     attend_tile<T, DP, 1, true>(a, f, s, st);
-    if (more) load_values<T, DP, FULL, NT>(a, vp, win, at, f);
     if (ends) {
       store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
       st.reset();
       b = nb;
       h = nh;
+    }
+  };
+  if constexpr (DP * sizeof(T) <= 256) {
+    L f, g;
+    load_keys<T, DP, FULL, NT>(a, kp, win, 0, f);
+    load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
+    for (int t = 0; t < n; t += 2) {
+      turn(t, f, g);
+      if (t + 1 < n) turn(t + 1, g, f);
+    }
+  } else {  // two tiles do not fit the registers
+    L f;
+    for (int t = 0; t < n; ++t) {
+      if (t == 0) {
+        load_keys<T, DP, FULL, NT>(a, kp, win, 0, f);
+        load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
+      }
+      const bool more = t + 1 < n;
+      const int at = (t + 1) % kSpan * L::kGroups;
+      int nb = b, nh = h;
+      f32x4 s[1][L::kGroups];
+      score_tile<T, DP, 1>(f, qf, s);
+      if (more) {
+        if (at == 0) fill(t + 1);
+        nb = __builtin_amdgcn_readlane(row, at);
+        nh = __builtin_amdgcn_readlane(head, at);
+        load_keys<T, DP, FULL, NT>(a, kp, win, at, f);
+      }
+      const bool ends = !more || nb != b || (nh >> 1) != (h >> 1);
+      if (more && ends) load_own_queries<T, DP, FULL>(a, nb, nh >> 1, qf);
+      attend_tile<T, DP, 1, true>(a, f, s, st);
+      if (more) load_values<T, DP, FULL, NT>(a, vp, win, at, f);
+      if (ends) {
+        store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
+        st.reset();
+        b = nb;
+        h = nh;
+      }
     }
   }
 }

@@ -1,5 +1,5 @@
-"""paged_attention_shared_prefix_hip against the softmax in 64 bits: the split form
-and the one-launch form, grouped heads, rows shorter than the shared blocks, NaN
+"""paged_attention_shared_prefix_hip against the softmax in 64 bits: the split form,
+its shared tiles from registers and from LDS, and the one-launch form, grouped heads, rows shorter than the shared blocks, NaN
 in every slot no row holds, masked entries, odd block sizes and strides, scores of
 -inf, graphs and streams, and a rotary decode step through the pool.
 
@@ -26,14 +26,15 @@ DEV = torch.device("cuda:0")
 U = 2.0 ** -24
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 DTYPES = pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
-ROUTES = pytest.mark.parametrize("route", ["split", "one"])
+ROUTES = pytest.mark.parametrize("route", ["registers", "lds", "one"])
 
 
 @pytest.fixture(autouse=True)
 def _route(request, monkeypatch):
     route = request.node.callspec.params.get("route") if hasattr(request.node, "callspec") else None
-    if route:
-        monkeypatch.setenv("MINIVLLM_HIP_SHARED_SPLIT", "1" if route == "split" else "0")
+    if route:  # (f32, wide heads and block sizes that are no multiple of 16 keep to registers)
+        monkeypatch.setenv("MINIVLLM_HIP_SHARED_SPLIT", "0" if route == "one" else "1")
+        monkeypatch.setenv("MINIVLLM_HIP_SHARED_LDS", "1" if route == "lds" else "0")
 
 
 def make(B, Hq, Hk, D, S, shared, ctx, dtype, seed=0, layers=2, layer=1, itype=torch.int64):
