@@ -836,9 +836,10 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   p.set_blocks = (int)((sets + 15) / 16);
   p.team = (int)((sets + p.set_blocks - 1) / p.set_blocks);
   const int64_t step = p.lds_tiles ? 64 : 4 * keys, tiles = (shared * S + step - 1) / step;
-  // Tile numbers are 32-bit, and the rows' prefix sums live in LDS.
+  // Tile numbers are 32-bit, the rows' prefix sums live in LDS, and rows by the
+  // thousand fill the CUs by themselves: no partials past 4 GiB.
   const int forced = env_int("MINIVLLM_HIP_SHARED_SPLIT", -1);
-  p.one_launch = B > mgi::kSharedMaxB || Hk * p.set_blocks * tiles >= (int64_t(1) << 30) ||
+  p.one_launch = B > mgi::kSharedMaxB || 2 * B * Hq * D * 4 > (int64_t(4) << 30) || Hk * p.set_blocks * tiles >= (int64_t(1) << 30) ||
                  B * ((M * S + keys - 1) / keys) * p.vheads >= (int64_t(1) << 30) ||
                  (forced >= 0 ? forced == 0
                               : shared_one_launch(B, Hk, p.vheads, rows, D, eb, keys, shared * S, M * S));
@@ -1287,7 +1288,7 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
   a.shared = (int)shared_blocks;
   a.P = (int)(shared_blocks * S);
   a.scale_log2 = scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f;
-  a.lazy = 6.f / a.scale_log2;
+  a.lazy = std::min(6.f / a.scale_log2, 1e30f);
   a.q_flip = scale < 0.f ? (dtype == MGI_F32 ? 0x80000000u : 0x80008000u) : 0u;
   a.q_zero = scale == 0.f;
   magic_of(S, &a.s_mul, &a.s_shift);

@@ -130,6 +130,8 @@ CASES = {
     "odd head dim": (4, 4, 2, 20, 16, 3, [48, 50, 64, 30]),
     "head dim 512": (3, 2, 1, 512, 16, 2, [32, 40, 33]),
     "long": (3, 4, 2, 128, 16, 130, [2080, 2500, 5000]),
+    "hundreds of rows": (301, 2, 1, 64, 16, 3, [48 + (i * 31) % 140 if i % 9 else i % 50 for i in range(301)]),
+    "teams of many sets": (150, 32, 2, 64, 16, 20, [320 + (i * 7) % 50 for i in range(150)]),
 }
 
 
@@ -146,6 +148,76 @@ def test_against_64_bits(name, dtype, route):
     assert torch.equal(got, again)
     for b, c in enumerate(ctx):
         assert c > 0 or not got[b].any()
+
+
+@DTYPES
+@ROUTES
+@pytest.mark.parametrize("B,H,shared,own", [(3, 1, 2_200_000, 5), (8, 8, 16, 41_000)], ids=["shared", "own"])
+def test_windows_of_the_table_move_on(B, H, shared, own, dtype, route):
+    """Runs of tiles past what one reading of the table covers (64 / 32 tiles a
+    wavefront). Eight tokens, spread to the last, hold nearly all of the weight (their
+    score is 25, 0 elsewhere), so a tile from a wrong place changes the output by about
+    an eighth. An accumulator takes at most the keys of one of eight wavefronts: 2 (n / 8
+    + 64) u of A and the rounding of weights and output."""
+    D, S, P = 8, 16, -(-shared // 16)
+    n = P * S + own
+    g = torch.Generator(device=DEV).manual_seed(5)
+    N = P + B * -(-own // S) + 2
+    perm = torch.randperm(N, generator=g, device=DEV)
+    tables = torch.empty((B, n // S + 1), dtype=torch.int32, device=DEV)
+    tables[:, :P] = perm[:P]
+    tables[:, P:] = perm[P:P + B * (tables.shape[1] - P)].view(B, -1)
+    pool = KVBlockPool(1, N, S, H, D, device=DEV, dtype=dtype)
+    pool.k.zero_()
+    pool.v.normal_(generator=g)
+    q = torch.zeros((B, H, D), dtype=dtype, device=DEV)
+    q[..., 0] = 4
+    at = torch.linspace(0, n - 1, 8, device=DEV, dtype=torch.float64).long()
+    for b in range(B):
+        pool.k[0, tables[b, at // S].long(), at % S, :, 0] = 25 * math.sqrt(D) / 4
+    lens = torch.full((B,), n, device=DEV)
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, 0, shared_blocks=P)
+    half, k = 0.5 * torch.finfo(dtype).eps, pool.k[0, :, :, 0, 0].double()
+    for b in range(B):
+        row = tables[b].long()
+        w = torch.softmax((k[row] * 4 / math.sqrt(D)).flatten()[:n], 0)
+        for h in range(H):
+            v = pool.v[0, row, :, h].flatten(0, 1)[:n].double()
+            out, A = (w[:, None] * v).sum(0), (w[:, None] * v.abs()).sum(0)
+            bound = (2 * (n / 8 + 64) * U + 2 * (D + 4) * U * 26 + (half if dtype != F32 else 0)) * A + half * out.abs()
+            assert ((got[b, h].double() - out).abs() <= 1.01 * bound).all(), (b, h)
+
+
+@DTYPES
+@ROUTES
+def test_a_row_of_nan_keeps_to_itself(dtype, route):
+    """NaN in one row's query, and in one row's own values, stays in that row; an
+    infinite shared value is every row's, in its dim."""
+    ctx = [100, 90, 130, 80, 64]
+    q, pool, tables, lens, layer = make(5, 4, 2, 64, 16, 4, ctx, dtype, seed=12)
+    want = reference(q, pool, tables, lens, layer, 4)
+    q[1, 2, 5] = float("nan")
+    pool.v[layer, tables[2, 7].long(), 3, 1, 9] = float("nan")
+    pool.v[layer, tables[0, 2].long(), 6, 0, 30] = float("inf")
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=4)
+    assert torch.isnan(got[1, 2]).all() and torch.isnan(got[2, 2:, 9]).all() and torch.isinf(got[[0, 2, 3, 4], :2, 30]).all()
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[1, 2] = hit[2, 2:, 9] = hit[:, :2, 30] = True
+    assert torch.isfinite(got[~hit]).all()
+    out, A, X, n = want
+    check(torch.where(hit, torch.zeros_like(got), got), (out.masked_fill(hit, 0), A, X, n), dtype)
+
+
+def test_more_rows_than_the_split_takes():
+    """4100 rows: one launch."""
+    ctx = [20 + i % 30 for i in range(4100)]
+    q, pool, tables, lens, layer = make(4100, 2, 1, 64, 16, 1, ctx, BF16, seed=13)
+    assert _native.lib().mgi_paged_decode_shared_workspace_bytes(4100, 2, 1, 64, 16, tables.shape[1], 1, 1) == 0
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=1)
+    pick = list(range(0, 4100, 37))
+    row0 = tables[:1].expand(len(pick), -1)
+    sub = torch.where(torch.arange(tables.shape[1], device=DEV) < 1, row0, tables[pick])
+    check(got[pick], reference(q[pick], pool, sub, lens[pick], layer, 1), BF16)
 
 
 @DTYPES
