@@ -722,7 +722,8 @@ int rope_args(const RopeSpec& r, mgi::RopeArgs* a) {
   if (!std::isfinite(r.eps) || r.eps < 0.f) return fail(MGI_EINVAL, "eps must be finite and non-negative");
   if (r.D > 512) return fail(MGI_EUNSUPPORTED, "head_dim larger than 512");
   // One launch's threads, 64 to a head row at most, are counted in 32 bits.
-  if (r.Hq > kMaxGridYZ || r.Hk > kMaxGridYZ || r.T >= (int64_t(1) << 24) || r.T * (r.Hq + 2 * r.Hk) >= (int64_t(1) << 25))
+  if (r.Hq > kMaxGridYZ || r.Hk > kMaxGridYZ || r.T >= (int64_t(1) << 24) ||
+      r.T * (r.Hq + 2 * r.Hk) >= (int64_t(1) << 25))
     return fail(MGI_EUNSUPPORTED, "rows x heads too large for one launch");
   a->q = r.q;
   a->q_st = r.qs[0], a->q_sh = r.qs[1], a->q_sd = r.qs[2];
@@ -757,7 +758,8 @@ int rope_args(const RopeSpec& r, mgi::RopeArgs* a) {
 // of every row must be aligned to its size, up to 16 bytes.
 int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
   const int64_t eb = dtype_bytes(a.dtype), ob = dtype_bytes(out_dtype);
-  auto fits = [](int64_t bytes, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides, int64_t e) {
+  auto fits = [](int64_t bytes, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides,
+                 int64_t e) {
     const int64_t al = std::min<int64_t>(16, bytes);
     for (const void* p : ptrs)
       if (reinterpret_cast<uintptr_t>(p) % (uintptr_t)al) return false;
@@ -765,11 +767,13 @@ int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
       if (s * e % al) return false;
     return true;
   };
-  const bool unit = a.q_sd == 1 && a.k_sd == 1 && a.qo_sd == 1 && a.ko_sd == 1 && (!a.Hv || (a.v_sd == 1 && a.vo_sd == 1));
+  const bool unit =
+      a.q_sd == 1 && a.k_sd == 1 && a.qo_sd == 1 && a.ko_sd == 1 && (!a.Hv || (a.v_sd == 1 && a.vo_sd == 1));
   a.chunk = 0;
   for (int c : {8, 4}) {
     if (c * eb > 16 || !unit || (a.R / 2) % c || (a.D - a.R) % (2 * c)) continue;
-    if (fits(c * (a.w_f32 ? 4 : eb), {a.qw, a.kw}, {}, 1) && fits(c * eb, {a.q, a.k, a.v}, {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh}, eb) &&
+    if (fits(c * (a.w_f32 ? 4 : eb), {a.qw, a.kw}, {}, 1) &&
+        fits(c * eb, {a.q, a.k, a.v}, {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh}, eb) &&
         fits(c * ob, {a.q_out, a.k_out, a.v_out},
              {a.qo_st, a.qo_sh, a.ko_sn, a.ko_st, a.ko_sh, a.vo_sn, a.vo_st, a.vo_sh}, ob)) {
       a.chunk = c;
@@ -827,7 +831,8 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   // with four tiles or more to a workgroup (65-128 rows: 15 % slower with fewer, 8-18
   // % faster with more; 257 and up, 16 tiles: 31 % faster).
   const int forced_lds = env_int("MINIVLLM_HIP_SHARED_LDS", -1);
-  const bool lds_pays = rows > 16 && (rows <= 64 || Hk * ((shared * S + 63) / 64) * ((rows + 127) / 128) >= 4 * p.wgs);
+  const bool lds_pays =
+      rows > 16 && (rows <= 64 || Hk * ((shared * S + 63) / 64) * ((rows + 127) / 128) >= 4 * p.wgs);
   p.lds_tiles = eb == 2 && D <= 128 && S % 16 == 0 && (forced_lds >= 0 ? forced_lds != 0 : lds_pays);
   p.row_tiles = rows > (p.lds_tiles ? 64 : 16) && D <= 128 ? 2 : 1;
   p.set_rows = (p.lds_tiles ? 64 : 16) * p.row_tiles;
@@ -1288,7 +1293,7 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
   a.shared = (int)shared_blocks;
   a.P = (int)(shared_blocks * S);
   a.scale_log2 = scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f;
-  a.lazy = std::min(6.f / a.scale_log2, 1e30f);
+  a.lazy = std::min(kSharedLazy / a.scale_log2, 1e30f);
   a.q_flip = scale < 0.f ? (dtype == MGI_F32 ? 0x80000000u : 0x80008000u) : 0u;
   a.q_zero = scale == 0.f;
   magic_of(S, &a.s_mul, &a.s_shift);
@@ -1305,7 +1310,8 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
     const SharedPlan p = shared_plan(B, Hq, Hk, D, S, M, shared_blocks, dtype);
     a.one_launch = p.one_launch;
     a.gsets = p.gsets, a.vheads = p.vheads, a.wgs = p.wgs, a.lds_tiles = p.lds_tiles, a.row_tiles = p.row_tiles;
-    a.set_rows = p.set_rows, a.team = p.team, a.set_blocks = p.set_blocks, a.s_units = p.s_units, a.s_tiles = p.s_tiles, a.s_cost = p.s_cost, a.s_piece = p.s_piece;
+    a.set_rows = p.set_rows, a.team = p.team, a.set_blocks = p.set_blocks;
+    a.s_units = p.s_units, a.s_tiles = p.s_tiles, a.s_cost = p.s_cost, a.s_piece = p.s_piece;
     a.s_cont = p.s_cont, a.own_slot = p.own_slot, a.own_cont = p.own_cont;
     if (!p.one_launch) {
       if (!workspace) return fail(MGI_EWORKSPACE, "workspace required for the split pass");

@@ -154,7 +154,8 @@ struct SharedArgs {
   int* ws_cum;             // [B] prefix sums of the rows' own tiles
   int* ws_split;           // the two lists' segment lengths
 };
-constexpr int kSharedMaxB = 4096;      // rows of the split form (their prefix sums live in LDS)
+constexpr int kSharedMaxB = 4096;    // rows of the split form (their prefix sums live in LDS)
+constexpr float kSharedLazy = 6.f;   // log2 units a score may pass the running maximum by
 hipError_t launch_paged_shared_f32(const SharedArgs& a, hipStream_t stream);
 hipError_t launch_paged_shared_bf16(const SharedArgs& a, hipStream_t stream);
 hipError_t launch_paged_shared_f16(const SharedArgs& a, hipStream_t stream);

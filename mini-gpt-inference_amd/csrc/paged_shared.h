@@ -8,13 +8,13 @@
 // anywhere: a piece leaves its largest score m (log2 units), l = sum 2^(s - m) and
 // o = sum 2^(s - m) V, and pieces join as
 //   M = max m_i,  L = sum l_i 2^(m_i - M),  out = sum o_i 2^(m_i - M) / L.
-// So the shared tokens are attended once for all rows together, as a matrix
-// product with up to 64 query rows per wavefront, each row's own tokens by
-// itself, and a second launch joins the pieces. A row shorter than P takes no part
-// in the shared piece (all of its tokens are its own then), so no key of either
-// kind is masked for one row and not for another.
+// So the shared tokens are attended once for all rows together, as one matrix
+// product, each row's own tokens by themselves, and a second launch joins the
+// pieces. A row shorter than P takes no part in the shared piece (all of its tokens
+// are its own then), so no key of either kind is masked for one row and not for
+// another.
 //
-// Both products run on the matrix cores, straight from registers, without LDS:
+// Both products run on the matrix cores. In the register form, without LDS:
 //   S^T = K Q^T   A: lane l holds 16 bytes of key l & 15; B: of query l & 15.
 //                 The result leaves lane l the scores of query l & 15 with keys
 //                 4 (l >> 4) + i -- which is the B operand the second needs.
@@ -24,13 +24,27 @@
 //                 whole row) and transposes the 8 x 8 block with 32 v_perm_b32,
 //                 tile t then standing for dims 8 m + t.
 // f32 uses the 16x16x4 product, one key per lane group, and needs no transpose.
-// The weights 2^(s - m) are rounded to the 16-bit type for the second product
-// (half a step of each weight, which the output's own rounding exceeds); the
-// sums l, the scores and the outputs are f32.
+// A row's own tokens take it with one query head's row in 16 filled, or G of them:
+// the products are idle lanes then, but 16 KiB of K and V take a CU 650 ns of its
+// share of HBM and a wavefront's products 110 ns. Many rows on the shared tokens
+// take tiles in LDS instead (below).
 //
-// The running maximum moves only when a score passes it by 2^kLazy, which costs
-// one comparison per tile instead of a reduction over lanes; weights stay below
-// 2^kLazy, well inside every type. A tile's K and V are loaded one tile ahead.
+// Rounding: the weights 2^(s - m) go to the 16-bit type for the second product, at
+// most half a step of each, as independent errors about as much in the output as
+// its own rounding (bf16: 0.0023 off 64 bits, relative, where rounding alone is
+// 0.0017; f16 0.00028 and 0.00021). Scores, sums l and outputs are f32.
+//
+// The running maximum moves only when a score passes it by kSharedLazy in log2
+// units, which costs one comparison per tile instead of a reduction over lanes;
+// weights stay below 2^kSharedLazy, well inside every type.
+//
+// What bounds it (MI355X; inputs from memory, another set each call): 64 x 32 heads
+// on 4096 shared tokens and 64-1024 of their own, bf16, 649 MB: 119 us, 5.45 TB/s; 128
+// x 32 on 8 KV heads over 65 536 shared, 138 GFLOP: 173 us, 795 TFLOP/s, the softmax's
+// VALU work beside the products (37 % of cycles in the matrix cores, LDS conflicts
+// none; with all keys in L2 it still takes 141 of the 146 us without own tokens).
+// Calls under about 30 us are chains: launch and the rows' prefix sums 4 us, a first
+// tile 3, the joining launch 5-8 us.
 #pragma once
 
 #include <type_traits>
@@ -52,14 +66,15 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kNegInf = -__builtin_inff();
-constexpr float kLazy = 6.f;
 
 template <typename T>
 __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
   if constexpr (std::is_same_v<T, bf16_t>)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
   else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -67,7 +82,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (std::is_same_v<T, bf16_t>) return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
 }
-__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
 __device__ __forceinline__ uint32_t word(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
 __device__ __forceinline__ float fword(const uint4& v, int i) { return __uint_as_float(word(v, i)); }
 __device__ __forceinline__ float across_groups_max(float x) {
@@ -132,9 +149,8 @@ __device__ __forceinline__ int64_t table_entry(const SharedArgs& a, int b, int j
 // Where the 16-key groups of a wavefront's next tiles lie (S a multiple of 16, so
 // each lies in one block): lane i holds group i % GR of tile i / GR, as byte offsets
 // into the pool, and how many of its keys count. One table load serves 64 / GR tiles,
-// and the next window's is issued a window ahead: read where it is used, an entry
-// costs a wait for every load in flight (the document case, 128 x 32 heads over
-// 65 536 tokens: 351 us so, see the table in the documentation for now).
+// and the next window's is issued a window ahead: an entry read where it is used
+// costs a wait for every load in flight.
 struct Window {
   uint32_t k_lo, k_hi, v_lo, v_hi;
   int n;
@@ -183,7 +199,8 @@ __device__ __forceinline__ void load_keys(const SharedArgs& a, const char* kp, c
     const uint32_t off = (uint32_t)min(row, max(n, 1) - 1) * ss + (uint32_t)kg * 16;
 #pragma unroll
     for (int s = 0; s < L::kKS; ++s)
-      f.k[g][s] = FULL || (kg + 4 * s) * L::kCE < a.D ? load_piece<NT, uint4>(base + off + 64 * s) : make_uint4(0, 0, 0, 0);
+      f.k[g][s] = FULL || (kg + 4 * s) * L::kCE < a.D ? load_piece<NT, uint4>(base + off + 64 * s)
+                                                      : make_uint4(0, 0, 0, 0);
   }
 }
 template <typename T, int DP, bool FULL, bool NT = false>
@@ -204,7 +221,9 @@ __device__ __forceinline__ void load_values(const SharedArgs& a, const char* vp,
       const uint32_t off = (uint32_t)min(4 * kg + j, max(n, 1) - 1) * ss + col;
 #pragma unroll
       for (int h = 0; h < L::kHF; ++h)
-        f.v[4 * g + j][h] = FULL || 16 * L::kEV * h + row * L::kEV < a.D ? load_piece<NT, V>(base + off + 16 * L::kEV * (int)sizeof(T) * h) : V{};
+        f.v[4 * g + j][h] = FULL || 16 * L::kEV * h + row * L::kEV < a.D
+                                ? load_piece<NT, V>(base + off + 16 * L::kEV * (int)sizeof(T) * h)
+                                : V{};
     }
   }
 }
@@ -366,15 +385,15 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, Tile<T, DP>& f,
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            st.acc[q][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fword(f.v[j][h], e), p[q][j], st.acc[q][4 * h + e], 0, 0, 0);
+            st.acc[q][4 * h + e] =
+                __builtin_amdgcn_mfma_f32_16x16x4f32(fword(f.v[j][h], e), p[q][j], st.acc[q][4 * h + e], 0, 0, 0);
   }
 }
 
 // Attends the tiles first, first + step, ... below end of row b's table. A tile's
 // keys are loaded into the registers the one before has given its scores from, and
 // its values where that one's products have been taken: half a tile is always on
-// its way. (A second set of registers, a whole tile ahead, changed nothing: 133 us
-// either way for 64 x 32 heads.)
+// its way. (A second set of registers, a whole tile ahead, changed no call's time.)
 template <typename T, int DP, int NQ, bool UNI, bool FULL>
 __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh, int first, int step, int end,
                                              const uint4 (&qf)[NQ][Tile<T, DP>::kKS], State<DP, NQ>& st) {
@@ -487,7 +506,8 @@ __device__ __forceinline__ void join_waves(const SharedArgs& a, const State<DP, 
     }
     each_run<T>(a, st, q, [&](int d, const float* x) {
 #pragma unroll
-      for (int e = 0; e < Tile<T, DP>::kEV; e += 4) *(f32x4*)&space.acc[wave][row][d + e] = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+      for (int e = 0; e < Tile<T, DP>::kEV; e += 4)
+        *(f32x4*)&space.acc[wave][row][d + e] = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
     });
   }
   __syncthreads();
@@ -520,7 +540,8 @@ __device__ __forceinline__ void store_partial(const SharedArgs& a, const State<D
   float* row = a.ws_acc + slot * a.D;
   each_run<T>(a, st, q, [&](int d, const float* x) {
 #pragma unroll
-    for (int e = 0; e < Tile<T, DP>::kEV; e += 4) *(float4*)(row + d + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+    for (int e = 0; e < Tile<T, DP>::kEV; e += 4)
+      *(f32x4*)(row + d + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
   });
 }
 
@@ -530,14 +551,16 @@ __device__ __forceinline__ int clamped_ctx(const SharedArgs& a, int b) {
 }
 
 constexpr int kSplitWaves = 4;
+
 // The work is two lists: the shared tokens' tiles, (KV head, block of row sets, tile)
 // in that order, each for a team of workgroups, one to a set of query rows, that
-// walk the same keys together and find them in their XCD's L2 (8 sets of 128 rows
-// over 65 536 tokens: 197 us with a list per set); and the rows' own, (row, virtual head, tile), a virtual head
-// being a KV head and a set of at most 16 of its query heads. The launch's
-// workgroups are dealt out between the lists by cost, and each list is cut into
-// equal segments: one per team of the first list, one per wavefront of the second. A segment's first piece may continue a run that another began: it leaves
-// its partial in the segment's slots, a piece that begins a run in the rows' own.
+// walk the same keys together and find them in their XCD's L2 (4 sets of 128 rows
+// over 65 536 tokens: 197 us with a list per set, 173 so); and the rows' own, (row,
+// virtual head, tile), a virtual head being a KV head and a set of at most 16 of its
+// query heads. The launch's workgroups are dealt out between the lists by cost, and
+// each list is cut into equal segments: one per team of the first, one per wavefront
+// of the second. A segment's first piece may continue a run that another began: it
+// leaves its partial in the segment's slots, a piece that begins a run in its row's.
 struct Split {
   int shared_wgs;  // workgroups of the first list, whole teams
   int seg_shared;  // tiles of a team's segment
@@ -568,7 +591,8 @@ struct Place {
 };
 __device__ __forceinline__ Place make_place(const SharedArgs& a, const Split& sp) {
   const int x = (int)blockIdx.x & 7, j = (int)blockIdx.x >> 3;
-  const int mine = sp.shared_wgs / 8 + (x < sp.shared_wgs % 8), before = x * (sp.shared_wgs / 8) + min(x, sp.shared_wgs % 8);
+  const int each = sp.shared_wgs / 8, rest = sp.shared_wgs % 8;
+  const int mine = each + (x < rest), before = x * each + min(x, rest);
   if (j < mine) return {true, before + j};
   return {false, x * (a.wgs / 8) - before + j - mine};
 }
@@ -627,10 +651,12 @@ __device__ __forceinline__ OwnTile find_own(const SharedArgs& a, const int* cum,
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void store_own(const SharedArgs& a, const State<DP, 1>& st, int wave_index, int b, int vh, bool begins) {
+__device__ __forceinline__ void store_own(const SharedArgs& a, const State<DP, 1>& st, int wave_index, int b, int vh,
+                                          bool begins) {
   const int lane = (int)threadIdx.x & 63, kvh = vh / a.gsets, g = (vh - kvh * a.gsets) * 16 + (lane & 15);
   const float l = coded_sum(across_groups_sum(st.l[0]), st.any);
-  const int64_t slot = begins ? a.own_slot + (int64_t)b * a.Hq + kvh * a.G + g : a.own_cont + (int64_t)wave_index * 16 + (lane & 15);
+  const int64_t slot = begins ? a.own_slot + (int64_t)b * a.Hq + kvh * a.G + g
+                              : a.own_cont + (int64_t)wave_index * 16 + (lane & 15);
   if (g < a.G) store_partial<T>(a, st, 0, slot, st.m[0] == kNegInf ? kNegInf : st.mc[0], l);
 }
 template <typename T, int DP, bool FULL>
@@ -641,96 +667,61 @@ __device__ __forceinline__ void load_own_queries(const SharedArgs& a, int b, int
 
 // A wavefront's segment of the rows' own tiles, as one stream over rows and heads:
 // the window's lanes find their own tiles, so a run's end costs no new chain of
-// loads (length, table, queries, keys), only its partial. With a loop over runs
-// instead each cost about 4 us: 13 x 16 heads, 14.9 us where a wavefront had one
-// tile and 19.0 where it had two.
+// loads (length, table, queries, keys), only its partial (24 x 12 heads of 64, f32:
+// 23.8 us with a loop over runs, 21.4 so; 13 x 16, whose wavefronts have a tile
+// each, 14.9 and 14.7).
 template <typename T, int DP, bool FULL, bool NT>
-__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum, const int* ctx) {
+__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum,
+                                           const int* ctx) {
   using L = Tile<T, DP>;
   constexpr int kSpan = 64 / L::kGroups;
   const int lane = (int)threadIdx.x & 63;
   if ((int64_t)wave_index * seg >= total) return;
   const int u0 = wave_index * seg, n = min(total - u0, seg);
+  const char* kp = (const char*)a.k;
+  const char* vp = (const char*)a.v;
   Window win{};
-  int row = 0, head = 0;  // of the lane's tile; head: virtual head, and whether the tile begins its run
+  int row = 0, head = 0;  // of the lane's tile; head: 2 x virtual head, + 1 where the tile begins its run
   auto fill = [&](int t) {
     const int u = u0 + t + lane / L::kGroups;
     if (u < u0 + n) {
       const OwnTile o = find_own(a, cum, u);
-      const int c = ctx[o.b], tok = (c < a.P ? 0 : a.P) + o.tile * L::kKeys + 16 * (lane % L::kGroups), kvh = o.vh / a.gsets;
-      win = make_window<T>(a, window_entry(a, o.b, tok), tok, c, kvh);
+      const int c = ctx[o.b], tok = (c < a.P ? 0 : a.P) + o.tile * L::kKeys + 16 * (lane % L::kGroups);
+      win = make_window<T>(a, window_entry(a, o.b, tok), tok, c, o.vh / a.gsets);
       row = o.b;
       head = 2 * o.vh + (o.tile == 0);
     }
   };
-  const char* kp = (const char*)a.k;
-  const char* vp = (const char*)a.v;
-  uint4 qf[1][L::kKS];
-  State<DP, 1> st;
   fill(0);
   int b = __builtin_amdgcn_readlane(row, 0), h = __builtin_amdgcn_readlane(head, 0);
+  uint4 qf[1][L::kKS];
+  State<DP, 1> st;
+  L f;
+  f32x4 s[1][L::kGroups];
   load_own_queries<T, DP, FULL>(a, b, h >> 1, qf);
+  load_keys<T, DP, FULL, NT>(a, kp, win, 0, f);
+  load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
   st.reset();
-  // Tile t, in f; the next one's loads go out first, into g.
-  auto turn = [&](int t, L& f, L& g) {
+  for (int t = 0; t < n; ++t) {  // as in stream_tiles
     const bool more = t + 1 < n;
     const int at = (t + 1) % kSpan * L::kGroups;
     int nb = b, nh = h;
+    score_tile<T, DP, 1>(f, qf, s);
     if (more) {
       if (at == 0) fill(t + 1);
       nb = __builtin_amdgcn_readlane(row, at);
       nh = __builtin_amdgcn_readlane(head, at);
-      load_keys<T, DP, FULL, NT>(a, kp, win, at, g);
-      load_values<T, DP, FULL, NT>(a, vp, win, at, g);
+      load_keys<T, DP, FULL, NT>(a, kp, win, at, f);
     }
     const bool ends = !more || nb != b || (nh >> 1) != (h >> 1);
-    f32x4 s[1][L::kGroups];
-    score_tile<T, DP, 1>(f, qf, s);
     if (more && ends) load_own_queries<T, DP, FULL>(a, nb, nh >> 1, qf);
     attend_tile<T, DP, 1, true>(a, f, s, st);
+    if (more) load_values<T, DP, FULL, NT>(a, vp, win, at, f);
     if (ends) {
       store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
       st.reset();
       b = nb;
       h = nh;
-    }
-  };
-  if constexpr (DP * sizeof(T) <= 256) {
-    L f, g;
-    load_keys<T, DP, FULL, NT>(a, kp, win, 0, f);
-    load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
-    for (int t = 0; t < n; t += 2) {
-      turn(t, f, g);
-      if (t + 1 < n) turn(t + 1, g, f);
-    }
-  } else {  // two tiles do not fit the registers
-    L f;
-    for (int t = 0; t < n; ++t) {
-      if (t == 0) {
-        load_keys<T, DP, FULL, NT>(a, kp, win, 0, f);
-        load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
-      }
-      const bool more = t + 1 < n;
-      const int at = (t + 1) % kSpan * L::kGroups;
-      int nb = b, nh = h;
-      f32x4 s[1][L::kGroups];
-      score_tile<T, DP, 1>(f, qf, s);
-      if (more) {
-        if (at == 0) fill(t + 1);
-        nb = __builtin_amdgcn_readlane(row, at);
-        nh = __builtin_amdgcn_readlane(head, at);
-        load_keys<T, DP, FULL, NT>(a, kp, win, at, f);
-      }
-      const bool ends = !more || nb != b || (nh >> 1) != (h >> 1);
-      if (more && ends) load_own_queries<T, DP, FULL>(a, nb, nh >> 1, qf);
-      attend_tile<T, DP, 1, true>(a, f, s, st);
-      if (more) load_values<T, DP, FULL, NT>(a, vp, win, at, f);
-      if (ends) {
-        store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
-        st.reset();
-        b = nb;
-        h = nh;
-      }
     }
   }
 }
@@ -740,7 +731,8 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
 // own tokens: 133 us without, 115 with; 64 x 1, 50 MB, called again and again: 31.5
 // and 34.3).
 template <typename T, int DP, bool FULL>
-__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum, const int* ctx) {
+__device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum,
+                                           const int* ctx) {
   if ((int64_t)total * Tile<T, DP>::kKeys * 2 * a.D * (int)sizeof(T) > (int64_t)192 << 20)
     attend_own<T, DP, FULL, true>(a, wave_index, seg, total, cum, ctx);
   else
@@ -749,7 +741,8 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
 
 // The same for any S, a run at a time.
 template <typename T, int DP>
-__device__ __forceinline__ void attend_own_any(const SharedArgs& a, int wave_index, int seg, int total, const int* cum, const int* ctx) {
+__device__ __forceinline__ void attend_own_any(const SharedArgs& a, int wave_index, int seg, int total, const int* cum,
+                                               const int* ctx) {
   using L = Tile<T, DP>;
   if ((int64_t)wave_index * seg >= total) return;
   const int stop = min(total, wave_index * seg + seg);
@@ -780,7 +773,8 @@ __device__ __forceinline__ int64_t shared_slot(const SharedArgs& a, int kvh, int
 // in LDS do not take: the workgroup's wavefronts take every fourth tile of a piece
 // (a tile of the list is four of theirs) and join in LDS.
 template <typename T, int DP, int NQ, bool UNI, bool FULL>
-__device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int seg, JoinSpace<DP, NQ, kSplitWaves>& space) {
+__device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int seg,
+                                              JoinSpace<DP, NQ, kSplitWaves>& space) {
   using L = Tile<T, DP>;
   const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int total = a.s_units * a.s_tiles, step = kSplitWaves * L::kKeys;
@@ -796,7 +790,8 @@ __device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int s
     if (r0 >= a.B * a.G) continue;
     load_queries<T, DP, NQ, FULL>(a, kvh, r0, a.B * a.G, qf);
     st.reset();
-    stream_tiles<T, DP, NQ, UNI, FULL>(a, 0, kvh, tile * step + wave * L::kKeys, step, min(a.P, (tile + n) * step), qf, st);
+    stream_tiles<T, DP, NQ, UNI, FULL>(a, 0, kvh, tile * step + wave * L::kKeys, step, min(a.P, (tile + n) * step), qf,
+                                       st);
     __syncthreads();  // the joins before are done with the space
     join_waves<T>(a, st, wave, 16 * NQ, space, [&](int row, int d, f32x4 o, float m, float l) {
       const int64_t slot = shared_slot(a, kvh, r0 + row, r0, tile == 0, wg);
@@ -827,13 +822,16 @@ __global__ void __launch_bounds__(64 * kSplitWaves, DP > 128 ? 1 : 2) paged_shar
 }
 
 // ------------------------------------------------- shared tiles in LDS
-// More than 32 query rows: the workgroup's four wavefronts hold 16 QB rows each and
-// read the same 64-key tiles from LDS, copied there straight from memory one tile
-// ahead, so a key is read from L2 once per 64 QB rows. Each wavefront copies 16 of
-// a tile's rows: one group of the block table's, at a scalar base. As in
-// paged_prefill_tr, S^T's rows are the keys 32 c + 8 (r / 4) + 4 h + r % 4 for block
-// 2 c + h, which puts 8 consecutive keys of its column into a lane, and V^T comes
-// out of ds_read_b64_tr_b16; the weights' sums are one more product, with ones.
+// For more query rows than registers hold: the workgroup's four wavefronts hold 16 QB
+// rows each and read the same 64-key tiles from LDS, copied there straight from
+// memory one tile ahead, so a key is read from L2 once per 64 QB rows (128 x 32 heads
+// on 8 KV heads over 65 536 tokens: 360 us from registers with 64 rows to a
+// wavefront, 204 through LDS). Each wavefront copies 16 of a tile's rows: one group
+// of the block table's, at a scalar base. As in paged_prefill_tr, S^T's rows are the
+// keys 32 c + 8 (r / 4) + 4 h + r % 4 for block 2 c + h, which puts 8 consecutive keys
+// of its column into a lane, and V^T comes out of ds_read_b64_tr_b16; the weights'
+// sums are one more product, with ones. s_setprio puts a wavefront's products before
+// the other's softmax on its SIMD (156 -> 149 us without own tokens).
 template <typename T, int DP, int QB>
 struct LdsState {
   f32x4 acc[QB][DP / 16], sum[QB];
@@ -853,7 +851,8 @@ __device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char*
   auto read = [&](int kb) {
 #pragma unroll
     for (int f = 0; f < DP / 32; ++f)
-      kv[kb & 1][f] = *(const uint4*)(kl + (kr + 32 * (kb >> 1) + 4 * (kb & 1)) * kRowB + (((4 * f + g) ^ k_swz<kCPR>(kr)) << 4));
+      kv[kb & 1][f] = *(const uint4*)(kl + (kr + 32 * (kb >> 1) + 4 * (kb & 1)) * kRowB +
+                                      (((4 * f + g) ^ k_swz<kCPR>(kr)) << 4));
   };
   read(0);
   __builtin_amdgcn_s_setprio(1);
@@ -874,7 +873,8 @@ __device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char*
   const int vrow = 8 * g + (col >> 2), vq = lane & 3;
   uint4 vv[DP / 16];
   auto value = [&](int h, int t) {
-    const uint32_t at = vl + vrow * kRowB + ((vq & 1) << 3) + (((2 * t + (vq >> 1)) ^ v_swz<kCPR>(vrow)) << 4) + 32 * h * kRowB;
+    const uint32_t at = vl + (vrow + 32 * h) * kRowB + ((vq & 1) << 3) +
+                        (((2 * t + (vq >> 1)) ^ v_swz<kCPR>(vrow)) << 4);
     const uint2 lo = TrRead<T>::at(at), hi = TrRead<T>::at(at + 4 * kRowB);
     vv[t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
   };
@@ -979,7 +979,8 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
       if (i % 64 == 0) {
         counts = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) counts |= (uint32_t)(entry[j] < 0 ? 0 : max(0, min(16, a.P - tok - 16 * j))) << (8 * j);
+        for (int j = 0; j < 4; ++j)
+          counts |= (uint32_t)(entry[j] < 0 ? 0 : max(0, min(16, a.P - tok - 16 * j))) << (8 * j);
         const int e = wave == 0 ? entry[0] : wave == 1 ? entry[1] : wave == 2 ? entry[2] : entry[3];
         win = make_window<T>(a, e, tok + 16 * wave, a.P, kvh);
         tok += 64 * 64;
@@ -1004,8 +1005,9 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
         for (int c = 0; c < kCopies; ++c) {
           const int kc = k_chunk(c, l), vc = v_chunk(c, l);
           const bool ok = copy_row(c, l) < m;
-          const void* ks = ok && kc * 8 < a.D ? (const void*)(kb + ko[c]) : (const void*)(kZeroRow + kc * 16);
-          const void* vs = ok && vc * 8 < a.D ? (const void*)(vb + vo[c]) : (const void*)(kZeroRow + vc * 16);
+          const char* zero = (const char*)kZeroRow;
+          const char* ks = ok && kc * 8 < a.D ? kb + ko[c] : zero + kc * 16;
+          const char* vs = ok && vc * 8 < a.D ? vb + vo[c] : zero + vc * 16;
           copy16_to_lds(ks, kd + 1024 * c);
           copy16_to_lds(vs, vd + 1024 * c);
         }
@@ -1041,7 +1043,8 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
       wait_and_barrier<0>();  // tile i has landed, and tile i - 1 is done with
       if (i + 1 < n) copy(i + 1, S ^ 1);
       any |= now != 0;
-      if (active) attend_lds_tile<T, DP, QB>(a, lds + S * 2 * kTileB, lds_addr(lds) + S * 2 * kTileB + kTileB, now, qf, st);
+      if (active)
+        attend_lds_tile<T, DP, QB>(a, lds + S * 2 * kTileB, lds_addr(lds) + S * 2 * kTileB + kTileB, now, qf, st);
     };
     for (int i = 0; i < n; i += 2) {
       turn(i, Stage<0>{});
@@ -1051,7 +1054,8 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
     for (int q = 0; q < QB; ++q) {
       const int64_t slot = shared_slot(a, kvh, mine + 16 * q + col, r0, tile0 == 0, wg);
       if (slot < 0) continue;
-      if (lane < 16) a.ws_ml[slot] = make_float2(st.m[q] == kNegInf ? kNegInf : st.mc[q], coded_sum(st.sum[q][0], any));
+      if (lane < 16)
+        a.ws_ml[slot] = make_float2(st.m[q] == kNegInf ? kNegInf : st.mc[q], coded_sum(st.sum[q][0], any));
       float* out = a.ws_acc + slot * a.D + 4 * g;
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t)
@@ -1104,7 +1108,8 @@ __global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
   }
   const int n = live ? shared + pieces : 0;
   auto slot = [&](int i) -> int64_t {
-    if (i < shared) return i == 0 ? unit : a.s_cont + ((int64_t)(s0 + i) * a.team + member) * a.set_rows + r % a.set_rows;
+    if (i < shared)
+      return i == 0 ? unit : a.s_cont + ((int64_t)(s0 + i) * a.team + member) * a.set_rows + r % a.set_rows;
     i -= shared;
     return i == 0 ? a.own_slot + unit : a.own_cont + (int64_t)(w0 + i) * 16 + (g - set * 16);
   };
@@ -1255,16 +1260,19 @@ hipError_t launch_tiles(const SharedArgs& a, hipStream_t stream) {
     if (a.row_tiles == 2) fn = (const void*)&paged_shared_split<T, DP, 2, UNI, FULL>;
   if constexpr (sizeof(T) == 2 && DP <= 128 && UNI) {
     if (a.lds_tiles)
-      fn = a.row_tiles == 2 ? (const void*)&paged_shared_split_lds<T, DP, 2, FULL> : (const void*)&paged_shared_split_lds<T, DP, 1, FULL>;
+      fn = a.row_tiles == 2 ? (const void*)&paged_shared_split_lds<T, DP, 2, FULL>
+                            : (const void*)&paged_shared_split_lds<T, DP, 1, FULL>;
   }
   const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)a.wgs), dim3(64 * kSplitWaves), kargs, 0, stream);
   if (e != hipSuccess) return e;
   // Four wavefronts join a row's pieces where there are many: at most so many of either kind.
   const int64_t units = (int64_t)a.B * a.Hq;
-  const int64_t most = 2 + (int64_t)a.wgs * kSplitWaves / ((int64_t)a.B * a.vheads) + (a.s_units ? a.wgs / (a.s_units * a.team) : 0);
+  const int64_t most = 2 + (int64_t)a.wgs * kSplitWaves / ((int64_t)a.B * a.vheads) +
+                       (a.s_units ? a.wgs / (a.s_units * a.team) : 0);
   if (most > 24)
     return hipLaunchKernel((const void*)&paged_shared_join<T, 4>, dim3((unsigned)units), dim3(256), kargs, 0, stream);
-  return hipLaunchKernel((const void*)&paged_shared_join<T, 1>, dim3((unsigned)((units + 3) / 4)), dim3(256), kargs, 0, stream);
+  return hipLaunchKernel((const void*)&paged_shared_join<T, 1>, dim3((unsigned)((units + 3) / 4)), dim3(256), kargs, 0,
+                         stream);
 }
 
 template <typename T, int DP>
@@ -1278,9 +1286,12 @@ hipError_t launch_type(const SharedArgs& a, hipStream_t stream) {
   if (!a.tiles) {
     SharedArgs c = a;
     void* kargs[] = {&c};
-    return hipLaunchKernel((const void*)&paged_shared_any<T>, dim3((unsigned)a.Hq, (unsigned)a.B), dim3(64), kargs, 0, stream);
+    return hipLaunchKernel((const void*)&paged_shared_any<T>, dim3((unsigned)a.Hq, (unsigned)a.B), dim3(64), kargs, 0,
+                           stream);
   }
-  return a.D <= 64 ? launch_width<T, 64>(a, stream) : a.D <= 128 ? launch_width<T, 128>(a, stream) : launch_width<T, 256>(a, stream);
+  return a.D <= 64    ? launch_width<T, 64>(a, stream)
+         : a.D <= 128 ? launch_width<T, 128>(a, stream)
+                      : launch_width<T, 256>(a, stream);
 }
 
 }  // namespace

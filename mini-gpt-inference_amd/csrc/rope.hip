@@ -282,7 +282,8 @@ template <typename TI, typename TO>
 const void* rope_kernel(int chunk, int interleaved) {
   if (chunk == 0) return (const void*)&rope_any<TI, TO>;
   if constexpr (sizeof(TI) == 2)
-    if (chunk == 8) return interleaved ? (const void*)&rope_vec<TI, TO, 8, true> : (const void*)&rope_vec<TI, TO, 8, false>;
+    if (chunk == 8)
+      return interleaved ? (const void*)&rope_vec<TI, TO, 8, true> : (const void*)&rope_vec<TI, TO, 8, false>;
   return interleaved ? (const void*)&rope_vec<TI, TO, 4, true> : (const void*)&rope_vec<TI, TO, 4, false>;
 }
 

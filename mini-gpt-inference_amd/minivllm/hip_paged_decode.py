@@ -8,7 +8,7 @@ paged_attention_batch_online_v1:
     block_tables:    [B, M] (logical -> physical; -1 only in the unused tail)
     context_lengths: [B] (>= 1, include the KV written this step)
 
-Both entry points validate on the host exactly like
+The entry points validate on the host exactly like
 paged_attention_batch_triton_v0 (minivllm/triton_paged_decode.py:109-144):
 ValueError for contract violations, RuntimeError when the HIP library or its
 PyTorch binding is unavailable. The checks, allocations and launches run in
@@ -28,9 +28,11 @@ minivllm/attention.py:229-267): causal attention of one chunk's queries over
 the sequence's cached prefix and the chunk itself, read from the pool.
 
 qk_norm_rope_hip and kv_append_rope_hip norm and rotate query and key heads by
-their positions, the latter on the way into the pool. They are inference-only
-(RuntimeError for tensors that require gradients while grad mode is on) and run
-on their tensors' device, current or not.
+their positions, the latter on the way into the pool.
+paged_attention_shared_prefix_hip is decode attention, with grouped query
+heads, for sequences that begin with the same cached blocks. These three are
+inference-only (RuntimeError for tensors that require gradients while grad mode
+is on) and run on their tensors' device, current or not.
 """
 from __future__ import annotations
 
