@@ -357,7 +357,8 @@ size_t mgi_decode_linear_norm_workspace_bytes(int64_t B, int64_t N, int64_t K);
  * position is outside the table has no angles: its rotated dims come out NaN.
  * q_weight, k_weight: [D] contiguous, of weight_dtype (dtype or MGI_F32), or both
  * null. q, k, q_out, k_out share one dtype and have any strides; the outputs must
- * not overlap the inputs. D <= 512.
+ * not overlap the inputs. D <= 512, Hq and Hk <= 65535, T < 2^24,
+ * T*(Hq + 2*Hk) < 2^25.
  */
 int mgi_qk_norm_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
                      void* k_out, const int64_t* k_out_strides, /* [3] */
@@ -408,8 +409,9 @@ int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
  * included; a sequence shorter than shared_blocks * S reads its first tokens from
  * row 0's blocks all the same, by itself. Lengths are clamped to [0, M*S], a table
  * entry outside [0, N) masks its block, a row without keys gives 0, and only the
- * tokens of some row's context enter any result. Arithmetic is f32, but that 2-byte types round
- * the softmax weights to their type for the second product (as mgi_paged_prefill).
+ * tokens of some row's context enter any result. Arithmetic is f32, but that
+ * 2-byte types round the softmax weights to their type for the second product
+ * (as mgi_paged_prefill).
  * 0 <= shared_blocks <= M. B <= 65535, B*Hq < 2^25, M*S < 2^30, D <= 512.
  *
  * workspace: mgi_paged_decode_shared_workspace_bytes(...) bytes for the same sizes,

@@ -44,7 +44,7 @@
 // VALU work beside the products (37 % of cycles in the matrix cores, LDS conflicts
 // none; with all keys in L2 it still takes 141 of the 146 us without own tokens).
 // Calls under about 30 us are chains: launch and the rows' prefix sums 4 us, a first
-// tile 3, the joining launch 5-8 us.
+// tile 3, the joining launch 5-7 us.
 #pragma once
 
 #include <type_traits>
@@ -1114,12 +1114,21 @@ __global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
     return i == 0 ? a.own_slot + unit : a.own_cont + (int64_t)(w0 + i) * 16 + (g - set * 16);
   };
   const int lpr = a.D <= 64 ? 16 : a.D <= 128 ? 32 : 64, at = lane / lpr, d = 4 * (lane % lpr), per = 64 / lpr;
+  constexpr int kEarly = 8;
   float top = kNegInf, sum = 0.f;
   bool dead = false;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   const int share = (n + JW - 1) / JW, stop = min(n, (wave % JW + 1) * share);  // the wavefront's pieces
   for (int i0 = wave % JW * share; i0 < stop; i0 += 64) {
     const int m = min(64, stop - i0);
+    // The first pieces' rows load beside the weights that say whether they count (64 x 8
+    // heads, some 20 pieces each: 6.6 us after them, 5.5 so; 128 x 32: 11.2 and 9.8).
+    f32x4 early[kEarly];
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j) {
+      const int i = j * per + at;
+      early[j] = i < m && d < a.D ? *(const f32x4*)(a.ws_acc + slot(i0 + i) * a.D + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     const float2 x = lane < m ? a.ws_ml[slot(i0 + lane)] : make_float2(kNegInf, 0.f);
     const bool counts = !(x.y <= 0.f);
     dead |= x.y < 0.f;
@@ -1129,9 +1138,16 @@ __global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
     sum = sum * alpha + wave_sum(counts ? x.y * w : 0.f);
     acc *= alpha;
     top = mn;
+    // Every lane takes part in the exchanges: a lane reads one that is switched off as 0.
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j) {
+      if (j * per >= m) break;
+      const float wi = __shfl(w, j * per + at, 64);
+      const int use = __shfl((int)counts, j * per + at, 64);
+      if (use && j * per + at < m) acc += wi * early[j];
+    }
 #pragma unroll 8
-    for (int i = 0; i < m; i += per) {
-      // Every lane takes part in the exchange: a lane reads one that is switched off as 0.
+    for (int i = kEarly * per; i < m; i += per) {
       const float wi = __shfl(w, i + at, 64);
       const int use = __shfl((int)counts, i + at, 64);
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
