@@ -681,6 +681,15 @@ int launch_append(const AppendSpec& ap, const int64_t* k_pool_strides, const int
   return MGI_OK;
 }
 
+// n / d = umulhi(n, mul) >> shift for 0 <= n < 2^31 and d >= 2: with 2^(s-1) < d <=
+// 2^s, mul = ceil(2^(31+s) / d) exceeds the quotient by less than 2^s / d.
+void magic_of(int64_t d, uint32_t* mul, int* shift) {
+  int s = 1;
+  while ((int64_t(1) << s) < d) ++s;
+  *mul = d < 2 ? 0 : (uint32_t)(((uint64_t(1) << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d);
+  *shift = s - 1;
+}
+
 // The arguments mgi_qk_norm_rope and mgi_kv_append_rope share.
 struct RopeSpec {
   void* q_out;
@@ -769,9 +778,16 @@ int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
   };
   const bool unit =
       a.q_sd == 1 && a.k_sd == 1 && a.qo_sd == 1 && a.ko_sd == 1 && (!a.Hv || (a.v_sd == 1 && a.vo_sd == 1));
+  // Offsets are products of two 31-bit numbers.
+  bool narrow = a.P < (int64_t(1) << 31) && (!a.slots || a.N < (int64_t(1) << 31) / a.S);
+  for (int64_t x : {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh, a.qo_st, a.qo_sh, a.ko_sn, a.ko_st, a.ko_sh,
+                    a.vo_sn, a.vo_st, a.vo_sh, a.pos_s, a.sl_s, a.table_s})
+    narrow &= x < (int64_t(1) << 31);
+  magic_of(a.Hq + a.Hk + a.Hv, &a.h_mul, &a.h_shift);
+  if (a.slots) magic_of(a.S, &a.s_mul, &a.s_shift);
   a.chunk = 0;
   for (int c : {8, 4}) {
-    if (c * eb > 16 || !unit || (a.R / 2) % c || (a.D - a.R) % (2 * c)) continue;
+    if (c * eb > 16 || !unit || !narrow || (a.R / 2) % c || (a.D - a.R) % (2 * c)) continue;
     if (fits(c * (a.w_f32 ? 4 : eb), {a.qw, a.kw}, {}, 1) &&
         fits(c * eb, {a.q, a.k, a.v}, {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh}, eb) &&
         fits(c * ob, {a.q_out, a.k_out, a.v_out},
@@ -864,15 +880,6 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   p.cum_offset = (size_t)round_up((int64_t)p.ml_offset + p.slots * 8, kWorkspaceAlign);
   p.total = p.cum_offset + (size_t)(B * 4 + 8);
   return p;
-}
-
-// n / d = umulhi(n, mul) >> shift for 0 <= n < 2^31 and d >= 2: with 2^(s-1) < d <=
-// 2^s, mul = ceil(2^(31+s) / d) exceeds the quotient by less than 2^s / d.
-void magic_of(int64_t d, uint32_t* mul, int* shift) {
-  int s = 1;
-  while ((int64_t(1) << s) < d) ++s;
-  *mul = d < 2 ? 0 : (uint32_t)(((uint64_t(1) << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d);
-  *shift = s - 1;
 }
 
 // Checks the two decode-step linear calls share.

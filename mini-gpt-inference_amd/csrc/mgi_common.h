@@ -58,6 +58,11 @@ template <> struct Elem<f16_t> {
   __device__ static void store(f16_t* p, float x) { p->bits = f32_to_f16(x); }
 };
 
+// n / d for 0 <= n < 2^31 (see magic_of).
+__device__ __forceinline__ int fast_div(int n, uint32_t mul, int shift, int d) {
+  return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift);
+}
+
 // ------------------------------------------------------------ index loading
 
 // Loads element i of an int32 or int64 index array (wave-uniform when the
@@ -66,6 +71,21 @@ __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i
   return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }
 
+// Element i of an int32 or int64 array: both words of an int64, the same word twice of
+// an int32. Without a branch, whose end would wait for the load.
+struct Index {
+  uint32_t lo, hi;
+  __device__ __forceinline__ void load(const void* p, int is64, uint64_t i) {
+    const char* at = (const char*)p + (i << (is64 ? 3 : 2));
+    int second = is64 ? 4 : 0;
+    asm volatile("" : "+s"(second));  // kept as an offset
+    lo = *(const uint32_t*)at;
+    hi = *(const uint32_t*)(at + second);
+  }
+  __device__ __forceinline__ int64_t value(int is64) const {
+    return (int64_t)((uint64_t)lo | ((uint64_t)(is64 ? hi : (uint32_t)((int)lo >> 31)) << 32));
+  }
+};
 // -------------------------------------------------------------- DPP / swizzle
 
 // DPP controls (gfx9 encoding).

@@ -107,6 +107,8 @@ struct RopeArgs {
   int interleaved;
   int chunk;           // elements of a lane's chunk (8 or 4), 0: the kernel for any strides
   int gp_shift;        // log2(lanes per head row), set by the launcher
+  uint32_t h_mul, s_mul;  // division by Hq + Hk + Hv and by S (magic_of)
+  int h_shift, s_shift;
   int cus;
 };
 hipError_t launch_rope(const RopeArgs& a, int in_dtype, int out_dtype, hipStream_t stream);

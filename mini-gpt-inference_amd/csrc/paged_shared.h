@@ -136,11 +136,6 @@ struct State {
   }
 };
 
-// n / d for 0 <= n < 2^31 (see magic_of).
-__device__ __forceinline__ int fast_div(int n, uint32_t mul, int shift, int d) {
-  return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift);
-}
-
 // Entry j of row b's table: the shared blocks are row 0's.
 __device__ __forceinline__ int64_t table_entry(const SharedArgs& a, int b, int j) {
   return load_index(a.bt, a.bt_i64, (int64_t)(j < a.shared ? 0 : b) * a.bt_sb + (int64_t)j * a.bt_sm);
@@ -156,13 +151,20 @@ struct Window {
   int n;
 };
 
-// The lane's table entry (-1: none, or outside the pool) for its group, whose first
-// token is tok. Entries past a row's length are read too (and not used), so that the
-// load does not wait for the length.
-__device__ __forceinline__ int window_entry(const SharedArgs& a, int b, int tok) {
-  if (tok >= a.M * a.S) return -1;
-  const int64_t id = table_entry(a, b, fast_div(tok, a.s_mul, a.s_shift, a.S));
-  return id >= 0 && id < a.N ? (int)id : -1;
+// The lane's table entry, as loaded, for its group, whose first token is tok. Entries
+// past a row's length are read too (and not used), so that the load does not wait for
+// the length; past the table its last one stands in, as a load under a condition is
+// waited for where the condition ends, with all others in flight.
+__device__ __forceinline__ Index window_entry(const SharedArgs& a, int b, int tok) {
+  const int j = fast_div(min(tok, a.M * a.S - 1), a.s_mul, a.s_shift, a.S);
+  Index x;
+  x.load(a.bt, a.bt_i64, (uint64_t)(j < a.shared ? 0 : b) * (uint64_t)a.bt_sb + (uint64_t)j * (uint64_t)a.bt_sm);
+  return x;
+}
+// The entry's block, -1 for none or one outside the pool.
+__device__ __forceinline__ int entry_block(const SharedArgs& a, const Index& x, int tok) {
+  const int64_t id = x.value(a.bt_i64);
+  return tok < a.M * a.S && id >= 0 && id < a.N ? (int)id : -1;
 }
 template <typename T>
 __device__ __forceinline__ Window make_window(const SharedArgs& a, int id, int tok, int end, int kvh) {
@@ -185,8 +187,8 @@ __device__ __forceinline__ V load_piece(const char* p) {
 }
 
 // Loads the keys, and the values, of the tile whose groups are lanes at .. of the
-// window (kp, vp: the pools). Rows past a group's last key read that one again.
-// FULL: D == DP.
+// window (kp, vp: the pools). Rows past a group's last key read that one again, chunks
+// past D zeros: no load is under a condition. FULL: D == DP.
 template <typename T, int DP, bool FULL, bool NT = false>
 __device__ __forceinline__ void load_keys(const SharedArgs& a, const char* kp, const Window& w, int at, Tile<T, DP>& f) {
   using L = Tile<T, DP>;
@@ -198,9 +200,14 @@ __device__ __forceinline__ void load_keys(const SharedArgs& a, const char* kp, c
     const char* base = kp + lane_offset(w.k_lo, w.k_hi, at + g);
     const uint32_t off = (uint32_t)min(row, max(n, 1) - 1) * ss + (uint32_t)kg * 16;
 #pragma unroll
-    for (int s = 0; s < L::kKS; ++s)
-      f.k[g][s] = FULL || (kg + 4 * s) * L::kCE < a.D ? load_piece<NT, uint4>(base + off + 64 * s)
-                                                      : make_uint4(0, 0, 0, 0);
+    for (int s = 0; s < L::kKS; ++s) {
+      if constexpr (FULL) {
+        f.k[g][s] = load_piece<NT, uint4>(base + off + 64 * s);
+      } else {
+        const bool in = (kg + 4 * s) * L::kCE < a.D;
+        f.k[g][s] = load_piece<NT, uint4>(in ? base + off + 64 * s : (const char*)kZeroRow);
+      }
+    }
   }
 }
 template <typename T, int DP, bool FULL, bool NT = false>
@@ -220,10 +227,11 @@ __device__ __forceinline__ void load_values(const SharedArgs& a, const char* vp,
     for (int j = 0; j < 4; ++j) {
       const uint32_t off = (uint32_t)min(4 * kg + j, max(n, 1) - 1) * ss + col;
 #pragma unroll
-      for (int h = 0; h < L::kHF; ++h)
-        f.v[4 * g + j][h] = FULL || 16 * L::kEV * h + row * L::kEV < a.D
-                                ? load_piece<NT, V>(base + off + 16 * L::kEV * (int)sizeof(T) * h)
-                                : V{};
+      for (int h = 0; h < L::kHF; ++h) {
+        // Dims past D load the row's first ones and are not stored.
+        const bool in = FULL || 16 * L::kEV * h + row * L::kEV < a.D;
+        f.v[4 * g + j][h] = load_piece<NT, V>(base + (in ? off + 16 * L::kEV * (uint32_t)sizeof(T) * h : off - col));
+      }
     }
   }
 }
@@ -402,7 +410,8 @@ __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh
   const char* vp = (const char*)a.v + (int64_t)kvh * a.v_sh * (int)sizeof(T);
   constexpr int kSpan = 64 / L::kGroups;  // tiles of a window
   const int lane = (int)threadIdx.x & 63;
-  int tok = 0, entry = -1;                // the lane's group of the next window
+  int tok = 0;  // the lane's group of the next window
+  Index entry = {0, 0};
   Window win{};
   if constexpr (UNI) {
     tok = first + lane / L::kGroups * step + 16 * (lane % L::kGroups);
@@ -413,7 +422,7 @@ __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh
   auto keys = [&](int i) {
     if constexpr (UNI) {
       if (i % kSpan == 0) {
-        win = make_window<T>(a, entry, tok, end, kvh);
+        win = make_window<T>(a, entry_block(a, entry, tok), tok, end, kvh);
         tok += kSpan * step;
         entry = window_entry(a, b, tok);
       }
@@ -429,17 +438,21 @@ __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh
   const int n = (end - first + step - 1) / step;
   f32x4 s[NQ][L::kGroups];
   keys(0);
+  __builtin_amdgcn_sched_barrier(0);  // keys before values, as in the loop: their wait leaves the values in flight
   values(0);
-  for (int i = 0; i < n; ++i) {
+  __builtin_amdgcn_sched_barrier(0);
+  for (int i = 0; i + 1 < n; ++i) {
     score_tile<T, DP, NQ>(f, qf, s);
-    if (i + 1 < n) keys(i + 1);
+    keys(i + 1);
     attend_tile<T, DP, NQ, UNI>(a, f, s, st);
-    if (i + 1 < n) values(i + 1);
+    values(i + 1);
   }
+  score_tile<T, DP, NQ>(f, qf, s);  // the last apart: loads under no condition in the loop
+  attend_tile<T, DP, NQ, UNI>(a, f, s, st);
 }
 
 // Query fragments of NQ x 16 rows of one KV head's query heads: row r is sequence
-// r / G's head r % G, from row r0 on; rows past `rows` are zero.
+// r / G's head r % G, from row r0 on; past `rows` the last one again (and not stored).
 template <typename T, int DP, int NQ, bool FULL>
 __device__ __forceinline__ void load_queries(const SharedArgs& a, int kvh, int r0, int rows,
                                              uint4 (&qf)[NQ][Tile<T, DP>::kKS]) {
@@ -447,17 +460,23 @@ __device__ __forceinline__ void load_queries(const SharedArgs& a, int kvh, int r
   const int lane = (int)threadIdx.x & 63, kg = lane >> 4;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    const int r = r0 + 16 * q + (lane & 15), bb = fast_div(r, a.g_mul, a.g_shift, a.G), g = r - bb * a.G;
+    const int r = min(r0 + 16 * q + (lane & 15), rows - 1), bb = fast_div(r, a.g_mul, a.g_shift, a.G), g = r - bb * a.G;
     const T* p = (const T*)a.q + (int64_t)bb * a.q_sb + (int64_t)(kvh * a.G + g) * a.q_sh + kg * L::kCE;
 #pragma unroll
     for (int s = 0; s < L::kKS; ++s) {
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < rows && (FULL || (kg + 4 * s) * L::kCE < a.D)) {
-        x = *(const uint4*)(p + 4 * L::kCE * s);
-        x = make_uint4(x.x ^ a.q_flip, x.y ^ a.q_flip, x.z ^ a.q_flip, x.w ^ a.q_flip);
-      }
-      qf[q][s] = a.q_zero ? make_uint4(0, 0, 0, 0) : x;
+      if constexpr (FULL) qf[q][s] = *(const uint4*)(p + 4 * L::kCE * s);
+      else qf[q][s] = *((kg + 4 * s) * L::kCE < a.D ? (const uint4*)(p + 4 * L::kCE * s) : (const uint4*)kZeroRow);
     }
+  }
+  if (a.q_flip | a.q_zero) {  // a scale that is not positive
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int s = 0; s < L::kKS; ++s) {
+        const uint4 x = qf[q][s];
+        qf[q][s] = a.q_zero ? make_uint4(0, 0, 0, 0)
+                            : make_uint4(x.x ^ a.q_flip, x.y ^ a.q_flip, x.z ^ a.q_flip, x.w ^ a.q_flip);
+      }
   }
 }
 
@@ -687,7 +706,7 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
     if (u < u0 + n) {
       const OwnTile o = find_own(a, cum, u);
       const int c = ctx[o.b], tok = (c < a.P ? 0 : a.P) + o.tile * L::kKeys + 16 * (lane % L::kGroups);
-      win = make_window<T>(a, window_entry(a, o.b, tok), tok, c, o.vh / a.gsets);
+      win = make_window<T>(a, entry_block(a, window_entry(a, o.b, tok), tok), tok, c, o.vh / a.gsets);
       row = o.b;
       head = 2 * o.vh + (o.tile == 0);
     }
@@ -699,24 +718,22 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
   L f;
   f32x4 s[1][L::kGroups];
   load_own_queries<T, DP, FULL>(a, b, h >> 1, qf);
+  __builtin_amdgcn_sched_barrier(0);
   load_keys<T, DP, FULL, NT>(a, kp, win, 0, f);
+  __builtin_amdgcn_sched_barrier(0);
   load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
+  __builtin_amdgcn_sched_barrier(0);
   st.reset();
-  for (int t = 0; t < n; ++t) {  // as in stream_tiles
-    const bool more = t + 1 < n;
+  for (int t = 0; t + 1 < n; ++t) {  // as in stream_tiles
     const int at = (t + 1) % kSpan * L::kGroups;
-    int nb = b, nh = h;
     score_tile<T, DP, 1>(f, qf, s);
-    if (more) {
-      if (at == 0) fill(t + 1);
-      nb = __builtin_amdgcn_readlane(row, at);
-      nh = __builtin_amdgcn_readlane(head, at);
-      load_keys<T, DP, FULL, NT>(a, kp, win, at, f);
-    }
-    const bool ends = !more || nb != b || (nh >> 1) != (h >> 1);
-    if (more && ends) load_own_queries<T, DP, FULL>(a, nb, nh >> 1, qf);
+    if (at == 0) fill(t + 1);
+    const int nb = __builtin_amdgcn_readlane(row, at), nh = __builtin_amdgcn_readlane(head, at);
+    load_keys<T, DP, FULL, NT>(a, kp, win, at, f);
+    const bool ends = nb != b || (nh >> 1) != (h >> 1);
+    if (ends) load_own_queries<T, DP, FULL>(a, nb, nh >> 1, qf);
     attend_tile<T, DP, 1, true>(a, f, s, st);
-    if (more) load_values<T, DP, FULL, NT>(a, vp, win, at, f);
+    load_values<T, DP, FULL, NT>(a, vp, win, at, f);
     if (ends) {
       store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
       st.reset();
@@ -724,6 +741,9 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
       h = nh;
     }
   }
+  score_tile<T, DP, 1>(f, qf, s);
+  attend_tile<T, DP, 1, true>(a, f, s, st);
+  store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
 }
 
 // Own keys and values are read once a call: past what the 256 MB memory-side cache
@@ -967,24 +987,24 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
     if (r0 >= a.B * a.G) continue;  // the last block's teams may be short
     // A window of 64 tiles: lane i holds tile i's four groups' key counts and the
     // place of the wavefront's own.
-    int tok = (tile0 + lane) * 64, entry[4];
-    auto look = [&]() {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) entry[j] = window_entry(a, 0, tok + 16 * j);
-    };
     Window win{};
     uint32_t counts = 0;
     uint32_t now = 0, next = 0;  // key counts of the tile computed and of the one copied
     auto copy = [&](int i, int stage) {
       if (i % 64 == 0) {
-        counts = 0;
+        const int tok = (tile0 + i + lane) * 64;
+        Index entry[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          counts |= (uint32_t)(entry[j] < 0 ? 0 : max(0, min(16, a.P - tok - 16 * j))) << (8 * j);
-        const int e = wave == 0 ? entry[0] : wave == 1 ? entry[1] : wave == 2 ? entry[2] : entry[3];
-        win = make_window<T>(a, e, tok + 16 * wave, a.P, kvh);
-        tok += 64 * 64;
-        look();
+        for (int j = 0; j < 4; ++j) entry[j] = window_entry(a, 0, tok + 16 * j);
+        counts = 0;
+        int id_own = -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int id = entry_block(a, entry[j], tok + 16 * j);
+          counts |= (uint32_t)(id < 0 ? 0 : max(0, min(16, a.P - tok - 16 * j))) << (8 * j);
+          if (wave == j) id_own = id;
+        }
+        win = make_window<T>(a, id_own, tok + 16 * wave, a.P, kvh);
       }
       const int at = i % 64;
       next = (uint32_t)__builtin_amdgcn_readlane((int)counts, at);
@@ -1013,20 +1033,9 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
         }
       }
     };
-    look();
+    load_queries<T, DP, QB, false>(a, kvh, mine, a.B * a.G, qf);
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
-      const int r = mine + 16 * q + col, bb = fast_div(r, a.g_mul, a.g_shift, a.G);
-      const T* p = (const T*)a.q + (int64_t)bb * a.q_sb + (int64_t)(kvh * a.G + r - bb * a.G) * a.q_sh + 8 * g;
-#pragma unroll
-      for (int f = 0; f < DP / 32; ++f) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < a.B * a.G && 32 * f + 8 * g < a.D && !a.q_zero) {
-          x = *(const uint4*)(p + 32 * f);
-          x = make_uint4(x.x ^ a.q_flip, x.y ^ a.q_flip, x.z ^ a.q_flip, x.w ^ a.q_flip);
-        }
-        qf[q][f] = x;
-      }
       st.sum[q] = f32x4{0.f, 0.f, 0.f, 0.f};
       st.m[q] = kNegInf;
       st.mc[q] = 0.f;

@@ -28,6 +28,10 @@ namespace mgi {
 
 constexpr int kRopeThreads = 256;
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 // N consecutive elements from f32, with one rounding each. Pointers are aligned to the
 // chunk's bytes, 16 at most.
 template <int N>
@@ -37,25 +41,14 @@ __device__ __forceinline__ void store_chunk(float* p, const float (&x)[N]) {
 }
 template <int N, typename T>
 __device__ __forceinline__ void store_chunk(T* p, const float (&x)[N]) {
+  using Two = std::conditional_t<std::is_same_v<T, bf16_t>, bf16x2, f16x2>;
   uint32_t w[N / 2];
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
-    if constexpr (std::is_same_v<T, bf16_t>)
-      w[i] = (uint32_t)f32_to_bf16(x[2 * i]) | ((uint32_t)f32_to_bf16(x[2 * i + 1]) << 16);
-    else
-      w[i] = (uint32_t)f32_to_f16(x[2 * i]) | ((uint32_t)f32_to_f16(x[2 * i + 1]) << 16);
-  }
+  for (int i = 0; i < N / 2; ++i)
+    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, Two));
   if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
-// Element i of an int32 or int64 array without a branch (whose end would wait for the
-// load): both words of an int64, the same word twice of an int32.
-__device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
-  const char* at = (const char*)p + i * (is64 ? 8 : 4);
-  const uint32_t lo = *(const uint32_t*)at, hi = *(const uint32_t*)(at + (is64 ? 4 : 0));
-  return is64 ? (int64_t)((uint64_t)lo | ((uint64_t)hi << 32)) : (int64_t)(int32_t)lo;
-}
-
 // Where row t's key and value go: the pool's slot, or row t of k_out (no v).
 // False when nothing is to be written.
 __device__ __forceinline__ bool rope_target(const RopeArgs& a, int64_t t, bool placed, int64_t* k_off, int64_t* v_off) {
@@ -63,7 +56,7 @@ __device__ __forceinline__ bool rope_target(const RopeArgs& a, int64_t t, bool p
     *k_off = t * a.ko_st;
     return true;
   }
-  const int64_t slot = index_at(a.slots, a.sl_i64, t * a.sl_s);
+  const int64_t slot = load_index(a.slots, a.sl_i64, t * a.sl_s);
   if (!placed || slot < 0 || slot >= a.N * (int64_t)a.S) return false;
   const int64_t blk = slot / a.S, off = slot - blk * a.S;
   *k_off = blk * a.ko_sn + off * a.ko_st;
@@ -100,122 +93,165 @@ struct Raw {
   }
 };
 
-// TI: q, k, v; TO: q_out and the keys' and values' target. C: elements per chunk.
+// The sum over aligned groups of gp lanes, gp a power of two.
+__device__ __forceinline__ float group_sum(float x, int gp) {
+  if (gp > 1) x += dpp<DPP_QUAD_XOR1>(x);
+  if (gp > 2) x += dpp<DPP_QUAD_XOR2>(x);
+  if (gp > 4) x += dpp<DPP_ROW_HALF_MIRROR>(x);
+  if (gp > 8) x += dpp<DPP_ROW_MIRROR>(x);
+  if (gp > 16) x += swizzle_xor16(x);
+  if (gp > 32) x += __shfl_xor(x, 32, 64);
+  return x;
+}
+
+// n * stride, both below 2^31: one instruction, where a 64-bit stride takes three of a
+// quarter of the rate.
+__device__ __forceinline__ uint64_t times(int n, int64_t stride) { return (uint64_t)(uint32_t)n * (uint32_t)stride; }
+
+// TI: q, k, v; TO: q_out and the keys' and values' target. C: elements per chunk. All
+// strides, positions and slots are below 2^31.
 template <typename TI, typename TO, int C, bool INTER>
 __global__ void __launch_bounds__(kRopeThreads) rope_vec(const RopeArgs a) {
   const int gp = 1 << a.gp_shift;  // lanes per head row
   const int sub = (int)threadIdx.x & (gp - 1), slots = (int)blockDim.x >> a.gp_shift;
   const int heads = a.Hq + a.Hk + a.Hv, total = a.T * heads;
   // The lane's two chunks: R / 2 apart inside the rotated dims, half of the
-  // others apart past them.
+  // others apart past them. Lanes and items too many load item 0's first dims.
   const int half = a.R >> 1, rot = half / C, rest = (a.D - a.R) >> 1;
-  const bool live = sub < a.D / (2 * C), turns = sub < rot;
-  const int d0 = turns ? sub * C : a.R + (sub - rot) * C, d1 = d0 + (turns ? half : rest);
-
-  const int64_t item = (int64_t)blockIdx.x * slots + ((int)threadIdx.x >> a.gp_shift);
-  const bool in = item < total;
-  const int t = in ? (int)((uint32_t)item / (uint32_t)heads) : 0, h = in ? (int)item - t * heads : 0;
+  const int item = (int)blockIdx.x * slots + ((int)threadIdx.x >> a.gp_shift);
+  const bool in = item < total, mine = in && sub < a.D / (2 * C), turns = sub < rot;
+  const int d0 = turns ? sub * C : mine ? a.R + (sub - rot) * C : 0, d1 = d0 + (turns ? half : mine ? rest : 0);
+  const int t = in ? fast_div(item, a.h_mul, a.h_shift, heads) : 0, h = in ? item - t * heads : 0;
   const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hk;
   const int hh = is_q ? h : is_v ? h - a.Hq - a.Hk : h - a.Hq;
-  const bool mine = in && live;
-  const int64_t pos = index_at(a.positions, a.pos_i64, t * a.pos_s);
+  // These loads are under no condition, so that waiting for the position leaves the
+  // others on their way.
+  Index at_pos, at_slot;
+  at_pos.load(a.positions, a.pos_i64, times(t, a.pos_s));
+  at_slot.load(a.slots ? a.slots : a.positions, a.slots ? a.sl_i64 : a.pos_i64, times(t, a.slots ? a.sl_s : a.pos_s));
   Raw<TI, C> x[2];
-  if (mine) {
-    const TI* src = is_q   ? (const TI*)a.q + t * a.q_st + (int64_t)hh * a.q_sh
-                    : is_v ? (const TI*)a.v + t * a.v_st + (int64_t)hh * a.v_sh
-                           : (const TI*)a.k + t * a.k_st + (int64_t)hh * a.k_sh;
-    x[0].load(src + d0);
-    x[1].load(src + d1);
+  const TI* src = (const TI*)(is_q ? a.q : is_v ? a.v : a.k);
+  src += times(t, is_q ? a.q_st : is_v ? a.v_st : a.k_st) + times(hh, is_q ? a.q_sh : is_v ? a.v_sh : a.k_sh);
+  x[0].load(src + d0);
+  x[1].load(src + d1);
+  const int64_t pos = at_pos.value(a.pos_i64), slot = at_slot.value(a.sl_i64);
+  const bool placed = pos >= 0 && pos < a.P;
+  // Half-split: pairs (d0 + i, d1 + i) with cs[i]. Interleaved: pair i of the
+  // first chunk with cs[i], of the second with cs[C/2 + i].
+  float cs[C], sn[C];
+  const float* line = a.table + times(placed ? (int)pos : 0, a.table_s);
+  const int a0 = turns ? d0 : 0, a1 = turns ? d1 : half;  // lanes without pairs load some angles
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int p = INTER ? (i < C / 2 ? a0 / 2 + i : a1 / 2 + i - C / 2) : a0 + i;
+    cs[i] = line[p], sn[i] = line[half + p];
   }
-  float w[2][C];  // the norm's weights
-  if (a.qw && mine && !is_v) {
+  // The norm's weights as loaded: C words of f32, else C / 2.
+  uint32_t wr[2][C];
+  if (a.qw) {
+    const void* p = is_q ? a.qw : a.kw;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const void* p = is_q ? a.qw : a.kw;
       const int d = s ? d1 : d0;
       if (a.w_f32) {
-        Raw<float, 4> r[C / 4];
 #pragma unroll
-        for (int i = 0; i < C / 4; ++i) r[i].load((const float*)p + d + 4 * i);
-#pragma unroll
-        for (int i = 0; i < C; ++i) w[s][i] = r[i / 4][i % 4];
+        for (int i = 0; i < C; i += 4) {
+          const uint4 v = *(const uint4*)((const float*)p + d + i);
+          wr[s][i] = v.x, wr[s][i + 1] = v.y, wr[s][i + 2] = v.z, wr[s][i + 3] = v.w;
+        }
       } else if constexpr (sizeof(TI) == 2) {
         Raw<TI, C> r;
         r.load((const TI*)p + d);
 #pragma unroll
-        for (int i = 0; i < C; ++i) w[s][i] = r[i];
+        for (int i = 0; i < C / 2; ++i) wr[s][i] = r.w[i];
       }
     }
   }
-  const bool placed = pos >= 0 && pos < a.P;
-  int64_t k_off = 0, v_off = 0;
-  const bool keeps = is_q || (in && rope_target(a, t, placed, &k_off, &v_off));
-  TO* dst = is_q   ? (TO*)a.q_out + t * a.qo_st + (int64_t)hh * a.qo_sh
-            : is_v ? (TO*)a.v_out + v_off + (int64_t)hh * a.vo_sh
-                   : (TO*)a.k_out + k_off + (int64_t)hh * a.ko_sh;
-  float y[2][C];
+  // Where the row goes: q_out, or k_out or the pools.
+  TO* dst = (TO*)(is_q ? a.q_out : is_v ? a.v_out : a.k_out);
+  bool keeps = mine;
+  if (is_q || !a.slots) {
+    dst += times(t, is_q ? a.qo_st : a.ko_st) + times(hh, is_q ? a.qo_sh : a.ko_sh);
+  } else {
+    keeps = mine && placed && slot >= 0 && slot < a.N * (int64_t)a.S;
+    const int at = keeps ? (int)slot : 0, blk = fast_div(at, a.s_mul, a.s_shift, a.S);
+    dst += times(blk, is_v ? a.vo_sn : a.ko_sn) + times(at - blk * a.S, is_v ? a.vo_st : a.ko_st) +
+           times(hh, is_v ? a.vo_sh : a.ko_sh);
+  }
   if (is_v) {
-    if (!mine || !keeps) return;
+    if (!keeps) return;
     if constexpr (std::is_same_v<TI, TO>) {  // a copy, bit for bit
       x[0].store(dst + d0);
       x[1].store(dst + d1);
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < C; ++i) y[0][i] = x[0][i], y[1][i] = x[1][i];
-  } else {
-    // Half-split: pairs (d0 + i, d1 + i) with cs[i]. Interleaved: pair i of the
-    // first chunk with cs[i], of the second with cs[C/2 + i].
-    float z[2][C], cs[C], sn[C];
-    const float none = __builtin_nanf("");
-#pragma unroll
-    for (int i = 0; i < C; ++i) z[0][i] = x[0][i], z[1][i] = x[1][i], cs[i] = sn[i] = none;
-    if (mine && turns && placed) {
-      const float* line = a.table + pos * a.table_s;
+    } else {  // the conversion of the append without rotation, NaN included
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        const int p = INTER ? (i < C / 2 ? d0 / 2 + i : d1 / 2 + i - C / 2) : d0 + i;
-        cs[i] = line[p], sn[i] = line[half + p];
+        Elem<TO>::store(dst + d0 + i, x[0][i]);
+        Elem<TO>::store(dst + d1 + i, x[1][i]);
       }
     }
-    if (a.qw) {  // lanes without chunks only pass the others' sums on
-      float ss = 0.f;
-      if (mine) {
+    return;
+  }
+  float z[2][C];
 #pragma unroll
-        for (int i = 0; i < C; ++i) ss = fmaf(z[0][i], z[0][i], fmaf(z[1][i], z[1][i], ss));
-      }
-      for (int m = gp >> 1; m > 0; m >>= 1) ss += __shfl_xor(ss, m, 64);
-      const float r = 1.0f / sqrtf(ss * a.inv_d + a.eps);
-      if (mine) {
+  for (int i = 0; i < C; ++i) z[0][i] = x[0][i], z[1][i] = x[1][i];
+  float r = 1.f;
+  if (a.qw) {  // lanes without chunks only pass the others' sums on
+    float ss = 0.f;
+    if (mine) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int i = 0; i < C; ++i) z[s][i] = z[s][i] * r * w[s][i];
-      }
+      for (int i = 0; i < C; ++i) ss = fmaf(z[0][i], z[0][i], fmaf(z[1][i], z[1][i], ss));
     }
-    if (!mine || !keeps) return;
-    if (!turns) {  // past the rotated dims: as it is (an infinity times 0 is no 0)
+    ss = group_sum(ss, gp);
+    r = rsqrtf(ss * a.inv_d + a.eps);
+  }
+  if (!keeps) return;
+  if (turns && !placed) r = __builtin_nanf("");  // a query without angles
+  if (a.qw) {
 #pragma unroll
-      for (int i = 0; i < C; ++i) y[0][i] = z[0][i], y[1][i] = z[1][i];
-    } else if constexpr (INTER) {
+    for (int s = 0; s < 2; ++s) {
+      float w[C];
+#pragma unroll
+      for (int i = 0; i < C; ++i) w[i] = __uint_as_float(wr[s][i]);
+      if constexpr (sizeof(TI) == 2) {
+        if (!a.w_f32) {
+          Raw<TI, C> raw;
+#pragma unroll
+          for (int i = 0; i < C / 2; ++i) raw.w[i] = wr[s][i];
+#pragma unroll
+          for (int i = 0; i < C; ++i) w[i] = raw[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < C; ++i) z[s][i] = z[s][i] * r * w[i];
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < C; ++i) z[s][i] *= r;
+  }
+  if (turns) {  // past the rotated dims: as it is (an infinity times 0 is no 0)
+    if constexpr (INTER) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int i = 0; i < C / 2; ++i) {
           const float c = cs[s * C / 2 + i], n = sn[s * C / 2 + i], p = z[s][2 * i], q = z[s][2 * i + 1];
-          y[s][2 * i] = p * c - q * n;
-          y[s][2 * i + 1] = q * c + p * n;
+          z[s][2 * i] = p * c - q * n;
+          z[s][2 * i + 1] = q * c + p * n;
         }
     } else {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        y[0][i] = z[0][i] * cs[i] - z[1][i] * sn[i];
-        y[1][i] = z[1][i] * cs[i] + z[0][i] * sn[i];
+        const float p = z[0][i], q = z[1][i];
+        z[0][i] = p * cs[i] - q * sn[i];
+        z[1][i] = q * cs[i] + p * sn[i];
       }
     }
   }
-  store_chunk(dst + d0, y[0]);
-  store_chunk(dst + d1, y[1]);
+  store_chunk(dst + d0, z[0]);
+  store_chunk(dst + d1, z[1]);
 }
 
 // Any strides and any even R: one wavefront per head row, lanes over the dims.
