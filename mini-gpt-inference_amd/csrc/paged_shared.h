@@ -398,13 +398,40 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, Tile<T, DP>& f,
   }
 }
 
-// Attends the tiles first, first + step, ... below end of row b's table. A tile's
+// A scale that is not positive, put into the queries (apart from their loads: it waits
+// for them).
+template <int NQ, int KS>
+__device__ __forceinline__ void sign_queries(const SharedArgs& a, uint4 (&qf)[NQ][KS]) {
+  if (!(a.q_flip | a.q_zero)) return;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const uint4 x = qf[q][s];
+      qf[q][s] = a.q_zero ? make_uint4(0, 0, 0, 0)
+                          : make_uint4(x.x ^ a.q_flip, x.y ^ a.q_flip, x.z ^ a.q_flip, x.w ^ a.q_flip);
+    }
+}
+
+// Row b's length, from the load and its value.
+__device__ __forceinline__ Index ctx_load(const SharedArgs& a, int b) {
+  Index x;
+  x.load(a.cl, a.cl_i64, (uint64_t)b * (uint64_t)a.cl_s);
+  return x;
+}
+__device__ __forceinline__ int ctx_value(const SharedArgs& a, const Index& x) {
+  const int64_t c = x.value(a.cl_i64), top = (int64_t)a.M * a.S;
+  return (int)(c < 0 ? 0 : c > top ? top : c);
+}
+__device__ __forceinline__ int clamped_ctx(const SharedArgs& a, int b) { return ctx_value(a, ctx_load(a, b)); }
+
+// Attends the tiles first, first + step, ... below end_of() of row b's table. A tile's
 // keys are loaded into the registers the one before has given its scores from, and
 // its values where that one's products have been taken: half a tile is always on
 // its way. (A second set of registers, a whole tile ahead, changed no call's time.)
-template <typename T, int DP, int NQ, bool UNI, bool FULL>
-__device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh, int first, int step, int end,
-                                             const uint4 (&qf)[NQ][Tile<T, DP>::kKS], State<DP, NQ>& st) {
+template <typename T, int DP, int NQ, bool UNI, bool FULL, typename End>
+__device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh, int first, int step, End end_of,
+                                             uint4 (&qf)[NQ][Tile<T, DP>::kKS], State<DP, NQ>& st) {
   using L = Tile<T, DP>;
   const char* kp = (const char*)a.k + (int64_t)kvh * a.k_sh * (int)sizeof(T);
   const char* vp = (const char*)a.v + (int64_t)kvh * a.v_sh * (int)sizeof(T);
@@ -417,6 +444,8 @@ __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh
     tok = first + lane / L::kGroups * step + 16 * (lane % L::kGroups);
     entry = window_entry(a, b, tok);
   }
+  __builtin_amdgcn_sched_barrier(0);
+  const int end = uniform(end_of());
   if (first >= end) return;
   L f;
   auto keys = [&](int i) {
@@ -441,6 +470,7 @@ __device__ __forceinline__ void stream_tiles(const SharedArgs& a, int b, int kvh
   __builtin_amdgcn_sched_barrier(0);  // keys before values, as in the loop: their wait leaves the values in flight
   values(0);
   __builtin_amdgcn_sched_barrier(0);
+  sign_queries(a, qf);
   for (int i = 0; i + 1 < n; ++i) {
     score_tile<T, DP, NQ>(f, qf, s);
     keys(i + 1);
@@ -467,16 +497,6 @@ __device__ __forceinline__ void load_queries(const SharedArgs& a, int kvh, int r
       if constexpr (FULL) qf[q][s] = *(const uint4*)(p + 4 * L::kCE * s);
       else qf[q][s] = *((kg + 4 * s) * L::kCE < a.D ? (const uint4*)(p + 4 * L::kCE * s) : (const uint4*)kZeroRow);
     }
-  }
-  if (a.q_flip | a.q_zero) {  // a scale that is not positive
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-      for (int s = 0; s < L::kKS; ++s) {
-        const uint4 x = qf[q][s];
-        qf[q][s] = a.q_zero ? make_uint4(0, 0, 0, 0)
-                            : make_uint4(x.x ^ a.q_flip, x.y ^ a.q_flip, x.z ^ a.q_flip, x.w ^ a.q_flip);
-      }
   }
 }
 
@@ -509,6 +529,7 @@ __device__ __forceinline__ void each_run(const SharedArgs& a, const State<DP, NQ
 template <int DP, int NQ, int WAVES>
 struct JoinSpace {
   float acc[WAVES][NQ * 16][DP + 4], m[WAVES][NQ * 16], l[WAVES][NQ * 16];
+  int64_t slot[NQ * 16];  // of the rows' partials, where the workgroup leaves any
 };
 template <typename T, int DP, int NQ, int WAVES, typename F>
 __device__ __forceinline__ void join_waves(const SharedArgs& a, const State<DP, NQ>& st, int wave, int rows,
@@ -562,11 +583,6 @@ __device__ __forceinline__ void store_partial(const SharedArgs& a, const State<D
     for (int e = 0; e < Tile<T, DP>::kEV; e += 4)
       *(f32x4*)(row + d + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
   });
-}
-
-__device__ __forceinline__ int clamped_ctx(const SharedArgs& a, int b) {
-  const int64_t c = load_index(a.cl, a.cl_i64, (int64_t)b * a.cl_s), top = (int64_t)a.M * a.S;
-  return (int)(c < 0 ? 0 : c > top ? top : c);
 }
 
 constexpr int kSplitWaves = 4;
@@ -623,13 +639,14 @@ __device__ __forceinline__ int scan_own(const SharedArgs& a, int* cum, int* ctx,
   const int wave = uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int per = (a.B + 64 * kSplitWaves - 1) / (64 * kSplitWaves), b0 = (int)threadIdx.x * per;
   int sum = 0;
-  for (int i = 0; i < per; ++i)
+  for (int i = 0; i < per; ++i) {
+    const int c = clamped_ctx(a, min(b0 + i, a.B - 1));
     if (b0 + i < a.B) {
-      const int c = clamped_ctx(a, b0 + i);
       sum += (c - (c < a.P ? 0 : a.P) + KEYS - 1) / KEYS;
       cum[b0 + i] = sum;
       ctx[b0 + i] = c;
     }
+  }
   int incl = sum;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -723,6 +740,7 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
   __builtin_amdgcn_sched_barrier(0);
   load_values<T, DP, FULL, NT>(a, vp, win, 0, f);
   __builtin_amdgcn_sched_barrier(0);
+  sign_queries(a, qf);
   st.reset();
   for (int t = 0; t + 1 < n; ++t) {  // as in stream_tiles
     const int at = (t + 1) % kSpan * L::kGroups;
@@ -736,6 +754,7 @@ __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, 
     load_values<T, DP, FULL, NT>(a, vp, win, at, f);
     if (ends) {
       store_own<T>(a, st, wave_index, b, h >> 1, h & 1);
+      sign_queries(a, qf);
       st.reset();
       b = nb;
       h = nh;
@@ -775,18 +794,18 @@ __device__ __forceinline__ void attend_own_any(const SharedArgs& a, int wave_ind
     load_own_queries<T, DP, false>(a, b, vh, qf);
     st.reset();
     const int first = (c < a.P ? 0 : a.P) + tile * L::kKeys;
-    stream_tiles<T, DP, 1, false, false>(a, b, vh / a.gsets, first, L::kKeys, min(c, first + n * L::kKeys), qf, st);
+    stream_tiles<T, DP, 1, false, false>(
+        a, b, vh / a.gsets, first, L::kKeys, [&] { return min(c, first + n * L::kKeys); }, qf, st);
     store_own<T>(a, st, wave_index, b, vh, tile == 0);
   }
 }
 
-// The slot of the lane's query row r (of a shared piece that begins its run or
-// continues it), or -1 where the row takes no part.
+// The slot of query row r (of a shared piece that begins its run or continues it), or
+// -1 where the row takes no part.
 __device__ __forceinline__ int64_t shared_slot(const SharedArgs& a, int kvh, int r, int r0, bool begins, int wg) {
-  if (r >= a.B * a.G) return -1;
-  const int b = fast_div(r, a.g_mul, a.g_shift, a.G), g = r - b * a.G;
-  if (clamped_ctx(a, b) < a.P) return -1;
-  return begins ? (int64_t)b * a.Hq + kvh * a.G + g : a.s_cont + (int64_t)wg * a.set_rows + (r - r0);
+  const int rr = min(r, a.B * a.G - 1), b = fast_div(rr, a.g_mul, a.g_shift, a.G), g = rr - b * a.G;
+  const int64_t slot = begins ? (int64_t)b * a.Hq + kvh * a.G + g : a.s_cont + (int64_t)wg * a.set_rows + (rr - r0);
+  return clamped_ctx(a, b) >= a.P && r == rr ? slot : -1;
 }
 
 // Shared pieces from registers, for up to 32 query rows a set and for what the tiles
@@ -809,12 +828,14 @@ __device__ __forceinline__ void attend_shared(const SharedArgs& a, int wg, int s
     n = min(a.s_tiles - tile, stop - u);
     if (r0 >= a.B * a.G) continue;
     load_queries<T, DP, NQ, FULL>(a, kvh, r0, a.B * a.G, qf);
+    const int64_t slot = shared_slot(a, kvh, r0 + lane % (16 * NQ), r0, tile == 0, wg);
     st.reset();
-    stream_tiles<T, DP, NQ, UNI, FULL>(a, 0, kvh, tile * step + wave * L::kKeys, step, min(a.P, (tile + n) * step), qf,
-                                       st);
+    stream_tiles<T, DP, NQ, UNI, FULL>(
+        a, 0, kvh, tile * step + wave * L::kKeys, step, [&] { return min(a.P, (tile + n) * step); }, qf, st);
     __syncthreads();  // the joins before are done with the space
+    if ((int)threadIdx.x < 16 * NQ) space.slot[threadIdx.x] = slot;
     join_waves<T>(a, st, wave, 16 * NQ, space, [&](int row, int d, f32x4 o, float m, float l) {
-      const int64_t slot = shared_slot(a, kvh, r0 + row, r0, tile == 0, wg);
+      const int64_t slot = space.slot[row];
       if (slot < 0) return;
       *(f32x4*)(a.ws_acc + slot * a.D + d) = o;
       if (d == 0) a.ws_ml[slot] = make_float2(m, l);
@@ -1046,6 +1067,7 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
     const bool active = mine < a.B * a.G;
     __syncthreads();  // the tiles of the piece before, and the scan's sums, are done with
     copy(0, 0);
+    sign_queries(a, qf);
     auto turn = [&](int i, auto stage) {
       constexpr int S = decltype(stage)::value;
       now = next;
@@ -1059,9 +1081,12 @@ __device__ __forceinline__ void attend_shared_lds(const SharedArgs& a, int wg, i
       turn(i, Stage<0>{});
       if (i + 1 < n) turn(i + 1, Stage<1>{});
     }
+    int64_t slots[QB];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) slots[q] = shared_slot(a, kvh, mine + 16 * q + col, r0, tile0 == 0, wg);
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
-      const int64_t slot = shared_slot(a, kvh, mine + 16 * q + col, r0, tile0 == 0, wg);
+      const int64_t slot = slots[q];
       if (slot < 0) continue;
       if (lane < 16)
         a.ws_ml[slot] = make_float2(st.m[q] == kNegInf ? kNegInf : st.mc[q], coded_sum(st.sum[q][0], any));
@@ -1101,10 +1126,10 @@ __global__ void __launch_bounds__(256) paged_shared_join(const SharedArgs a) {
   const bool live = unit < (int64_t)a.B * a.Hq;
   const int b = live ? (int)(unit / a.Hq) : 0, hq = live ? (int)(unit - (int64_t)b * a.Hq) : 0;
   const int kvh = hq / a.G, g = hq - kvh * a.G, set = g / 16, r = b * a.G + g;
-  const int before = b ? a.ws_cum[b - 1] : 0, tiles = a.ws_cum[b] - before;
-  const int seg_shared = a.ws_split[0], seg_own = a.ws_split[1];
+  const int last = a.ws_cum[max(b - 1, 0)], upto = a.ws_cum[b], seg_shared = a.ws_split[0], seg_own = a.ws_split[1];
+  const int ctx = clamped_ctx(a, b), before = b ? last : 0, tiles = upto - before;
   int shared = 0, s0 = 0, member = 0, pieces = 0, w0 = 0;
-  if (a.s_tiles && clamped_ctx(a, b) >= a.P) {
+  if (a.s_tiles && ctx >= a.P) {
     const int rs = r / a.set_rows, u = (kvh * a.set_blocks + rs / a.team) * a.s_tiles;
     member = rs % a.team;
     s0 = u / seg_shared;
@@ -1213,8 +1238,10 @@ __global__ void __launch_bounds__(64 * kOneWaves<DP>) paged_shared_one(const Sha
   uint4 qf[1][L::kKS];
   State<DP, 1> st;
   load_queries<T, DP, 1, FULL>(a, kvh, b * a.G + g0, (b + 1) * a.G, qf);
+  const Index ctx = ctx_load(a, b);
   st.reset();
-  stream_tiles<T, DP, 1, UNI, FULL>(a, b, kvh, wave * L::kKeys, kOneWaves<DP> * L::kKeys, clamped_ctx(a, b), qf, st);
+  stream_tiles<T, DP, 1, UNI, FULL>(
+      a, b, kvh, wave * L::kKeys, kOneWaves<DP> * L::kKeys, [&] { return ctx_value(a, ctx); }, qf, st);
   join_waves<T>(a, st, wave, min(16, a.G - g0), space, [&](int row, int d, f32x4 o, float, float l) {
     const f32x4 x = o * (l == 0.f ? 0.f : l < 0.f ? __builtin_nanf("") : 1.f / l);
     T* p = (T*)a.out + (int64_t)b * a.o_sb + (int64_t)(kvh * a.G + g0 + row) * a.o_sh + d;
