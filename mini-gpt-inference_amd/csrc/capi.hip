@@ -803,7 +803,8 @@ int launch_rope_checked(mgi::RopeArgs& a, int out_dtype, hipStream_t stream) {
 
 // How mgi_paged_decode_shared runs a call of these sizes on the matrix-core kernels.
 struct SharedPlan {
-  int one_launch, gsets, vheads, wgs, lds_tiles, row_tiles, set_rows, team, set_blocks, s_units, s_tiles, s_cost, s_piece;
+  int one_launch, gsets, vheads, wgs, lds_tiles, row_tiles, set_rows, team, set_blocks;
+  int s_units, s_tiles, s_cost, s_piece;
   int64_t s_cont, own_slot, own_cont, slots;
   size_t ml_offset, cum_offset, total;
 };
@@ -823,12 +824,13 @@ bool shared_one_launch(int64_t B, int64_t Hk, int64_t vheads, int64_t rows, int6
   const double width = D <= 64 ? 64 : D <= 128 ? 128 : 256, cus = (double)device_cus();
   const double own = (double)(tokens - shared_tokens), row_mb = 2e-6 * (double)(D * eb);
   // Eight wavefronts take a row's tiles in turn, 1.7 us a 16 KiB tile.
-  const double turns = (double)((tokens + keys - 1) / keys + 7) / 8, tile_us = 1.72 * std::pow(width * (double)eb / 256, 0.73);
+  const double turns = (double)((tokens + keys - 1) / keys + 7) / 8;
+  const double tile_us = 1.72 * std::pow(width * (double)eb / 256, 0.73);
   const double wgs = (double)(B * vheads);
   const double one_us = 4.5 + std::max(std::floor(turns) * tile_us * std::max(1.0, wgs / (0.83 * cus)),
                                        wgs * (double)tokens * row_mb / 10.6);
   const double mflop = 4e-6 * (double)(rows * Hk * shared_tokens * D);
-  const double split_us = 13.9 + (double)Hk * ((double)shared_tokens + 0.6 * (double)B * own) * row_mb / 5.0 +
+  const double split_us = 13.0 + (double)Hk * ((double)shared_tokens + 0.6 * (double)B * own) * row_mb / 6.0 +
                           mflop / (eb == 2 ? 507.0 : 63.0);
   return one_us <= split_us;
 }
@@ -860,7 +862,8 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   // Tile numbers are 32-bit, the rows' prefix sums live in LDS, and rows by the
   // thousand fill the CUs by themselves: no partials past 4 GiB.
   const int forced = env_int("MINIVLLM_HIP_SHARED_SPLIT", -1);
-  p.one_launch = B > mgi::kSharedMaxB || 2 * B * Hq * D * 4 > (int64_t(4) << 30) || Hk * p.set_blocks * tiles >= (int64_t(1) << 30) ||
+  p.one_launch = B > mgi::kSharedMaxB || 2 * B * Hq * D * 4 > (int64_t(4) << 30) ||
+                 Hk * p.set_blocks * tiles >= (int64_t(1) << 30) ||
                  B * ((M * S + keys - 1) / keys) * p.vheads >= (int64_t(1) << 30) ||
                  (forced >= 0 ? forced == 0
                               : shared_one_launch(B, Hk, p.vheads, rows, D, eb, keys, shared * S, M * S));
