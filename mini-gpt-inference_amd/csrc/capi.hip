@@ -813,12 +813,12 @@ struct SharedPlan {
 // itself, is estimated faster than the split over all workgroups and its joining
 // launch. Only the table's width is known here: rows are taken to fill it in the
 // first estimate, whose longest row ends the call, and 0.6 of it in the second. In us,
-// fitted to 1500 shapes on MI355X (2-256 rows, 1-32 KV heads, 1-8 query heads each,
+// fitted to 2000 shapes on MI355X (2-256 rows, 1-32 KV heads, 1-8 query heads each,
 // head_dim 32-128, 64 to 65 536 shared tokens, the three types); the slower one is
-// taken by more than 10 % in 1 of 27, the mean loss is 1 %. One launch / split:
-// 4 x 8 heads of 32, f32, 200-256 tokens, 128 shared: 7.1 / 12.2; 8 x 30, bf16,
-// 842: 17.8 / 25; 13 x 16, 820-1300, 800 shared: 15.3 / 15.0; 24 x 12, f32, 1520-1900,
-// 1504 shared: 40 / 21; 64 x 32, 4160-5120, 4096 shared: 409 / 115.
+// taken by more than 10 % in 1 of 40, the mean loss is 0.7 %. One launch / split:
+// 4 x 8 heads of 32, f32, 200-256 tokens, 128 shared: 6.9 / 11.6; 13 x 16, bf16,
+// 820-1300, 800 shared: 14.7 / 13.1; 24 x 12, f32, 1520-1900, 1504 shared: 37 / 18;
+// 64 x 32, 4160-5120, 4096 shared: 401 / 113.
 bool shared_one_launch(int64_t B, int64_t Hk, int64_t vheads, int64_t rows, int64_t D, int64_t eb, int64_t keys,
                        int64_t shared_tokens, int64_t tokens) {
   const double width = D <= 64 ? 64 : D <= 128 ? 128 : 256, cus = (double)device_cus();

@@ -39,8 +39,8 @@
 // weights stay below 2^kSharedLazy, well inside every type.
 //
 // What bounds it (MI355X; inputs from memory, another set each call): 64 x 32 heads
-// on 4096 shared tokens and 64-1024 of their own, bf16, 649 MB: 119 us, 5.45 TB/s; 128
-// x 32 on 8 KV heads over 65 536 shared, 138 GFLOP: 173 us, 795 TFLOP/s, the softmax's
+// on 4096 shared tokens and 64-1024 of their own, bf16, 649 MB: 116 us, 5.6 TB/s; 128
+// x 32 on 8 KV heads over 65 536 shared, 138 GFLOP: 172 us, 800 TFLOP/s, the softmax's
 // VALU work beside the products (37 % of cycles in the matrix cores, LDS conflicts
 // none; with all keys in L2 it still takes 141 of the 146 us without own tokens).
 // Calls under about 30 us are chains: launch and the rows' prefix sums 4 us, a first
@@ -704,8 +704,7 @@ __device__ __forceinline__ void load_own_queries(const SharedArgs& a, int b, int
 // A wavefront's segment of the rows' own tiles, as one stream over rows and heads:
 // the window's lanes find their own tiles, so a run's end costs no new chain of
 // loads (length, table, queries, keys), only its partial (24 x 12 heads of 64, f32:
-// 23.8 us with a loop over runs, 21.4 so; 13 x 16, whose wavefronts have a tile
-// each, 14.9 and 14.7).
+// 23.8 us with a loop over runs, 21.4 so, then 18.3 with all loads unconditional).
 template <typename T, int DP, bool FULL, bool NT>
 __device__ __forceinline__ void attend_own(const SharedArgs& a, int wave_index, int seg, int total, const int* cum,
                                            const int* ctx) {

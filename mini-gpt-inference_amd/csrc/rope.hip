@@ -13,11 +13,13 @@
 // staged: a lane holds two chunks of a head row that a rotation needs together
 // (dims C p .. C p + C-1 and the same plus R/2), loads them with one instruction
 // each and shares only the sum of squares, over the lanes of the head. Everything
-// but the angles loads at once, the angles once the position is there. One head row
-// to a lane: 8192 rows of 32 + 8 bf16 heads of 128 take 35.4 us, 4.9 TB/s, what a
-// large copy reaches; two rows 36.2, four 45.6 (more registers, fewer wavefronts),
-// and a workgroup per row walking its heads 62. 13 rows appended take 3.1 us replayed
-// from a graph (5.4 with the host's call).
+// but the angles loads at once, the angles once the position is there, and no load is
+// under a condition: its end would wait for all of them. 8192 rows of 32 + 8 bf16 heads
+// of 128 take 28 us on cached inputs (6.1 TB/s) and 33 from memory (5.2; a large copy
+// 4.9). With conditions, 64-bit offsets and rounding by hand: 37 and 43; in that form
+// two head rows to a lane took 2 % more, four 29 % (more registers, fewer wavefronts),
+// and a workgroup per row walking its heads 75 %. 13 rows appended take 2.9 us (6.2
+// with the host's call).
 #include <type_traits>
 
 #include "mgi_common.h"
