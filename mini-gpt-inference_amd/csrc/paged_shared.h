@@ -211,7 +211,8 @@ __device__ __forceinline__ void load_keys(const SharedArgs& a, const char* kp, c
   }
 }
 template <typename T, int DP, bool FULL, bool NT = false>
-__device__ __forceinline__ void load_values(const SharedArgs& a, const char* vp, const Window& w, int at, Tile<T, DP>& f) {
+__device__ __forceinline__ void load_values(const SharedArgs& a, const char* vp, const Window& w, int at,
+                                            Tile<T, DP>& f) {
   using L = Tile<T, DP>;
   using V = typename L::VVec;
   const int lane = (int)threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
@@ -249,7 +250,8 @@ __device__ __forceinline__ Found find_key(const SharedArgs& a, int b, int key, i
   return {ok ? id : 0, ok ? k - blk * a.S : 0, ok};
 }
 template <typename T, int DP>
-__device__ __forceinline__ void load_keys_any(const SharedArgs& a, const char* kp, int b, int t0, int end, Tile<T, DP>& f) {
+__device__ __forceinline__ void load_keys_any(const SharedArgs& a, const char* kp, int b, int t0, int end,
+                                              Tile<T, DP>& f) {
   using L = Tile<T, DP>;
   const int lane = (int)threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
 #pragma unroll
@@ -262,7 +264,8 @@ __device__ __forceinline__ void load_keys_any(const SharedArgs& a, const char* k
   }
 }
 template <typename T, int DP>
-__device__ __forceinline__ void load_values_any(const SharedArgs& a, const char* vp, int b, int t0, int end, Tile<T, DP>& f) {
+__device__ __forceinline__ void load_values_any(const SharedArgs& a, const char* vp, int b, int t0, int end,
+                                                Tile<T, DP>& f) {
   using L = Tile<T, DP>;
   using V = typename L::VVec;
   const int lane = (int)threadIdx.x & 63, row = lane & 15, kg = lane >> 4;

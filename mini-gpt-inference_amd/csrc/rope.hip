@@ -95,6 +95,20 @@ struct Raw {
   }
 };
 
+// A value converted as the append without rotation converts it, NaN included.
+template <int N, typename T>
+__device__ __forceinline__ void store_value(T* p, const float (&x)[N]) {
+  if constexpr (std::is_same_v<T, bf16_t>) {
+    Raw<bf16_t, N> r;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      r.w[i] = (uint32_t)f32_to_bf16(x[2 * i]) | ((uint32_t)f32_to_bf16(x[2 * i + 1]) << 16);
+    r.store(p);
+  } else {
+    store_chunk(p, x);
+  }
+}
+
 // The sum over aligned groups of gp lanes, gp a power of two.
 __device__ __forceinline__ float group_sum(float x, int gp) {
   if (gp > 1) x += dpp<DPP_QUAD_XOR1>(x);
@@ -185,12 +199,12 @@ __global__ void __launch_bounds__(kRopeThreads) rope_vec(const RopeArgs a) {
     if constexpr (std::is_same_v<TI, TO>) {  // a copy, bit for bit
       x[0].store(dst + d0);
       x[1].store(dst + d1);
-    } else {  // the conversion of the append without rotation, NaN included
+    } else {
+      float y[2][C];
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        Elem<TO>::store(dst + d0 + i, x[0][i]);
-        Elem<TO>::store(dst + d1 + i, x[1][i]);
-      }
+      for (int i = 0; i < C; ++i) y[0][i] = x[0][i], y[1][i] = x[1][i];
+      store_value(dst + d0, y[0]);
+      store_value(dst + d1, y[1]);
     }
     return;
   }

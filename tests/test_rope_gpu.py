@@ -199,6 +199,35 @@ def test_empty_calls_and_far_positions():
     _check(qo, want, size, "far")  # the table's own rounding is one more u of each term
 
 
+def test_index_types_wide_strides_and_converted_nan_values():
+    """int32 and strided positions and slots, and a stride past 31 bits (of a single
+    row), give the bits of plain int64 ones; a NaN value converts as kv_append does."""
+    T, Hq, H, D = 9, 4, 2, 128
+    table = hpd.rope_table(64, D, device=DEV)
+    q, k, v = _randn((T, Hq, D), F32, 90), _randn((T, H, D), F32, 91), _randn((T, H, D), F32, 92)
+    v[3, 1, 5], v[4, 0, 0] = float("nan"), -float("nan")
+    w = _randn((D,), F32, 93), _randn((D,), F32, 94)
+    pos, slots = torch.arange(T, device=DEV) * 7, torch.tensor([3, 40, -1, 8, 30, 2, 99, 17, 0], device=DEV)
+    pools = [KVBlockPool(1, 3, 16, H, D, device=DEV, dtype=BF16) for _ in range(4)]
+    for p in pools:
+        p.k.zero_(), p.v.zero_()
+    wide = lambda t: torch.stack((t, t + 1), 1)[:, 0]
+    got = [hpd.kv_append_rope_hip(p, 0, q, k, v, s, i, table, *w)
+           for p, s, i in zip(pools, (slots, slots.int(), wide(slots)), (pos, wide(pos.int()), wide(pos)))]
+    hpd.kv_append(pools[3], 0, k, v, slots)
+    for p, out in zip(pools[1:3], got[1:]):
+        assert torch.equal(_bits(out), _bits(got[0]))
+        assert torch.equal(_bits(p.k), _bits(pools[0].k)) and torch.equal(_bits(p.v), _bits(pools[0].v))
+    assert torch.equal(_bits(pools[3].v), _bits(pools[0].v))
+    one = [t[:1].contiguous() for t in (q, k)]
+    far = [t.as_strided(t.shape, (2 ** 31, D, 1)) for t in one]
+    a, b = (hpd.qk_norm_rope_hip(*x, pos[1:2], table, *w) for x in (one, far))
+    for x, y, src, wt in zip(a, b, one, w):
+        want, size = _formula(src, wt, table[pos[1:2]], D, False, 1e-6)
+        _check(x, want, size, "row")
+        _check(y, want, size, "far row")
+
+
 def test_graph_replays_and_streams():
     """Captured together, replayed on new inputs, equal to the eager calls; another
     stream than the tensors' own."""
