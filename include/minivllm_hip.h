@@ -83,8 +83,8 @@ int mgi_abi_version(void);
  * is touched. With new_dtype == pool_dtype the copy is bit-exact; otherwise
  * the value is converted with round-to-nearest-even (f32 -> bf16/f16) or
  * exactly (bf16/f16 -> f32). Other conversions return MGI_EUNSUPPORTED.
- * If two rows name the same slot, which one lands is unspecified (as for
- * torch index_put_ without accumulate).
+ * If rows name the same slot, each element of it is one of theirs, and which
+ * is unspecified, for K and V apart (as for torch index_put_ without accumulate).
  */
 int mgi_kv_append(void* k_pool, void* v_pool,
                   const int64_t* k_pool_strides, /* [5] */
@@ -374,12 +374,13 @@ int mgi_qk_norm_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
 /*
  * KV append with the same norms and rotation on the way: keys are normed, rotated
  * and written to the pool's slots, values copied there, as mgi_kv_append writes
- * rows k_new, v_new of Hk heads (skipped rows, conversions and repeated slots as
- * there; values are bit-exact where the dtypes agree), and the normed, rotated
+ * rows k_new, v_new of Hk heads (skipped rows and conversions as there; values
+ * are bit-exact where the dtypes agree), and the normed, rotated
  * queries go to q_out, which has the pool's dtype, as the attention that
  * follows takes them. q, k and v share one dtype. A row whose position is outside
  * the table is not written to the pool, and its query comes out NaN in the
- * rotated dims.
+ * rotated dims. If rows that are written name the same slot, it holds the last
+ * one's K and V where T <= 256; in longer calls as in mgi_kv_append.
  */
 int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
                        void* k_pool, void* v_pool,

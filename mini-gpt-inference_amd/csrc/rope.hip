@@ -18,8 +18,9 @@
 // of 128 take 28 us on cached inputs (6.1 TB/s) and 33 from memory (5.2; a large copy
 // 4.9). With conditions, 64-bit offsets and rounding by hand: 37 and 43; in that form
 // two head rows to a lane took 2 % more, four 29 % (more registers, fewer wavefronts),
-// and a workgroup per row walking its heads 75 %. 13 rows appended take 2.9 us (6.2
-// with the host's call).
+// and a workgroup per row walking its heads 75 %. 13 rows appended take 3.1 us (5.6-6.2
+// with the host's call), 256 rows of 32 + 2 x 32 heads 5.0; without a look at the later
+// rows' slots (LaterRows) 2.8 and 4.5.
 #include <type_traits>
 
 #include "mgi_common.h"
@@ -120,13 +121,63 @@ __device__ __forceinline__ float group_sum(float x, int gp) {
   return x;
 }
 
+// Rows on one slot: a slot's head rows are many wavefronts', K and V apart, and nothing
+// orders two rows' stores, so left alone a slot may hold heads (or 16-byte pieces) of
+// one row and of the other. In calls of up to kOrderedRows rows every wavefront looks
+// through the later rows' slots and leaves out a row that one of them replaces: K and V
+// are the last row's, whole. 256 slots are 2 KB, no more than a wavefront's own eight head
+// rows of 128, and load beside them; a long chunk's would be many times that, so longer
+// calls do not look.
+constexpr int kOrderedRows = 256;
+
+// The low words of the slots of a wavefront's rows (t is its first lane's, the lowest)
+// and of those after them: lane l holds rows l, l + 64, ...
+struct LaterRows {
+  uint32_t low[kOrderedRows / 64];
+  __device__ __forceinline__ static bool holds(const RopeArgs& a, int i, int t) { return 64 * i < a.T && 64 * i + 63 > t; }
+  __device__ __forceinline__ void load(const RopeArgs& a, int t) {
+    const int first = __builtin_amdgcn_readfirstlane(t), lane = (int)threadIdx.x & 63;
+    const char* p = (const char*)a.slots;
+#pragma unroll
+    for (int i = 0; i < kOrderedRows / 64; ++i)
+      if (holds(a, i, first))
+        low[i] = *(const uint32_t*)(p + (((uint64_t)min(lane + 64 * i, a.T - 1) * (uint64_t)a.sl_s) << (a.sl_i64 ? 3 : 2)));
+  }
+  // For the lanes that ask: whether a row after theirs is written to their slot. Every
+  // lane of the wavefront takes part.
+  __device__ __forceinline__ bool replace(const RopeArgs& a, int t, int64_t slot, bool asks) const {
+    const int first = __builtin_amdgcn_readfirstlane(t), lane = (int)threadIdx.x & 63;
+    bool out = false;
+    for (uint64_t left = __ballot(asks); left;) {  // a row at a time
+      const int src = __builtin_ctzll(left), row = __builtin_amdgcn_readlane(t, src);
+      const uint32_t want = (uint32_t)__builtin_amdgcn_readlane((int)slot, src);
+      uint32_t same = 0;
+#pragma unroll
+      for (int i = 0; i < kOrderedRows / 64; ++i)
+        if (holds(a, i, first)) same |= (low[i] == want && lane + 64 * i > row && lane + 64 * i < a.T ? 1u : 0u) << i;
+      bool hit = false;
+      for (; same; same &= same - 1) {  // the rest of the slot, and its row's position
+        const int64_t r = lane + 64 * __builtin_ctz(same);
+        const int64_t pos = load_index(a.positions, a.pos_i64, r * a.pos_s);
+        const uint32_t high = (uint32_t)__builtin_amdgcn_readlane((int)(slot >> 32), src);
+        hit |= (uint32_t)(load_index(a.slots, a.sl_i64, r * a.sl_s) >> 32) == high &&
+               pos >= 0 && pos < a.P;  // without angles a row is not written
+      }
+      const bool hits = __any(hit);
+      if (t == row) out = hits;
+      left &= ~__ballot(t == row);
+    }
+    return out;
+  }
+};
+
 // n * stride, both below 2^31: one instruction, where a 64-bit stride takes three of a
 // quarter of the rate.
 __device__ __forceinline__ uint64_t times(int n, int64_t stride) { return (uint64_t)(uint32_t)n * (uint32_t)stride; }
 
 // TI: q, k, v; TO: q_out and the keys' and values' target. C: elements per chunk. All
-// strides, positions and slots are below 2^31.
-template <typename TI, typename TO, int C, bool INTER>
+// strides, positions and slots are below 2^31. ORDERED: of rows on one slot the last.
+template <typename TI, typename TO, int C, bool INTER, bool ORDERED>
 __global__ void __launch_bounds__(kRopeThreads) rope_vec(const RopeArgs a) {
   const int gp = 1 << a.gp_shift;  // lanes per head row
   const int sub = (int)threadIdx.x & (gp - 1), slots = (int)blockDim.x >> a.gp_shift;
@@ -150,6 +201,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_vec(const RopeArgs a) {
   src += times(t, is_q ? a.q_st : is_v ? a.v_st : a.k_st) + times(hh, is_q ? a.q_sh : is_v ? a.v_sh : a.k_sh);
   x[0].load(src + d0);
   x[1].load(src + d1);
+  LaterRows later;
+  if constexpr (ORDERED) later.load(a, t);
   const int64_t pos = at_pos.value(a.pos_i64), slot = at_slot.value(a.sl_i64);
   const bool placed = pos >= 0 && pos < a.P;
   // Half-split: pairs (d0 + i, d1 + i) with cs[i]. Interleaved: pair i of the
@@ -185,11 +238,12 @@ __global__ void __launch_bounds__(kRopeThreads) rope_vec(const RopeArgs a) {
   }
   // Where the row goes: q_out, or k_out or the pools.
   TO* dst = (TO*)(is_q ? a.q_out : is_v ? a.v_out : a.k_out);
-  bool keeps = mine;
+  bool keeps = mine, replaced = false;
+  if constexpr (ORDERED) replaced = later.replace(a, t, slot, mine && !is_q);
   if (is_q || !a.slots) {
     dst += times(t, is_q ? a.qo_st : a.ko_st) + times(hh, is_q ? a.qo_sh : a.ko_sh);
   } else {
-    keeps = mine && placed && slot >= 0 && slot < a.N * (int64_t)a.S;
+    keeps = mine && placed && !replaced && slot >= 0 && slot < a.N * (int64_t)a.S;
     const int at = keeps ? (int)slot : 0, blk = fast_div(at, a.s_mul, a.s_shift, a.S);
     dst += times(blk, is_v ? a.vo_sn : a.ko_sn) + times(at - blk * a.S, is_v ? a.vo_st : a.ko_st) +
            times(hh, is_v ? a.vo_sh : a.ko_sh);
@@ -271,7 +325,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_vec(const RopeArgs a) {
 }
 
 // Any strides and any even R: one wavefront per head row, lanes over the dims.
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool ORDERED>
 __global__ void __launch_bounds__(kRopeThreads) rope_any(const RopeArgs a) {
   const int heads = a.Hq + a.Hk + a.Hv;
   const int64_t unit = (int64_t)blockIdx.x * (kRopeThreads / 64) + threadIdx.x / 64;
@@ -284,6 +338,13 @@ __global__ void __launch_bounds__(kRopeThreads) rope_any(const RopeArgs a) {
   const bool placed = pos >= 0 && pos < a.P;
   int64_t k_off = 0, v_off = 0;
   if (!rope_target(a, t, placed, &k_off, &v_off) && !is_q) return;
+  if constexpr (ORDERED) {
+    if (!is_q) {
+      LaterRows later;
+      later.load(a, (int)t);
+      if (later.replace(a, (int)t, load_index(a.slots, a.sl_i64, t * a.sl_s), true)) return;
+    }
+  }
   const TI* src = is_q   ? (const TI*)a.q + t * a.q_st + (int64_t)hh * a.q_sh
                   : is_v ? (const TI*)a.v + t * a.v_st + (int64_t)hh * a.v_sh
                          : (const TI*)a.k + t * a.k_st + (int64_t)hh * a.k_sh;
@@ -330,13 +391,20 @@ __global__ void __launch_bounds__(kRopeThreads) rope_any(const RopeArgs a) {
 
 namespace {
 
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool ORDERED>
 const void* rope_kernel(int chunk, int interleaved) {
-  if (chunk == 0) return (const void*)&rope_any<TI, TO>;
+  if (chunk == 0) return (const void*)&rope_any<TI, TO, ORDERED>;
   if constexpr (sizeof(TI) == 2)
     if (chunk == 8)
-      return interleaved ? (const void*)&rope_vec<TI, TO, 8, true> : (const void*)&rope_vec<TI, TO, 8, false>;
-  return interleaved ? (const void*)&rope_vec<TI, TO, 4, true> : (const void*)&rope_vec<TI, TO, 4, false>;
+      return interleaved ? (const void*)&rope_vec<TI, TO, 8, true, ORDERED>
+                         : (const void*)&rope_vec<TI, TO, 8, false, ORDERED>;
+  return interleaved ? (const void*)&rope_vec<TI, TO, 4, true, ORDERED>
+                     : (const void*)&rope_vec<TI, TO, 4, false, ORDERED>;
+}
+template <typename TI, typename TO>
+const void* rope_kernel(const RopeArgs& a) {
+  return a.slots && a.T > 1 && a.T <= kOrderedRows ? rope_kernel<TI, TO, true>(a.chunk, a.interleaved)
+                                                   : rope_kernel<TI, TO, false>(a.chunk, a.interleaved);
 }
 
 }  // namespace
@@ -351,15 +419,15 @@ hipError_t launch_rope(const RopeArgs& args, int in_dtype, int out_dtype, hipStr
   const int threads = (total << a.gp_shift) < 4 * 64 * (int64_t)a.cus ? 64 : kRopeThreads;
   const void* fn = nullptr;
   if (in_dtype == out_dtype)
-    fn = in_dtype == MGI_F32    ? rope_kernel<float, float>(c, a.interleaved)
-         : in_dtype == MGI_BF16 ? rope_kernel<bf16_t, bf16_t>(c, a.interleaved)
-                                : rope_kernel<f16_t, f16_t>(c, a.interleaved);
+    fn = in_dtype == MGI_F32    ? rope_kernel<float, float>(a)
+         : in_dtype == MGI_BF16 ? rope_kernel<bf16_t, bf16_t>(a)
+                                : rope_kernel<f16_t, f16_t>(a);
   else if (in_dtype == MGI_F32)
-    fn = out_dtype == MGI_BF16 ? rope_kernel<float, bf16_t>(c, a.interleaved)
-                               : rope_kernel<float, f16_t>(c, a.interleaved);
+    fn = out_dtype == MGI_BF16 ? rope_kernel<float, bf16_t>(a)
+                               : rope_kernel<float, f16_t>(a);
   else if (out_dtype == MGI_F32)
-    fn = in_dtype == MGI_BF16 ? rope_kernel<bf16_t, float>(c, a.interleaved)
-                              : rope_kernel<f16_t, float>(c, a.interleaved);
+    fn = in_dtype == MGI_BF16 ? rope_kernel<bf16_t, float>(a)
+                              : rope_kernel<f16_t, float>(a);
   else
     return hipErrorInvalidValue;
   void* kargs[] = {&a};

@@ -148,7 +148,8 @@ def kv_append_rope_hip(pool: KVBlockPool, layer_idx: int, q: torch.Tensor, k: to
     q: [T, Hq, D]; k, v: [T, H, D] of the pool's H heads; a chunk's T rows or a decode
     batch's. Returns the queries, [T, Hq, D] in the pool's dtype, for the attention
     that follows. Rows with a negative slot, or a position outside the table,
-    leave the pool as it was.
+    leave the pool as it was. Of rows on one slot the last is kept, K and V both, in
+    calls of up to 256 rows; in longer ones each element is one of theirs.
     """
     return _native.ops().kv_append_rope(pool.k, pool.v, int(layer_idx), q, k, v, slot_mapping, positions, cos_sin,
                                         q_weight, k_weight, float(eps), bool(interleaved))

@@ -309,3 +309,57 @@ def test_ctypes_path_is_bit_identical_and_refuses_alike():
                 getattr(_ctypes_ops, fn)(*args)
             assert str(a.value) == str(b.value), name
     assert torch.equal(p.k, before)
+
+
+def _rows_on_few_slots(T, Hq, H, D, R, S, new, pool_t, strided, itype):
+    """An append of T rows to few slots, some of them skipped: (per slot the rows
+    that are written, in order; what the pool holds after; the rows' keys and their
+    terms in 64 bits; the values as the pool's type)."""
+    g = torch.Generator().manual_seed(T)
+    N, P = max(2, -(-T // (3 * S))), 500
+    table = hpd.rope_table(P, R, device=DEV)
+    pool = KVBlockPool(2, N, S, H, D, device=DEV, dtype=pool_t)
+    if strided:
+        pool.k, pool.v = (torch.zeros((2, N, S, H, D, 2), dtype=pool_t, device=DEV)[..., 1] for _ in range(2))
+    pool.k.fill_(7), pool.v.fill_(7)
+    q, k, v = (_randn((T, h, D), new, 100 + i) for i, h in enumerate((Hq, H, H)))
+    w = _randn((D,), new, 103), _randn((D,), new, 104)
+    pos, few = torch.randint(0, P, (T,), generator=g), torch.randperm(N * S, generator=g)[:max(1, T // 4)]
+    slots = few[torch.randint(0, few.numel(), (T,), generator=g)]
+    slots[torch.rand(T, generator=g) < 0.05] = -1
+    if itype == torch.int64:  # past the pool, the low word a slot's
+        slots[torch.rand(T, generator=g) < 0.1] += 2 ** 32
+    pos[torch.rand(T, generator=g) < 0.2] = P  # not written: the row before on its slot stays
+    hpd.kv_append_rope_hip(pool, 1, q, k, v, slots.to(itype).to(DEV), pos.to(itype).to(DEV), table, *w)
+    rows = [[t for t in range(T) if slots[t] == s and pos[t] < P] for s in range(N * S)]
+    assert T < 13 or any(len(r) > 1 for r in rows)
+    want, size = _formula(k, w[1], table[pos.clamp_max(P - 1).to(DEV)], R, False, 1e-6)
+    flat = [t[1].reshape(N * S, H, D) for t in (pool.k, pool.v)]
+    assert (pool.k[0] == 7).all() and (pool.v[0] == 7).all()
+    for s, r in enumerate(rows):
+        if not r:
+            assert (flat[0][s] == 7).all() and (flat[1][s] == 7).all()
+    return rows, *flat, want, size, v.to(pool_t)
+
+
+@pytest.mark.parametrize("itype", [torch.int64, torch.int32], ids=["i64", "i32"])
+@pytest.mark.parametrize("T", [2, 13, 64, 65, 200, 256])
+@pytest.mark.parametrize("Hq,H,D,R,S,new,pool_t,strided", [
+    (8, 4, 128, 128, 16, BF16, BF16, False), (2, 1, 64, 24, 4, F32, F16, False), (1, 1, 16, 16, 3, F16, F16, False),
+    (3, 2, 20, 6, 4, BF16, F32, False), (2, 2, 64, 64, 4, BF16, BF16, True)])
+def test_of_rows_on_one_slot_the_last_written_is_kept(T, itype, Hq, H, D, R, S, new, pool_t, strided):
+    rows, kk, vv, want, size, v = _rows_on_few_slots(T, Hq, H, D, R, S, new, pool_t, strided, itype)
+    at = [s for s, r in enumerate(rows) if r]
+    last = [rows[s][-1] for s in at]
+    _check(kk[at], want[last], size[last], "k")
+    assert torch.equal(_bits(vv[at]), _bits(v[last]))
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_longer_calls_keep_one_of_the_rows_in_every_element(strided):
+    rows, kk, vv, want, size, v = _rows_on_few_slots(400, 4, 2, 64, 64, 16, BF16, BF16, strided, torch.int64)
+    for s, r in enumerate(rows):
+        if r:
+            bound = 24 * U * size[r] + 2.0 ** -8 * want[r].abs().clamp_min(torch.finfo(BF16).tiny) * 1.0001
+            assert ((kk[s].double() - want[r]).abs() <= bound).any(0).all(), s
+            assert (vv[s] == v[r]).any(0).all(), s
