@@ -1303,7 +1303,7 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
   a.shared = (int)shared_blocks;
   a.P = (int)(shared_blocks * S);
   a.scale_log2 = scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f;
-  a.lazy = std::min(kSharedLazy / a.scale_log2, 1e30f);
+  a.lazy = std::min((dtype == MGI_F16 ? kSharedLazyF16 : kSharedLazy) / a.scale_log2, 1e30f);
   a.q_flip = scale < 0.f ? (dtype == MGI_F32 ? 0x80000000u : 0x80008000u) : 0u;
   a.q_zero = scale == 0.f;
   magic_of(S, &a.s_mul, &a.s_shift);

@@ -157,7 +157,11 @@ struct SharedArgs {
   int* ws_split;           // the two lists' segment lengths
 };
 constexpr int kSharedMaxB = 4096;    // rows of the split form (their prefix sums live in LDS)
-constexpr float kSharedLazy = 6.f;   // log2 units a score may pass the running maximum by
+// log2 units a score may pass the running maximum by.
+constexpr float kSharedLazy = 6.f;
+// f16's are fewer, for its weights are scaled to the top of the type: kSharedF16Scale in
+// log2 units and these stay below its largest, 65 504.
+constexpr float kSharedLazyF16 = 2.f, kSharedF16Scale = 13.f;
 hipError_t launch_paged_shared_f32(const SharedArgs& a, hipStream_t stream);
 hipError_t launch_paged_shared_bf16(const SharedArgs& a, hipStream_t stream);
 hipError_t launch_paged_shared_f16(const SharedArgs& a, hipStream_t stream);

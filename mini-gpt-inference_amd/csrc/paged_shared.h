@@ -32,11 +32,14 @@
 // Rounding: the weights 2^(s - m) go to the 16-bit type for the second product, at
 // most half a step of each, as independent errors about as much in the output as
 // its own rounding (bf16: 0.0023 off 64 bits, relative, where rounding alone is
-// 0.0017; f16 0.00028 and 0.00021). Scores, sums l and outputs are f32.
+// 0.0017; f16 0.00028 and 0.00021). f16 holds that down to 2^-14 only, so its weights
+// are 2^(s - m + 13) (the sums' too, so that it divides out): half a step down to 2^-27
+// of the largest, 2^-38 of it below. Scores, sums l and outputs are f32; l sums the
+// weights before their rounding in the register form, the rounded ones in LDS's.
 //
-// The running maximum moves only when a score passes it by kSharedLazy in log2
-// units, which costs one comparison per tile instead of a reduction over lanes;
-// weights stay below 2^kSharedLazy, well inside every type.
+// The running maximum moves only when a score passes it by kSharedLazy (f16:
+// kSharedLazyF16) in log2 units, which costs one comparison per tile instead of a
+// reduction over lanes; weights stay inside every type.
 //
 // What bounds it (MI355X; inputs from memory, another set each call): 64 x 32 heads
 // on 4096 shared tokens and 64-1024 of their own, bf16, 649 MB: 116 us, 5.6 TB/s; 128
@@ -97,6 +100,16 @@ __device__ __forceinline__ float across_groups_sum(float x) {
 }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// What the exponents of weights are taken from, in log2 units, for a maximum m (raw): m c,
+// for f16 lowered by its scale. Scores past 2^20, whose product with c is off by a
+// sixteenth and more, keep it as it is: the scale leaves them no room for that.
+template <typename T>
+__device__ __forceinline__ float exponent_base(float m, float c) {
+  if (m == kNegInf) return 0.f;
+  if constexpr (std::is_same_v<T, f16_t>) return fabsf(m * c) < 0x1p20f ? fmaf(m, c, -kSharedF16Scale) : m * c;
+  else return m * c;
+}
+
 // Sizes of one tile: KEYS keys, held by a wavefront.
 template <typename T, int DP>
 struct Tile {
@@ -121,7 +134,7 @@ template <int DP, int NQ>
 struct State {
   f32x4 acc[NQ][DP / 16];  // O^T
   float m[NQ];             // running maximum, raw scores
-  float mc[NQ];            // the same times the scale, 0 while it is -inf
+  float mc[NQ];            // its exponent_base, 0 while it is -inf
   float l[NQ];             // this lane group's part of the sum
   bool any;                // some key counted
   __device__ __forceinline__ void reset() {
@@ -345,7 +358,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, Tile<T, DP>& f,
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       const float mn = fmaxf(st.m[q], across_groups_max(top[q]));
-      const float mcn = mn == kNegInf ? 0.f : mn * c;
+      const float mcn = exponent_base<T>(mn, c);
       const float alpha = st.m[q] == kNegInf ? 0.f : fast_exp2(st.mc[q] - mcn);
       st.m[q] = mn;
       st.mc[q] = mcn;
@@ -944,7 +957,7 @@ __device__ __forceinline__ void attend_lds_tile(const SharedArgs& a, const char*
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[q][kb][i]);
     if (__any(top > st.m[q] + a.lazy)) {
-      const float mn = fmaxf(st.m[q], across_groups_max(top)), mcn = mn == kNegInf ? 0.f : mn * c;
+      const float mn = fmaxf(st.m[q], across_groups_max(top)), mcn = exponent_base<T>(mn, c);
       const float alpha = st.m[q] == kNegInf ? 0.f : fast_exp2(st.mc[q] - mcn);
       st.m[q] = mn;
       st.mc[q] = mcn;

@@ -423,3 +423,57 @@ def test_ctypes_path_is_bit_identical_and_refuses_alike():
         with pytest.raises(kind) as y:
             _ctypes_ops.paged_decode_shared(*args)
         assert str(x.value) == str(y.value), name
+
+
+@DTYPES
+@ROUTES
+@pytest.mark.parametrize("nats", [12.5, 17.5, 24.5])
+def test_keys_far_below_a_sink_keep_their_weight(nats, dtype, route):
+    """Every 32nd key scores ``nats`` above the others and has no value, so the output
+    is the others', whose weights are 2^-18, 2^-25 and 2^-35 of the largest: below
+    what f16 holds to half a step, unless scaled. Scaled by 2^13 they are off by
+    half a step down to 2^-27 and by 2^-38 of the largest below, which adds 2^-38
+    sum_t |V_t| / sum_t (w_t / max w)."""
+    B, H, D, S, shared, ctx = 3, 2, 64, 16, 160, [3200, 2561, 3000]
+    q, pool, tables, lens, layer = make(B, H, H, D, S, shared, ctx, dtype, seed=31)
+    q.zero_()
+    q[..., 0] = 4
+    k, v = pool.k[layer], pool.v[layer]
+    k.copy_(torch.where(k.isnan(), k, 0))
+    v.mul_(100).add_(torch.where(v.isnan(), v, 1000))
+    for b, c in enumerate(ctx):
+        t = torch.arange(5, c, 32, device=DEV)
+        row = torch.where(t // S < shared, tables[0, t // S], tables[b, t // S])
+        k[row, t % S, :, 0], v[row, t % S] = 2 * nats, 0
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=shared)
+    out, A, X, n = reference(q, pool, tables, lens, layer, shared)
+    if dtype == F16:  # |V| < 1600, 31 of 32 keys; of the sum the sinks alone are n / 32
+        A = A + 2.0 ** -38 * 1600 * 32 / (0.5 * torch.finfo(F16).eps)
+    check(got, (out, A, X, n), dtype, f"{nats}")
+
+
+@DTYPES
+@ROUTES
+def test_scores_in_the_millions(dtype, route):
+    """Scores of 8 to 11 million, thousands apart: the largest key's value, to the
+    rounding of its weight and of the output."""
+    B, H, D, S, shared, ctx = 3, 2, 64, 16, 10, [300, 161, 259]
+    q, pool, tables, lens, layer = make(B, H, H, D, S, shared, ctx, dtype, seed=32)
+    q.zero_()
+    q[..., 0] = 30000
+    g = torch.Generator().manual_seed(33)
+    k, best = pool.k[layer], torch.empty((B, H, D), dtype=torch.float64, device=DEV)
+    step = 32 if dtype == BF16 else 2  # of the type at 2048 .. 4096, doubled for bf16
+    rank = torch.stack([torch.randperm(k.shape[0] * S, generator=g) for _ in range(H)], 1).view(-1, S, H).to(DEV)
+    k.copy_(torch.where(k.isnan(), k, 0))
+    k[..., 0] = torch.where(k[..., 0].isnan(), k[..., 0], (2048 + step * (rank % (2000 // step))).to(dtype))
+    for b, c in enumerate(ctx):
+        t = torch.arange(c, device=DEV)
+        row = torch.where(t // S < shared, tables[0, t // S], tables[b, t // S])
+        for h in range(H):
+            score, value = k[row, t % S, h, 0].double(), pool.v[layer, row, t % S, h].double()
+            top = score == score.max()
+            best[b, h] = value[top].mean(0)
+            bound = value[top].abs().mean(0) * torch.finfo(dtype).eps * 1.01
+            got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=shared)[b, h]
+            assert ((got.double() - best[b, h]).abs() <= bound).all(), (b, h)
