@@ -477,3 +477,23 @@ def test_scores_in_the_millions(dtype, route):
             bound = value[top].abs().mean(0) * torch.finfo(dtype).eps * 1.01
             got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, layer, shared_blocks=shared)[b, h]
             assert ((got.double() - best[b, h]).abs() <= bound).all(), (b, h)
+
+
+@DTYPES
+@pytest.mark.parametrize("route", ["registers", "lds"])
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_own_tiles_past_the_caches(D, dtype, route):
+    """More than 192 MB of own keys and values (rows may name the same blocks): read
+    as non-temporal, whole and padded head dims, runs that end inside tiles."""
+    B, H, S, shared, N = 64, 16, 16, 3, 200
+    g = torch.Generator().manual_seed(D)
+    own = torch.randint(850, 1000, (B,), generator=g)
+    own[7], own[20] = 0, -30  # no own tokens; shorter than the shared blocks
+    assert (own.clamp_min(0) // 32 * 32).sum() * H * 2 * D * torch.finfo(dtype).bits // 8 > 192 << 20
+    pool = KVBlockPool(1, N, S, H, D, device=DEV, dtype=dtype)
+    pool.k.copy_(torch.randn(pool.k.shape, generator=g)), pool.v.copy_(torch.randn(pool.v.shape, generator=g))
+    tables = torch.randint(0, N, (B, shared + 63), generator=g).to(DEV)
+    lens = (own + shared * S).to(DEV)
+    q = torch.randn((B, H, D), generator=g).to(dtype).to(DEV)
+    got = hpd.paged_attention_shared_prefix_hip(q, pool, tables, lens, 0, shared_blocks=shared)
+    check(got, reference(q, pool, tables, lens, 0, shared), dtype, f"{D}")
