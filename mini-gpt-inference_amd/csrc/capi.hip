@@ -811,28 +811,40 @@ struct SharedPlan {
 
 // Whether one workgroup per (row, virtual head), each reading the shared tokens by
 // itself, is estimated faster than the split over all workgroups and its joining
-// launch. Only the table's width is known here: rows are taken to fill it in the
-// first estimate, whose longest row ends the call, and 0.6 of it in the second. In us,
-// fitted to 2000 shapes on MI355X (2-256 rows, 1-32 KV heads, 1-8 query heads each,
-// head_dim 32-128, 64 to 65 536 shared tokens, the three types); the slower one is
-// taken by more than 10 % in 1 of 40, the mean loss is 0.7 %. One launch / split:
-// 4 x 8 heads of 32, f32, 200-256 tokens, 128 shared: 6.9 / 11.6; 13 x 16, bf16,
-// 820-1300, 800 shared: 14.7 / 13.1; 24 x 12, f32, 1520-1900, 1504 shared: 37 / 18;
-// 64 x 32, 4160-5120, 4096 shared: 401 / 113.
+// launch. Only the table's width is known here, and rows fill it or do not, so one
+// launch has to be the faster one for rows of a range (the longest full, 0.6 of it the
+// mean), and at most a tenth slower with every row at the end of the shared tokens (each
+// reads them all, the split once) and with one of them full (its workgroup ends the
+// call). Mixes between lie between. In us, fitted to 2000 shapes on MI355X (2-256 rows,
+// 1-32 KV heads, 1-8 query heads each, head_dim 32-128, 64 to 65 536 shared tokens, the
+// three types, lengths of a range that fills the table): the slower one is taken by
+// more than 10 % in 1 of 40, the mean loss is 0.7 %. Of 700 shapes with six mixes each
+// (own lengths full, half of them, one, none, a range) one launch is taken where it is
+// over 25 % slower in 15 of 4200, never 2 times as slow (158 and 54 by the first
+// estimate alone). One launch / split: 4 x 8 heads of 32, f32, 200-256 tokens, 128 shared:
+// 6.9 / 11.6; 13 x 16, bf16, 820-1300, 800 shared: 14.7 / 13.1; 24 x 12, f32, 1520-1900,
+// 1504 shared: 37 / 18; 64 x 32, 4160-5120, 4096 shared: 401 / 113.
 bool shared_one_launch(int64_t B, int64_t Hk, int64_t vheads, int64_t rows, int64_t D, int64_t eb, int64_t keys,
                        int64_t shared_tokens, int64_t tokens) {
   const double width = D <= 64 ? 64 : D <= 128 ? 128 : 256, cus = (double)device_cus();
   const double own = (double)(tokens - shared_tokens), row_mb = 2e-6 * (double)(D * eb);
-  // Eight wavefronts take a row's tiles in turn, 1.7 us a 16 KiB tile.
-  const double turns = (double)((tokens + keys - 1) / keys + 7) / 8;
+  // Eight wavefronts take a row's tiles in turn, 1.7 us a 16 KiB tile, the first turn
+  // whatever there is; 0.83 workgroups to a CU run together.
   const double tile_us = 1.72 * std::pow(width * (double)eb / 256, 0.73);
-  const double wgs = (double)(B * vheads);
-  const double one_us = 4.5 + std::max(std::floor(turns) * tile_us * std::max(1.0, wgs / (0.83 * cus)),
-                                       wgs * (double)tokens * row_mb / 10.6);
+  const double wgs = (double)(B * vheads), rounds = std::max(1.0, wgs / (0.83 * cus));
+  auto turns_us = [&](int64_t n) { return (double)(((std::max<int64_t>(n, 1) + keys - 1) / keys + 7) / 8) * tile_us; };
+  // With `full` rows filling the table and the others at the end of the shared tokens.
+  auto one_us = [&](double full) {
+    const double longest = turns_us(full > 0 ? tokens : shared_tokens);
+    const double in_turn = (full * turns_us(tokens) + ((double)B - full) * turns_us(shared_tokens)) / (double)B * rounds;
+    return 4.5 + std::max({longest, in_turn, (wgs * (double)shared_tokens + full * (double)vheads * own) * row_mb / 10.6});
+  };
   const double mflop = 4e-6 * (double)(rows * Hk * shared_tokens * D);
-  const double split_us = 13.0 + (double)Hk * ((double)shared_tokens + 0.6 * (double)B * own) * row_mb / 6.0 +
-                          mflop / (eb == 2 ? 507.0 : 63.0);
-  return one_us <= split_us;
+  auto split_us = [&](double full) {
+    return 13.0 + (double)Hk * ((double)shared_tokens + full * own) * row_mb / 6.0 + mflop / (eb == 2 ? 507.0 : 63.0);
+  };
+  return one_us((double)B) <= split_us(0.6 * (double)B) && one_us(0) <= 1.1 * split_us(0) &&
+         one_us(1) <= 1.1 * split_us(1);
 }
 
 // MINIVLLM_HIP_SHARED_SPLIT = 0 or 1 takes one launch or the split, and

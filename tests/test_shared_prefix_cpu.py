@@ -60,3 +60,58 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(ValueError, match="q must be on a GPU device"):
         hpd.paged_attention_shared_prefix_hip(torch.zeros(1, 2, 64), pool, torch.zeros(1, 1, dtype=torch.long),
                                               torch.ones(1, dtype=torch.long), 0, shared_blocks=1)
+
+
+def one_launch(B, Hq, Hk, D, shared, tokens, dtype=1, S=16):
+    """Whether a call whose table holds `tokens` takes one launch (no workspace)."""
+    return _native.lib().mgi_paged_decode_shared_workspace_bytes(B, Hq, Hk, D, S, -(-tokens // S), shared // S, dtype) == 0
+
+
+@pytest.mark.parametrize("B,Hq,Hk,D,shared,tokens,dtype", [
+    # what each row reads again of the shared tokens: 401 us against 113 with 64 x 32 heads
+    (64, 32, 32, 128, 4096, 5120, 1), (64, 32, 8, 128, 4096, 8192, 1), (64, 32, 32, 128, 1024, 4096, 1),
+    (32, 32, 8, 128, 2048, 4096, 1), (24, 12, 12, 64, 1504, 1904, 0),
+    # one full row among short ones, however wide the table
+    (16, 16, 16, 128, 0, 8192, 1), (64, 32, 8, 128, 128, 16384, 2), (256, 32, 32, 128, 0, 4096, 1),
+    # rows by the thousand, with few tokens or none: 48 us against 18 and more
+    (178, 33, 33, 128, 0, 64, 1), (232, 46, 46, 128, 0, 128, 0)])
+def test_wide_tables_keep_the_split(B, Hq, Hk, D, shared, tokens, dtype, monkeypatch):
+    for name in ("SPLIT", "LDS"):
+        monkeypatch.delenv("MINIVLLM_HIP_SHARED_" + name, raising=False)
+    for wider in (1, 2, 4, 16, 64, 256):
+        assert not one_launch(B, Hq, Hk, D, shared, shared + (tokens - shared) * wider, dtype), wider
+
+
+def test_small_calls_take_one_launch(monkeypatch):
+    monkeypatch.delenv("MINIVLLM_HIP_SHARED_SPLIT", raising=False)
+    for call in ((4, 8, 8, 32, 128, 256, 0), (13, 16, 16, 128, 800, 1312, 1), (1, 8, 2, 128, 0, 512, 2),
+                 (8, 8, 8, 64, 64, 512, 1), (32, 8, 8, 128, 16, 256, 1)):
+        assert one_launch(*call), call
+
+
+def test_one_long_row_ends_soon_where_one_launch_is_taken(monkeypatch):
+    """Over the ranges calls come in: one workgroup's turns of eight tiles for a full
+    row, 1.7 us each 16 KiB, stay below what the split takes for that row and the shared
+    tokens, and so does reading the shared tokens by every row, a tenth aside."""
+    monkeypatch.delenv("MINIVLLM_HIP_SHARED_SPLIT", raising=False)
+    taken = 0
+    for dtype, eb, keys in ((1, 2, 32), (0, 4, 16)):
+        for Hk in (1, 2, 8, 32):
+            for G in (1, 8, 40):
+                for D, width in ((32, 64), (64, 64), (128, 128), (256, 256)):
+                    for B in (1, 4, 13, 64, 256):
+                        for shared in (0, 128, 4096, 65536):
+                            for own in (16, 256, 1024, 4096, 16384, 131072):
+                                if not one_launch(B, Hk * G, Hk, D, shared, shared + own, dtype):
+                                    continue
+                                if B * Hk * ((G + 15) // 16) >= 1 << 14 and 2 * B * Hk * G * D * 4 > 4 << 30:
+                                    continue  # no partials past 4 GiB
+                                taken += 1
+                                mb, vheads = 2e-6 * D * eb, Hk * -(-G // 16)
+                                mflop = 4e-6 * B * G * Hk * shared * D / (507 if eb == 2 else 63)
+                                split = 13 + Hk * shared * mb / 6 + mflop
+                                turns = -(-(shared + own) // keys) // 8
+                                long = 4.5 + 1.72 * (width * eb / 256) ** 0.73 * turns
+                                assert long <= 1.1 * (split + Hk * own * mb / 6), (B, Hk, G, D, shared, own, dtype)
+                                assert 4.5 + B * vheads * shared * mb / 10.6 <= 1.1 * split, (B, Hk, G, D, shared, own, dtype)
+    assert taken > 300
