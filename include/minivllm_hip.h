@@ -403,7 +403,11 @@ int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
  * Decode attention of a batch whose sequences begin with the same cached blocks:
  * mgi_paged_decode's result (one query token per sequence), with the first
  * shared_blocks entries of every row of block_tables taken from row 0, and those
- * blocks read once for all rows. No counterpart in the reference.
+ * blocks read once for all rows. Each row reads them by itself in calls too small
+ * for a second launch to pay, with more than 4096 rows, where the partial results of
+ * every (row, head) would take more than 4 GiB, and, token by token in one wavefront
+ * per (row, head), where head_dim is over 256, no multiple of 8 or strided, or head
+ * rows are not 16-byte aligned. No counterpart in the reference.
  *
  * q and out are [B, Hq, D] with Hq a multiple of the pool's Hk heads: query head h
  * reads KV head h / (Hq / Hk). Context lengths count all tokens, the shared ones
@@ -411,8 +415,9 @@ int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
  * row 0's blocks all the same, by itself. Lengths are clamped to [0, M*S], a table
  * entry outside [0, N) masks its block, a row without keys gives 0, and only the
  * tokens of some row's context enter any result. Arithmetic is f32, but that
- * 2-byte types round the softmax weights to their type for the second product
- * (as mgi_paged_prefill).
+ * 2-byte types round the softmax weights to their type for the second product (as
+ * mgi_paged_prefill; f16's scaled by 2^13, so that far keys keep theirs), which
+ * mgi_paged_decode does not.
  * 0 <= shared_blocks <= M. B <= 65535, B*Hq < 2^25, M*S < 2^30, D <= 512.
  *
  * workspace: mgi_paged_decode_shared_workspace_bytes(...) bytes for the same sizes,

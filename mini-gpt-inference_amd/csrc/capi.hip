@@ -882,9 +882,10 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   if (p.one_launch) return p;
   p.s_tiles = (int)tiles;
   p.s_units = (int)(Hk * p.set_blocks);
-  // By bytes; a piece costs two tiles more, its chain of loads (with none a list of
-  // two-tile pieces ended last: 130 x 13 heads, 128 shared tokens, 92 us, so 66; 100 x
-  // 4, D = 64, 3200: 26.5 and 22.3).
+  // In own tiles, by bytes; a piece costs eight more, its chain of loads: two tiles of
+  // the register form, four of the LDS form (with none a list of two-tile pieces ended
+  // last: 130 x 13 heads, 128 shared tokens, 92 us, so 66; 100 x 4, D = 64, 3200: 26.5
+  // and 22.3).
   p.s_cost = (int)(step / keys);
   p.s_piece = 8;
   p.s_cont = B * Hq;

@@ -32,7 +32,7 @@
 // Rounding: the weights 2^(s - m) go to the 16-bit type for the second product, at
 // most half a step of each, as independent errors about as much in the output as
 // its own rounding (bf16: 0.0023 off 64 bits, relative, where rounding alone is
-// 0.0017; f16 0.00028 and 0.00021). f16 holds that down to 2^-14 only, so its weights
+// 0.0017; f16 0.00027 and 0.00021). f16 holds that down to 2^-14 only, so its weights
 // are 2^(s - m + 13) (the sums' too, so that it divides out): half a step down to 2^-27
 // of the largest, 2^-38 of it below. Scores, sums l and outputs are f32; l sums the
 // weights before their rounding in the register form, the rounded ones in LDS's.
@@ -44,7 +44,7 @@
 // What bounds it (MI355X; inputs from memory, another set each call): 64 x 32 heads
 // on 4096 shared tokens and 64-1024 of their own, bf16, 649 MB: 116 us, 5.6 TB/s; 128
 // x 32 on 8 KV heads over 65 536 shared, 138 GFLOP: 172 us, 800 TFLOP/s, the softmax's
-// VALU work beside the products (37 % of cycles in the matrix cores, LDS conflicts
+// VALU work in line with the products (37 % of cycles in the matrix cores, LDS conflicts
 // none; with all keys in L2 it still takes 141 of the 146 us without own tokens).
 // Calls under about 30 us are chains: launch and the rows' prefix sums 4 us, a first
 // tile 3, the joining launch 5-7 us.

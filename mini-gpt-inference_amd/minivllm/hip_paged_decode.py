@@ -86,15 +86,19 @@ def paged_attention_shared_prefix_hip(q: torch.Tensor, pool: KVBlockPool, block_
     """paged_attention_batch_hip for sequences that begin with the same cached
     blocks: the first ``shared_blocks`` entries of every row of block_tables are
     taken from row 0 (the others' are not read), and those blocks' keys and
-    values are read once for all rows, on the matrix cores.
+    values are read once for all rows, on the matrix cores; by each row itself in
+    calls too small for that to pay, past 4096 rows, and where head_dim is over 256 or
+    no multiple of 8 or rows are not contiguous and 16-byte aligned (the last by a slow
+    kernel).
 
     q: [B, Hq, D] with Hq a multiple of the pool's heads H; query head h reads KV
     head h // (Hq // H). context_lengths count a sequence's tokens, the shared ones
     included; a sequence shorter than the shared blocks (a padding row of
-    length 0, say) is attended by itself. shared_blocks = 0 is plain decode
-    attention with grouped query heads. Returns a fresh [B, Hq, D] tensor of
-    q.dtype. 2-byte types round the softmax weights to their type for the product
-    with the values, as paged_prefill_hip does; sums are float32.
+    length 0, say) is attended by itself. shared_blocks = 0 is decode attention
+    with grouped query heads. Returns a fresh [B, Hq, D] tensor of q.dtype. 2-byte
+    types round the softmax weights to their type for the product with the values, as
+    paged_prefill_hip does and paged_attention_batch_hip does not (bfloat16: 0.0023 off
+    64 bits, relative, instead of 0.0017); sums are float32.
     """
     return _native.ops().paged_decode_shared(q, pool.k, pool.v, block_tables, context_lengths, int(layer_idx),
                                              int(shared_blocks))
