@@ -417,7 +417,7 @@ int mgi_kv_append_rope(void* q_out, const int64_t* q_out_strides, /* [3] */
  * tokens of some row's context enter any result. Arithmetic is f32, but that
  * 2-byte types round the softmax weights to their type for the second product (as
  * mgi_paged_prefill; f16's scaled by 2^13, so that far keys keep theirs), which
- * mgi_paged_decode does not.
+ * mgi_paged_decode does not; scores up to 2^27 in size.
  * 0 <= shared_blocks <= M. B <= 65535, B*Hq < 2^25, M*S < 2^30, D <= 512.
  *
  * workspace: mgi_paged_decode_shared_workspace_bytes(...) bytes for the same sizes,

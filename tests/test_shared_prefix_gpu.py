@@ -454,19 +454,20 @@ def test_keys_far_below_a_sink_keep_their_weight(nats, dtype, route):
 
 @DTYPES
 @ROUTES
-def test_scores_in_the_millions(dtype, route):
-    """Scores of 8 to 11 million, thousands apart: the largest key's value, to the
-    rounding of its weight and of the output."""
+@pytest.mark.parametrize("dims", [1, 6])
+def test_scores_in_the_millions(dims, dtype, route):
+    """Scores of 16 to 22 million, or 94 to 131 (2^27 is 134), thousands apart, exact
+    in 32 bits: the largest key's value, to the rounding of its weight and of the output."""
     B, H, D, S, shared, ctx = 3, 2, 64, 16, 10, [300, 161, 259]
     q, pool, tables, lens, layer = make(B, H, H, D, S, shared, ctx, dtype, seed=32)
     q.zero_()
-    q[..., 0] = 30000
+    q[..., :dims] = 61440
     g = torch.Generator().manual_seed(33)
     k, best = pool.k[layer], torch.empty((B, H, D), dtype=torch.float64, device=DEV)
     step = 32 if dtype == BF16 else 2  # of the type at 2048 .. 4096, doubled for bf16
     rank = torch.stack([torch.randperm(k.shape[0] * S, generator=g) for _ in range(H)], 1).view(-1, S, H).to(DEV)
     k.copy_(torch.where(k.isnan(), k, 0))
-    k[..., 0] = torch.where(k[..., 0].isnan(), k[..., 0], (2048 + step * (rank % (2000 // step))).to(dtype))
+    k[..., :dims] = torch.where(k[..., :dims].isnan(), k[..., :dims], (2048 + step * (rank % (800 // step))).to(dtype)[..., None])
     for b, c in enumerate(ctx):
         t = torch.arange(c, device=DEV)
         row = torch.where(t // S < shared, tables[0, t // S], tables[b, t // S])
