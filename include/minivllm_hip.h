@@ -63,8 +63,8 @@ const char* mgi_last_error(void);
  * mgi_paged_prefill_workspace_bytes); 1.03 mgi_paged_decode_noalloc; 1.04
  * mgi_paged_decode_append. mgi_decode_linear, mgi_decode_linear_norm, their
  * queries, mgi_paged_decode_workgroup_waves, mgi_qk_norm_rope,
- * mgi_kv_append_rope and mgi_paged_decode_shared came later without a change to
- * the others. */
+ * mgi_kv_append_rope, mgi_paged_decode_shared, the 4-bit pool's calls (*_fp4)
+ * and mgi_prompt_attention came later without a change to the others. */
 int mgi_abi_version(void);
 
 /*
@@ -441,6 +441,82 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, /* [3] */
  * device (0 if none). */
 size_t mgi_paged_decode_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S,
                                                int64_t M, int64_t shared_blocks, int dtype);
+
+/*
+ * The 4-bit KV pool. No counterpart in the reference, whose pool holds f32. A head's row
+ * of D <= 256 dims is held in groups of 32 dims (the last padded with zeros): e2m1 codes
+ * (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) and one e8m0 byte per group, as the OCP
+ * microscaling formats have them. The scale is the least 2^e, -125 <= e <= 125, with
+ * max |x| <= 7 * 2^e; codes are nearest, ties to the even code; a group with an
+ * infinity or a NaN is held as NaN. 17/64 of the bytes of bf16.
+ *
+ * One (layer, block, head) is a slab of mgi_fp4_slab_bytes(S, D) bytes, 16-byte aligned:
+ *   K codes [S][g * 16] (two to a byte, the even dim low), V codes [S][g * 16],
+ *   K scales [S][g], V scales [g][S],    g = ceil(D / 32),
+ * at pool + layer * pool_strides[0] + block * pool_strides[1] + head * pool_strides[2]
+ * (bytes, multiples of 16). S <= 2^20, N < 2^31.
+ */
+size_t mgi_fp4_slab_bytes(int64_t S, int64_t D);
+
+/*
+ * KV append into the 4-bit pool: rows k_new, v_new [T, H, D] (any strides; f32, bf16 or
+ * f16) as mgi_kv_append writes them, quantised on the way. Rows with a slot outside
+ * [0, N*S) are skipped. If rows name the same slot, it holds the last one. T < 2^24.
+ */
+int mgi_kv_append_fp4(void* pool, const int64_t* pool_strides, /* [3], bytes */
+                      const void* k_new, const void* v_new,
+                      const int64_t* k_new_strides, /* [3] */
+                      const int64_t* v_new_strides, /* [3] */
+                      int new_dtype,
+                      const void* slot_mapping, int64_t slot_stride, int slot_itype,
+                      int64_t T, int64_t H, int64_t D,
+                      int64_t S, int64_t N, int64_t L, int64_t layer_idx,
+                      void* stream);
+
+/*
+ * The other way: k_out[t], v_out[t] [T, H, D] (any strides; f32, bf16 or f16) = the values
+ * slot_mapping[t] holds, each rounded once (exact in f32 and bf16; f16 where it is in
+ * range). A row whose slot is outside [0, N*S) comes out 0. T < 2^24.
+ */
+int mgi_kv_gather_fp4(void* k_out, void* v_out,
+                      const int64_t* k_out_strides, /* [3] */
+                      const int64_t* v_out_strides, /* [3] */
+                      int out_dtype,
+                      const void* pool, const int64_t* pool_strides, /* [3], bytes */
+                      const void* slot_mapping, int64_t slot_stride, int slot_itype,
+                      int64_t T, int64_t H, int64_t D,
+                      int64_t S, int64_t N, int64_t L, int64_t layer_idx,
+                      void* stream);
+
+/*
+ * Decode attention over the 4-bit pool (one query token per sequence): mgi_paged_decode's
+ * result for the values the pool holds, with grouped query heads as in
+ * mgi_paged_decode_shared (q and out [B, Hq, D], Hq a multiple of the pool's Hk). Lengths
+ * are clamped to [0, M*S], a table entry outside [0, N) masks its block, a row without keys
+ * gives 0, and only the tokens of a row's context enter its result. Sums are f32; the
+ * products take q and the softmax weights as sums of bf16 terms (q exactly; weights to
+ * 2^-17, 2^-25 for f32). One launch or two, by sizes alone. Same inputs, same bits.
+ * B and Hq <= 65535, B*Hq < 2^25, M*S < 2^30, B*M*S < 2^35.
+ *
+ * workspace: mgi_paged_decode_fp4_workspace_bytes(...) bytes for the same sizes, 16-byte
+ * aligned; may be NULL when that is 0. Contents need no initialisation; calls that
+ * overlap in time need separate workspaces. MINIVLLM_HIP_FP4_SPLIT (read on every call,
+ * by both functions) forces one launch (0) or two (1).
+ */
+int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, /* [3] */
+                         const void* q, const int64_t* q_strides, /* [3] */
+                         int dtype,
+                         const void* pool, const int64_t* pool_strides, /* [3], bytes */
+                         const void* block_tables, const int64_t* bt_strides, /* [2] */
+                         int bt_itype,
+                         const void* context_lens, int64_t cl_stride, int cl_itype,
+                         int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t N,
+                         int64_t M, int64_t L, int64_t layer_idx, float scale,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes mgi_paged_decode_fp4 needs for these sizes on the current device (0 if
+ * none). */
+size_t mgi_paged_decode_fp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M);
 
 #ifdef __cplusplus
 }

@@ -11,6 +11,7 @@
 #include <mutex>
 #include <string>
 
+#include "fp4_kv.h"
 #include "mgi_internal.h"
 #include "minivllm_hip.h"
 
@@ -898,6 +899,86 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, 
   return p;
 }
 
+// How mgi_paged_decode_fp4 runs a call of these sizes.
+struct Fp4Plan {
+  int one_launch, waves, q_tiles;
+  int64_t ml_offset, cum_offset;
+  size_t total;
+};
+
+constexpr int64_t kFp4OneLaunchTiles = 8;  // tiles of 32 tokens per wavefront, at most, of the one-launch form
+
+Fp4Plan fp4_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M) {
+  Fp4Plan p{};
+  const int64_t G = Hq / Hk, rows = std::min<int64_t>(G, 16), dims = mgi::fp4_groups(D) * 32;
+  p.q_tiles = (int)((G + 15) / 16);
+  const int64_t tiles = (M * S + 31) / 32, pairs = B * Hk * p.q_tiles;
+  int64_t waves = 8;
+  while (waves > 1 && (waves * rows * (dims + 4) * 4 > 65536 || waves / 2 >= tiles)) waves /= 2;
+  const int forced = env_int("MINIVLLM_HIP_FP4_SPLIT", -1);
+  if (forced < 0 ? tiles <= kFp4OneLaunchTiles * waves : forced == 0) {
+    p.one_launch = 1;
+    p.waves = (int)waves;
+    return p;
+  }
+  int64_t most = 16 * (int64_t)device_cus();
+  waves = 4;
+  while (waves < most && waves < pairs * tiles) waves *= 2;
+  p.waves = (int)waves;
+  p.ml_offset = round_up(2 * waves * rows * dims * 4, kWorkspaceAlign);
+  p.cum_offset = round_up(p.ml_offset + 2 * waves * 16 * 8, kWorkspaceAlign);
+  p.total = (size_t)(p.cum_offset + (B + 1) * 4);
+  return p;
+}
+
+// Limits the 4-bit pool's calls share.
+int check_fp4_pool(const void* pool, const int64_t* strides, int64_t H, int64_t D, int64_t S, int64_t N, int64_t L,
+                   int64_t layer_idx) {
+  if (!pool) return fail(MGI_EINVAL, "null tensor pointer");
+  if (!strides) return fail(MGI_EINVAL, "null stride array");
+  if (H <= 0 || D <= 0 || S <= 0 || N <= 0 || L <= 0) return fail(MGI_EINVAL, "pool dimensions must be nonzero");
+  if (layer_idx < 0 || layer_idx >= L) return fail(MGI_EINVAL, "layer_idx outside KV pool");
+  if (D > mgi::kFp4MaxDim) return fail(MGI_EUNSUPPORTED, "head_dim larger than 256");
+  if (H > kMaxGridYZ) return fail(MGI_EUNSUPPORTED, "more than 65535 heads");
+  if (S > (int64_t(1) << 20)) return fail(MGI_EUNSUPPORTED, "block size larger than 2^20");
+  if (N >= (int64_t(1) << 31)) return fail(MGI_EUNSUPPORTED, "2^31 blocks or more");
+  if (!nonneg(strides, 3)) return fail(MGI_EINVAL, "strides must be non-negative");
+  if (!aligned16(pool) || strides[0] % 16 || strides[1] % 16 || strides[2] % 16)
+    return fail(MGI_EINVAL, "pool slabs must be 16-byte aligned");
+  return MGI_OK;
+}
+
+// Checks and fills what append and gather share (T > 0).
+int fp4_row_args(const void* pool, const int64_t* ps, const void* k, const void* v, const int64_t* ks,
+                 const int64_t* vs, int dtype, const void* slots, int64_t slot_stride, int slot_itype, int64_t T,
+                 int64_t H, int64_t D, int64_t S, int64_t N, int64_t L, int64_t layer_idx, mgi::Fp4RowArgs* a) {
+  const int rc = check_fp4_pool(pool, ps, H, D, S, N, L, layer_idx);
+  if (rc != MGI_OK) return rc;
+  if (!k || !v || !slots) return fail(MGI_EINVAL, "null tensor pointer");
+  if (!ks || !vs) return fail(MGI_EINVAL, "null stride array");
+  if (!valid_dtype(dtype)) return fail(MGI_EINVAL, "unknown dtype code");
+  if (!valid_itype(slot_itype)) return fail(MGI_EINVAL, "slot_mapping must be int32 or int64");
+  if (!nonneg(ks, 3) || !nonneg(vs, 3) || slot_stride < 0) return fail(MGI_EINVAL, "strides must be non-negative");
+  if (T >= (int64_t(1) << 24)) return fail(MGI_EUNSUPPORTED, "too many rows for one launch");
+  const int64_t eb = dtype_bytes(dtype), groups = mgi::fp4_groups(D);
+  if (2 * H * groups * 4 * 32 >= (int64_t(1) << 31)) return fail(MGI_EUNSUPPORTED, "rows too long for one launch");
+  a->pool = static_cast<unsigned char*>(const_cast<void*>(pool)) + layer_idx * ps[0];
+  a->p_sn = ps[1], a->p_sh = ps[2];
+  a->k = const_cast<void*>(k), a->v = const_cast<void*>(v);
+  a->k_st = ks[0], a->k_sh = ks[1], a->k_sd = ks[2];
+  a->v_st = vs[0], a->v_sh = vs[1], a->v_sd = vs[2];
+  a->slots = slots;
+  a->sl_s = slot_stride;
+  a->sl_i64 = slot_itype == MGI_I64;
+  a->T = (int)T, a->H = (int)H, a->D = (int)D, a->S = (int)S, a->groups = (int)groups;
+  a->N = N;
+  a->vec = D % 8 == 0 && ks[2] == 1 && vs[2] == 1 && aligned16(k) && aligned16(v) && mult16(ks[0], eb) &&
+           mult16(ks[1], eb) && mult16(vs[0], eb) && mult16(vs[1], eb);
+  magic_of(groups, &a->g_mul, &a->g_shift);
+  magic_of(2 * H * groups * 4, &a->o_mul, &a->o_shift);
+  return MGI_OK;
+}
+
 // Checks the two decode-step linear calls share.
 int check_linear(std::initializer_list<const void*> tensors, int dtype, int64_t B, int64_t N, int64_t K) {
   using namespace mgi;
@@ -1351,6 +1432,118 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
   const hipError_t e = dtype == MGI_F32    ? launch_paged_shared_f32(a, st)
                        : dtype == MGI_BF16 ? launch_paged_shared_bf16(a, st)
                                            : launch_paged_shared_f16(a, st);
+  if (e != hipSuccess) return fail(MGI_ELAUNCH, std::string("launch failed: ") + hipGetErrorString(e));
+  return MGI_OK;
+}
+
+size_t mgi_fp4_slab_bytes(int64_t S, int64_t D) {
+  return S <= 0 || D <= 0 || D > mgi::kFp4MaxDim || S > (int64_t(1) << 20) ? 0 : (size_t)mgi::fp4_slab_bytes(S, D);
+}
+
+int mgi_kv_append_fp4(void* pool, const int64_t* pool_strides, const void* k_new, const void* v_new,
+                      const int64_t* k_new_strides, const int64_t* v_new_strides, int new_dtype,
+                      const void* slot_mapping, int64_t slot_stride, int slot_itype, int64_t T, int64_t H, int64_t D,
+                      int64_t S, int64_t N, int64_t L, int64_t layer_idx, void* stream) {
+  g_err.clear();
+  if (T < 0) return fail(MGI_EINVAL, "row count must be non-negative");
+  if (T == 0) return MGI_OK;
+  mgi::Fp4RowArgs a{};
+  const int rc = fp4_row_args(pool, pool_strides, k_new, v_new, k_new_strides, v_new_strides, new_dtype, slot_mapping,
+                              slot_stride, slot_itype, T, H, D, S, N, L, layer_idx, &a);
+  if (rc != MGI_OK) return rc;
+  const hipError_t e = mgi::launch_fp4_append(a, new_dtype, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MGI_ELAUNCH, std::string("launch failed: ") + hipGetErrorString(e));
+  return MGI_OK;
+}
+
+int mgi_kv_gather_fp4(void* k_out, void* v_out, const int64_t* k_out_strides, const int64_t* v_out_strides,
+                      int out_dtype, const void* pool, const int64_t* pool_strides, const void* slot_mapping,
+                      int64_t slot_stride, int slot_itype, int64_t T, int64_t H, int64_t D, int64_t S, int64_t N,
+                      int64_t L, int64_t layer_idx, void* stream) {
+  g_err.clear();
+  if (T < 0) return fail(MGI_EINVAL, "row count must be non-negative");
+  if (T == 0) return MGI_OK;
+  mgi::Fp4RowArgs a{};
+  const int rc = fp4_row_args(pool, pool_strides, k_out, v_out, k_out_strides, v_out_strides, out_dtype, slot_mapping,
+                              slot_stride, slot_itype, T, H, D, S, N, L, layer_idx, &a);
+  if (rc != MGI_OK) return rc;
+  const hipError_t e = mgi::launch_fp4_gather(a, out_dtype, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MGI_ELAUNCH, std::string("launch failed: ") + hipGetErrorString(e));
+  return MGI_OK;
+}
+
+size_t mgi_paged_decode_fp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M) {
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk != 0 || D <= 0 || D > mgi::kFp4MaxDim || S <= 0 || M <= 0 ||
+      M >= (int64_t(1) << 30) / S || B > kMaxGridYZ || Hq > kMaxGridYZ)
+    return 0;
+  return fp4_plan(B, Hq, Hk, D, S, M).total;
+}
+
+int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides, int dtype,
+                         const void* pool, const int64_t* pool_strides, const void* block_tables,
+                         const int64_t* bt_strides, int bt_itype, const void* context_lens, int64_t cl_stride,
+                         int cl_itype, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t N, int64_t M,
+                         int64_t L, int64_t layer_idx, float scale, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  using namespace mgi;
+  g_err.clear();
+  if (!out || !q || !block_tables || !context_lens) return fail(MGI_EINVAL, "null tensor pointer");
+  if (!out_strides || !q_strides || !bt_strides) return fail(MGI_EINVAL, "null stride array");
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || D <= 0) return fail(MGI_EINVAL, "q dimensions must be nonzero");
+  if (Hq % Hk != 0) return fail(MGI_EINVAL, "query heads must be a multiple of the pool's heads");
+  const int rc = check_fp4_pool(pool, pool_strides, Hk, D, S, N, L, layer_idx);
+  if (rc != MGI_OK) return rc;
+  if (M < 1) return fail(MGI_EINVAL, "block_tables need at least one block column");
+  if (!valid_dtype(dtype)) return fail(MGI_EINVAL, "unknown dtype code");
+  if (!valid_itype(bt_itype) || !valid_itype(cl_itype)) return fail(MGI_EINVAL, "index arrays must be int32 or int64");
+  if (!std::isfinite(scale)) return fail(MGI_EINVAL, "scale must be finite");
+  if (!nonneg(out_strides, 3) || !nonneg(q_strides, 3) || !nonneg(bt_strides, 2) || cl_stride < 0)
+    return fail(MGI_EINVAL, "strides must be non-negative");
+  if (B > kMaxGridYZ || Hq > kMaxGridYZ) return fail(MGI_EUNSUPPORTED, "batch or heads larger than 65535");
+  if (B * Hq >= (int64_t(1) << 25)) return fail(MGI_EUNSUPPORTED, "rows x heads too large for one launch");
+  if (M >= (int64_t(1) << 30) / S) return fail(MGI_EUNSUPPORTED, "M*S must be < 2^30");
+  if (B * ((M * S + 31) / 32) >= (int64_t(1) << 30)) return fail(MGI_EUNSUPPORTED, "B*M*S must be < 2^35");
+  const int64_t eb = dtype_bytes(dtype);
+  const Fp4Plan p = fp4_plan(B, Hq, Hk, D, S, M);
+  Fp4DecodeArgs a{};
+  a.out = out;
+  a.o_sb = out_strides[0], a.o_sh = out_strides[1], a.o_sd = out_strides[2];
+  a.q = q;
+  a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_sd = q_strides[2];
+  a.pool = static_cast<const unsigned char*>(pool) + layer_idx * pool_strides[0];
+  a.p_sn = pool_strides[1], a.p_sh = pool_strides[2];
+  a.bt = block_tables;
+  a.bt_sb = bt_strides[0], a.bt_sm = bt_strides[1];
+  a.bt_i64 = bt_itype == MGI_I64;
+  a.cl = context_lens;
+  a.cl_s = cl_stride;
+  a.cl_i64 = cl_itype == MGI_I64;
+  a.B = (int)B, a.Hk = (int)Hk, a.G = (int)(Hq / Hk), a.D = (int)D, a.S = (int)S, a.M = (int)M;
+  a.N = N;
+  a.q_tiles = p.q_tiles;
+  a.scale_log2 = scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f;
+  a.q_flip = scale < 0.f ? 0x80000000u : 0u;
+  a.q_zero = scale == 0.f;
+  a.vec = D % 8 == 0 && q_strides[2] == 1 && out_strides[2] == 1 && aligned16(q) && aligned16(out) &&
+          mult16(q_strides[0], eb) && mult16(q_strides[1], eb) && mult16(out_strides[0], eb) &&
+          mult16(out_strides[1], eb);
+  magic_of(S, &a.s_mul, &a.s_shift);
+  a.one_launch = p.one_launch;
+  a.waves = p.waves;
+  while ((1 << a.waves_log2) < a.waves) ++a.waves_log2;
+  if (!p.one_launch) {
+    if (!workspace) return fail(MGI_EWORKSPACE, "workspace required for the split pass");
+    if (workspace_bytes < p.total)
+      return fail(MGI_EWORKSPACE, "workspace smaller than mgi_paged_decode_fp4_workspace_bytes()");
+    if (!aligned16(workspace)) return fail(MGI_EINVAL, "workspace must be 16-byte aligned");
+    a.ws_acc = static_cast<float*>(workspace);
+    a.ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.ml_offset);
+    a.ws_cum = reinterpret_cast<int*>(static_cast<char*>(workspace) + p.cum_offset);
+  }
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const hipError_t e = dtype == MGI_F32    ? launch_paged_fp4_f32(a, st)
+                       : dtype == MGI_BF16 ? launch_paged_fp4_bf16(a, st)
+                                           : launch_paged_fp4_f16(a, st);
   if (e != hipSuccess) return fail(MGI_ELAUNCH, std::string("launch failed: ") + hipGetErrorString(e));
   return MGI_OK;
 }

@@ -348,6 +348,100 @@ at::Tensor paged_decode_shared(const at::Tensor& q, const at::Tensor& kp, const 
   return out;
 }
 
+// Checks of a 4-bit pool: data [L, N, H, slab] bytes of blocks of S tokens and heads of D
+// dims.
+void check_fp4_pool(const at::Tensor& pool, int64_t S, int64_t D, int64_t layer_idx) {
+  if (!pool.is_cuda()) value_error("KV pool must be on a GPU device for the HIP backend");
+  if (S <= 0) value_error("block_size must be positive");
+  if (D <= 0 || D > 256) value_error("4-bit KV pool supports head_dim from 1 to 256");
+  if (pool.dim() != 4 || pool.scalar_type() != at::kByte || pool.size(3) != (int64_t)mgi_fp4_slab_bytes(S, D) ||
+      pool.stride(3) != 1)
+    value_error("4-bit KV data must be uint8 [L,P,H,slab] of the pool's block size and head dimension");
+  if (layer_idx < 0 || layer_idx >= pool.size(0)) value_error("layer_idx outside KV pool");
+}
+
+// kv_append_fp4(pool, block_size, head_dim, layer_idx, k, v, slot_mapping): rows k[t], v[t]
+// into the 4-bit pool's slots.
+void kv_append_fp4(const at::Tensor& pool, int64_t S, int64_t D, int64_t layer_idx, const at::Tensor& k,
+                   const at::Tensor& v, const at::Tensor& slots) {
+  check_fp4_pool(pool, S, D, layer_idx);
+  if (k.dim() != 3 || v.sizes() != k.sizes()) value_error("k and v must have matching shape [T,H,D]");
+  const int64_t T = k.size(0), H = pool.size(2);
+  if (k.size(1) != H || k.size(2) != D) value_error("k/v head dimensions do not match the KV pool");
+  const int nd = dtype_code(k.scalar_type());
+  if (nd < 0 || v.scalar_type() != k.scalar_type()) value_error("k and v must share a float dtype");
+  if (slots.dim() != 1 || slots.size(0) != T) value_error("slot_mapping must have shape [T]");
+  const int st = index_code(slots.scalar_type());
+  if (st < 0) value_error("slot_mapping must contain integer slots");
+  const auto dev = pool.device();
+  if (k.device() != dev || v.device() != dev || slots.device() != dev)
+    value_error("all inputs must reside on same GPU device");
+  check_plain({&pool, &k, &v, &slots});
+  if (T == 0) return;
+  const c10::DeviceGuard guard(dev);
+  check_status(mgi_kv_append_fp4(pool.data_ptr(), pool.strides().data(), k.data_ptr(), v.data_ptr(),
+                                 k.strides().data(), v.strides().data(), nd, slots.data_ptr(), slots.stride(0), st, T,
+                                 H, D, S, pool.size(1), pool.size(0), layer_idx, stream_of(pool)));
+}
+
+// kv_gather_fp4(pool, block_size, head_dim, layer_idx, slot_mapping, dtype) -> (k, v)
+// [T, H, D]: the values of the slots, 0 where a slot is outside the pool.
+py::tuple kv_gather_fp4(const at::Tensor& pool, int64_t S, int64_t D, int64_t layer_idx, const at::Tensor& slots,
+                        at::ScalarType dtype) {
+  check_fp4_pool(pool, S, D, layer_idx);
+  if (slots.dim() != 1) value_error("slot_mapping must have shape [T]");
+  const int st = index_code(slots.scalar_type());
+  if (st < 0) value_error("slot_mapping must contain integer slots");
+  const int od = dtype_code(dtype);
+  if (od < 0) value_error("dtype must be float32, bfloat16 or float16");
+  const auto dev = pool.device();
+  if (slots.device() != dev) value_error("all inputs must reside on same GPU device");
+  check_plain({&pool, &slots});
+  const c10::DeviceGuard guard(dev);
+  const int64_t T = slots.size(0), H = pool.size(2);
+  at::Tensor k = at::empty({T, H, D}, pool.options().dtype(dtype)), v = at::empty_like(k);
+  if (T != 0)
+    check_status(mgi_kv_gather_fp4(k.data_ptr(), v.data_ptr(), k.strides().data(), v.strides().data(), od,
+                                   pool.data_ptr(), pool.strides().data(), slots.data_ptr(), slots.stride(0), st, T, H,
+                                   D, S, pool.size(1), pool.size(0), layer_idx, stream_of(pool)));
+  return py::make_tuple(k, v);
+}
+
+// paged_decode_fp4(q, pool, block_size, head_dim, block_tables, context_lengths,
+// layer_idx) -> [B, Hq, D] of q's dtype: decode attention over the 4-bit pool.
+at::Tensor paged_decode_fp4(const at::Tensor& q, const at::Tensor& pool, int64_t S, int64_t D, const at::Tensor& bt,
+                            const at::Tensor& cl, int64_t layer_idx) {
+  if (!q.is_cuda()) value_error("q must be on a GPU device for the HIP backend");
+  if (q.dim() != 3) value_error("q must have shape [B,H,D]");
+  const int64_t b = q.size(0), h = q.size(1), d = q.size(2);
+  if (b == 0 || h == 0 || d == 0) value_error("q dimensions must be nonzero");
+  const int qd = dtype_code(q.scalar_type());
+  if (qd < 0) value_error("q must be float32, bfloat16 or float16");
+  check_fp4_pool(pool, S, D, layer_idx);
+  const int64_t hk = pool.size(2);
+  if (hk <= 0 || h % hk != 0 || D != d) value_error("q heads must be a multiple of the KV pool's, of its head dimension");
+  if (bt.dim() != 2 || bt.size(0) != b) value_error("block_tables must have shape [B,M]");
+  if (cl.dim() != 1 || cl.size(0) != b) value_error("context_lengths must have shape [B]");
+  if (index_code(bt.scalar_type()) < 0) value_error("block_tables must contain integer indices");
+  if (index_code(cl.scalar_type()) < 0) value_error("context_lengths must be integer");
+  const auto dev = q.device();
+  if (pool.device() != dev || bt.device() != dev || cl.device() != dev)
+    value_error("all inputs must reside on same GPU device");
+  const int64_t M = bt.size(1);
+  if (M < 1) value_error("block_tables need at least one block column");
+  check_plain({&q, &pool, &bt, &cl});
+  const c10::DeviceGuard guard(dev);
+  at::Tensor out = at::empty({b, h, d}, q.options()), ws;
+  const size_t ws_bytes = mgi_paged_decode_fp4_workspace_bytes(b, h, hk, d, S, M);
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte));
+  check_status(mgi_paged_decode_fp4(
+      out.data_ptr(), out.strides().data(), q.data_ptr(), q.strides().data(), qd, pool.data_ptr(),
+      pool.strides().data(), bt.data_ptr(), bt.strides().data(), index_code(bt.scalar_type()), cl.data_ptr(),
+      cl.stride(0), index_code(cl.scalar_type()), b, h, hk, d, S, pool.size(1), M, pool.size(0), layer_idx,
+      (float)(1.0 / std::sqrt((double)d)), ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q)));
+  return out;
+}
+
 // Whether t is a plain contiguous, 16-byte aligned tensor of x's dtype and
 // (current) device with `numel` elements: what the decode-step linear kernels
 // take.
@@ -418,7 +512,8 @@ py::object decode_linear_norm(const c10::optional<at::Tensor>& x, const c10::opt
 
 PYBIND11_MODULE(_hip_ops, m) {
   m.doc() = "PyTorch binding of libminivllm_hip.so (kv_append, kv_append_rope, qk_norm_rope, paged_decode, "
-            "paged_decode_append, paged_decode_shared, paged_prefill, decode_linear, decode_linear_norm)";
+            "paged_decode_append, paged_decode_shared, paged_prefill, decode_linear, decode_linear_norm, "
+            "kv_append_fp4, kv_gather_fp4, paged_decode_fp4)";
   m.def("kv_append", &kv_append);
   m.def("paged_decode", &paged_decode);
   m.def("paged_decode_append", &paged_decode_append);
@@ -426,6 +521,12 @@ PYBIND11_MODULE(_hip_ops, m) {
   m.def("paged_decode_shared", &paged_decode_shared);
   m.def("qk_norm_rope", &qk_norm_rope);
   m.def("kv_append_rope", &kv_append_rope);
+  m.def("kv_append_fp4", &kv_append_fp4);
+  m.def("kv_gather_fp4", [](const at::Tensor& pool, int64_t S, int64_t D, int64_t layer_idx, const at::Tensor& slots,
+                            const py::object& dtype) {
+    return kv_gather_fp4(pool, S, D, layer_idx, slots, torch::python::detail::py_object_to_dtype(dtype));
+  });
+  m.def("paged_decode_fp4", &paged_decode_fp4);
   m.def("decode_linear", &decode_linear);
   m.def("decode_linear_norm", &decode_linear_norm);
 }

@@ -380,6 +380,120 @@ def paged_decode_shared(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, bt:
     return out
 
 
+def _check_fp4_pool(pool: torch.Tensor, S: int, D: int, layer_idx: int) -> None:
+    if not pool.is_cuda:
+        raise ValueError("KV pool must be on a GPU device for the HIP backend")
+    if S <= 0:
+        raise ValueError("block_size must be positive")
+    if not 1 <= D <= 256:
+        raise ValueError("4-bit KV pool supports head_dim from 1 to 256")
+    if pool.ndim != 4 or pool.dtype != torch.uint8 or pool.shape[3] != _native.lib().mgi_fp4_slab_bytes(S, D) \
+            or pool.stride(3) != 1:
+        raise ValueError("4-bit KV data must be uint8 [L,P,H,slab] of the pool's block size and head dimension")
+    if not 0 <= layer_idx < pool.shape[0]:
+        raise ValueError("layer_idx outside KV pool")
+
+
+def kv_append_fp4(pool: torch.Tensor, S: int, D: int, layer_idx: int, k: torch.Tensor, v: torch.Tensor,
+                  slots: torch.Tensor) -> None:
+    """Rows k[t], v[t] into the 4-bit pool's slots slots[t]."""
+    _check_fp4_pool(pool, S, D, layer_idx)
+    if k.ndim != 3 or v.shape != k.shape:
+        raise ValueError("k and v must have matching shape [T,H,D]")
+    L, N, H = pool.shape[:3]
+    T = k.shape[0]
+    if k.shape[1] != H or k.shape[2] != D:
+        raise ValueError("k/v head dimensions do not match the KV pool")
+    if k.dtype not in _FLOATS or v.dtype != k.dtype:
+        raise ValueError("k and v must share a float dtype")
+    if slots.ndim != 1 or slots.shape[0] != T:
+        raise ValueError("slot_mapping must have shape [T]")
+    if slots.dtype not in _INDEX:
+        raise ValueError("slot_mapping must contain integer slots")
+    if any(x.device != pool.device for x in (k, v, slots)):
+        raise ValueError("all inputs must reside on same GPU device")
+    _check_plain(pool, k, v, slots)
+    if T == 0:
+        return
+    with torch.cuda.device(pool.device):
+        _native.check(_native.lib().mgi_kv_append_fp4(
+            pool.data_ptr(), _native.strides(pool), k.data_ptr(), v.data_ptr(), _native.strides(k),
+            _native.strides(v), _native.DTYPE_CODES[k.dtype],
+            slots.data_ptr(), slots.stride(0), _native.ITYPE_CODES[slots.dtype],
+            T, H, D, S, N, L, int(layer_idx), _native.stream_handle(pool.device)))
+
+
+def kv_gather_fp4(pool: torch.Tensor, S: int, D: int, layer_idx: int, slots: torch.Tensor,
+                  dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [T, H, D]: the values of the 4-bit pool's slots."""
+    _check_fp4_pool(pool, S, D, layer_idx)
+    if slots.ndim != 1:
+        raise ValueError("slot_mapping must have shape [T]")
+    if slots.dtype not in _INDEX:
+        raise ValueError("slot_mapping must contain integer slots")
+    if dtype not in _FLOATS:
+        raise ValueError("dtype must be float32, bfloat16 or float16")
+    if slots.device != pool.device:
+        raise ValueError("all inputs must reside on same GPU device")
+    _check_plain(pool, slots)
+    L, N, H = pool.shape[:3]
+    T = slots.shape[0]
+    with torch.cuda.device(pool.device):
+        k = torch.empty((T, H, D), dtype=dtype, device=pool.device)
+        v = torch.empty_like(k)
+        if T:
+            _native.check(_native.lib().mgi_kv_gather_fp4(
+                k.data_ptr(), v.data_ptr(), _native.strides(k), _native.strides(v), _native.DTYPE_CODES[dtype],
+                pool.data_ptr(), _native.strides(pool),
+                slots.data_ptr(), slots.stride(0), _native.ITYPE_CODES[slots.dtype],
+                T, H, D, S, N, L, int(layer_idx), _native.stream_handle(pool.device)))
+    return k, v
+
+
+def paged_decode_fp4(q: torch.Tensor, pool: torch.Tensor, S: int, D: int, bt: torch.Tensor, cl: torch.Tensor,
+                     layer_idx: int) -> torch.Tensor:
+    """[B, Hq, D] decode attention over the 4-bit pool."""
+    if not q.is_cuda:
+        raise ValueError("q must be on a GPU device for the HIP backend")
+    if q.ndim != 3:
+        raise ValueError("q must have shape [B,H,D]")
+    b, h, d = q.shape
+    if b == 0 or h == 0 or d == 0:
+        raise ValueError("q dimensions must be nonzero")
+    if q.dtype not in _FLOATS:
+        raise ValueError("q must be float32, bfloat16 or float16")
+    _check_fp4_pool(pool, S, D, layer_idx)
+    L, N, hk = pool.shape[:3]
+    if hk <= 0 or h % hk != 0 or D != d:
+        raise ValueError("q heads must be a multiple of the KV pool's, of its head dimension")
+    if bt.ndim != 2 or bt.shape[0] != b:
+        raise ValueError("block_tables must have shape [B,M]")
+    if cl.ndim != 1 or cl.shape[0] != b:
+        raise ValueError("context_lengths must have shape [B]")
+    if bt.dtype not in _INDEX:
+        raise ValueError("block_tables must contain integer indices")
+    if cl.dtype not in _INDEX:
+        raise ValueError("context_lengths must be integer")
+    if any(x.device != q.device for x in (pool, bt, cl)):
+        raise ValueError("all inputs must reside on same GPU device")
+    M = bt.shape[1]
+    if M < 1:
+        raise ValueError("block_tables need at least one block column")
+    _check_plain(q, pool, bt, cl)
+    lib = _native.lib()
+    with torch.cuda.device(q.device):
+        out = torch.empty((b, h, d), dtype=q.dtype, device=q.device)
+        ws_bytes = int(lib.mgi_paged_decode_fp4_workspace_bytes(b, h, hk, d, S, M))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        _native.check(lib.mgi_paged_decode_fp4(
+            out.data_ptr(), _native.strides(out), q.data_ptr(), _native.strides(q), _native.DTYPE_CODES[q.dtype],
+            pool.data_ptr(), _native.strides(pool), bt.data_ptr(), _native.strides(bt), _native.ITYPE_CODES[bt.dtype],
+            cl.data_ptr(), cl.stride(0), _native.ITYPE_CODES[cl.dtype],
+            b, h, hk, d, S, N, M, L, int(layer_idx), 1.0 / math.sqrt(d), _ptr(ws), ws_bytes,
+            _native.stream_handle(q.device)))
+    return out
+
+
 def _linear_ok(t: torch.Tensor | None, x: torch.Tensor, numel: int) -> bool:
     """Whether t (or no tensor) is plain, contiguous and 16-byte aligned, of x's
     dtype and (current) device, with numel elements."""

@@ -49,6 +49,11 @@ EXPORTED_SYMBOLS = (
     "mgi_kv_append_rope",
     "mgi_paged_decode_shared",
     "mgi_paged_decode_shared_workspace_bytes",
+    "mgi_fp4_slab_bytes",
+    "mgi_kv_append_fp4",
+    "mgi_kv_gather_fp4",
+    "mgi_paged_decode_fp4",
+    "mgi_paged_decode_fp4_workspace_bytes",
 )
 
 _lock = threading.Lock()
@@ -179,6 +184,31 @@ def _declare(lib: ctypes.CDLL) -> None:
     ]
     lib.mgi_paged_decode_shared_workspace_bytes.restype = ctypes.c_size_t
     lib.mgi_paged_decode_shared_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i]
+    lib.mgi_fp4_slab_bytes.restype = ctypes.c_size_t
+    lib.mgi_fp4_slab_bytes.argtypes = [_i64, _i64]
+    rows = [
+        _p, _i64, _i,                      # slot mapping, stride, itype
+        _i64, _i64, _i64, _i64, _i64, _i64, _i64,  # T H D S N L layer
+        _p,                                # stream
+    ]
+    lib.mgi_kv_append_fp4.restype = _i
+    lib.mgi_kv_append_fp4.argtypes = [_p, _pi64, _p, _p, _pi64, _pi64, _i, *rows]  # pool, new k/v
+    lib.mgi_kv_gather_fp4.restype = _i
+    lib.mgi_kv_gather_fp4.argtypes = [_p, _p, _pi64, _pi64, _i, _p, _pi64, *rows]  # k/v out, pool
+    lib.mgi_paged_decode_fp4.restype = _i
+    lib.mgi_paged_decode_fp4.argtypes = [
+        _p, _pi64,                         # out, strides
+        _p, _pi64, _i,                     # q, strides, dtype
+        _p, _pi64,                         # pool, strides (bytes)
+        _p, _pi64, _i,                     # block tables, strides, itype
+        _p, _i64, _i,                      # context lengths, stride, itype
+        _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,  # B Hq Hk D S N M L layer
+        ctypes.c_float,                    # scale
+        _p, ctypes.c_size_t,               # workspace, bytes
+        _p,                                # stream
+    ]
+    lib.mgi_paged_decode_fp4_workspace_bytes.restype = ctypes.c_size_t
+    lib.mgi_paged_decode_fp4_workspace_bytes.argtypes = [_i64] * 6
 
 
 def lib() -> ctypes.CDLL:
@@ -209,7 +239,8 @@ def lib() -> ctypes.CDLL:
 def ops():
     """The eager path's binding: kv_append, paged_decode, paged_decode_append,
     paged_prefill, decode_linear, decode_linear_norm, qk_norm_rope,
-    kv_append_rope and paged_decode_shared on tensors, validated,
+    kv_append_rope, paged_decode_shared, kv_append_fp4, kv_gather_fp4 and
+    paged_decode_fp4 on tensors, validated,
     calling the C ABI on the current stream.
 
     Normally the PyTorch extension _hip_ops (csrc/torch_ops.cpp). When the

@@ -30,7 +30,9 @@ the sequence's cached prefix and the chunk itself, read from the pool.
 qk_norm_rope_hip and kv_append_rope_hip norm and rotate query and key heads by
 their positions, the latter on the way into the pool.
 paged_attention_shared_prefix_hip is decode attention, with grouped query
-heads, for sequences that begin with the same cached blocks. These three are
+heads, for sequences that begin with the same cached blocks. kv_append_fp4,
+kv_gather_fp4 and paged_attention_fp4_hip write, read back and attend over a
+FP4KVBlockPool, whose keys and values are 4 bits. These six are
 inference-only (RuntimeError for tensors that require gradients while grad mode
 is on) and run on their tensors' device, current or not.
 """
@@ -39,7 +41,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .kv_block_pool import KVBlockPool
+from .kv_block_pool import FP4KVBlockPool, KVBlockPool
 
 
 def paged_attention_batch_hip(q: torch.Tensor, pool: KVBlockPool, block_tables: torch.Tensor,
@@ -157,6 +159,37 @@ def kv_append_rope_hip(pool: KVBlockPool, layer_idx: int, q: torch.Tensor, k: to
     """
     return _native.ops().kv_append_rope(pool.k, pool.v, int(layer_idx), q, k, v, slot_mapping, positions, cos_sin,
                                         q_weight, k_weight, float(eps), bool(interleaved))
+
+
+def kv_append_fp4(pool: FP4KVBlockPool, layer_idx: int, k: torch.Tensor, v: torch.Tensor,
+                  slot_mapping: torch.Tensor) -> None:
+    """kv_append into a 4-bit pool: rows k[t], v[t] ([T, H, D], any strides; float32,
+    bfloat16 or float16) are quantised (FP4KVBlockPool says how) on their way to slots
+    slot_mapping[t]. Rows with a slot outside the pool are skipped; of rows on one slot
+    the last is kept.
+    """
+    _native.ops().kv_append_fp4(pool.data, pool.block_size, pool.head_dim, int(layer_idx), k, v, slot_mapping)
+
+
+def kv_gather_fp4(pool: FP4KVBlockPool, layer_idx: int, slot_mapping: torch.Tensor, *,
+                  dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values slots slot_mapping[t] of a 4-bit pool hold: fresh (k, v), [T, H, D] of
+    ``dtype`` (float32 and bfloat16 exactly; float16 as far as it reaches). Rows whose
+    slot is outside the pool are 0.
+    """
+    return _native.ops().kv_gather_fp4(pool.data, pool.block_size, pool.head_dim, int(layer_idx), slot_mapping, dtype)
+
+
+def paged_attention_fp4_hip(q: torch.Tensor, pool: FP4KVBlockPool, block_tables: torch.Tensor,
+                            context_lengths: torch.Tensor, layer_idx: int) -> torch.Tensor:
+    """paged_attention_batch_hip over the values a 4-bit pool holds, with grouped query
+    heads: q is [B, Hq, D] with Hq a multiple of the pool's heads H, and query head h reads
+    KV head h // (Hq // H). float32, bfloat16 or float16 queries; head_dim up to 256; any
+    block size (16-token runs of a block are read fastest: a multiple of 16). Sums are
+    float32 and the result is rounded once. Returns a fresh [B, Hq, D] tensor of q.dtype.
+    """
+    return _native.ops().paged_decode_fp4(q, pool.data, pool.block_size, pool.head_dim, block_tables,
+                                          context_lengths, int(layer_idx))
 
 
 def paged_prefill_hip(q: torch.Tensor, pool: KVBlockPool, block_table: torch.Tensor,
