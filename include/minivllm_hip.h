@@ -518,6 +518,30 @@ int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, /* [3] */
  * none). */
 size_t mgi_paged_decode_fp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M);
 
+/*
+ * Causal attention of whole prompts, packed one after the other, over their own keys and
+ * values as a projection makes them (no pool). No counterpart in the reference, which
+ * prefills one sequence at a time through its pool (minivllm/attention.py:190-299).
+ * q and out [T, Hq, D], k and v [T, Hk, D], any strides, one dtype; Hq a multiple of Hk,
+ * query head h uses KV head h / (Hq / Hk). seq_starts [B + 1], int32 or int64, never
+ * falling: sequence b is rows seq_starts[b] .. seq_starts[b + 1] - 1 (clamped to [0, T]).
+ *   out[i,h] = sum_{j <= i, j in i's sequence} softmax_j(scale * q[i,h] . k[j]) * v[j]
+ * A sequence may be empty. Rows of no sequence (before the first start, behind the last)
+ * are left as they were, or become 0 with zero_rest. A row's result depends on the rows
+ * it sees alone, whatever the others hold (infinities and NaN too). Sums are f32; 2-byte
+ * types round the softmax weights to their type for the second product, as
+ * mgi_paged_prefill; f32 products are f32. Same inputs, same bits. No workspace.
+ * D <= 256, T and B < 2^28, (T / 32 + B + 1) * Hq < 2^31.
+ */
+int mgi_prompt_attention(void* out, const int64_t* out_strides, /* [3] */
+                         const void* q, const int64_t* q_strides, /* [3] */
+                         const void* k, const int64_t* k_strides, /* [3] */
+                         const void* v, const int64_t* v_strides, /* [3] */
+                         int dtype,
+                         const void* seq_starts, int64_t starts_stride, int starts_itype,
+                         int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D,
+                         float scale, int zero_rest, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

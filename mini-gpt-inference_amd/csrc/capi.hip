@@ -13,6 +13,7 @@
 
 #include "fp4_kv.h"
 #include "mgi_internal.h"
+#include "prompt_args.h"
 #include "minivllm_hip.h"
 
 namespace {
@@ -1432,6 +1433,58 @@ int mgi_paged_decode_shared(void* out, const int64_t* out_strides, const void* q
   const hipError_t e = dtype == MGI_F32    ? launch_paged_shared_f32(a, st)
                        : dtype == MGI_BF16 ? launch_paged_shared_bf16(a, st)
                                            : launch_paged_shared_f16(a, st);
+  if (e != hipSuccess) return fail(MGI_ELAUNCH, std::string("launch failed: ") + hipGetErrorString(e));
+  return MGI_OK;
+}
+
+int mgi_prompt_attention(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides, const void* k,
+                         const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
+                         const void* seq_starts, int64_t starts_stride, int starts_itype, int64_t B, int64_t T,
+                         int64_t Hq, int64_t Hk, int64_t D, float scale, int zero_rest, void* stream) {
+  using namespace mgi;
+  g_err.clear();
+  if (T < 0 || B < 0) return fail(MGI_EINVAL, "row and sequence counts must be non-negative");
+  if (T == 0) return MGI_OK;
+  if (!out || !q || !k || !v || !seq_starts) return fail(MGI_EINVAL, "null tensor pointer");
+  if (!out_strides || !q_strides || !k_strides || !v_strides) return fail(MGI_EINVAL, "null stride array");
+  if (Hq <= 0 || Hk <= 0 || D <= 0) return fail(MGI_EINVAL, "q and k dimensions must be nonzero");
+  if (Hq % Hk != 0) return fail(MGI_EINVAL, "query heads must be a multiple of the KV heads");
+  if (!valid_dtype(dtype)) return fail(MGI_EINVAL, "unknown dtype code");
+  if (!valid_itype(starts_itype)) return fail(MGI_EINVAL, "index arrays must be int32 or int64");
+  if (!std::isfinite(scale)) return fail(MGI_EINVAL, "scale must be finite");
+  if (!nonneg(out_strides, 3) || !nonneg(q_strides, 3) || !nonneg(k_strides, 3) || !nonneg(v_strides, 3) ||
+      starts_stride < 0)
+    return fail(MGI_EINVAL, "strides must be non-negative");
+  if (D > kPromptMaxDim) return fail(MGI_EUNSUPPORTED, "head_dim larger than 256");
+  if (T >= (int64_t(1) << 28) || B >= (int64_t(1) << 28) || Hq > kMaxGridYZ ||
+      (T / 32 + std::min(B, T) + 1) * Hq >= (int64_t(1) << 31))
+    return fail(MGI_EUNSUPPORTED, "rows x heads too large for one launch");
+  const int64_t eb = dtype_bytes(dtype);
+  PromptArgs a{};
+  a.out = out;
+  a.o_st = out_strides[0], a.o_sh = out_strides[1], a.o_sd = out_strides[2];
+  a.q = q, a.k = k, a.v = v;
+  a.q_st = q_strides[0], a.q_sh = q_strides[1], a.q_sd = q_strides[2];
+  a.k_st = k_strides[0], a.k_sh = k_strides[1], a.k_sd = k_strides[2];
+  a.v_st = v_strides[0], a.v_sh = v_strides[1], a.v_sd = v_strides[2];
+  a.starts = seq_starts;
+  a.cu_s = starts_stride;
+  a.cu_i64 = starts_itype == MGI_I64;
+  a.B = (int)B, a.T = (int)T, a.Hq = (int)Hq, a.G = (int)(Hq / Hk), a.D = (int)D;
+  a.heads = a.G % 4 == 0 ? 4 : a.G % 2 == 0 ? 2 : 1;
+  a.zero_rest = zero_rest != 0;
+  a.scale_log2 = scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f;
+  a.q_flip = scale < 0.f ? (dtype == MGI_F32 ? 0x80000000u : 0x80008000u) : 0u;
+  a.q_zero = scale == 0.f;
+  a.vec = D % (16 / eb) == 0 && q_strides[2] == 1 && k_strides[2] == 1 && v_strides[2] == 1 && out_strides[2] == 1 &&
+          aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && mult16(q_strides[0], eb) &&
+          mult16(q_strides[1], eb) && mult16(k_strides[0], eb) && mult16(k_strides[1], eb) && mult16(v_strides[0], eb) &&
+          mult16(v_strides[1], eb) && mult16(out_strides[0], eb) && mult16(out_strides[1], eb) &&
+          std::max(k_strides[0], v_strides[0]) * eb < (int64_t(1) << 24);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const hipError_t e = dtype == MGI_F32    ? launch_prompt_f32(a, st)
+                       : dtype == MGI_BF16 ? launch_prompt_bf16(a, st)
+                                           : launch_prompt_f16(a, st);
   if (e != hipSuccess) return fail(MGI_ELAUNCH, std::string("launch failed: ") + hipGetErrorString(e));
   return MGI_OK;
 }

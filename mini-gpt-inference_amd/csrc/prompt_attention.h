@@ -1,0 +1,591 @@
+// prompt_attention.h -- causal attention of whole prompts, packed one after the other, on
+// the matrix cores of gfx950. Keys and values are the projection's own rows (no pool);
+// query heads may share KV heads.
+//
+//   out[i,h] = sum_{j <= i} softmax_j(scale * q[i,h] . k[j, h / G]) v[j, h / G]
+// over the rows j of i's sequence. 4 D flops per (query head, visible pair of rows), and
+// each K and V row is used by every later row: bound by the matrix cores and by the
+// exponentials beside them (per score 2 D / 512 matrix cycles of a SIMD, 16 for the
+// exponential, about 10 for the rest), from a few hundred tokens on.
+//
+// A workgroup is four wavefronts of 32 query rows each: the same 32 positions of four heads
+// that share a KV head, 64 positions of two, or 128 of one. Keys and values stream
+// through LDS in tiles, two in flight, copied there straight from memory. Each wavefront
+// computes S^T = K Q^T and O^T += V^T P^T with 32x32 MFMAs, so a lane's column is one
+// query row: its running maximum and sum are the lane's own (two lanes share a row), and
+// S^T's rows (keys 8 (r / 4) + 4 (lane / 32) + r % 4) are the order in which P^T enters the
+// second product when V^T's keys are read in the same order.
+//
+// Work order: the work of a tile of positions grows with its index in its sequence, so
+// workgroups take all sequences' tiles in falling index, which every workgroup finds from
+// the sequence starts by itself: nothing is read on the host, and no launch precedes it.
+//
+// Numerics: f32 sums and softmax (log2 domain). 2-byte types round the weights to their
+// type for the second product, half a step each (bf16 2^-9 of a weight, whose errors
+// are independent), and the sum that divides is that of the rounded weights; f16 weights are scaled by 2^13, so that
+// far keys keep theirs. f32 multiplies in f32.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "lds_tiles.h"
+#include "mgi_common.h"
+#include "minivllm_hip.h"
+#include "prompt_args.h"
+
+namespace mgi {
+
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+template <typename T> struct PM;  // the products of a type
+template <> struct PM<bf16_t> {
+  typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  static constexpr float slack = 8.f, bias = 0.f;  // log2: a score may pass the maximum by slack; weights are 2^bias too large
+  static constexpr uint32_t inf = 0x7f80u;  // bits
+  __device__ static __forceinline__ f32x16_t mfma(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ uint32_t pack2(float lo, float hi) {
+    const f32x2_t x = {lo, hi};  // converted as a vector: one instruction (three, element by element)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, v2));
+  }
+  __device__ static __forceinline__ float sum2(uint32_t w, float acc) {
+    const v2 one = {(__bf16)1.f, (__bf16)1.f};
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w), one, acc, false);
+  }
+};
+template <> struct PM<f16_t> {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  static constexpr float slack = 2.f, bias = 13.f;
+  static constexpr uint32_t inf = 0x7c00u;
+  __device__ static __forceinline__ f32x16_t mfma(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ uint32_t pack2(float lo, float hi) {
+    const v2 v = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  __device__ static __forceinline__ float sum2(uint32_t w, float acc) {
+    const v2 one = {(_Float16)1.f, (_Float16)1.f};
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, w), one, acc, false);
+  }
+};
+template <> struct PM<float> {
+  static constexpr float slack = 8.f, bias = 0.f;
+};
+
+template <typename T> struct PElem {
+  __device__ static __forceinline__ uint32_t bits(const T* p) { return p->bits; }
+};
+template <> struct PElem<float> {
+  __device__ static __forceinline__ uint32_t bits(const float* p) { return __float_as_uint(*p); }
+};
+
+__device__ __forceinline__ int wave_sum_int(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_max_int(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d, 64));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The next N instructions of the kinds in MASK, in the order of issue.
+template <int MASK, int N>
+__device__ __forceinline__ void sched() {
+  if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(MASK, N, 0);
+}
+
+struct Span {
+  int start, rows;
+};
+__device__ __forceinline__ Span span_of(const PromptArgs& a, int b) {
+  const int64_t s = load_index(a.starts, a.cu_i64, (int64_t)b * a.cu_s);
+  const int64_t e = load_index(a.starts, a.cu_i64, (int64_t)(b + 1) * a.cu_s);
+  const int64_t lo = s < 0 ? 0 : s > a.T ? a.T : s, hi = e < lo ? lo : e > a.T ? a.T : e;
+  return Span{(int)lo, (int)(hi - lo)};
+}
+
+// Tiles (of `rows` positions) of lane's sequence b0 + lane.
+__device__ __forceinline__ int tiles_of(const PromptArgs& a, int b, int rows) {
+  return b < a.B ? (span_of(a, b).rows + rows - 1) / rows : 0;
+}
+
+// The `rank`-th tile in falling order of its index in its sequence: (sequence, index),
+// or sequence -1 past the last.
+struct PromptTile {
+  int b, index;
+};
+__device__ __forceinline__ PromptTile tile_at(const PromptArgs& a, int rank, int rows) {
+  const int lane = (int)(threadIdx.x & 63);
+  const int first = tiles_of(a, lane, rows);  // of the first 64 sequences, kept
+  const auto each = [&](auto f) {
+    f(first, 0);
+    for (int b0 = 64; b0 < a.B; b0 += 64) f(tiles_of(a, b0 + lane, rows), b0);
+  };
+  int most = 0;
+  each([&](int n, int) { most = max(most, n); });
+  most = wave_max_int(most);
+  const auto from = [&](int index) {  // tiles with this index or a higher one
+    int sum = 0;
+    each([&](int n, int) { sum += max(0, n - index); });
+    return wave_sum_int(sum);
+  };
+  if (rank >= from(0)) return PromptTile{-1, 0};
+  int lo = 0, hi = most;  // from(lo) > rank >= from(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (from(mid) > rank) lo = mid; else hi = mid;
+  }
+  int left = rank - from(lo + 1), b = -1;
+  each([&](int n, int b0) {
+    if (b >= 0) return;
+    const uint64_t has = __ballot(n > lo);
+    const int count = __popcll(has);
+    if (left < count) {
+      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+      b = b0 + __ffsll((unsigned long long)__ballot(n > lo && before == left)) - 1;
+    } else {
+      left -= count;
+    }
+  });
+  return PromptTile{b, lo};
+}
+
+// DP: head dim, padded to a multiple of 16 (D <= DP). VEC: rows are copied in 16-byte pieces.
+template <typename T, int DP, bool VEC>
+struct Prompt {
+  static constexpr int EB = (int)sizeof(T);
+  static constexpr bool F32 = EB == 4;
+  static constexpr int NDB = (DP + 31) / 32;        // 32-wide blocks of O^T's dims
+  static constexpr int ROWB = NDB * 32 * EB;        // bytes of a row in LDS
+  static constexpr int CPR = ROWB / 16;             // 16-byte chunks of a row
+  static constexpr int EPC = 16 / EB;               // elements of a chunk
+  static constexpr int KT = F32 ? 32 : 64;          // keys of a tile
+  static constexpr int TILEB = KT * ROWB;
+  static constexpr int COPIES = TILEB / 4096;       // 16-byte copies per lane, tile and tensor
+  static_assert(COPIES * 4096 == TILEB, "the workgroup copies whole tiles");
+  static constexpr int NF = DP / (2 * EPC);         // steps of the first product: two chunks each
+  static constexpr int NKB = KT / 32;
+  static constexpr int RESIDENT = 4 * TILEB > 80 * 1024 ? 1 : 2;  // workgroups of a CU, by their LDS
+  static constexpr int PREGS = F32 ? 16 : 8;        // registers of a 32-key block's weights
+  using M = PM<T>;
+
+  // A chunk's place in its row: spread over the banks that rows would share. K reads take
+  // one chunk of 32 rows; V reads 8 (f32: 2) neighbouring rows' chunks of one block of dims.
+  __device__ static __forceinline__ int k_place(int row, int c) {
+    constexpr int bits = CPR % 16 == 0 ? 15 : CPR % 8 == 0 ? 7 : 3;
+    return c ^ (row & bits);
+  }
+  __device__ static __forceinline__ int v_place(int row, int c) {
+    if constexpr (F32) return c;
+    else return CPR % 16 == 0 ? c ^ (4 * (row & 3)) : CPR % 8 == 0 ? c ^ (4 * ((row >> 1) & 1)) : c;
+  }
+
+  // A word of V (f32, or two halves) with 0 for what is not a number or infinite.
+  __device__ static __forceinline__ uint32_t finite(uint32_t w) {
+    if constexpr (F32) {
+      return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+    } else {
+      if ((w & 0x7fffu) >= M::inf) w &= 0xffff0000u;
+      return ((w >> 16) & 0x7fffu) >= M::inf ? w & 0xffffu : w;
+    }
+  }
+
+  // One tile (keys key0 .. of this sequence) of K or V into LDS at `dst`, by all four wavefronts.
+  template <bool KEYS>
+  __device__ static __forceinline__ void copy(const PromptArgs& a, const T* head, int64_t st, int64_t sd, int key0, int n,
+                                              uint32_t dst, unsigned char* lds) {
+    // Chunks past D: of K zeros, which queries padded with zeros need; of V anything, for
+    // the dims past D are not written.
+    const bool whole = key0 + KT <= n && (!KEYS || a.D == DP);
+    const char* base = (const char*)(head + (int64_t)key0 * st);
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int at = i * 256 + (int)threadIdx.x, row = at / CPR, place = at % CPR;
+        const int c = KEYS ? k_place(row, place) : v_place(row, place);  // its own inverse
+        const uint32_t off = (uint32_t)row * (uint32_t)(st * EB) + (c * EPC < a.D ? (uint32_t)c * 16 : 0u);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(dst + (uint32_t)(i * 256 + ((int)threadIdx.x & ~63)) * 16);
+        if (whole) {
+          copy16_to_lds(base, off, to);
+        } else {
+          const bool in = key0 + row < n && c * EPC < a.D;
+          copy16_to_lds(in ? base + off : (const char*)kZeroRow, to);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < COPIES; ++i) {
+        const int at = i * 256 + (int)threadIdx.x, row = at / CPR, place = at % CPR;
+        const int c = KEYS ? k_place(row, place) : v_place(row, place);
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (key0 + row < n) {
+          const T* p = (const T*)base + (int64_t)row * st;
+#pragma unroll
+          for (int e = 0; e < EPC; ++e)
+            if (c * EPC + e < a.D) w[e * EB / 4] |= PElem<T>::bits(p + (c * EPC + e) * sd) << (8 * (e * EB % 4));
+        }
+        *(uint4*)(lds + at * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+};
+
+template <typename T, int DP, bool VEC>
+__global__ void __launch_bounds__(256, (Prompt<T, DP, VEC>::RESIDENT))
+prompt_attention_kernel(const PromptArgs a) {
+  using P = Prompt<T, DP, VEC>;
+  using M = PM<T>;
+  constexpr int NDB = P::NDB, NF = P::NF, NKB = P::NKB, KT = P::KT, ROWB = P::ROWB, TILEB = P::TILEB;
+  __shared__ __align__(1024) unsigned char k_lds[2][TILEB];
+  __shared__ __align__(1024) unsigned char v_lds[2][TILEB];
+
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, kg = lane >> 5;
+
+  // Rows of no sequence: before the first start, behind the last.
+  if (a.zero_rest) {
+    const int64_t s0 = load_index(a.starts, a.cu_i64, 0), s1 = load_index(a.starts, a.cu_i64, (int64_t)a.B * a.cu_s);
+    const int lo = (int)(s0 < 0 ? 0 : s0 > a.T ? a.T : s0), hi = (int)(s1 < lo ? lo : s1 > a.T ? a.T : s1);
+    const int rest = lo + a.T - hi;
+    for (int r = (int)blockIdx.x; r < rest; r += (int)gridDim.x) {
+      T* row = (T*)a.out + (int64_t)(r < lo ? r : hi + r - lo) * a.o_st;
+      for (int i = tid; i < a.Hq * a.D; i += 256) {
+        const int h = i / a.D;
+        Elem<T>::store(row + h * a.o_sh + (i - h * a.D) * a.o_sd, 0.f);
+      }
+    }
+  }
+
+  // This workgroup's tile of positions and heads; head groups fastest, so that those of
+  // one KV head tend to one XCD.
+  const int hgroups = a.Hq / a.heads, rows = kPromptRows / a.heads;
+  const int rank = (int)blockIdx.x / hgroups, hg = (int)blockIdx.x - rank * hgroups;
+  const PromptTile tile = tile_at(a, rank, rows);
+  if (tile.b < 0) return;
+  const Span seq = span_of(a, tile.b);
+  const int n = __builtin_amdgcn_readfirstlane(seq.rows), start = __builtin_amdgcn_readfirstlane(seq.start);
+  const int per_head = 4 / a.heads;                    // wavefronts of one head
+  const int h = hg * a.heads + wave / per_head, kvh = h / a.G;
+  const int first = tile.index * rows + wave % per_head * 32;  // this wavefront's first position
+  const int last = min(n, first + 32) - 1;             // below first: the wavefront has no rows
+  const int pos = first + col;
+  const int end = min(n, (tile.index + 1) * rows);     // positions the workgroup's keys reach
+  const int steps = (end + KT - 1) / KT;
+
+  // ---- this lane's query: chunks 2 f + kg
+  uint4 qf[NF];
+  {
+    const bool have = pos < n && !a.q_zero;
+    const T* row = (const T*)a.q + (int64_t)(start + (pos < n ? pos : 0)) * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const int d = (2 * f + kg) * P::EPC;
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (have && d < a.D) {
+        if constexpr (VEC) {
+          const uint4 x = *(const uint4*)(row + d);
+          w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < P::EPC; ++e)
+            if (d + e < a.D) w[e * P::EB / 4] |= PElem<T>::bits(row + (int64_t)(d + e) * a.q_sd) << (8 * (e * P::EB % 4));
+        }
+      }
+      qf[f] = make_uint4(w[0] ^ a.q_flip, w[1] ^ a.q_flip, w[2] ^ a.q_flip, w[3] ^ a.q_flip);
+    }
+  }
+
+  const T* kh = (const T*)a.k + (int64_t)start * a.k_st + (int64_t)kvh * a.k_sh;
+  const T* vh = (const T*)a.v + (int64_t)start * a.v_st + (int64_t)kvh * a.v_sh;
+  const auto issue_keys = [&](int step, int buf) __attribute__((always_inline)) {
+    P::template copy<true>(a, kh, a.k_st, a.k_sd, step * KT, n, lds_addr(k_lds[buf]), k_lds[buf]);
+  };
+  const auto issue_values = [&](int step, int buf) __attribute__((always_inline)) {
+    P::template copy<false>(a, vh, a.v_st, a.v_sd, step * KT, n, lds_addr(v_lds[buf]), v_lds[buf]);
+  };
+
+  // A wavefront's last tile holds its own positions; all before are seen whole.
+  const int mine = first < n ? first / KT : -1;
+  f32x16_t o[NDB];
+  float m, neg_m, thr, l;
+  const float cs = a.scale_log2, inv_cs = 1.f / cs;
+
+  // Scores of a tile of keys at `kl`: register r of block kb is key 32 kb + 8 (r / 4) + 4 kg + r % 4.
+  const auto scores = [&](const unsigned char* kl, f32x16_t (&s)[NKB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[kb][j] = 0.f;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const uint4 x = *(const uint4*)(kl + (kb * 32 + col) * ROWB + P::k_place(col, 2 * f + kg) * 16);
+        if constexpr (P::F32) {
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.x), __uint_as_float(qf[f].x), s[kb], 0, 0, 0);
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.y), __uint_as_float(qf[f].y), s[kb], 0, 0, 0);
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.z), __uint_as_float(qf[f].z), s[kb], 0, 0, 0);
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.w), __uint_as_float(qf[f].w), s[kb], 0, 0, 0);
+        } else {
+          s[kb] = M::mfma(x, qf[f], s[kb]);
+        }
+      }
+    }
+  };
+  const auto mask = [&](int step, f32x16_t (&s)[NKB]) __attribute__((always_inline)) {
+    int base = step * KT + 4 * kg - pos;
+    asm volatile("" : "+v"(base));  // defined here, so that no index arithmetic of this path is hoisted
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (base + 32 * kb + 8 * (r / 4) + r % 4 > 0) s[kb][r] = -INFINITY;
+  };
+  const auto rescale = [&](const f32x16_t (&s)[NKB]) __attribute__((always_inline)) {
+    float top = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+    if (__builtin_amdgcn_ballot_w64(top > thr)) {
+      const float m2 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * cs);
+      const float f = m == -INFINITY ? 0.f : fast_exp2(m - m2);
+      m = m2;
+      neg_m = m2 == -INFINITY ? 0.f : M::bias - m2;
+      thr = m2 == -INFINITY ? -INFINITY : (m2 + M::slack) * inv_cs;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) o[i] *= f;
+    }
+  };
+  // Weights of a 32-key block.
+  const auto weights = [&](f32x16_t& s, uint32_t (&w)[P::PREGS]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], cs, neg_m));
+#pragma unroll
+    for (int r = 0; r < P::PREGS; ++r) {
+      if constexpr (P::F32) {
+        l += s[r];
+        w[r] = __float_as_uint(s[r]);
+      } else {
+        w[r] = M::pack2(s[2 * r], s[2 * r + 1]);
+        l = M::sum2(w[r], l);
+      }
+    }
+  };
+  // O^T += V^T P^T for 32 keys' values at `vl`; clean: what is not finite in V counts as 0.
+  const int v_row = 4 * kg + ((lane & 15) >> 2);  // of 16 keys' first (and, + 8, second) 4-row piece
+  const int v_c0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const auto add_values = [&](const unsigned char* vl, const uint32_t (&w)[P::PREGS], auto clean)
+      __attribute__((always_inline)) {
+    if constexpr (P::F32) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = 8 * (r / 4) + 4 * kg + r % 4;
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) {
+          uint32_t x = *(const uint32_t*)(vl + key * ROWB + (32 * i + col) * 4);
+          if constexpr (decltype(clean)::value) x = P::finite(x);
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x), __uint_as_float(w[r]), o[i], 0, 0, 0);
+        }
+      }
+    } else {
+      const uint32_t vb = lds_addr(vl) + v_row * ROWB + (lane & 1) * 8;
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) {
+          const uint2 lo = TrRead<T>::at(vb + (16 * sl) * ROWB + P::v_place(v_row, 4 * i + v_c0) * 16);
+          const uint2 hi = TrRead<T>::at(vb + (16 * sl + 8) * ROWB + P::v_place(v_row + 8, 4 * i + v_c0) * 16);
+          uint4 x = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          if constexpr (decltype(clean)::value) x = make_uint4(P::finite(x.x), P::finite(x.y), P::finite(x.z), P::finite(x.w));
+          o[i] = M::mfma(x, make_uint4(w[4 * sl], w[4 * sl + 1], w[4 * sl + 2], w[4 * sl + 3]), o[i]);
+        }
+    }
+  };
+  const auto begin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+    m = -INFINITY, neg_m = 0.f, thr = -INFINITY, l = 0.f;
+  };
+  f32x16_t sa[NKB], sb[NKB];
+  uint32_t w[NKB][P::PREGS];
+
+  // A tile's keys are copied a step ahead of its values, and its scores are made beside
+  // the exponentials of the tile before: the matrix cores and the vector units each have
+  // work that does not wait for the other's.
+  begin();
+  issue_keys(0, 0);
+  issue_values(0, 0);
+  if (steps > 1) issue_keys(1, 1);
+  wait_and_barrier<0>();
+  scores(k_lds[0], sa);
+  const auto arrive = [&](int step, int buf) __attribute__((always_inline)) {
+    wait_and_barrier<0>();  // the next keys and these values have landed, and the buffers below are done with
+    if (step + 2 < steps) issue_keys(step + 2, buf);
+    if (step + 1 < steps) issue_values(step + 1, buf ^ 1);
+  };
+  const auto full = [&](int step, auto buf, f32x16_t (&s)[NKB], f32x16_t (&next)[NKB]) __attribute__((always_inline)) {
+    constexpr int B = decltype(buf)::value;
+    arrive(step, B);
+    rescale(s);
+    __builtin_amdgcn_sched_barrier(0);
+    scores(k_lds[B ^ 1], next);
+    if constexpr (P::F32) {
+      weights(s[0], w[0]);
+      add_values(v_lds[B], w[0], std::false_type{});
+    } else {
+      weights(s[0], w[0]);
+      add_values(v_lds[B], w[0], std::false_type{});
+      weights(s[1], w[1]);
+      add_values(v_lds[B] + 32 * ROWB, w[1], std::false_type{});
+      // The order of issue: each product followed by a share of the vector work.
+      sched<0x100, 2>();
+#pragma unroll
+      for (int i = 0; i < 2 * NF; ++i) {  // scores beside block 0's weights
+        sched<0x100, 1>();
+        sched<0x008, 1>();
+        sched<0x400, 16 / (2 * NF)>();
+        sched<0x002, 32 / (2 * NF)>();
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * NDB; ++i) {  // block 0's values beside block 1's weights
+        sched<0x100, 2>();
+        sched<0x008, 1>();
+        sched<0x400, 16 / (2 * NDB)>();
+        sched<0x002, 32 / (2 * NDB)>();
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * NDB; ++i) {
+        sched<0x100, 2>();
+        sched<0x008, 1>();
+      }
+    }
+  };
+  int step = 0;
+  for (; step + 1 < mine; step += 2) {
+    full(step, Stage<0>{}, sa, sb);
+    full(step + 1, Stage<1>{}, sb, sa);
+  }
+  if (step < mine) {
+    full(step, Stage<0>{}, sa, sb);
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) sa[kb] = sb[kb];
+    ++step;
+  }
+  if (mine >= 0) {
+    arrive(step, step & 1);
+    mask(step, sa);
+    rescale(sa);
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+      weights(sa[kb], w[kb]);
+      add_values(v_lds[step & 1] + kb * 32 * ROWB, w[kb], std::false_type{});
+    }
+    ++step;
+  }
+  for (; step < steps; ++step) arrive(step, step & 1);
+
+  // With a masked weight of 0, an infinity or a NaN in a value that a row does not see
+  // still makes a NaN of it in the matrix product. That shows in the output; then the
+  // workgroup goes over its tiles again, with such values taken out of the product and
+  // added to the rows that see them.
+  float lost = l * 0.f;
+#pragma unroll
+  for (int i = 0; i < NDB; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) lost = __builtin_fmaf(o[i][j], 0.f, lost);
+  if (__syncthreads_or(pos < n && lost != lost)) {
+    begin();
+#pragma unroll 1
+    for (step = 0; step < steps; ++step) {
+      __syncthreads();
+      issue_keys(step, 0);
+      issue_values(step, 0);
+      wait_and_barrier<0>();
+      if (step > mine) continue;
+      scores(k_lds[0], sa);
+      mask(step, sa);
+      rescale(sa);
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        weights(sa[kb], w[kb]);
+        add_values(v_lds[0] + kb * 32 * ROWB, w[kb], std::true_type{});
+      }
+#pragma unroll 1
+      for (int key = 0; key < KT; ++key) {
+        const bool seen = step * KT + key <= pos;
+#pragma unroll
+        for (int i = 0; i < NDB; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int d = 32 * i + 8 * j + 4 * kg;
+            const unsigned char* at = v_lds[0] + key * ROWB + P::v_place(key, d / P::EPC) * 16 + d % P::EPC * P::EB;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = Elem<T>::load((const T*)at + e);
+              if (seen && !(fabsf(x) < INFINITY)) o[i][4 * j + e] += x;
+            }
+          }
+      }
+    }
+  }
+
+  // ---- out: registers 4 j .. 4 j + 3 of block i are dims 32 i + 8 j + 4 kg ..
+  if (pos >= n) return;
+  const float total = l + __shfl_xor(l, 32, 64), inv = total == 0.f ? 0.f : 1.f / total;
+  T* row = (T*)a.out + (int64_t)(start + pos) * a.o_st + (int64_t)h * a.o_sh;
+#pragma unroll
+  for (int i = 0; i < NDB; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = 32 * i + 8 * j + 4 * kg;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = o[i][4 * j + e] * inv;
+      if constexpr (VEC) {
+        if (d >= a.D) continue;
+        if constexpr (P::F32) *(float4*)(row + d) = make_float4(x[0], x[1], x[2], x[3]);
+        else *(uint2*)(row + d) = make_uint2(M::pack2(x[0], x[1]), M::pack2(x[2], x[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < a.D) Elem<T>::store(row + (d + e) * a.o_sd, x[e]);
+      }
+    }
+}
+
+template <typename T, int DP>
+hipError_t launch_prompt_dp(PromptArgs a, hipStream_t stream) {
+  const int rows = kPromptRows / a.heads;
+  const int64_t tiles = (int64_t)a.T / rows + std::min<int64_t>(a.B, a.T);
+  const int64_t grid = std::max<int64_t>(1, tiles * (a.Hq / a.heads));
+  void* args[] = {&a};
+  const void* fn = a.vec ? (const void*)&prompt_attention_kernel<T, DP, true> : (const void*)&prompt_attention_kernel<T, DP, false>;
+  return hipLaunchKernel(fn, dim3((unsigned)grid), dim3(256), args, 0, stream);
+}
+
+template <typename T>
+hipError_t launch_prompt(const PromptArgs& a, hipStream_t stream) {
+  if (a.D <= 32) return launch_prompt_dp<T, 32>(a, stream);
+  if (a.D <= 64) return launch_prompt_dp<T, 64>(a, stream);
+  if (a.D <= 80) return launch_prompt_dp<T, 80>(a, stream);
+  if (a.D <= 96) return launch_prompt_dp<T, 96>(a, stream);
+  if (a.D <= 128) return launch_prompt_dp<T, 128>(a, stream);
+  if (a.D <= 192) return launch_prompt_dp<T, 192>(a, stream);
+  if (a.D <= 256) return launch_prompt_dp<T, 256>(a, stream);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+}  // namespace mgi

@@ -442,6 +442,38 @@ at::Tensor paged_decode_fp4(const at::Tensor& q, const at::Tensor& pool, int64_t
   return out;
 }
 
+// prompt_attention(q, k, v, cu_seqlens) -> [T, Hq, D] of q's dtype: causal attention of
+// packed whole prompts.
+at::Tensor prompt_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu) {
+  if (!q.is_cuda()) value_error("q must be on a GPU device for the HIP backend");
+  if (q.dim() != 3) value_error("q must have shape [T,H,D]");
+  const int64_t t = q.size(0), h = q.size(1), d = q.size(2);
+  if (h == 0 || d == 0) value_error("q dimensions must be nonzero");
+  if (d > 256) value_error("prompt attention supports head_dim <= 256");
+  const int qd = dtype_code(q.scalar_type());
+  if (qd < 0) value_error("q must be float32, bfloat16 or float16");
+  if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
+    value_error("q, k and v must share a float dtype");
+  if (k.dim() != 3 || v.sizes() != k.sizes()) value_error("k and v must have matching shape [T,H,D]");
+  const int64_t hk = k.size(1);
+  if (k.size(0) != t || k.size(2) != d || hk == 0 || h % hk != 0)
+    value_error("k and v must have q's rows and head dimension, and heads that divide q's");
+  if (cu.dim() != 1 || cu.size(0) < 1) value_error("cu_seqlens must have shape [B+1]");
+  const int ci = index_code(cu.scalar_type());
+  if (ci < 0) value_error("cu_seqlens must be integer");
+  const auto dev = q.device();
+  if (k.device() != dev || v.device() != dev || cu.device() != dev)
+    value_error("all inputs must reside on same GPU device");
+  check_plain({&q, &k, &v, &cu});
+  const c10::DeviceGuard guard(dev);
+  at::Tensor out = at::empty({t, h, d}, q.options());
+  check_status(mgi_prompt_attention(out.data_ptr(), out.strides().data(), q.data_ptr(), q.strides().data(),
+                                    k.data_ptr(), k.strides().data(), v.data_ptr(), v.strides().data(), qd,
+                                    cu.data_ptr(), cu.stride(0), ci, cu.size(0) - 1, t, h, hk, d,
+                                    (float)(1.0 / std::sqrt((double)d)), 1, stream_of(q)));
+  return out;
+}
+
 // Whether t is a plain contiguous, 16-byte aligned tensor of x's dtype and
 // (current) device with `numel` elements: what the decode-step linear kernels
 // take.
@@ -513,7 +545,7 @@ py::object decode_linear_norm(const c10::optional<at::Tensor>& x, const c10::opt
 PYBIND11_MODULE(_hip_ops, m) {
   m.doc() = "PyTorch binding of libminivllm_hip.so (kv_append, kv_append_rope, qk_norm_rope, paged_decode, "
             "paged_decode_append, paged_decode_shared, paged_prefill, decode_linear, decode_linear_norm, "
-            "kv_append_fp4, kv_gather_fp4, paged_decode_fp4)";
+            "kv_append_fp4, kv_gather_fp4, paged_decode_fp4, prompt_attention)";
   m.def("kv_append", &kv_append);
   m.def("paged_decode", &paged_decode);
   m.def("paged_decode_append", &paged_decode_append);
@@ -527,6 +559,7 @@ PYBIND11_MODULE(_hip_ops, m) {
     return kv_gather_fp4(pool, S, D, layer_idx, slots, torch::python::detail::py_object_to_dtype(dtype));
   });
   m.def("paged_decode_fp4", &paged_decode_fp4);
+  m.def("prompt_attention", &prompt_attention);
   m.def("decode_linear", &decode_linear);
   m.def("decode_linear_norm", &decode_linear_norm);
 }

@@ -44,7 +44,8 @@ HIP_FLAGS = [
 # for the softmax (64 v_accvgpr moves per key tile).
 MFMA_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 MFMA_SOURCES = {"decode_linear.hip", "paged_prefill.hip", "paged_shared_f32.hip", "paged_shared_bf16.hip",
-                "paged_shared_f16.hip", "paged_fp4_f32.hip", "paged_fp4_bf16.hip", "paged_fp4_f16.hip"}
+                "paged_shared_f16.hip", "paged_fp4_f32.hip", "paged_fp4_bf16.hip", "paged_fp4_f16.hip",
+                "prompt_attention_f32.hip", "prompt_attention_bf16.hip", "prompt_attention_f16.hip"}
 
 
 def library_path() -> Path:

@@ -494,6 +494,43 @@ def paged_decode_fp4(q: torch.Tensor, pool: torch.Tensor, S: int, D: int, bt: to
     return out
 
 
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor) -> torch.Tensor:
+    """[T, Hq, D] causal attention of packed whole prompts."""
+    if not q.is_cuda:
+        raise ValueError("q must be on a GPU device for the HIP backend")
+    if q.ndim != 3:
+        raise ValueError("q must have shape [T,H,D]")
+    t, h, d = q.shape
+    if h == 0 or d == 0:
+        raise ValueError("q dimensions must be nonzero")
+    if d > 256:
+        raise ValueError("prompt attention supports head_dim <= 256")
+    if q.dtype not in _FLOATS:
+        raise ValueError("q must be float32, bfloat16 or float16")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must share a float dtype")
+    if k.ndim != 3 or v.shape != k.shape:
+        raise ValueError("k and v must have matching shape [T,H,D]")
+    hk = k.shape[1]
+    if k.shape[0] != t or k.shape[2] != d or hk == 0 or h % hk != 0:
+        raise ValueError("k and v must have q's rows and head dimension, and heads that divide q's")
+    if cu.ndim != 1 or cu.shape[0] < 1:
+        raise ValueError("cu_seqlens must have shape [B+1]")
+    if cu.dtype not in _INDEX:
+        raise ValueError("cu_seqlens must be integer")
+    if any(x.device != q.device for x in (k, v, cu)):
+        raise ValueError("all inputs must reside on same GPU device")
+    _check_plain(q, k, v, cu)
+    with torch.cuda.device(q.device):
+        out = torch.empty((t, h, d), dtype=q.dtype, device=q.device)
+        _native.check(_native.lib().mgi_prompt_attention(
+            out.data_ptr(), _native.strides(out), q.data_ptr(), _native.strides(q), k.data_ptr(), _native.strides(k),
+            v.data_ptr(), _native.strides(v), _native.DTYPE_CODES[q.dtype],
+            cu.data_ptr(), cu.stride(0), _native.ITYPE_CODES[cu.dtype], cu.shape[0] - 1, t, h, hk, d,
+            1.0 / math.sqrt(d), 1, _native.stream_handle(q.device)))
+    return out
+
+
 def _linear_ok(t: torch.Tensor | None, x: torch.Tensor, numel: int) -> bool:
     """Whether t (or no tensor) is plain, contiguous and 16-byte aligned, of x's
     dtype and (current) device, with numel elements."""

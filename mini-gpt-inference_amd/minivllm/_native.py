@@ -54,6 +54,7 @@ EXPORTED_SYMBOLS = (
     "mgi_kv_gather_fp4",
     "mgi_paged_decode_fp4",
     "mgi_paged_decode_fp4_workspace_bytes",
+    "mgi_prompt_attention",
 )
 
 _lock = threading.Lock()
@@ -209,6 +210,15 @@ def _declare(lib: ctypes.CDLL) -> None:
     ]
     lib.mgi_paged_decode_fp4_workspace_bytes.restype = ctypes.c_size_t
     lib.mgi_paged_decode_fp4_workspace_bytes.argtypes = [_i64] * 6
+    lib.mgi_prompt_attention.restype = _i
+    lib.mgi_prompt_attention.argtypes = [
+        _p, _pi64, _p, _pi64,              # out, q, strides
+        _p, _pi64, _p, _pi64, _i,          # k, v, strides, dtype
+        _p, _i64, _i,                      # sequence starts, stride, itype
+        _i64, _i64, _i64, _i64, _i64,      # B T Hq Hk D
+        ctypes.c_float, _i,                # scale, zero_rest
+        _p,                                # stream
+    ]
 
 
 def lib() -> ctypes.CDLL:
@@ -239,8 +249,8 @@ def lib() -> ctypes.CDLL:
 def ops():
     """The eager path's binding: kv_append, paged_decode, paged_decode_append,
     paged_prefill, decode_linear, decode_linear_norm, qk_norm_rope,
-    kv_append_rope, paged_decode_shared, kv_append_fp4, kv_gather_fp4 and
-    paged_decode_fp4 on tensors, validated,
+    kv_append_rope, paged_decode_shared, kv_append_fp4, kv_gather_fp4,
+    paged_decode_fp4 and prompt_attention on tensors, validated,
     calling the C ABI on the current stream.
 
     Normally the PyTorch extension _hip_ops (csrc/torch_ops.cpp). When the

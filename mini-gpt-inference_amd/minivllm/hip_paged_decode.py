@@ -32,7 +32,8 @@ their positions, the latter on the way into the pool.
 paged_attention_shared_prefix_hip is decode attention, with grouped query
 heads, for sequences that begin with the same cached blocks. kv_append_fp4,
 kv_gather_fp4 and paged_attention_fp4_hip write, read back and attend over a
-FP4KVBlockPool, whose keys and values are 4 bits. These six are
+FP4KVBlockPool, whose keys and values are 4 bits. prompt_attention_hip is causal
+attention of packed whole prompts over their own keys and values. These seven are
 inference-only (RuntimeError for tensors that require gradients while grad mode
 is on) and run on their tensors' device, current or not.
 """
@@ -203,3 +204,17 @@ def paged_prefill_hip(q: torch.Tensor, pool: KVBlockPool, block_table: torch.Ten
     tensor of q.dtype with out[t] = softmax(q[t] K[0..start_pos+t]^T / sqrt(D)) V.
     """
     return _native.ops().paged_prefill(q, pool.k, pool.v, block_table, int(start_pos), int(layer_idx))
+
+
+def prompt_attention_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor) -> torch.Tensor:
+    """Causal attention of whole prompts, packed one after the other, over their own keys
+    and values as the projection made them (no pool: append them to any pool beside it).
+
+    q: [T, Hq, D]; k, v: [T, Hk, D] with Hq a multiple of Hk, any strides; query head h
+    reads KV head h // (Hq // Hk). cu_seqlens: [B + 1] integers that never fall, sequence b
+    being rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (none, for an empty one); it is read
+    on the GPU alone, so a captured graph follows it. float32, bfloat16 or float16;
+    head_dim up to 256. Returns a fresh [T, Hq, D] tensor of q.dtype; rows of no sequence
+    are 0. A row's result does not depend on rows it does not see, whatever they hold.
+    """
+    return _native.ops().prompt_attention(q, k, v, cu_seqlens)
