@@ -87,77 +87,81 @@ template <> struct PElem<float> {
   __device__ static __forceinline__ uint32_t bits(const float* p) { return __float_as_uint(*p); }
 };
 
-__device__ __forceinline__ int wave_sum_int(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
-  return __builtin_amdgcn_readfirstlane(x);
-}
-__device__ __forceinline__ int wave_max_int(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d, 64));
-  return __builtin_amdgcn_readfirstlane(x);
-}
-
-// The next N instructions of the kinds in MASK, in the order of issue.
-template <int MASK, int N>
-__device__ __forceinline__ void sched() {
-  if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(MASK, N, 0);
+// Sum and maximum over the wavefront of numbers that are not negative, by DPP.
+template <typename Op>
+__device__ __forceinline__ int wave_reduce(int x, Op op) {
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));  // lanes 1, 2, 4 and 8 below in the row
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true));  // row 0's last to row 1, 2's to 3
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true));  // row 1's last to rows 2 and 3
+  return __builtin_amdgcn_readlane(x, 63);
 }
 
 struct Span {
   int start, rows;
 };
 __device__ __forceinline__ Span span_of(const PromptArgs& a, int b) {
+  if (b >= a.B) return Span{0, 0};
   const int64_t s = load_index(a.starts, a.cu_i64, (int64_t)b * a.cu_s);
   const int64_t e = load_index(a.starts, a.cu_i64, (int64_t)(b + 1) * a.cu_s);
   const int64_t lo = s < 0 ? 0 : s > a.T ? a.T : s, hi = e < lo ? lo : e > a.T ? a.T : e;
   return Span{(int)lo, (int)(hi - lo)};
 }
 
-// Tiles (of `rows` positions) of lane's sequence b0 + lane.
-__device__ __forceinline__ int tiles_of(const PromptArgs& a, int b, int rows) {
-  return b < a.B ? (span_of(a, b).rows + rows - 1) / rows : 0;
-}
-
-// The `rank`-th tile in falling order of its index in its sequence: (sequence, index),
-// or sequence -1 past the last.
+// The `rank`-th tile (of `rows` positions) in falling order of its index in its sequence:
+// the sequence's rows and the index, or no rows past the last. The first kKept sequences'
+// lengths stay in registers, the others' are read again in each step of the search.
 struct PromptTile {
-  int b, index;
+  Span seq;
+  int index;
 };
 __device__ __forceinline__ PromptTile tile_at(const PromptArgs& a, int rank, int rows) {
-  const int lane = (int)(threadIdx.x & 63);
-  const int first = tiles_of(a, lane, rows);  // of the first 64 sequences, kept
-  const auto each = [&](auto f) {
-    f(first, 0);
-    for (int b0 = 64; b0 < a.B; b0 += 64) f(tiles_of(a, b0 + lane, rows), b0);
+  constexpr int kKept = 4;
+  const int lane = (int)(threadIdx.x & 63), shift = __builtin_ctz(rows);
+  const auto tiles = [&](Span x) { return (x.rows + rows - 1) >> shift; };
+  Span kept[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) kept[i] = 64 * i < a.B ? span_of(a, 64 * i + lane) : Span{0, 0};
+  const auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kKept; ++i)
+      if (64 * i < a.B) f(kept[i]);
+    for (int b0 = 64 * kKept; b0 < a.B; b0 += 64) f(span_of(a, b0 + lane));
   };
+  const auto sum = [](int x, int y) { return x + y; };
+  const auto larger = [](int x, int y) { return max(x, y); };
   int most = 0;
-  each([&](int n, int) { most = max(most, n); });
-  most = wave_max_int(most);
-  const auto from = [&](int index) {  // tiles with this index or a higher one
-    int sum = 0;
-    each([&](int n, int) { sum += max(0, n - index); });
-    return wave_sum_int(sum);
+  each([&](Span x) { most = max(most, tiles(x)); });
+  most = wave_reduce(most, larger);
+  const auto from = [&](int index) __attribute__((always_inline)) {  // tiles with this index or a higher one
+    int n = 0;
+    each([&](Span x) { n += max(0, tiles(x) - index); });
+    return wave_reduce(n, sum);
   };
-  if (rank >= from(0)) return PromptTile{-1, 0};
-  int lo = 0, hi = most;  // from(lo) > rank >= from(hi)
+  if (rank >= from(0)) return PromptTile{Span{0, 0}, 0};
+  int lo = 0, hi = most, above = 0;  // from(lo) > rank >= from(hi) = above
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (from(mid) > rank) lo = mid; else hi = mid;
+    const int mid = (lo + hi) >> 1, n = from(mid);
+    if (n > rank) lo = mid;
+    else hi = mid, above = n;
   }
-  int left = rank - from(lo + 1), b = -1;
-  each([&](int n, int b0) {
-    if (b >= 0) return;
-    const uint64_t has = __ballot(n > lo);
-    const int count = __popcll(has);
+  int left = rank - above;
+  PromptTile found{Span{0, 0}, lo};
+  each([&](Span x) {
+    if (left < 0) return;
+    const bool has = tiles(x) > lo;
+    const uint64_t all = __ballot(has);
+    const int count = __popcll(all);
     if (left < count) {
-      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
-      b = b0 + __ffsll((unsigned long long)__ballot(n > lo && before == left)) - 1;
-    } else {
-      left -= count;
+      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+      const int at = __ffsll((unsigned long long)__ballot(has && before == left)) - 1;
+      found.seq = Span{__builtin_amdgcn_readlane(x.start, at), __builtin_amdgcn_readlane(x.rows, at)};
     }
+    left -= count;
   });
-  return PromptTile{b, lo};
+  return found;
 }
 
 // DP: head dim, padded to a multiple of 16 (D <= DP). VEC: rows are copied in 16-byte pieces.
@@ -198,6 +202,15 @@ struct Prompt {
       if ((w & 0x7fffu) >= M::inf) w &= 0xffff0000u;
       return ((w >> 16) & 0x7fffu) >= M::inf ? w & 0xffffu : w;
     }
+  }
+
+  // Copy i of a whole tile (see copy): from `base`, its first key's row.
+  template <bool KEYS, int I>
+  __device__ static __forceinline__ void copy_piece(const PromptArgs& a, const char* base, int64_t st, uint32_t dst) {
+    const int at = I * 256 + (int)threadIdx.x, row = at / CPR, place = at % CPR;
+    const int c = KEYS ? k_place(row, place) : v_place(row, place);  // its own inverse
+    const uint32_t off = (uint32_t)row * (uint32_t)(st * EB) + (c * EPC < a.D ? (uint32_t)c * 16 : 0u);
+    copy16_to_lds(base, off, __builtin_amdgcn_readfirstlane(dst + (uint32_t)(I * 256 + ((int)threadIdx.x & ~63)) * 16));
   }
 
   // One tile (keys key0 .. of this sequence) of K or V into LDS at `dst`, by all four wavefronts.
@@ -246,8 +259,9 @@ prompt_attention_kernel(const PromptArgs a) {
   using P = Prompt<T, DP, VEC>;
   using M = PM<T>;
   constexpr int NDB = P::NDB, NF = P::NF, NKB = P::NKB, KT = P::KT, ROWB = P::ROWB, TILEB = P::TILEB;
-  __shared__ __align__(1024) unsigned char k_lds[2][TILEB];
-  __shared__ __align__(1024) unsigned char v_lds[2][TILEB];
+  __shared__ __align__(1024) unsigned char lds[4][TILEB];  // two tiles of keys, two of values
+  unsigned char(*k_lds)[TILEB] = lds;
+  unsigned char(*v_lds)[TILEB] = lds + 2;
 
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, kg = lane >> 5;
@@ -271,9 +285,8 @@ prompt_attention_kernel(const PromptArgs a) {
   const int hgroups = a.Hq / a.heads, rows = kPromptRows / a.heads;
   const int rank = (int)blockIdx.x / hgroups, hg = (int)blockIdx.x - rank * hgroups;
   const PromptTile tile = tile_at(a, rank, rows);
-  if (tile.b < 0) return;
-  const Span seq = span_of(a, tile.b);
-  const int n = __builtin_amdgcn_readfirstlane(seq.rows), start = __builtin_amdgcn_readfirstlane(seq.start);
+  const int n = tile.seq.rows, start = tile.seq.start;
+  if (n == 0) return;
   const int per_head = 4 / a.heads;                    // wavefronts of one head
   const int h = hg * a.heads + wave / per_head, kvh = h / a.G;
   const int first = tile.index * rows + wave % per_head * 32;  // this wavefront's first position
@@ -281,6 +294,19 @@ prompt_attention_kernel(const PromptArgs a) {
   const int pos = first + col;
   const int end = min(n, (tile.index + 1) * rows);     // positions the workgroup's keys reach
   const int steps = (end + KT - 1) / KT;
+
+  const T* kh = (const T*)a.k + (int64_t)start * a.k_st + (int64_t)kvh * a.k_sh;
+  const T* vh = (const T*)a.v + (int64_t)start * a.v_st + (int64_t)kvh * a.v_sh;
+  const auto issue_keys = [&](int step, int buf) __attribute__((always_inline)) {
+    P::template copy<true>(a, kh, a.k_st, a.k_sd, step * KT, n, lds_addr(k_lds[buf]), k_lds[buf]);
+  };
+  const auto issue_values = [&](int step, int buf) __attribute__((always_inline)) {
+    P::template copy<false>(a, vh, a.v_st, a.v_sd, step * KT, n, lds_addr(v_lds[buf]), v_lds[buf]);
+  };
+
+  issue_keys(0, 0);
+  issue_values(0, 0);
+  if (steps > 1) issue_keys(1, 1);
 
   // ---- this lane's query: chunks 2 f + kg
   uint4 qf[NF];
@@ -305,111 +331,106 @@ prompt_attention_kernel(const PromptArgs a) {
     }
   }
 
-  const T* kh = (const T*)a.k + (int64_t)start * a.k_st + (int64_t)kvh * a.k_sh;
-  const T* vh = (const T*)a.v + (int64_t)start * a.v_st + (int64_t)kvh * a.v_sh;
-  const auto issue_keys = [&](int step, int buf) __attribute__((always_inline)) {
-    P::template copy<true>(a, kh, a.k_st, a.k_sd, step * KT, n, lds_addr(k_lds[buf]), k_lds[buf]);
-  };
-  const auto issue_values = [&](int step, int buf) __attribute__((always_inline)) {
-    P::template copy<false>(a, vh, a.v_st, a.v_sd, step * KT, n, lds_addr(v_lds[buf]), v_lds[buf]);
-  };
-
   // A wavefront's last tile holds its own positions; all before are seen whole.
   const int mine = first < n ? first / KT : -1;
   f32x16_t o[NDB];
   float m, neg_m, thr, l;
   const float cs = a.scale_log2, inv_cs = 1.f / cs;
 
-  // Scores of a tile of keys at `kl`: register r of block kb is key 32 kb + 8 (r / 4) + 4 kg + r % 4.
-  const auto scores = [&](const unsigned char* kl, f32x16_t (&s)[NKB]) __attribute__((always_inline)) {
+  // One step of the first product over 32 keys at `kl`: register r of the scores is key
+  // 8 (r / 4) + 4 kg + r % 4.
+  const auto key_operand = [&](const unsigned char* kl, auto step) __attribute__((always_inline)) -> uint4 {
+    return *(const uint4*)(kl + col * ROWB + P::k_place(col, 2 * decltype(step)::value + kg) * 16);
+  };
+  const auto score = [&](uint4 x, auto step, f32x16_t& s) __attribute__((always_inline)) {
+    constexpr int f = decltype(step)::value;
+    if constexpr (f == 0) {
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[kb][j] = 0.f;
-#pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const uint4 x = *(const uint4*)(kl + (kb * 32 + col) * ROWB + P::k_place(col, 2 * f + kg) * 16);
-        if constexpr (P::F32) {
-          s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.x), __uint_as_float(qf[f].x), s[kb], 0, 0, 0);
-          s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.y), __uint_as_float(qf[f].y), s[kb], 0, 0, 0);
-          s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.z), __uint_as_float(qf[f].z), s[kb], 0, 0, 0);
-          s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.w), __uint_as_float(qf[f].w), s[kb], 0, 0, 0);
-        } else {
-          s[kb] = M::mfma(x, qf[f], s[kb]);
-        }
-      }
+      for (int j = 0; j < 16; ++j) s[j] = 0.f;
+    }
+    if constexpr (P::F32) {
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.x), __uint_as_float(qf[f].x), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.y), __uint_as_float(qf[f].y), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.z), __uint_as_float(qf[f].z), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.w), __uint_as_float(qf[f].w), s, 0, 0, 0);
+    } else {
+      s = M::mfma(x, qf[f], s);
     }
   };
-  const auto mask = [&](int step, f32x16_t (&s)[NKB]) __attribute__((always_inline)) {
-    int base = step * KT + 4 * kg - pos;
+  const auto mask = [&](int key0, f32x16_t& s) __attribute__((always_inline)) {
+    int base = key0 + 4 * kg - pos;
     asm volatile("" : "+v"(base));  // defined here, so that no index arithmetic of this path is hoisted
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (base + 32 * kb + 8 * (r / 4) + r % 4 > 0) s[kb][r] = -INFINITY;
+    for (int r = 0; r < 16; ++r)
+      if (base + 8 * (r / 4) + r % 4 > 0) s[r] = -INFINITY;
   };
-  const auto rescale = [&](const f32x16_t (&s)[NKB]) __attribute__((always_inline)) {
-    float top = s[0][0];
+  // Whether the running maximum moves with these scores; then `f` takes sums made with the old one to the new.
+  const auto raise = [&](const f32x16_t& s, float& f) __attribute__((always_inline)) -> bool {
+    float top = s[0];
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb)
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    if (!__builtin_amdgcn_ballot_w64(top > thr)) return false;
+    const float m2 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * cs);
+    f = m == -INFINITY ? 0.f : fast_exp2(m - m2);
+    m = m2;
+    neg_m = m2 == -INFINITY ? 0.f : M::bias - m2;
+    thr = m2 == -INFINITY ? -INFINITY : (m2 + M::slack) * inv_cs;
+    l *= f;
+    return true;
+  };
+  const auto scale_output = [&](float f) __attribute__((always_inline)) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-    if (__builtin_amdgcn_ballot_w64(top > thr)) {
-      const float m2 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * cs);
-      const float f = m == -INFINITY ? 0.f : fast_exp2(m - m2);
-      m = m2;
-      neg_m = m2 == -INFINITY ? 0.f : M::bias - m2;
-      thr = m2 == -INFINITY ? -INFINITY : (m2 + M::slack) * inv_cs;
-      l *= f;
-#pragma unroll
-      for (int i = 0; i < NDB; ++i) o[i] *= f;
+    for (int i = 0; i < NDB; ++i) o[i] *= f;
+  };
+  // Weights of a 32-key block: element by element, then by pairs packed and summed.
+  const auto weight = [&](f32x16_t& s, int r) __attribute__((always_inline)) {
+    s[r] = fast_exp2(__builtin_fmaf(s[r], cs, neg_m));
+  };
+  const auto pack_pair = [&](const f32x16_t& s, int r, uint32_t (&w)[P::PREGS]) __attribute__((always_inline)) {
+    if constexpr (P::F32) {
+      l += s[2 * r] + s[2 * r + 1];
+      w[2 * r] = __float_as_uint(s[2 * r]);
+      w[2 * r + 1] = __float_as_uint(s[2 * r + 1]);
+    } else {
+      w[r] = M::pack2(s[2 * r], s[2 * r + 1]);
+      l = M::sum2(w[r], l);
     }
   };
-  // Weights of a 32-key block.
   const auto weights = [&](f32x16_t& s, uint32_t (&w)[P::PREGS]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], cs, neg_m));
+    for (int r = 0; r < 16; ++r) weight(s, r);
 #pragma unroll
-    for (int r = 0; r < P::PREGS; ++r) {
-      if constexpr (P::F32) {
-        l += s[r];
-        w[r] = __float_as_uint(s[r]);
-      } else {
-        w[r] = M::pack2(s[2 * r], s[2 * r + 1]);
-        l = M::sum2(w[r], l);
-      }
-    }
+    for (int r = 0; r < 8; ++r) pack_pair(s, r, w);
   };
-  // O^T += V^T P^T for 32 keys' values at `vl`; clean: what is not finite in V counts as 0.
+  // One step of O^T += V^T P^T for 32 keys' values at `vl`: 16 keys and a block of dims (f32:
+  // two keys). clean: what is not finite in V counts as 0.
   const int v_row = 4 * kg + ((lane & 15) >> 2);  // of 16 keys' first (and, + 8, second) 4-row piece
   const int v_c0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  const auto add_values = [&](const unsigned char* vl, const uint32_t (&w)[P::PREGS], auto clean)
-      __attribute__((always_inline)) {
+  constexpr int VSTEPS = P::F32 ? 16 * NDB : 2 * NDB;
+  const auto value_operand = [&](const unsigned char* vl, auto step) __attribute__((always_inline)) -> uint4 {
+    constexpr int n = decltype(step)::value, i = n % NDB, part = n / NDB;
     if constexpr (P::F32) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = 8 * (r / 4) + 4 * kg + r % 4;
-#pragma unroll
-        for (int i = 0; i < NDB; ++i) {
-          uint32_t x = *(const uint32_t*)(vl + key * ROWB + (32 * i + col) * 4);
-          if constexpr (decltype(clean)::value) x = P::finite(x);
-          o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x), __uint_as_float(w[r]), o[i], 0, 0, 0);
-        }
-      }
+      return make_uint4(*(const uint32_t*)(vl + (8 * (part / 4) + 4 * kg + part % 4) * ROWB + (32 * i + col) * 4), 0, 0, 0);
     } else {
       const uint32_t vb = lds_addr(vl) + v_row * ROWB + (lane & 1) * 8;
-#pragma unroll
-      for (int sl = 0; sl < 2; ++sl)
-#pragma unroll
-        for (int i = 0; i < NDB; ++i) {
-          const uint2 lo = TrRead<T>::at(vb + (16 * sl) * ROWB + P::v_place(v_row, 4 * i + v_c0) * 16);
-          const uint2 hi = TrRead<T>::at(vb + (16 * sl + 8) * ROWB + P::v_place(v_row + 8, 4 * i + v_c0) * 16);
-          uint4 x = make_uint4(lo.x, lo.y, hi.x, hi.y);
-          if constexpr (decltype(clean)::value) x = make_uint4(P::finite(x.x), P::finite(x.y), P::finite(x.z), P::finite(x.w));
-          o[i] = M::mfma(x, make_uint4(w[4 * sl], w[4 * sl + 1], w[4 * sl + 2], w[4 * sl + 3]), o[i]);
-        }
+      const uint2 lo = TrRead<T>::at(vb + (16 * part) * ROWB + P::v_place(v_row, 4 * i + v_c0) * 16);
+      const uint2 hi = TrRead<T>::at(vb + (16 * part + 8) * ROWB + P::v_place(v_row + 8, 4 * i + v_c0) * 16);
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
+  };
+  const auto value = [&](uint4 x, auto step, const uint32_t (&w)[P::PREGS], auto clean) __attribute__((always_inline)) {
+    constexpr int n = decltype(step)::value, i = n % NDB, part = n / NDB;
+    if constexpr (decltype(clean)::value) x = make_uint4(P::finite(x.x), P::finite(x.y), P::finite(x.z), P::finite(x.w));
+    if constexpr (P::F32)
+      o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.x), __uint_as_float(w[part]), o[i], 0, 0, 0);
+    else
+      o[i] = M::mfma(x, make_uint4(w[4 * part], w[4 * part + 1], w[4 * part + 2], w[4 * part + 3]), o[i]);
+  };
+  const auto all_scores = [&](const unsigned char* kl, f32x16_t& s) __attribute__((always_inline)) {
+    static_for<0, NF>([&](auto f) { score(key_operand(kl, f), f, s); });
+  };
+  const auto all_values = [&](const unsigned char* vl, const uint32_t (&w)[P::PREGS], auto clean) __attribute__((always_inline)) {
+    static_for<0, VSTEPS>([&](auto n) { value(value_operand(vl, n), n, w, clean); });
   };
   const auto begin = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -418,81 +439,148 @@ prompt_attention_kernel(const PromptArgs a) {
       for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
     m = -INFINITY, neg_m = 0.f, thr = -INFINITY, l = 0.f;
   };
-  f32x16_t sa[NKB], sb[NKB];
-  uint32_t w[NKB][P::PREGS];
+  f32x16_t sa, sb;
+  uint32_t wa[P::PREGS], wb[P::PREGS];
+  float f;
 
-  // A tile's keys are copied a step ahead of its values, and its scores are made beside
-  // the exponentials of the tile before: the matrix cores and the vector units each have
-  // work that does not wait for the other's.
+  // Three blocks of 32 keys are in work at once: block b's weights are made by the vector
+  // units while the matrix cores make block b + 1's scores and add block b - 1's values,
+  // and nothing among them waits for the others. So a tile's keys are needed a step before
+  // its values, and are copied a step ahead of them.
   begin();
-  issue_keys(0, 0);
-  issue_values(0, 0);
-  if (steps > 1) issue_keys(1, 1);
   wait_and_barrier<0>();
-  scores(k_lds[0], sa);
   const auto arrive = [&](int step, int buf) __attribute__((always_inline)) {
     wait_and_barrier<0>();  // the next keys and these values have landed, and the buffers below are done with
     if (step + 2 < steps) issue_keys(step + 2, buf);
     if (step + 1 < steps) issue_values(step + 1, buf ^ 1);
   };
-  const auto full = [&](int step, auto buf, f32x16_t (&s)[NKB], f32x16_t (&next)[NKB]) __attribute__((always_inline)) {
-    constexpr int B = decltype(buf)::value;
-    arrive(step, B);
-    rescale(s);
-    __builtin_amdgcn_sched_barrier(0);
-    scores(k_lds[B ^ 1], next);
-    if constexpr (P::F32) {
-      weights(s[0], w[0]);
-      add_values(v_lds[B], w[0], std::false_type{});
-    } else {
-      weights(s[0], w[0]);
-      add_values(v_lds[B], w[0], std::false_type{});
-      weights(s[1], w[1]);
-      add_values(v_lds[B] + 32 * ROWB, w[1], std::false_type{});
-      // The order of issue: each product followed by a share of the vector work.
-      sched<0x100, 2>();
-#pragma unroll
-      for (int i = 0; i < 2 * NF; ++i) {  // scores beside block 0's weights
-        sched<0x100, 1>();
-        sched<0x008, 1>();
-        sched<0x400, 16 / (2 * NF)>();
-        sched<0x002, 32 / (2 * NF)>();
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * NDB; ++i) {  // block 0's values beside block 1's weights
-        sched<0x100, 2>();
-        sched<0x008, 1>();
-        sched<0x400, 16 / (2 * NDB)>();
-        sched<0x002, 32 / (2 * NDB)>();
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * NDB; ++i) {
-        sched<0x100, 2>();
-        sched<0x008, 1>();
-      }
-    }
-  };
   int step = 0;
-  for (; step + 1 < mine; step += 2) {
-    full(step, Stage<0>{}, sa, sb);
-    full(step + 1, Stage<1>{}, sb, sa);
-  }
-  if (step < mine) {
-    full(step, Stage<0>{}, sa, sb);
-#pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) sa[kb] = sb[kb];
-    ++step;
-  }
-  if (mine >= 0) {
-    arrive(step, step & 1);
-    mask(step, sa);
-    rescale(sa);
-#pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-      weights(sa[kb], w[kb]);
-      add_values(v_lds[step & 1] + kb * 32 * ROWB, w[kb], std::false_type{});
+  if constexpr (P::F32) {
+    all_scores(k_lds[0], sa);
+    const auto full = [&](int step, auto buf, f32x16_t& s, f32x16_t& next) __attribute__((always_inline)) {
+      constexpr int B = decltype(buf)::value;
+      arrive(step, B);
+      if (raise(s, f)) scale_output(f);
+      all_scores(k_lds[B ^ 1], next);
+      weights(s, wa);
+      all_values(v_lds[B], wa, std::false_type{});
+    };
+    for (; step + 1 < mine; step += 2) {
+      full(step, Stage<0>{}, sa, sb);
+      full(step + 1, Stage<1>{}, sb, sa);
     }
-    ++step;
+    if (step < mine) {
+      full(step, Stage<0>{}, sa, sb);
+      sa = sb;
+      ++step;
+    }
+    if (mine >= 0) {
+      arrive(step, step & 1);
+      mask(step * KT, sa);
+      if (raise(sa, f)) scale_output(f);
+      weights(sa, wa);
+      all_values(v_lds[step & 1], wa, std::false_type{});
+      ++step;
+    }
+  } else {
+    // Block b: weights of `s` into `w`, beside the next block's scores (NEXT), the last one's
+    // values, and the copies of a later tile of keys and of values (COPY), which would hold
+    // the wavefront up for about 100 cycles each if they were issued one after the other.
+    const char *k_from = nullptr, *v_from = nullptr;
+    const auto block = [&](int b, const unsigned char* kl, const unsigned char* vl, f32x16_t& s, f32x16_t& next,
+                           const uint32_t (&before)[P::PREGS], uint32_t (&w)[P::PREGS], auto has_next, auto copy,
+                           uint32_t copy_to) __attribute__((always_inline)) {
+      constexpr bool NEXT = decltype(has_next)::value;
+      constexpr int COPY = decltype(copy)::value;  // 0: none, 1: keys, 2: values
+      // Operands are read LEAD steps ahead, the first before the maximum.
+      constexpr int LEAD = 2, KSTEPS = NEXT ? NF : 0, SLOTS = KSTEPS + VSTEPS, EACH = (16 + SLOTS - 1) / SLOTS;
+      constexpr int LONG = KSTEPS > VSTEPS ? KSTEPS : VSTEPS;
+      uint4 kx[NF], vx[VSTEPS];
+      static_for<0, LEAD>([&](auto i) {
+        constexpr int n = decltype(i)::value;
+        if constexpr (n < KSTEPS) kx[n] = key_operand(kl, i);
+        if constexpr (n < VSTEPS) vx[n] = value_operand(vl, i);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+      if (COPY == 0 && b >= 2 * mine) mask(32 * b, s);
+      const bool raised = raise(s, f);
+      // Each product is followed by its share of the weights, in this order.
+      const auto share = [&](auto slot) __attribute__((always_inline)) {
+        constexpr int n = decltype(slot)::value;
+#pragma unroll
+        for (int r = n * EACH; r < (n + 1) * EACH && r < 16; ++r) {
+          weight(s, r);
+          if (r >= 3 && r % 2 == 1) pack_pair(s, r / 2 - 1, w);
+        }
+        if constexpr (COPY != 0) {
+          constexpr int GAP = SLOTS / P::COPIES;
+          if constexpr (n % GAP == 0 && n / GAP < P::COPIES) {
+            if constexpr (COPY == 1) P::template copy_piece<true, n / GAP>(a, k_from, a.k_st, copy_to);
+            else P::template copy_piece<false, n / GAP>(a, v_from, a.v_st, copy_to);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<0, LONG>([&](auto i) {
+        constexpr int n = decltype(i)::value;
+        if constexpr (n + LEAD < KSTEPS) kx[n + LEAD] = key_operand(kl, Stage<n + LEAD>{});
+        if constexpr (n < KSTEPS) {
+          score(kx[n], i, next);
+          share(Stage<n + (n < VSTEPS ? n : VSTEPS)>{});
+        }
+        if constexpr (n + LEAD < VSTEPS) vx[n + LEAD] = value_operand(vl, Stage<n + LEAD>{});
+        if constexpr (n < VSTEPS) {
+          value(vx[n], i, before, std::false_type{});
+          share(Stage<n + (n + 1 < KSTEPS ? n + 1 : KSTEPS)>{});
+        }
+      });
+      pack_pair(s, 7, w);
+      // Made here, not where they are first used, behind the branch below.
+      asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]), "+v"(w[4]), "+v"(w[5]), "+v"(w[6]), "+v"(w[7]), "+v"(l));
+      __builtin_amdgcn_sched_barrier(0);
+      if (raised) scale_output(f);
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    // In the middle of a long prompt: two whole tiles to copy, and nothing to mask.
+    const int middle = VEC && a.D == DP ? min(min(mine - 1, steps - 2), n / KT - 2) : 0;  // steps below it
+    const auto full = [&](int step, auto buf) __attribute__((always_inline)) {
+      constexpr int B = decltype(buf)::value;
+      wait_and_barrier<0>();
+      k_from = (const char*)(kh + (int64_t)(step + 2) * KT * a.k_st);
+      v_from = (const char*)(vh + (int64_t)(step + 1) * KT * a.v_st);
+      block(2 * step + 1, k_lds[B ^ 1], v_lds[B], sa, sb, wa, wb, yes, Stage<2>{}, lds_addr(v_lds[B ^ 1]));
+      block(2 * step + 2, k_lds[B ^ 1] + 32 * ROWB, v_lds[B] + 32 * ROWB, sb, sa, wb, wa, yes, Stage<1>{}, lds_addr(k_lds[B]));
+    };
+    // Block 0: its weights beside block 1's scores.
+    all_scores(k_lds[0], sb);
+    all_scores(k_lds[0] + 32 * ROWB, sa);
+    if (mine == 0) mask(0, sb);
+    raise(sb, f);
+    weights(sb, wa);
+    for (; step + 1 < middle; step += 2) {
+      full(step, Stage<0>{});
+      full(step + 1, Stage<1>{});
+    }
+#pragma unroll 1
+    for (; step < mine; ++step) {
+      const int buf = step & 1;
+      arrive(step, buf);
+      const unsigned char *kl = k_lds[buf ^ 1], *vl = v_lds[buf];
+      block(2 * step + 1, kl, vl, sa, sb, wa, wb, yes, Stage<0>{}, 0);
+      block(2 * step + 2, kl + 32 * ROWB, vl + 32 * ROWB, sb, sa, wb, wa, yes, Stage<0>{}, 0);
+    }
+    if (mine >= 0) {
+      arrive(step, step & 1);
+      if (64 * step + 32 <= last) {
+        block(2 * step + 1, nullptr, v_lds[step & 1], sa, sb, wa, wb, no, Stage<0>{}, 0);
+        all_values(v_lds[step & 1] + 32 * ROWB, wb, no);
+      } else {  // the tile's second half lies behind this wavefront's rows
+        all_values(v_lds[step & 1], wa, no);
+      }
+      ++step;
+    }
   }
   for (; step < steps; ++step) arrive(step, step & 1);
 
@@ -514,13 +602,13 @@ prompt_attention_kernel(const PromptArgs a) {
       issue_values(step, 0);
       wait_and_barrier<0>();
       if (step > mine) continue;
-      scores(k_lds[0], sa);
-      mask(step, sa);
-      rescale(sa);
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
-        weights(sa[kb], w[kb]);
-        add_values(v_lds[0] + kb * 32 * ROWB, w[kb], std::true_type{});
+        all_scores(k_lds[0] + kb * 32 * ROWB, sa);
+        mask(step * KT + 32 * kb, sa);
+        if (raise(sa, f)) scale_output(f);
+        weights(sa, wa);
+        all_values(v_lds[0] + kb * 32 * ROWB, wa, std::true_type{});
       }
 #pragma unroll 1
       for (int key = 0; key < KT; ++key) {
@@ -539,30 +627,43 @@ prompt_attention_kernel(const PromptArgs a) {
           }
       }
     }
+    __syncthreads();  // the output goes through these tiles
   }
 
-  // ---- out: registers 4 j .. 4 j + 3 of block i are dims 32 i + 8 j + 4 kg ..
-  if (pos >= n) return;
+  // ---- out: registers 4 j .. 4 j + 3 of block i are dims 32 i + 8 j + 4 kg .. of row `pos`
   const float total = l + __shfl_xor(l, 32, 64), inv = total == 0.f ? 0.f : 1.f / total;
-  T* row = (T*)a.out + (int64_t)(start + pos) * a.o_st + (int64_t)h * a.o_sh;
+  if constexpr (VEC) {
+    // Through LDS, which no wavefront reads any more: whole rows leave in 16-byte pieces
+    // (straight from the registers, 8-byte pieces of 32 rows a store, it took four times as long).
+    unsigned char* mine_lds = &k_lds[0][0] + wave * (32 * ROWB);  // k_lds and v_lds hold 128 rows and more
 #pragma unroll
-  for (int i = 0; i < NDB; ++i)
+    for (int i = 0; i < NDB; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = 32 * i + 8 * j + 4 * kg;
-      float x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = o[i][4 * j + e] * inv;
-      if constexpr (VEC) {
-        if (d >= a.D) continue;
-        if constexpr (P::F32) *(float4*)(row + d) = make_float4(x[0], x[1], x[2], x[3]);
-        else *(uint2*)(row + d) = make_uint2(M::pack2(x[0], x[1]), M::pack2(x[2], x[3]));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d + e < a.D) Elem<T>::store(row + (d + e) * a.o_sd, x[e]);
+      for (int j = 0; j < 4; ++j) {
+        const float x0 = o[i][4 * j] * inv, x1 = o[i][4 * j + 1] * inv, x2 = o[i][4 * j + 2] * inv, x3 = o[i][4 * j + 3] * inv;
+        const int d = 32 * i + 8 * j + 4 * kg;
+        unsigned char* at = mine_lds + col * ROWB + P::k_place(col, d / P::EPC) * 16 + d % P::EPC * P::EB;
+        if constexpr (P::F32) *(float4*)at = make_float4(x0, x1, x2, x3);
+        else *(uint2*)at = make_uint2(M::pack2(x0, x1), M::pack2(x2, x3));
       }
+    __builtin_amdgcn_wave_barrier();
+    T* out = (T*)a.out + (int64_t)(start + first) * a.o_st + (int64_t)h * a.o_sh;
+#pragma unroll
+    for (int i = 0; i < 32 * P::CPR / 64; ++i) {
+      const int at = i * 64 + lane, row = at / P::CPR, c = at % P::CPR;
+      const uint4 x = *(const uint4*)(mine_lds + row * ROWB + P::k_place(row, c) * 16);
+      if (first + row < n && c * P::EPC < a.D) *(uint4*)(out + (int64_t)row * a.o_st + c * P::EPC) = x;
     }
+  } else if (pos < n) {
+    T* row = (T*)a.out + (int64_t)(start + pos) * a.o_st + (int64_t)h * a.o_sh;
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int d = 32 * i + 8 * (j / 4) + 4 * kg + j % 4;
+        if (d < a.D) Elem<T>::store(row + d * a.o_sd, o[i][j] * inv);
+      }
+  }
 }
 
 template <typename T, int DP>
