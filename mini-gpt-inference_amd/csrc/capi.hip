@@ -922,9 +922,8 @@ Fp4Plan fp4_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_
     p.waves = (int)waves;
     return p;
   }
-  int64_t most = 16 * (int64_t)device_cus();
-  waves = 4;
-  while (waves < most && waves < pairs * tiles) waves *= 2;
+  // As many wavefronts as a CU may hold (fewer where registers say so, which the launcher knows).
+  waves = std::min(16 * (int64_t)device_cus(), round_up(pairs * tiles, 4));
   p.waves = (int)waves;
   p.ml_offset = round_up(2 * waves * rows * dims * 4, kWorkspaceAlign);
   p.cum_offset = round_up(p.ml_offset + 2 * waves * 16 * 8, kWorkspaceAlign);
@@ -1583,7 +1582,7 @@ int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, const void* q, c
   magic_of(S, &a.s_mul, &a.s_shift);
   a.one_launch = p.one_launch;
   a.waves = p.waves;
-  while ((1 << a.waves_log2) < a.waves) ++a.waves_log2;
+  a.cus = device_cus();
   if (!p.one_launch) {
     if (!workspace) return fail(MGI_EWORKSPACE, "workspace required for the split pass");
     if (workspace_bytes < p.total)

@@ -78,8 +78,8 @@ struct Fp4DecodeArgs {
   uint32_t s_mul;          // division by S (magic_of)
   int s_shift;
   int one_launch;          // a workgroup of `waves` wavefronts per (sequence, KV head)
-  int waves;               // otherwise: wavefronts of the whole launch, a power of two
-  int waves_log2;
+  int waves;               // otherwise: wavefronts of the whole launch, at most, a multiple of 4
+  int cus;
   float* ws_acc;           // [2 * waves][min(G, 16)][groups * 32]
   float2* ws_ml;           // [2 * waves][16]  (max, sum), log2 domain
   int* ws_cum;             // [B + 1] exclusive prefix sums of tiles per sequence

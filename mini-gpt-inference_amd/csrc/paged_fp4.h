@@ -31,6 +31,7 @@ namespace mgi {
 namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -67,6 +68,13 @@ __device__ __forceinline__ int64_t unhoisted(int64_t x) {
   return x;
 }
 
+// Wavefronts per SIMD that the accumulators and queries leave registers for (none spills).
+template <typename T, int NG>
+constexpr int occupancy() {
+  constexpr int held = NG * (2 + Terms<T>::q);
+  return NG <= 2 ? 4 : held <= 12 ? 3 : 2;
+}
+
 template <int I> using Int = std::integral_constant<int, I>;
 template <int B, int E, typename F>
 __device__ __forceinline__ void each(F&& f) {
@@ -77,8 +85,8 @@ __device__ __forceinline__ void each(F&& f) {
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const bf16x2_t v = {(__bf16)lo, (__bf16)hi};
-  return __builtin_bit_cast(uint32_t, v);
+  const f32x2_t x = {lo, hi};  // converted as a vector: one instruction (three, element by element)
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
 }
 __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
@@ -109,17 +117,24 @@ struct Attend {
   using P = Pieces<NG>;
   static constexpr int NQ = Terms<T>::q, NP = Terms<T>::p;
 
-  // The codes and scales of 32 tokens: 16 + 16 rows of keys, 8 tokens' values.
-  struct Tile {
-    uint32_t k[2][NG];          // words of the lane's 16-token row, piece by piece
-    uint32_t ks[2][P::count];   // its group's byte
-    uint32_t v[8][P::count];    // the lane's dims of its tokens 0..3 and 16..19 (+ 4 (l / 16))
-    uint32_t vs[2][P::count];   // four tokens' bytes
+  // Where 32 tokens are: the slabs and offsets of each 16 (ANY: of token l % 16 of them).
+  struct Place {
+    const unsigned char* slab[2];
+    uint32_t off[2];
     uint32_t valid;             // bit t: token t is in the context and its block is in the pool
+  };
+  // Their codes and scales: 16 + 16 rows of keys, 8 tokens' values.
+  struct Keys {
+    uint32_t w[2][NG];          // words of the lane's 16-token row, piece by piece
+    uint32_t s[2][P::count];    // its group's byte
+  };
+  struct Values {
+    uint32_t w[8][P::count];    // the lane's dims of its tokens 0..3 and 16..19 (+ 4 (l / 16))
+    uint32_t s[2][P::count];    // four tokens' bytes
   };
 
   const Fp4DecodeArgs& a;
-  const int lane, c, kg;        // c: query, key row, or dims of V^T; kg: which of the four lanes
+  int lane, c, kg;              // c: query, key row, or dims of V^T; kg: which of the four lanes
   const unsigned char* head;    // the pool at this KV head
   const char* table;            // the sequence's row of the block table
   int ctx;
@@ -129,7 +144,7 @@ struct Attend {
   int entries, entries_at;      // block ids of 64 subtiles from subtile `entries_at` on, one per lane
 
   __device__ __forceinline__ Attend(const Fp4DecodeArgs& args)
-      : a(args), lane((int)(threadIdx.x & 63)), c(lane & 15), kg(lane >> 4) {}
+      : a(args) {}
 
   __device__ __forceinline__ int64_t entry(int blk) const {
     const int64_t e = load_index(table, a.bt_i64, (int64_t)blk * a.bt_sm);
@@ -138,6 +153,10 @@ struct Attend {
 
   // Queries of heads hq0 .. hq0 + 15 (fewer at the end of the group), as bf16 terms.
   __device__ __forceinline__ void begin(int b, int hk, int qt, int context) {
+    // Defined anew, so that addresses made of them are not kept over the loop over pairs.
+    lane = (int)(threadIdx.x & 63);
+    asm volatile("" : "+v"(lane));
+    c = lane & 15, kg = lane >> 4;
     ctx = context;
     head = a.pool + hk * a.p_sh;
     table = (const char*)a.bt + ((int64_t)b * a.bt_sb) * (a.bt_i64 ? 8 : 4);
@@ -218,95 +237,111 @@ struct Attend {
     }
   }
 
-  // Codes and scales of tokens 32 * tile ..; every address is inside the pool.
-  __device__ __forceinline__ void load(Tile& t, int tile) {
-    const uint32_t S = a.S;
-    const uint32_t vc = fp4_v_codes(S, NG), ks = fp4_k_scales(S, NG), vs = fp4_v_scales(S, NG);
+  // Tokens 32 * tile .. + 31. A token past the context, or in a block outside the pool, is given
+  // a place in block 0, so that every address is inside the pool.
+  __device__ __forceinline__ Place find(int tile) {
+    Place t;
+    const int S = a.S;
     t.valid = 0;
-    if constexpr (!ANY) {  // S is a multiple of 16: 16 tokens lie in one block
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2; ++j) {
+      if constexpr (!ANY) {  // S is a multiple of 16: 16 tokens lie in one block
         const int sub = 2 * tile + j, tok = sub * 16;
         if (sub - entries_at >= 64) {
           entries_at = sub;
           const int mine = (sub + lane) * 16;
-          entries = mine < ctx ? (int)entry(fast_div(mine, a.s_mul, a.s_shift, (int)S)) : -1;
+          entries = mine < ctx ? (int)entry(fast_div(mine, a.s_mul, a.s_shift, S)) : -1;
         }
         const int phys = __builtin_amdgcn_readlane(entries, sub - entries_at);
-        const int blk = fast_div(tok, a.s_mul, a.s_shift, (int)S);
-        const uint32_t off = (uint32_t)__builtin_amdgcn_readfirstlane(tok - blk * (int)S);
+        const int blk = fast_div(tok, a.s_mul, a.s_shift, S);
+        t.off[j] = (uint32_t)__builtin_amdgcn_readfirstlane(tok - blk * S);
         const int left = phys < 0 ? 0 : min(16, ctx - tok);
         t.valid |= (left <= 0 ? 0u : 0xffffu >> (16 - left)) << (16 * j);
-        const unsigned char* slab = head + (int64_t)(phys < 0 ? 0 : phys) * a.p_sn;
-        each<0, P::count>([&](auto pc) {
-          constexpr int s = P::size(pc), g0 = P::start(pc);
-          const unsigned char* kb = slab + off * (NG * 16) + g0 * 16;
-          load_k<pc>(&t.k[j][g0], kb + (uint32_t)(c * (NG * 16) + kg * (s * 4)));
-          t.ks[j][pc] = __builtin_nontemporal_load(slab + ks + off * NG + g0 + (uint32_t)(c * NG + kg * s / 4));
-          const unsigned char* vb = slab + vc + off * (NG * 16) + g0 * 16;
-          each<0, 4>([&](auto i) {
-            t.v[4 * j + i][pc] = load_v<pc>(vb + i * (NG * 16) + (uint32_t)(kg * 4 * (NG * 16) + c * s));
-          });
-          t.vs[j][pc] = load32(slab + vs + g0 * S + off + (uint32_t)(c * s / 16 * S + kg * 4));
-        });
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
+        t.slab[j] = head + (int64_t)(phys < 0 ? 0 : phys) * a.p_sn;
+      } else {
         const int tok = 32 * tile + 16 * j + c;
-        const int blk = fast_div(tok, a.s_mul, a.s_shift, (int)S);
+        const int blk = fast_div(tok, a.s_mul, a.s_shift, S);
         const int64_t phys = tok < ctx ? entry(blk) : -1;
-        const uint32_t off = phys < 0 ? 0u : (uint32_t)(tok - blk * (int)S);
+        t.off[j] = phys < 0 ? 0u : (uint32_t)(tok - blk * S);
         t.valid |= (uint32_t)(__ballot(phys >= 0) & 0xffffu) << (16 * j);
-        const unsigned char* slab = head + (phys < 0 ? 0 : phys) * a.p_sn;
-        const uint64_t base = (uint64_t)slab;
+        t.slab[j] = head + (phys < 0 ? 0 : phys) * a.p_sn;
+      }
+    }
+    return t;
+  }
+
+  __device__ __forceinline__ void load(Keys& k, const Place& t) {
+    const uint32_t ks = fp4_k_scales(a.S, NG);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      each<0, P::count>([&](auto pc) {
+        constexpr int s = P::size(pc), g0 = P::start(pc);
+        const int row = ANY ? 0 : c;  // behind the place
+        load_k<pc>(&k.w[j][g0], t.slab[j] + t.off[j] * (NG * 16) + g0 * 16 + (uint32_t)(row * (NG * 16) + kg * (s * 4)));
+        k.s[j][pc] = __builtin_nontemporal_load(t.slab[j] + ks + t.off[j] * NG + g0 + (uint32_t)(row * NG + kg * s / 4));
+      });
+  }
+
+  __device__ __forceinline__ void load(Values& v, const Place& t) {
+    const uint32_t S = a.S, vc = fp4_v_codes(S, NG), vs = fp4_v_scales(S, NG);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if constexpr (!ANY) {
         each<0, P::count>([&](auto pc) {
           constexpr int s = P::size(pc), g0 = P::start(pc);
-          load_k<pc>(&t.k[j][g0], slab + off * (NG * 16) + g0 * 16 + (uint32_t)(kg * (s * 4)));
-          t.ks[j][pc] = slab[ks + off * NG + g0 + kg * s / 4];
-          t.vs[j][pc] = 0;
+          const unsigned char* vb = t.slab[j] + vc + t.off[j] * (NG * 16) + g0 * 16;
+          each<0, 4>([&](auto i) {
+            v.w[4 * j + i][pc] = load_v<pc>(vb + i * (NG * 16) + (uint32_t)(kg * 4 * (NG * 16) + c * s));
+          });
+          v.s[j][pc] = load32(t.slab[j] + vs + g0 * S + t.off[j] + (uint32_t)(c * s / 16 * S + kg * 4));
         });
+      } else {
+        const uint64_t base = (uint64_t)t.slab[j];
+        each<0, P::count>([&](auto pc) { v.s[j][pc] = 0; });
         each<0, 4>([&](auto i) {  // lane t (< 16) knows token t's place
           const int from = kg * 4 + i;
-          const unsigned char* vslab = (const unsigned char*)(((uint64_t)(uint32_t)__shfl((int)(base >> 32), from, 64) << 32) |
-                                                              (uint32_t)__shfl((int)base, from, 64));
-          const uint32_t voff = (uint32_t)__shfl((int)off, from, 64);
+          const unsigned char* slab = (const unsigned char*)(((uint64_t)(uint32_t)__shfl((int)(base >> 32), from, 64) << 32) |
+                                                             (uint32_t)__shfl((int)base, from, 64));
+          const uint32_t off = (uint32_t)__shfl((int)t.off[j], from, 64);
           each<0, P::count>([&](auto pc) {
             constexpr int s = P::size(pc), g0 = P::start(pc);
-            t.v[4 * j + i][pc] = load_v<pc>(vslab + vc + voff * (NG * 16) + g0 * 16 + (uint32_t)(c * s));
-            t.vs[j][pc] |= (uint32_t)vslab[vs + (g0 + c * s / 16) * S + voff] << (8 * i);
+            v.w[4 * j + i][pc] = load_v<pc>(slab + vc + off * (NG * 16) + g0 * 16 + (uint32_t)(c * s));
+            v.s[j][pc] |= (uint32_t)slab[vs + (g0 + c * s / 16) * S + off] << (8 * i);
           });
         });
       }
     }
   }
 
-  __device__ __forceinline__ void add(Tile& t) {
-    // Scores: rows 4 kg .. + 3 of each 16 tokens, column c.
-    float s[8];
+  // Scores: rows 4 kg .. + 3 of each 16 tokens, column c.
+  __device__ __forceinline__ void scores(const Keys& k, float (&s)[8]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       f32x4_t r = {0.f, 0.f, 0.f, 0.f};
       each<0, P::count>([&](auto pc) {
         constexpr int sz = P::size(pc), g0 = P::start(pc);
-        const float scale = __uint_as_float(t.ks[j][pc] << 23);
+        const float scale = __uint_as_float(k.s[j][pc] << 23);
         each<0, sz>([&](auto i) {
-          const uint32_t w = t.k[j][g0 + i];
-          const u32x4_t k = {two_bf16<0>(w, scale), two_bf16<1>(w, scale), two_bf16<2>(w, scale), two_bf16<3>(w, scale)};
-          each<0, NQ>([&](auto n) { r = mfma(k, q[n][g0 + i], r); });
+          const uint32_t w = k.w[j][g0 + i];
+          const u32x4_t x = {two_bf16<0>(w, scale), two_bf16<1>(w, scale), two_bf16<2>(w, scale), two_bf16<3>(w, scale)};
+          each<0, NQ>([&](auto n) { r = mfma(x, q[n][g0 + i], r); });
         });
       });
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * j + i] = r[i];
     }
-    if (t.valid != 0xffffffffu) {  // the end of the context, or a block outside the pool
+  }
+
+  // Softmax weights of the scores, as bf16 terms; masked tokens' values are made finite.
+  __device__ __forceinline__ void weights(float (&s)[8], uint32_t valid, Values& v, u32x4_t (&w)[NP]) {
+    if (valid != 0xffffffffu) {  // the end of the context, or a block outside the pool
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const bool in = (t.valid >> (16 * (i / 4) + kg * 4 + i % 4)) & 1;
+        const bool in = (valid >> (16 * (i / 4) + kg * 4 + i % 4)) & 1;
         s[i] = in ? s[i] : -INFINITY;
         // What stands in a masked place has weight 0, and must not be NaN.
         each<0, P::count>([&](auto pc) {
-          if (!in) t.vs[i / 4][pc] = (t.vs[i / 4][pc] & ~(0xffu << (8 * (i % 4)))) | (127u << (8 * (i % 4)));
+          if (!in) v.s[i / 4][pc] = (v.s[i / 4][pc] & ~(0xffu << (8 * (i % 4)))) | (127u << (8 * (i % 4)));
         });
       }
     }
@@ -319,29 +354,30 @@ struct Attend {
 #pragma unroll
       for (int j = 0; j < 2 * NG; ++j) acc[j] *= f;
     }
-    float p[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = fast_exp2(__builtin_fmaf(s[i], a.scale_log2, -m));
-    l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-    u32x4_t w[NP];
+    for (int i = 0; i < 8; ++i) s[i] = fast_exp2(__builtin_fmaf(s[i], a.scale_log2, -m));
+    l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     each<0, NP>([&](auto n) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        w[n][e] = pack_bf16(p[2 * e], p[2 * e + 1]);
-        p[2 * e] -= bf16_lo(w[n][e]);
-        p[2 * e + 1] -= bf16_hi(w[n][e]);
+        w[n][e] = pack_bf16(s[2 * e], s[2 * e + 1]);
+        s[2 * e] -= bf16_lo(w[n][e]);
+        s[2 * e + 1] -= bf16_hi(w[n][e]);
       }
     });
+  }
+
+  __device__ __forceinline__ void add(const Values& v, const u32x4_t (&w)[NP]) {
     each<0, P::count>([&](auto pc) {
       constexpr int sz = P::size(pc), g0 = P::start(pc);
       float scale[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) scale[i] = __uint_as_float(((t.vs[i / 4][pc] >> (8 * (i % 4))) & 0xffu) << 23);
+      for (int i = 0; i < 8; ++i) scale[i] = __uint_as_float(((v.s[i / 4][pc] >> (8 * (i % 4))) & 0xffu) << 23);
       each<0, sz>([&](auto b) {  // byte b: dims 2 b and 2 b + 1 of the lane's
         u32x4_t even, odd;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t x = two_bf16<b>(t.v[2 * e][pc], scale[2 * e]), y = two_bf16<b>(t.v[2 * e + 1][pc], scale[2 * e + 1]);
+          const uint32_t x = two_bf16<b>(v.w[2 * e][pc], scale[2 * e]), y = two_bf16<b>(v.w[2 * e + 1][pc], scale[2 * e + 1]);
           even[e] = __builtin_amdgcn_perm(y, x, 0x05040100u);
           odd[e] = __builtin_amdgcn_perm(y, x, 0x07060302u);
         }
@@ -353,15 +389,29 @@ struct Attend {
     });
   }
 
-  // Tiles first, first + step, .. below end.
+  // Tiles first, first + step, .. below end. A tile's keys are asked for when the last one's have
+  // been multiplied, its values when the last one's have been: one set of registers of each,
+  // and four wavefronts to a SIMD, whose loads are in flight while others compute.
   __device__ __forceinline__ void run(int first, int end, int step) {
     if (first >= end) return;
-    Tile cur, next;
-    load(cur, first);
+    Keys k;
+    Values v;
+    Place t = find(first);
+    load(k, t);
+    load(v, t);
     for (int tile = first; tile < end; tile += step) {
-      if (tile + step < end) load(next, tile + step);
-      add(cur);
-      cur = next;
+      const uint32_t valid = t.valid;
+      float s[8];
+      scores(k, s);
+      const bool more = tile + step < end;
+      if (more) {
+        t = find(tile + step);
+        load(k, t);
+      }
+      u32x4_t w[NP];
+      weights(s, valid, v, w);
+      add(v, w);
+      if (more) load(v, t);
     }
   }
 
@@ -455,18 +505,23 @@ __global__ void __launch_bounds__(512) paged_fp4_one(const Fp4DecodeArgs a) {
   }
 }
 
-// Tiles of all (sequence, KV head, query tile), in that order, cut into equal runs, one per
-// wavefront. A (sequence, head) inside one run is finished by it; the others leave
-// (maximum, sum, unnormalised output) for paged_fp4_join: slot 2 w for a run's beginning
-// inside a (sequence, head), 2 w + 1 for its end. Where there are fewer tiles than
-// wavefronts, so many take part (a power of two) that none is without a tile.
-__device__ __forceinline__ int runs_log2(int64_t total, const Fp4DecodeArgs& a) {
-  const int most = total < 1 ? 0 : 63 - __clzll(total);
-  return min(most, a.waves_log2);
-}
+// Tiles of all (sequence, KV head, query tile), in that order, cut into runs that differ by
+// one tile at most, one per wavefront: as many as are resident at once. A (sequence, head)
+// inside one run is finished by it; the others leave (maximum, sum, unnormalised output) for
+// paged_fp4_join: slot 2 w for a run's beginning inside a (sequence, head), 2 w + 1 for its
+// end. Where there are fewer tiles than wavefronts the last ones have none.
+struct Runs {
+  int64_t size, longer;  // tiles of a run; so many first runs have one more
+  __device__ __forceinline__ Runs(int64_t total, int waves) : size(total / waves), longer(total - size * waves) {}
+  __device__ __forceinline__ int64_t start(int w) const { return size * w + (w < longer ? w : longer); }
+  __device__ __forceinline__ int of(int64_t pos) const {  // the run with tile pos
+    const int64_t at = longer * (size + 1);
+    return (int)(pos < at ? pos / (size + 1) : longer + (pos - at) / size);
+  }
+};
 
 template <typename T, int NG, bool ANY>
-__global__ void __launch_bounds__(256, 2) paged_fp4_split(const Fp4DecodeArgs a) {
+__global__ void __launch_bounds__(256, (occupancy<T, NG>())) paged_fp4_split(const Fp4DecodeArgs a) {
   const int wave = (int)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
   const int lane = (int)(threadIdx.x & 63), heads = a.Hk * a.q_tiles;
   // All tiles of one head, and from them this wavefront's run.
@@ -476,10 +531,10 @@ __global__ void __launch_bounds__(256, 2) paged_fp4_split(const Fp4DecodeArgs a)
   for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
   const int tiles = __builtin_amdgcn_readfirstlane(sum);
   const int64_t total = (int64_t)tiles * heads;
-  const int runs = runs_log2(total, a);
-  const int64_t start = (total * wave) >> runs;
-  int64_t left = ((total * (wave + 1)) >> runs) - start;
-  if (wave >= 1 << runs) return;
+  const Runs runs(total, a.waves);
+  const int64_t start = runs.start(wave);
+  int64_t left = runs.start(wave + 1) - start;
+  if (left <= 0 && wave != 0) return;
   // The sequence the run starts in: the first whose tiles, with those before it, pass start / heads.
   const int want = (int)(start / heads);
   int b = -1, b_before = 0, before = 0;
@@ -553,9 +608,8 @@ __global__ void __launch_bounds__(64) paged_fp4_join(const Fp4DecodeArgs a, int 
     return;
   }
   const int64_t p0 = (int64_t)at * heads + (int64_t)r * n, p1 = p0 + n;
-  // The run with position p: the last that starts at or before it.
-  const int runs = runs_log2(total, a);
-  const int w0 = (int)((((p0 + 1) << runs) - 1) / total), w1 = (int)(((p1 << runs) - 1) / total);
+  const Runs runs(total, a.waves);
+  const int w0 = runs.of(p0), w1 = runs.of(p1 - 1);
   if (w0 == w1) return;
   const int rows = min(a.G, 16);
   const auto slot_of = [&](int w) { return 2 * (int64_t)w + (w == w0); };
@@ -584,6 +638,7 @@ hipError_t launch_ng(Fp4DecodeArgs a, hipStream_t stream) {
     return hipLaunchKernel(reinterpret_cast<const void*>(&paged_fp4_one<T, NG, ANY>),
                            dim3((unsigned)(a.B * a.Hk * a.q_tiles)), dim3(a.waves * 64), args, lds, stream);
   }
+  if (a.waves > 4 * occupancy<T, NG>() * a.cus) a.waves = 4 * occupancy<T, NG>() * a.cus;
   hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&paged_fp4_split<T, NG, ANY>),
                                  dim3((unsigned)(a.waves / 4)), dim3(256), args, 0, stream);
   if (e != hipSuccess) return e;

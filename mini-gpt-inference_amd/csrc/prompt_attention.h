@@ -102,12 +102,13 @@ __device__ __forceinline__ int wave_reduce(int x, Op op) {
 struct Span {
   int start, rows;
 };
+__device__ __forceinline__ int64_t clamped(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 __device__ __forceinline__ Span span_of(const PromptArgs& a, int b) {
-  if (b >= a.B) return Span{0, 0};
-  const int64_t s = load_index(a.starts, a.cu_i64, (int64_t)b * a.cu_s);
-  const int64_t e = load_index(a.starts, a.cu_i64, (int64_t)(b + 1) * a.cu_s);
-  const int64_t lo = s < 0 ? 0 : s > a.T ? a.T : s, hi = e < lo ? lo : e > a.T ? a.T : e;
-  return Span{(int)lo, (int)(hi - lo)};
+  Index s, e;  // both loads before either's use
+  s.load(a.starts, a.cu_i64, (uint64_t)min(b, a.B) * (uint64_t)a.cu_s);
+  e.load(a.starts, a.cu_i64, (uint64_t)min(b + 1, a.B) * (uint64_t)a.cu_s);
+  const int lo = (int)clamped(s.value(a.cu_i64), 0, a.T), hi = (int)clamped(e.value(a.cu_i64), lo, a.T);
+  return Span{lo, hi - lo};
 }
 
 // The `rank`-th tile (of `rows` positions) in falling order of its index in its sequence:
