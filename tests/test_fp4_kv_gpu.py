@@ -89,6 +89,30 @@ def test_append_is_the_pools_own_write(T, H, D, S, itype, strided, dtype):
         assert (x[N * S:] == 0).all()
 
 
+@DTYPES
+def test_ties_borders_and_extremes(dtype):
+    """Every border between codes and its neighbours, at scales over the whole range."""
+    y = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, 6.0, 4.0, 3.0, 2.0, 1.5, 1.0, 0.5, 0.0])
+    eps = torch.finfo(dtype).eps
+    rows = []
+    for top in (7.0, 6.0, 4.0, 3.5, 7.0 * (1 - eps), 7.0 * (1 + eps), 3.5 * (1 + eps)):
+        for near in (1 - eps, 1.0, 1 + eps):
+            group = (y * near).clamp(max=top)
+            group[0] = top
+            rows.append(torch.cat((group, -group)))
+    rows = torch.stack(rows)  # [21, 32]
+    lo, hi = (-20, 12) if dtype == F16 else (-126, 124)
+    x = torch.cat([rows * 2.0 ** e for e in (lo, lo + 1, lo + 9, -3, 0, 5, hi)]).to(dtype)[:, None]  # [T, 1, 32]
+    x = torch.cat((x, torch.full_like(x[:1], 2.0 ** -149 if dtype == F32 else torch.finfo(dtype).tiny), torch.zeros_like(x[:1])))
+    T = len(x)
+    host = cpu_pool(1, T, 1, 1, 32)
+    pool = gpu_pool(host)
+    hpd.kv_append_fp4(pool, 0, x.to(DEV), -x.to(DEV), torch.arange(T, device=DEV))
+    for t in range(T):
+        host.write_layer(0, t, 0, x[t], -x[t])
+    assert torch.equal(pool.data.cpu(), host.data)
+
+
 def test_append_takes_any_strides():
     g = torch.Generator().manual_seed(3)
     T, H, D, S = 13, 3, 48, 16
