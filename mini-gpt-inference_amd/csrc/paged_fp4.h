@@ -68,11 +68,17 @@ __device__ __forceinline__ int64_t unhoisted(int64_t x) {
   return x;
 }
 
-// Wavefronts per SIMD that the accumulators and queries leave registers for (none spills).
+// Wavefronts per SIMD that the registers allow without spilling a vector register: 4 registers
+// per group for each query term and each of two accumulators, and the tile's own.
 template <typename T, int NG>
 constexpr int occupancy() {
   constexpr int held = NG * (2 + Terms<T>::q);
-  return NG <= 2 ? 4 : held <= 12 ? 3 : 2;
+  return held <= 8 ? 4 : held <= 12 ? 3 : held <= 32 ? 2 : 1;
+}
+// Wavefronts of a workgroup of paged_fp4_one.
+template <typename T, int NG>
+constexpr int one_waves() {
+  return occupancy<T, NG>() > 1 ? 8 : 4;
 }
 
 template <int I> using Int = std::integral_constant<int, I>;
@@ -469,7 +475,7 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 // The whole call in one launch: a workgroup per (sequence, KV head, query tile), whose
 // wavefronts take its tiles in turn and meet in LDS.
 template <typename T, int NG, bool ANY>
-__global__ void __launch_bounds__(512) paged_fp4_one(const Fp4DecodeArgs a) {
+__global__ void __launch_bounds__((64 * one_waves<T, NG>())) paged_fp4_one(const Fp4DecodeArgs a) {
   extern __shared__ float lds[];
   const int waves = (int)(blockDim.x >> 6), wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = a.Hk * a.q_tiles, b = (int)blockIdx.x / heads, r = (int)blockIdx.x - b * heads;
@@ -634,6 +640,7 @@ template <typename T, int NG, bool ANY>
 hipError_t launch_ng(Fp4DecodeArgs a, hipStream_t stream) {
   void* args[] = {&a, nullptr};
   if (a.one_launch) {
+    if (a.waves > one_waves<T, NG>()) a.waves = one_waves<T, NG>();
     const size_t lds = (size_t)a.waves * (a.G < 16 ? a.G : 16) * (NG * 32 + 4) * 4;
     return hipLaunchKernel(reinterpret_cast<const void*>(&paged_fp4_one<T, NG, ANY>),
                            dim3((unsigned)(a.B * a.Hk * a.q_tiles)), dim3(a.waves * 64), args, lds, stream);
@@ -656,7 +663,7 @@ hipError_t launch_any(const Fp4DecodeArgs& a, hipStream_t stream) {
 template <typename T>
 hipError_t launch_paged_fp4(const Fp4DecodeArgs& a, hipStream_t stream) {
   switch (fp4_groups(a.D)) {
-        case 1: return launch_any<T, 1>(a, stream);
+    case 1: return launch_any<T, 1>(a, stream);
     case 2: return launch_any<T, 2>(a, stream);
     case 3: return launch_any<T, 3>(a, stream);
     case 4: return launch_any<T, 4>(a, stream);

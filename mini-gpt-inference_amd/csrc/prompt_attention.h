@@ -180,7 +180,8 @@ struct Prompt {
   static_assert(COPIES * 4096 == TILEB, "the workgroup copies whole tiles");
   static constexpr int NF = DP / (2 * EPC);         // steps of the first product: two chunks each
   static constexpr int NKB = KT / 32;
-  static constexpr int RESIDENT = 4 * TILEB > 80 * 1024 ? 1 : 2;  // workgroups of a CU, by their LDS
+  // Workgroups of a CU, by their LDS (and for unaligned f32 rows by registers: two would spill them).
+  static constexpr int RESIDENT = 4 * TILEB > 80 * 1024 || (F32 && !VEC && DP >= 128) ? 1 : 2;
   static constexpr int PREGS = F32 ? 16 : 8;        // registers of a 32-key block's weights
   using M = PM<T>;
 

@@ -238,7 +238,8 @@ def test_attention(Hq, Hk, D, S, route, dtype):
 
 @DTYPES
 @ROUTES
-@pytest.mark.parametrize("Hq,Hk,D,S", [(4, 2, 64, 1), (4, 4, 128, 5), (8, 1, 96, 8), (2, 1, 256, 24), (3, 3, 33, 7)])
+@pytest.mark.parametrize("Hq,Hk,D,S", [(4, 2, 64, 1), (4, 4, 128, 5), (8, 1, 96, 8), (2, 1, 256, 24), (3, 3, 33, 7),
+                                       (5, 5, 224, 6), (18, 1, 160, 12), (4, 2, 192, 20)])
 def test_block_sizes_that_are_no_multiple_of_16(Hq, Hk, D, S, route, dtype):
     lens = [1, 0, 31, 70, 33, 200]
     case = make(len(lens), Hq, Hk, D, S, lens, dtype, seed=S)
