@@ -16,9 +16,15 @@
 // Keys: a lane's codes are 16 consecutive bytes of one token's row, one group. Values: a
 // lane's codes are the dims that are its row of V^T, for its 8 tokens.
 //
+// Measured on MI355X, D = 128, bf16, where a large copy reaches 5.05 TB/s: 64 sequences of 512-4096
+// tokens, 32 heads, 131 us (5.2 TB/s); 8 of 32k-128k, 32 heads on 8, 174 us (5.4 TB/s); 13 of
+// 100-1000, 16 heads, 11 us; 256 of 128-2048, 32 heads of 64 on 8, f16, 56 us (2.6 TB/s: 17
+// tiles a wavefront at most, whose chains of table entry, codes and products nothing hides).
+// Of a large call's wavefront cycles half are waits, 42 % have a vector instruction in work.
+//
 // Numerics: q is cut into bf16 terms that add up to it (1 for bf16, 2 for f16, 3 for f32),
 // so scores are f32 sums of exact products. The softmax weights are cut into 2 terms (3 for
-// f32 outputs), 2^-17 (2^-25) of a weight at most, where one term would cost 2^-9: the
+// f32 outputs), 2^-17 (2^-26) of a weight at most, where one term would cost 2^-8: the
 // matrix cores have the room, as 4-bit keys and values arrive slower than they multiply.
 #pragma once
 
@@ -69,7 +75,9 @@ __device__ __forceinline__ int64_t unhoisted(int64_t x) {
 }
 
 // Wavefronts per SIMD that the registers allow without spilling a vector register: 4 registers
-// per group for each query term and each of two accumulators, and the tile's own.
+// per group for each query term and each of two accumulators, and the tile's own. More
+// wavefronts hide more of the loads: 64 x 512-4096 tokens, 32 heads of 128, bf16 took 150 us at
+// two, 131 at three.
 template <typename T, int NG>
 constexpr int occupancy() {
   constexpr int held = NG * (2 + Terms<T>::q);
@@ -515,10 +523,19 @@ __global__ void __launch_bounds__((64 * one_waves<T, NG>())) paged_fp4_one(const
 // one tile at most, one per wavefront: as many as are resident at once. A (sequence, head)
 // inside one run is finished by it; the others leave (maximum, sum, unnormalised output) for
 // paged_fp4_join: slot 2 w for a run's beginning inside a (sequence, head), 2 w + 1 for its
-// end. Where there are fewer tiles than wavefronts the last ones have none.
+// end. A run has kShortestRun tiles or more (or all), so that little is left to join: with
+// runs of one tile, and a join of one wavefront, 2 sequences of 8k tokens on 2 KV heads took
+// 82 us, with this 18. Runs of 2 tiles or more: 1-3 us less on few rows of 1k-8k, 6 more on one
+// of 32k; of 8: 1-5 more on all of them.
+constexpr int kShortestRun = 4;
 struct Runs {
   int64_t size, longer;  // tiles of a run; so many first runs have one more
-  __device__ __forceinline__ Runs(int64_t total, int waves) : size(total / waves), longer(total - size * waves) {}
+  int count;
+  __device__ __forceinline__ Runs(int64_t total, int waves)
+      : count((int)max((int64_t)1, min((int64_t)waves, total / kShortestRun))) {
+    size = total / count;
+    longer = total - size * count;
+  }
   __device__ __forceinline__ int64_t start(int w) const { return size * w + (w < longer ? w : longer); }
   __device__ __forceinline__ int of(int64_t pos) const {  // the run with tile pos
     const int64_t at = longer * (size + 1);
@@ -539,7 +556,7 @@ __global__ void __launch_bounds__(256, (occupancy<T, NG>())) paged_fp4_split(con
   const int64_t total = (int64_t)tiles * heads;
   const Runs runs(total, a.waves);
   const int64_t start = runs.start(wave);
-  int64_t left = runs.start(wave + 1) - start;
+  int64_t left = wave < runs.count ? runs.start(wave + 1) - start : 0;
   if (left <= 0 && wave != 0) return;
   // The sequence the run starts in: the first whose tiles, with those before it, pass start / heads.
   const int want = (int)(start / heads);
@@ -600,17 +617,22 @@ __global__ void __launch_bounds__(256, (occupancy<T, NG>())) paged_fp4_split(con
   }
 }
 
-// Joins what the runs left of each (sequence, query head), one workgroup of one wavefront
-// each: lane i has dims 4 i .. + 3. Rows without keys come out 0.
+// Joins what the runs left of each (sequence, query head), a workgroup each: a thread has
+// four dims of every parts-th run, kJoinBatch of them asked for at once, and the threads
+// of the same dims meet in LDS. Rows without keys come out 0.
+constexpr int kJoinThreads = 256, kJoinBatch = 4;
 template <typename T>
-__global__ void __launch_bounds__(64) paged_fp4_join(const Fp4DecodeArgs a, int dims) {
-  const int b = (int)blockIdx.y, h = (int)blockIdx.x, lane = (int)threadIdx.x;
+__global__ void __launch_bounds__(kJoinThreads) paged_fp4_join(const Fp4DecodeArgs a, int dims) {
+  __shared__ float4 lds_x[kJoinThreads];
+  __shared__ float lds_sum[kJoinThreads];
+  const int b = (int)blockIdx.y, h = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63;
   const int hk = h / a.G, g = h - hk * a.G, qt = g >> 4, heads = a.Hk * a.q_tiles, r = hk * a.q_tiles + qt;
   const int at = a.ws_cum[b], n = a.ws_cum[b + 1] - at;
   const int64_t total = (int64_t)a.ws_cum[a.B] * heads;
   T* row = out_row<T>(a, b, h);
+  const int quads = dims / 4, parts = kJoinThreads / quads, part = tid / quads, d = (tid - part * quads) * 4;
   if (n == 0) {
-    if (lane * 4 < dims) store4(a, row, lane * 4, 0.f, 0.f, 0.f, 0.f);
+    if (part == 0) store4(a, row, d, 0.f, 0.f, 0.f, 0.f);
     return;
   }
   const int64_t p0 = (int64_t)at * heads + (int64_t)r * n, p1 = p0 + n;
@@ -623,17 +645,36 @@ __global__ void __launch_bounds__(64) paged_fp4_join(const Fp4DecodeArgs a, int 
   for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, a.ws_ml[slot_of(w) * 16 + (g & 15)].x);
   m = wave_max(m);
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int w = w0; w <= w1; ++w) {
-    const float2 ml = a.ws_ml[slot_of(w) * 16 + (g & 15)];
-    const float f = fast_exp2(ml.x - m);
-    sum += f * ml.y;
-    if (lane * 4 < dims) {
-      const float4 y = *(const float4*)(a.ws_acc + (slot_of(w) * rows + (g & 15)) * dims + lane * 4);
-      x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+  if (part < parts) {
+    for (int w = w0 + part; w <= w1; w += kJoinBatch * parts) {
+      float2 ml[kJoinBatch];
+      float4 y[kJoinBatch];
+#pragma unroll
+      for (int i = 0; i < kJoinBatch; ++i) {
+        const int64_t slot = slot_of(min(w + i * parts, w1));
+        ml[i] = a.ws_ml[slot * 16 + (g & 15)];
+        y[i] = *(const float4*)(a.ws_acc + (slot * rows + (g & 15)) * dims + d);
+      }
+#pragma unroll
+      for (int i = 0; i < kJoinBatch; ++i)
+        if (w + i * parts <= w1) {
+          const float f = fast_exp2(ml[i].x - m);
+          sum += f * ml[i].y;
+          x.x += f * y[i].x, x.y += f * y[i].y, x.z += f * y[i].z, x.w += f * y[i].w;
+        }
     }
   }
+  lds_x[tid] = x;
+  lds_sum[tid] = sum;
+  __syncthreads();
+  if (part != 0) return;
+  for (int p = 1; p < parts; ++p) {
+    const float4 y = lds_x[p * quads + tid];
+    sum += lds_sum[p * quads + tid];
+    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+  }
   const float inv = inverse(sum);
-  if (lane * 4 < dims) store4(a, row, lane * 4, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  store4(a, row, d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
 }
 
 template <typename T, int NG, bool ANY>
@@ -651,8 +692,8 @@ hipError_t launch_ng(Fp4DecodeArgs a, hipStream_t stream) {
   if (e != hipSuccess) return e;
   int dims = NG * 32;
   args[1] = &dims;
-  return hipLaunchKernel(reinterpret_cast<const void*>(&paged_fp4_join<T>), dim3(a.Hk * a.G, a.B), dim3(64), args, 0,
-                         stream);
+  return hipLaunchKernel(reinterpret_cast<const void*>(&paged_fp4_join<T>), dim3(a.Hk * a.G, a.B),
+                         dim3(kJoinThreads), args, 0, stream);
 }
 
 template <typename T, int NG>

@@ -246,6 +246,15 @@ def test_block_sizes_that_are_no_multiple_of_16(Hq, Hk, D, S, route, dtype):
     check(hpd.paged_attention_fp4_hip(*case), *case)
 
 
+@DTYPES
+@pytest.mark.parametrize("Hq,Hk,D,S", [(2, 1, 128, 16), (3, 1, 96, 32), (1, 1, 20, 16), (17, 1, 64, 6)])
+def test_few_long_sequences(Hq, Hk, D, S, dtype):
+    """Many runs to join for one head."""
+    lens = [9001, 1, 0, 4100]
+    case = make(len(lens), Hq, Hk, D, S, lens, dtype, seed=D)
+    check(hpd.paged_attention_fp4_hip(*case), *case)
+
+
 @ROUTES
 @pytest.mark.parametrize("S", [16, 6])
 def test_blocks_outside_the_pool_are_masked(S, route):

@@ -82,7 +82,8 @@ LENS = [1, 0, 31, 32, 33, 130, 64, 65, 200]
 
 @DTYPES
 @pytest.mark.parametrize("Hq,Hk,D", [(1, 1, 128), (8, 2, 128), (6, 3, 64), (3, 3, 32), (4, 1, 80), (12, 1, 96), (2, 1, 256),
-                                     (5, 1, 192), (2, 2, 8), (4, 4, 136), (8, 1, 48), (2, 1, 20), (3, 1, 1), (4, 2, 253)])
+                                     (5, 1, 192), (2, 2, 8), (4, 4, 136), (8, 1, 48), (2, 1, 20), (3, 1, 1), (4, 2, 253),
+                                     (2, 1, 125), (4, 1, 70), (2, 2, 90), (1, 1, 190)])
 def test_lengths_heads_dims(Hq, Hk, D, dtype):
     case = make(LENS, Hq, Hk, D, dtype, seed=Hq + D)
     check(hpd.prompt_attention_hip(*case), *case)
