@@ -282,10 +282,25 @@ hipError_t launch_rows(F* kernel, Fp4RowArgs a, hipStream_t stream) {
 
 }  // namespace
 
+// Rows of a launch: what looking through the later rows' slots costs grows with their square, and
+// of two launches the later one's rows are kept by itself. 131072 rows of 8 heads of 128, bf16, slots in
+// random order: 493 us in one launch, 316 by 32768 rows, 372 by 16384 (32768 rows: 68, and 81).
+constexpr int kAppendRows = 32768;
+
 hipError_t launch_fp4_append(const Fp4RowArgs& a, int dtype, hipStream_t stream) {
-  return dtype == MGI_F32    ? launch_rows(&fp4_append_kernel<float>, a, stream)
-         : dtype == MGI_BF16 ? launch_rows(&fp4_append_kernel<bf16_t>, a, stream)
-                             : launch_rows(&fp4_append_kernel<f16_t>, a, stream);
+  for (int t = 0; t < a.T; t += kAppendRows) {
+    const int64_t bytes = dtype == MGI_F32 ? 4 : 2;
+    Fp4RowArgs part = a;
+    part.T = std::min(a.T - t, kAppendRows);
+    part.k = static_cast<char*>(a.k) + t * a.k_st * bytes;
+    part.v = static_cast<char*>(a.v) + t * a.v_st * bytes;
+    part.slots = static_cast<const char*>(a.slots) + t * a.sl_s * (a.sl_i64 ? 8 : 4);
+    const hipError_t e = dtype == MGI_F32    ? launch_rows(&fp4_append_kernel<float>, part, stream)
+                         : dtype == MGI_BF16 ? launch_rows(&fp4_append_kernel<bf16_t>, part, stream)
+                                             : launch_rows(&fp4_append_kernel<f16_t>, part, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_fp4_gather(const Fp4RowArgs& a, int dtype, hipStream_t stream) {
