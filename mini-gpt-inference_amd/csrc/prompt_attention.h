@@ -30,7 +30,9 @@
 // Numerics: f32 sums and softmax (log2 domain). 2-byte types round the weights to their
 // type for the second product, half a step each (bf16 2^-8 of a weight at most, f16 2^-11; the
 // errors are independent), and the sum that divides is that of the rounded weights; f16 weights are scaled by 2^13, so that
-// far keys keep theirs. f32 multiplies in f32.
+// far keys keep theirs. f32 multiplies in f32. The maximum is taken from the scores themselves where
+// they are large, not from their rounded products with the scale: any finite score gives a
+// finite weight (one more test per 32 keys: 0.6-1.1 % of the calls above).
 #pragma once
 
 #include <algorithm>
@@ -104,6 +106,10 @@ __device__ __forceinline__ int wave_reduce(int x, Op op) {
   x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true));  // row 0's last to row 1, 2's to 3
   x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true));  // row 1's last to rows 2 and 3
   return __builtin_amdgcn_readlane(x, 63);
+}
+
+__device__ __forceinline__ float uniform(float x) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
 }
 
 struct Span {
@@ -343,8 +349,16 @@ prompt_attention_kernel(const PromptArgs a) {
   // A wavefront's last tile holds its own positions; all before are seen whole.
   const int mine = first < n ? first / KT : -1;
   f32x16_t o[NDB];
-  float m, neg_m, thr, l;
-  const float cs = a.scale_log2, inv_cs = 1.f / cs;
+  // A score's weight is exp2((s - base) * cs + neg): around the row's maximum m, which is kept in
+  // the scores' own units. Up to kFar the maximum enters through neg, as one rounded product, which
+  // saves the difference; beyond, that product's rounding (2^-24 of it) would pass what a weight's exponent
+  // has room for, and base is the maximum itself, so that its weight is 2^bias whatever its size.
+  constexpr float kFar = 65536.f;
+  float m, neg, base, l;
+  bool far;                                            // some row of the wavefront has a base
+  const float cs = a.scale_log2;
+  // How far above m a score may be. Finite, so that an overflowing difference is above it.
+  const float slack = uniform(fminf(M::slack / cs, 3.4e38f));
 
   // One step of the first product over 32 keys at `kl`: register r of the scores is key
   // 8 (r / 4) + 4 kg + r % 4.
@@ -373,19 +387,27 @@ prompt_attention_kernel(const PromptArgs a) {
     for (int r = 0; r < 16; ++r)
       if (base + 8 * (r / 4) + r % 4 > 0) s[r] = -INFINITY;
   };
-  // Whether the running maximum moves with these scores; then `f` takes sums made with the old one to the new.
-  const auto raise = [&](const f32x16_t& s, float& f) __attribute__((always_inline)) -> bool {
+  // Whether the running maximum moves with these scores; then `f` takes sums made with the old one to
+  // the new. Takes the base from the scores.
+  const auto raise = [&](f32x16_t& s, float& f) __attribute__((always_inline)) -> bool {
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-    if (!__builtin_amdgcn_ballot_w64(top > thr)) return false;
-    const float m2 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * cs);
-    f = m == -INFINITY ? 0.f : fast_exp2(m - m2);
-    m = m2;
-    neg_m = m2 == -INFINITY ? 0.f : M::bias - m2;
-    thr = m2 == -INFINITY ? -INFINITY : (m2 + M::slack) * inv_cs;
-    l *= f;
-    return true;
+    const bool moves = __builtin_amdgcn_ballot_w64(top - m > slack) != 0;
+    if (moves) {
+      const float m2 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))), e = m2 * cs;
+      const bool none = m2 == -INFINITY, away = !none && !(fabsf(e) <= kFar);
+      const float base2 = away ? m2 : 0.f, neg2 = none ? 0.f : away ? M::bias : M::bias - e;
+      f = m == -INFINITY ? 0.f : fast_exp2(__builtin_fmaf(base - base2, cs, neg2 - neg));
+      m = m2, base = base2, neg = neg2;
+      far = __builtin_amdgcn_ballot_w64(away) != 0;
+      l *= f;
+    }
+    if (far) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] -= base;
+    }
+    return moves;
   };
   const auto scale_output = [&](float f) __attribute__((always_inline)) {
 #pragma unroll
@@ -393,7 +415,7 @@ prompt_attention_kernel(const PromptArgs a) {
   };
   // Weights of a 32-key block: element by element, then by pairs packed and summed.
   const auto weight = [&](f32x16_t& s, int r) __attribute__((always_inline)) {
-    s[r] = fast_exp2(__builtin_fmaf(s[r], cs, neg_m));
+    s[r] = fast_exp2(__builtin_fmaf(s[r], cs, neg));
   };
   const auto pack_pair = [&](const f32x16_t& s, int r, uint32_t (&w)[P::PREGS]) __attribute__((always_inline)) {
     if constexpr (P::F32) {
@@ -446,7 +468,7 @@ prompt_attention_kernel(const PromptArgs a) {
     for (int i = 0; i < NDB; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-    m = -INFINITY, neg_m = 0.f, thr = -INFINITY, l = 0.f;
+    m = -INFINITY, neg = 0.f, base = 0.f, l = 0.f, far = false;
   };
   f32x16_t sa, sb;
   uint32_t wa[P::PREGS], wb[P::PREGS];

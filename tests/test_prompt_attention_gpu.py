@@ -303,3 +303,51 @@ def test_a_requests_life_with_a_4_bit_cache(dtype):
             tol = (2 * (D + 4) * U * X + 8 * U + 2 * (n + 32) * U + 2.0 ** -18) * A + torch.finfo(dtype).eps / 2 * want.abs()
             assert ((got[b].double() - want).abs() <= tol).all()
     assert torch.equal(pool.data.cpu(), twin.data)
+
+
+def exact_scores(power, Hq, Hk, dtype, lens, seed):
+    """q, k, v, starts and a scale: scores near 2^power (of e) for two rows of three, a few units
+    for the third, every one a sum of two products that f32 holds exactly."""
+    q, k, v, cu = make(lens, Hq, Hk, 64, dtype, seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    q, k = torch.zeros_like(q), torch.zeros_like(k)
+    q[..., 0], k[..., 0] = 2.0 ** 15, 2.0 ** 15
+    q[..., 1] = 2.0 ** 7  # a step of 2^30 in f32
+    q[::3, :, 0] = 0
+    k[..., 1] = torch.randint(0, 9, (sum(lens), Hk), generator=g).to(DEV)
+    return q, k, v, cu, 2.0 ** (power - 30)
+
+
+def check_exact_scores(got, q, k, v, cu, scale):
+    """Scores have no error here, nor has what they differ by. A weight's exponent is off by 3 u of
+    itself (the scale's factor, its product), which moves a weight w = 2^-d by 3 u d w <= 2 u,
+    exp2 and the sums as in `tolerance`."""
+    out, A, _ = reference(q, k, v, cu, scale)
+    half, n = torch.finfo(q.dtype).eps / 2, int((cu[1:] - cu[:-1]).max())
+    tol = (16 * U + 2 * (n + 32) * U + 2 * half * (q.dtype != F32)) * A + half * out.abs()
+    if q.dtype == F16:
+        tol = tol + n * 2.0 ** -38 * float(v.abs().amax()) + 2.0 ** -25
+    assert not torch.isnan(got).any()
+    off = (got.double() - out).abs()
+    assert (off <= tol).all(), f"worst {float((off / tol.clamp_min(1e-300)).max()):.3g} of the tolerance"
+
+
+@DTYPES
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [4, 12, 15, 16, 18, 20, 22, 24, 27, 30, 34, 60])
+def test_scores_of_any_size(power, sign, dtype):
+    """Where a score's product with the scale rounds by more than a weight's exponent may."""
+    q, k, v, cu, scale = exact_scores(power, 4, 2, dtype, [1, 1, 2, 130, 300], seed=power)
+    got = torch.empty(q.shape, dtype=dtype, device=DEV)
+    entry(q, k, v, cu, got, sign * scale, 1)
+    check_exact_scores(got, q, k, v, cu, sign * scale)
+
+
+@DTYPES
+@pytest.mark.parametrize("size", [2.0 ** 8, 2.0 ** 11, 2.0 ** 13, 2.0 ** 18])
+def test_a_row_alone_is_its_value_at_any_score(size, dtype):
+    lens, size = [1] * 300, min(size, 2.0 ** 13) if dtype == F16 else size
+    q, k, v, cu = make(lens, 2, 1, 64, dtype, seed=11)
+    got = hpd.prompt_attention_hip(q * size, k * size, v, cu)
+    want = v.expand(-1, 2, -1).double()
+    assert ((got.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + 4 * U) * want.abs()).all()
