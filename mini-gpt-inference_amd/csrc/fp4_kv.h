@@ -72,6 +72,7 @@ struct Fp4DecodeArgs {
   int64_t N;
   int q_tiles;             // tiles of 16 query heads per KV head
   float scale_log2;        // |scale| * log2(e) (1 for a scale of 0)
+  float slack;             // the running maximum moves when a score, before the scale, passes it by this
   uint32_t q_flip;         // sign bit of q, for a negative scale
   int q_zero;              // scale is 0
   int vec;                 // q and out rows contiguous and 16-byte aligned, D a multiple of 8
@@ -81,7 +82,7 @@ struct Fp4DecodeArgs {
   int waves;               // otherwise: wavefronts of the whole launch, at most, a multiple of 4
   int cus;
   float* ws_acc;           // [2 * waves][min(G, 16)][groups * 32]
-  float2* ws_ml;           // [2 * waves][16]  (max, sum), log2 domain
+  float2* ws_ml;           // [2 * waves][16]  (max, before the scale, and sum)
   int* ws_cum;             // [B + 1] exclusive prefix sums of tiles per sequence
 };
 hipError_t launch_paged_fp4_f32(const Fp4DecodeArgs& a, hipStream_t stream);

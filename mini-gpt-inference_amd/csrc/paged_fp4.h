@@ -26,6 +26,8 @@
 // so scores are f32 sums of exact products. The softmax weights are cut into 2 terms (3 for
 // f32 outputs), 2^-17 (2^-26) of a weight at most, where one term would cost 2^-8: the
 // matrix cores have the room, as 4-bit keys and values arrive slower than they multiply.
+// A weight's exponent is (score - maximum) * scale, the difference first: a product of each
+// would round by 2^-24 of itself, which overflows weights of scores far from 0.
 #pragma once
 
 #include <type_traits>
@@ -44,8 +46,7 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 32;          // tokens per step of a wavefront
-constexpr float kNoMax = -3.0e38f; // below every score; finite, so that differences are
-constexpr float kSlack = 8.f;      // the running maximum moves when a score passes it by this (log2)
+constexpr float kNoMax = -3.4028234e38f;  // no score yet: the lowest finite number, so that differences are no NaN
 
 // A row of NG groups is handled in pieces of 4, 2 or 1 groups, so that a lane's share of a
 // piece is a power of two: piece p starts at group start(p) and has size(p) groups.
@@ -154,7 +155,7 @@ struct Attend {
   int ctx;
   u32x4_t q[NQ][NG];
   f32x4_t acc[2 * NG];
-  float m, l;
+  float m, l;                   // maximum, in the scores' own units (before the scale), and sum
   int entries, entries_at;      // block ids of 64 subtiles from subtile `entries_at` on, one per lane
 
   __device__ __forceinline__ Attend(const Fp4DecodeArgs& args)
@@ -360,16 +361,15 @@ struct Attend {
       }
     }
     float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    top *= a.scale_log2;
-    if (__any(top > m + kSlack)) {
-      const float m2 = fmaxf(m, across_max(top)), f = fast_exp2(m - m2);
+    if (__any(top - m > a.slack)) {
+      const float m2 = fmaxf(m, across_max(top)), f = fast_exp2((m - m2) * a.scale_log2);
       m = m2;
       l *= f;
 #pragma unroll
       for (int j = 0; j < 2 * NG; ++j) acc[j] *= f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = fast_exp2(__builtin_fmaf(s[i], a.scale_log2, -m));
+    for (int i = 0; i < 8; ++i) s[i] = fast_exp2((s[i] - m) * a.scale_log2);
     l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     each<0, NP>([&](auto n) {
 #pragma unroll
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__((64 * one_waves<T, NG>())) paged_fp4_one(const
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int w = 0; w < waves; ++w) {
       const float* part = lds + (w * rows + row) * width;
-      const float f = fast_exp2(part[NG * 32] - m);
+      const float f = fast_exp2((part[NG * 32] - m) * a.scale_log2);
       const float4 y = *(const float4*)(part + d);
       sum += f * part[NG * 32 + 1];
       x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_fp4_join(const Fp4DecodeAr
 #pragma unroll
       for (int i = 0; i < kJoinBatch; ++i)
         if (w + i * parts <= w1) {
-          const float f = fast_exp2(ml[i].x - m);
+          const float f = fast_exp2((ml[i].x - m) * a.scale_log2);
           sum += f * ml[i].y;
           x.x += f * y[i].x, x.y += f * y[i].y, x.z += f * y[i].z, x.w += f * y[i].w;
         }

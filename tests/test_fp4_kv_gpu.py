@@ -463,3 +463,43 @@ def test_refusals():
         # Nothing to do.
         append(0, rows[:0], rows[:0], ids[:0])
         assert ops.kv_gather_fp4(pool.data, 16, 64, 0, ids[:0], F32)[0].shape == (0, 2, 64)
+
+
+@DTYPES
+@ROUTES
+@pytest.mark.parametrize("S", [16, 6])
+@pytest.mark.parametrize("power", [4, 16, 20, 24, 30, 32, 34, 40, 60])
+def test_scores_of_any_size(power, S, route, dtype):
+    """Scores near 2^power (of e), or a few units (a third of the rows), every one a sum of two products that
+    f32 holds exactly: what is left is 3 u of a weight's exponent (the scale's factor, its
+    product), which moves a weight 2^-d by 3 u d 2^-d <= 2 u, exp2 and the sums. Weights below
+    2^-118 of the largest may be 0 in f32 (its least normal number is 2^-126, and the
+    running maximum is up to 2^8 off): n 2^-118 max |v|, which counts where every larger
+    weight meets a value of 0."""
+    lens = [1, 2, 33, 300, 290, 700]
+    g = torch.Generator().manual_seed(power)
+    B, H, D, n = len(lens), 2, 64, [-(-c // S) for c in lens]
+    pool = gpu_pool(cpu_pool(1, sum(n), S, H, D))
+    tables = torch.full((B, max(n)), -1, dtype=torch.int64)
+    at = 0
+    for b in range(B):
+        tables[b, :n[b]] = torch.arange(at, at + n[b])
+        at += n[b]
+    rows = sum(n) * S
+    k, v = torch.zeros((rows, H, D)), torch.randn((rows, H, D), generator=g)
+    k[..., 0] = 2.0 ** 15
+    k[..., 32] = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6])[torch.randint(0, 8, (rows, H), generator=g)]
+    hpd.kv_append_fp4(pool, 0, k.to(DEV), v.to(DEV), torch.arange(rows, device=DEV))
+    q = torch.zeros((B, 4, D), dtype=dtype, device=DEV)
+    q[..., 0], q[..., 32] = 2.0 ** 15, 2.0 ** 8  # a code's half is a step of 2^30 in f32
+    q[::3, :, 0] = 0
+    ctx, tables, half = torch.tensor(lens, device=DEV), tables.to(DEV), torch.finfo(dtype).eps / 2
+    for scale in (2.0 ** (power - 30), -2.0 ** (power - 30)):
+        got = entry(q, pool, tables, ctx, 0, scale, torch.empty_like(q))
+        out, A, _, most = reference(q, pool, tables, ctx, 0, scale)
+        cut = 2.0 ** -26 if dtype == F32 else 2.0 ** -17
+        tol = (16 * U + 2 * (most + 32) * U + cut) * A + half * out.abs() + 2.0 ** -25 * (dtype == F16)
+        tol += most * 2.0 ** -118 * float(v.abs().amax())
+        off = (got.double() - out).abs()
+        assert not torch.isnan(got).any()
+        assert (off <= tol).all(), f"worst {float((off / tol.clamp_min(1e-300)).max()):.3g} of the tolerance"
