@@ -528,7 +528,7 @@ size_t mgi_paged_decode_fp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, i
  *   out[i,h] = sum_{j <= i, j in i's sequence} softmax_j(scale * q[i,h] . k[j]) * v[j]
  * A sequence may be empty. Rows of no sequence (before the first start, behind the last)
  * are left as they were, or become 0 with zero_rest. A row's result depends on the rows
- * it sees alone, whatever the others hold (infinities and NaN too). Sums are f32; 2-byte
+ * it sees alone, to the bit, whatever the others hold (infinities and NaN too). Sums are f32; 2-byte
  * types round the softmax weights to their type for the second product, as
  * mgi_paged_prefill; f32 products are f32. Same inputs, same bits. No workspace.
  * D <= 256, T and B < 2^28, (T / 32 + B + 1) * Hq < 2^31.

@@ -387,15 +387,16 @@ prompt_attention_kernel(const PromptArgs a) {
     for (int r = 0; r < 16; ++r)
       if (base + 8 * (r / 4) + r % 4 > 0) s[r] = -INFINITY;
   };
-  // Whether the running maximum moves with these scores; then `f` takes sums made with the old one to
-  // the new. Takes the base from the scores.
+  // Whether some row's running maximum moves with these scores; then `f` takes sums made with the old
+  // one to the new (1 where it stays). Takes the base from the scores.
   const auto raise = [&](f32x16_t& s, float& f) __attribute__((always_inline)) -> bool {
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
     const bool moves = __builtin_amdgcn_ballot_w64(top - m > slack) != 0;
     if (moves) {
-      const float m2 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))), e = m2 * cs;
+      // Of the rows whose own scores ask for it: a row's bits are those of what it sees.
+      const float both = fmaxf(top, __shfl_xor(top, 32, 64)), m2 = both - m > slack ? both : m, e = m2 * cs;
       const bool none = m2 == -INFINITY, away = !none && !(fabsf(e) <= kFar);
       const float base2 = away ? m2 : 0.f, neg2 = none ? 0.f : away ? M::bias : M::bias - e;
       f = m == -INFINITY ? 0.f : fast_exp2(__builtin_fmaf(base - base2, cs, neg2 - neg));

@@ -215,6 +215,6 @@ def prompt_attention_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     being rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (none, for an empty one); it is read
     on the GPU alone, so a captured graph follows it. float32, bfloat16 or float16;
     head_dim up to 256. Returns a fresh [T, Hq, D] tensor of q.dtype; rows of no sequence
-    are 0. A row's result does not depend on rows it does not see, whatever they hold.
+    are 0. A row's bits do not depend on rows it does not see, whatever they hold.
     """
     return _native.ops().prompt_attention(q, k, v, cu_seqlens)

@@ -351,3 +351,27 @@ def test_a_row_alone_is_its_value_at_any_score(size, dtype):
     got = hpd.prompt_attention_hip(q * size, k * size, v, cu)
     want = v.expand(-1, 2, -1).double()
     assert ((got.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + 4 * U) * want.abs()).all()
+
+
+@DTYPES
+@pytest.mark.parametrize("Hq,Hk,D", [(4, 1, 64), (2, 1, 128), (1, 1, 128), (3, 3, 80), (4, 2, 20)])
+def test_a_rows_bits_are_those_of_the_rows_it_sees(Hq, Hk, D, dtype):
+    """The same first rows before other ones, which move the others' maxima, hold what is not a
+    number, or have scores that are far from 0."""
+    lens, same = [333, 41], 100
+    q, k, v, cu = make(lens, Hq, Hk, D, dtype, seed=12)
+    q = q * 4
+    first = hpd.prompt_attention_hip(q, k, v, cu)
+    for n in (101, 140, 500):
+        for what in ("larger", "far", "nan", "inf"):
+            q2, k2, v2, cu2 = make([n, 3], Hq, Hk, D, dtype, seed=13)
+            q2, k2, v2 = q2 * 12, k2 * 3, v2 * 2
+            for x, y in ((q2, q), (k2, k), (v2, v)):
+                x[:same] = y[:same]
+            if what == "far":
+                q2[same:], k2[same:] = q2[same:] * 2.0 ** 7, k2[same:] * 2.0 ** 7
+            elif what != "larger":
+                v2[same:, 0, D // 2], k2[same] = float(what), float(what)
+            got = hpd.prompt_attention_hip(q2, k2, v2, cu2)
+            assert not torch.isnan(got[:same]).any()
+            assert torch.equal(got[:same], first[:same]), f"{n} rows, {what}: {int((got[:same] != first[:same]).sum())} values"
