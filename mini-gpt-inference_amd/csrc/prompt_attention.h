@@ -54,7 +54,8 @@ template <typename T> struct PM;  // the products of a type
 template <> struct PM<bf16_t> {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
-  static constexpr float slack = 8.f, bias = 0.f;  // log2: a score may pass the maximum by slack; weights are 2^bias too large
+  // log2: a score may pass the maximum by slack; weights are 2^bias too large, so that no sum is larger than the softmax's.
+  static constexpr float slack = 8.f, bias = -8.f;
   static constexpr uint32_t inf = 0x7f80u;  // bits
   __device__ static __forceinline__ f32x16_t mfma(uint4 a, uint4 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -71,7 +72,7 @@ template <> struct PM<bf16_t> {
 template <> struct PM<f16_t> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-  static constexpr float slack = 2.f, bias = 13.f;
+  static constexpr float slack = 2.f, bias = 13.f;  // f16 values leave f32 sums the room
   static constexpr uint32_t inf = 0x7c00u;
   __device__ static __forceinline__ f32x16_t mfma(uint4 a, uint4 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -86,7 +87,7 @@ template <> struct PM<f16_t> {
   }
 };
 template <> struct PM<float> {
-  static constexpr float slack = 8.f, bias = 0.f;
+  static constexpr float slack = 8.f, bias = -8.f;
 };
 
 template <typename T> struct PElem {

@@ -375,3 +375,16 @@ def test_a_rows_bits_are_those_of_the_rows_it_sees(Hq, Hk, D, dtype):
             got = hpd.prompt_attention_hip(q2, k2, v2, cu2)
             assert not torch.isnan(got[:same]).any()
             assert torch.equal(got[:same], first[:same]), f"{n} rows, {what}: {int((got[:same] != first[:same]).sum())} values"
+
+
+@DTYPES
+def test_values_near_the_largest_number(dtype):
+    """A key somewhat above the running maximum, later: its weight times its value must not
+    overflow where the softmax's sum does not."""
+    n = 200
+    q, k, v = (torch.zeros((n, 1, 64), dtype=dtype, device=DEV) for _ in range(3))
+    q[..., 0], k[..., 0] = 8, -30
+    k[0, 0, 0], k[40, 0, 0] = 0, 5
+    v[:] = 6e4 if dtype == F16 else 2.0 ** 127
+    v[..., ::2] *= -1
+    check(hpd.prompt_attention_hip(q, k, v, torch.tensor([0, n], device=DEV)), q, k, v, torch.tensor([0, n], device=DEV))
