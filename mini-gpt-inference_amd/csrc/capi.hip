@@ -1582,7 +1582,7 @@ int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, const void* q, c
   a.N = N;
   a.q_tiles = p.q_tiles;
   a.scale_log2 = scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f;
-  a.slack = std::min(8.f / a.scale_log2, 3.4e38f);  // weights up to 2^8; finite, so that an overflowing difference is above it
+  a.slack = std::min(kFp4Slack / a.scale_log2, 3.4e38f);  // finite, so that an overflowing difference is above it
   a.q_flip = scale < 0.f ? 0x80000000u : 0u;
   a.q_zero = scale == 0.f;
   a.vec = D % 8 == 0 && q_strides[2] == 1 && out_strides[2] == 1 && aligned16(q) && aligned16(out) &&

@@ -23,6 +23,7 @@ namespace mgi {
 
 constexpr int kFp4Group = 32;
 constexpr int kFp4MaxDim = 256;
+constexpr float kFp4Slack = 8.f;  // log2: a score may pass the running maximum by this before it moves
 
 __host__ __device__ inline int64_t fp4_groups(int64_t D) { return (D + kFp4Group - 1) / kFp4Group; }
 // Bytes of one (layer, block, head), a multiple of 16.

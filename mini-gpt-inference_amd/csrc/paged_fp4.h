@@ -347,7 +347,8 @@ struct Attend {
     }
   }
 
-  // Softmax weights of the scores, as bf16 terms; masked tokens' values are made finite.
+  // Softmax weights of the scores, as bf16 terms; masked tokens' values are made finite. Weights
+  // carry a factor of 2^-kFp4Slack, so that no sum of them times values passes the softmax's.
   __device__ __forceinline__ void weights(float (&s)[8], uint32_t valid, Values& v, u32x4_t (&w)[NP]) {
     if (valid != 0xffffffffu) {  // the end of the context, or a block outside the pool
 #pragma unroll
@@ -369,7 +370,7 @@ struct Attend {
       for (int j = 0; j < 2 * NG; ++j) acc[j] *= f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = fast_exp2((s[i] - m) * a.scale_log2);
+    for (int i = 0; i < 8; ++i) s[i] = fast_exp2(__builtin_fmaf(s[i] - m, a.scale_log2, -kFp4Slack));
     l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     each<0, NP>([&](auto n) {
 #pragma unroll

@@ -503,3 +503,23 @@ def test_scores_of_any_size(power, S, route, dtype):
         off = (got.double() - out).abs()
         assert not torch.isnan(got).any()
         assert (off <= tol).all(), f"worst {float((off / tol.clamp_min(1e-300)).max()):.3g} of the tolerance"
+
+
+@DTYPES
+@ROUTES
+def test_values_near_the_largest_number(route, dtype):
+    """Keys somewhat above the running maximum, later: a weight times its value must not
+    overflow where the softmax's sum does not."""
+    S, n, B = 16, 40, 3
+    pool = gpu_pool(cpu_pool(1, B * n, S, 1, 64))
+    k, v = torch.zeros((2, B * n * S, 1, 64))
+    k[..., 0], v[:] = -24, 2.0 ** 127 if dtype != F16 else 6 * 2.0 ** 13
+    v[..., ::2] *= -1
+    for b, later in enumerate((40, 8 * 32 + 3, 600)):
+        k[b * n * S, 0, 0], k[b * n * S + later, 0, 0] = 0, 4
+    hpd.kv_append_fp4(pool, 0, k.to(DEV), v.to(DEV), torch.arange(B * n * S, device=DEV))
+    tables, ctx = torch.arange(B * n, device=DEV).view(B, n), torch.full((B,), n * S - 3, device=DEV)
+    q = torch.zeros((B, 2, 64), dtype=dtype, device=DEV)
+    q[..., 0] = 8
+    case = (q, pool, tables, ctx, 0)
+    check(hpd.paged_attention_fp4_hip(*case), *case)
