@@ -217,7 +217,11 @@ struct Attend {
         each<0, NQ>([&](auto n) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t w = pack_bf16(x[2 * e], x[2 * e + 1]);
+            uint32_t w;
+            if constexpr (NQ == 3)  // cut off: three times 8 bits are all 24, and the largest numbers stay finite
+              w = __builtin_amdgcn_perm(__float_as_uint(x[2 * e + 1]), __float_as_uint(x[2 * e]), 0x07060302u);
+            else
+              w = pack_bf16(x[2 * e], x[2 * e + 1]);
             q[n][g0 + i][e] = w;
             x[2 * e] -= bf16_lo(w);
             x[2 * e + 1] -= bf16_hi(w);

@@ -523,3 +523,20 @@ def test_values_near_the_largest_number(route, dtype):
     q[..., 0] = 8
     case = (q, pool, tables, ctx, 0)
     check(hpd.paged_attention_fp4_hip(*case), *case)
+
+
+@ROUTES
+@pytest.mark.parametrize("sign", [1, -1])
+def test_f32_queries_up_to_the_largest_number(sign, route):
+    """Such a query rounds up to no bf16 number; its terms must add up to it all the same."""
+    S, n = 16, 5
+    g = torch.Generator().manual_seed(5)
+    pool = gpu_pool(cpu_pool(1, n, S, 1, 64))
+    k, v = torch.zeros((n * S, 1, 64)), torch.randn((n * S, 1, 64), generator=g)
+    k[..., 3] = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6])[torch.randint(0, 8, (n * S, 1), generator=g)] * 2.0 ** -100
+    hpd.kv_append_fp4(pool, 0, k.to(DEV), v.to(DEV), torch.arange(n * S, device=DEV))
+    tables, ctx = torch.arange(n, device=DEV)[None], torch.tensor([n * S - 2], device=DEV)
+    q = torch.zeros((1, 2, 64), device=DEV)
+    q[0, 0, 3], q[0, 1, 3] = sign * torch.finfo(F32).max, sign * 1.999 * 2.0 ** 126
+    got = entry(q, pool, tables, ctx, 0, 2.0 ** -28, torch.empty_like(q))
+    check(got, q, pool, tables, ctx, 0, 2.0 ** -28)
