@@ -494,8 +494,8 @@ int mgi_kv_gather_fp4(void* k_out, void* v_out,
  * mgi_paged_decode_shared (q and out [B, Hq, D], Hq a multiple of the pool's Hk). Lengths
  * are clamped to [0, M*S], a table entry outside [0, N) masks its block, a row without keys
  * gives 0, and only the tokens of a row's context enter its result. Sums are f32; the
- * products take q and the softmax weights as sums of bf16 terms (q exactly; weights to
- * 2^-17, 2^-26 for f32). One launch or two, by sizes alone. Same inputs, same bits.
+ * products take q and the softmax weights as sums of bf16 terms (q exactly, but for what
+ * an f32 element has below 2^-133; weights to 2^-17, 2^-26 for f32). One launch or two, by sizes alone. Same inputs, same bits.
  * B and Hq <= 65535, B*Hq < 2^25, M*S < 2^30, B*M*S < 2^35.
  *
  * workspace: mgi_paged_decode_fp4_workspace_bytes(...) bytes for the same sizes, 16-byte

@@ -22,8 +22,8 @@
 // tiles a wavefront at most, whose chains of table entry, codes and products nothing hides).
 // Of a large call's wavefront cycles half are waits, 42 % have a vector instruction in work.
 //
-// Numerics: q is cut into bf16 terms that add up to it (1 for bf16, 2 for f16, 3 for f32),
-// so scores are f32 sums of exact products. The softmax weights are cut into 2 terms (3 for
+// Numerics: q is cut into bf16 terms that add up to it (1 for bf16, 2 for f16, 3 for f32; what an
+// f32 element has below 2^-133, bf16's least number, is left out), so scores are f32 sums of exact products. The softmax weights are cut into 2 terms (3 for
 // f32 outputs), 2^-17 (2^-26) of a weight at most, where one term would cost 2^-8: the
 // matrix cores have the room, as 4-bit keys and values arrive slower than they multiply.
 // A weight's exponent is (score - maximum) * scale, the difference first: a product of each

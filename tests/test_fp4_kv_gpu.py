@@ -540,3 +540,27 @@ def test_f32_queries_up_to_the_largest_number(sign, route):
     q[0, 0, 3], q[0, 1, 3] = sign * torch.finfo(F32).max, sign * 1.999 * 2.0 ** 126
     got = entry(q, pool, tables, ctx, 0, 2.0 ** -28, torch.empty_like(q))
     check(got, q, pool, tables, ctx, 0, 2.0 ** -28)
+
+
+@DTYPES
+@ROUTES
+def test_tiny_queries_and_large_keys(route, dtype):
+    """Queries whose further terms are no normal numbers. bf16's least number is 2^-133: of an f32
+    query less than that is left out, and a score is off by up to 2^-133 max |k|, by which
+    the weight and the sum that divides it are each off."""
+    S, n, low = 16, 5, -20 if dtype == F16 else -122
+    g = torch.Generator().manual_seed(6)
+    pool = gpu_pool(cpu_pool(1, n, S, 1, 64))
+    k, v = torch.zeros((n * S, 1, 64)), torch.randn((n * S, 1, 64), generator=g)
+    k[..., 3] = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6])[torch.randint(0, 8, (n * S, 1), generator=g)] * 2.0 ** -low
+    hpd.kv_append_fp4(pool, 0, k.to(DEV), v.to(DEV), torch.arange(n * S, device=DEV))
+    tables, ctx = torch.arange(n, device=DEV)[None], torch.tensor([n * S - 2], device=DEV)
+    q = torch.zeros((1, 4, 64), dtype=dtype, device=DEV)
+    q[0, :, 3] = (torch.tensor([1.9999, 1.2345678, -1.7182818, 0.9876543]) * 2.0 ** low).to(dtype)
+    got = entry(q, pool, tables, ctx, 0, 1.0, torch.empty_like(q))
+    if dtype != F32:
+        return check(got, q, pool, tables, ctx, 0, 1.0)
+    out, A, X, n = reference(q, pool, tables, ctx, 0, 1.0)
+    lost = 2.0 ** -133 * float(k.abs().amax())
+    tol = (2 * 68 * U * X + 8 * U + 2 * (n + 32) * U + 2.0 ** -26 + 2 * lost) * A + U * out.abs()
+    assert ((got.double() - out).abs() <= tol).all()
