@@ -1456,6 +1456,7 @@ int mgi_prompt_attention(void* out, const int64_t* out_strides, const void* q, c
   if (!valid_dtype(dtype)) return fail(MGI_EINVAL, "unknown dtype code");
   if (!valid_itype(starts_itype)) return fail(MGI_EINVAL, "index arrays must be int32 or int64");
   if (!std::isfinite(scale)) return fail(MGI_EINVAL, "scale must be finite");
+  if (std::fabs(scale) >= 0x1p127f) return fail(MGI_EUNSUPPORTED, "scale must be below 2^127");  // times log2(e): finite
   if (!nonneg(out_strides, 3) || !nonneg(q_strides, 3) || !nonneg(k_strides, 3) || !nonneg(v_strides, 3) ||
       starts_stride < 0)
     return fail(MGI_EINVAL, "strides must be non-negative");
@@ -1557,6 +1558,7 @@ int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, const void* q, c
   if (!valid_dtype(dtype)) return fail(MGI_EINVAL, "unknown dtype code");
   if (!valid_itype(bt_itype) || !valid_itype(cl_itype)) return fail(MGI_EINVAL, "index arrays must be int32 or int64");
   if (!std::isfinite(scale)) return fail(MGI_EINVAL, "scale must be finite");
+  if (std::fabs(scale) >= 0x1p127f) return fail(MGI_EUNSUPPORTED, "scale must be below 2^127");  // times log2(e): finite
   if (!nonneg(out_strides, 3) || !nonneg(q_strides, 3) || !nonneg(bt_strides, 2) || cl_stride < 0)
     return fail(MGI_EINVAL, "strides must be non-negative");
   if (B > kMaxGridYZ || Hq > kMaxGridYZ) return fail(MGI_EUNSUPPORTED, "batch or heads larger than 65535");

@@ -161,3 +161,10 @@ def test_cpu_tensors_are_refused(ops, monkeypatch):
         hpd.kv_gather_fp4(pool, 0, ids)
     with pytest.raises(ValueError, match="^q must be on a GPU device for the HIP backend$"):
         hpd.paged_attention_fp4_hip(rows, pool, ids[:, None], ids, 0)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, -3.4e38])
+def test_a_scale_whose_exponent_overflows_is_refused(scale):
+    lib = _native.lib()
+    assert lib.mgi_paged_decode_fp4(*{**DECODE, "scale": scale}.values()) == _native.MGI_EUNSUPPORTED
+    assert "2^127" in lib.mgi_last_error().decode()

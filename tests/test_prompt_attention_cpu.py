@@ -42,3 +42,10 @@ def test_cpu_tensors_are_refused(ops, monkeypatch):
     x = torch.zeros(3, 2, 64)
     with pytest.raises(ValueError, match="^q must be on a GPU device for the HIP backend$"):
         hpd.prompt_attention_hip(x, x, x, torch.tensor([0, 3]))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, -3.4e38])
+def test_a_scale_whose_exponent_overflows_is_refused(scale):
+    lib = _native.lib()
+    assert lib.mgi_prompt_attention(*{**CALL, "scale": scale}.values()) == _native.MGI_EUNSUPPORTED
+    assert "2^127" in lib.mgi_last_error().decode()
