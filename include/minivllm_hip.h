@@ -514,8 +514,8 @@ int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, /* [3] */
                          int64_t M, int64_t L, int64_t layer_idx, float scale,
                          void* workspace, size_t workspace_bytes, void* stream);
 
-/* Workspace bytes mgi_paged_decode_fp4 needs for these sizes on the current device (0 if
- * none). */
+/* Workspace bytes mgi_paged_decode_fp4 needs at most for these sizes on the current device,
+ * whatever the query type (0 if none). */
 size_t mgi_paged_decode_fp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M);
 
 /*

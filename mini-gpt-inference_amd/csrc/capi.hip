@@ -911,15 +911,18 @@ struct Fp4Plan {
 // its partials but has no more than 8 wavefronts for a (sequence, KV head). One launch against split and join
 // (us; heads of 128, bf16, lengths of half to all of the table): 1 sequence, 32 heads on 8, 1024
 // tokens 9/15, 4096 23/17, 32k 148/24; 4 of 8 heads 1024 10/15, 2048 17/18, 4096 30/18; 64, 32 heads
-// on 8, 1024 20/28, 2048 33/38, 4096 60/56. The host knows the table's width, not the lengths.
+// on 8, 1024 20/28, 2048 33/38, 4096 60/56; f32 heads of 256, whose workgroups have 4 wavefronts: 1 of 8 heads
+// 1024 18/20, 1536 19/20, 2048 26/20, 4 of 8 21/24, 29/21, 33/24, 64, 32 on 8 43/49, 57/59, 73/72. The host
+// knows the table's width, not the lengths.
 constexpr int64_t kFp4OneLaunchTiles = 8;
 
-Fp4Plan fp4_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M) {
+Fp4Plan fp4_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_t M, int dtype) {
   Fp4Plan p{};
   const int64_t G = Hq / Hk, rows = std::min<int64_t>(G, 16), dims = mgi::fp4_groups(D) * 32;
+  const int groups = (int)mgi::fp4_groups(D), terms = mgi::fp4_query_terms((int)dtype_bytes(dtype), dtype == MGI_BF16);
   p.q_tiles = (int)((G + 15) / 16);
   const int64_t tiles = (M * S + 31) / 32, pairs = B * Hk * p.q_tiles;
-  int64_t waves = 8;
+  int64_t waves = mgi::fp4_one_waves(groups, terms);
   while (waves > 1 && (waves * rows * (dims + 4) * 4 > 65536 || waves / 2 >= tiles)) waves /= 2;
   const int forced = env_int("MINIVLLM_HIP_FP4_SPLIT", -1);
   if (forced < 0 ? tiles <= kFp4OneLaunchTiles * waves : forced == 0) {
@@ -927,8 +930,8 @@ Fp4Plan fp4_plan(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t S, int64_
     p.waves = (int)waves;
     return p;
   }
-  // As many wavefronts as a CU may hold (fewer where registers say so, which the launcher knows).
-  waves = std::min(16 * (int64_t)device_cus(), round_up(pairs * tiles, 4));
+  // As many wavefronts as the CUs hold.
+  waves = std::min(4 * mgi::fp4_occupancy(groups, terms) * (int64_t)device_cus(), round_up(pairs * tiles, 4));
   p.waves = (int)waves;
   p.ml_offset = round_up(2 * waves * rows * dims * 4, kWorkspaceAlign);
   p.cum_offset = round_up(p.ml_offset + 2 * waves * 16 * 8, kWorkspaceAlign);
@@ -1537,7 +1540,9 @@ size_t mgi_paged_decode_fp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, i
   if (B <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk != 0 || D <= 0 || D > mgi::kFp4MaxDim || S <= 0 || M <= 0 ||
       M >= (int64_t(1) << 30) / S || B > kMaxGridYZ || Hq > kMaxGridYZ)
     return 0;
-  return fp4_plan(B, Hq, Hk, D, S, M).total;
+  size_t most = 0;  // of any query type
+  for (const int dtype : {MGI_F32, MGI_BF16, MGI_F16}) most = std::max(most, fp4_plan(B, Hq, Hk, D, S, M, dtype).total);
+  return most;
 }
 
 int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides, int dtype,
@@ -1566,7 +1571,7 @@ int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, const void* q, c
   if (M >= (int64_t(1) << 30) / S) return fail(MGI_EUNSUPPORTED, "M*S must be < 2^30");
   if (B * ((M * S + 31) / 32) >= (int64_t(1) << 30)) return fail(MGI_EUNSUPPORTED, "B*M*S must be < 2^35");
   const int64_t eb = dtype_bytes(dtype);
-  const Fp4Plan p = fp4_plan(B, Hq, Hk, D, S, M);
+  const Fp4Plan p = fp4_plan(B, Hq, Hk, D, S, M, dtype);
   Fp4DecodeArgs a{};
   a.out = out;
   a.o_sb = out_strides[0], a.o_sh = out_strides[1], a.o_sd = out_strides[2];
@@ -1593,7 +1598,6 @@ int mgi_paged_decode_fp4(void* out, const int64_t* out_strides, const void* q, c
   magic_of(S, &a.s_mul, &a.s_shift);
   a.one_launch = p.one_launch;
   a.waves = p.waves;
-  a.cus = device_cus();
   if (!p.one_launch) {
     if (!workspace) return fail(MGI_EWORKSPACE, "workspace required for the split pass");
     if (workspace_bytes < p.total)

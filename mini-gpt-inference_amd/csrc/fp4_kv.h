@@ -56,6 +56,23 @@ struct Fp4RowArgs {
 hipError_t launch_fp4_append(const Fp4RowArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_fp4_gather(const Fp4RowArgs& a, int dtype, hipStream_t stream);
 
+// bf16 terms of a query element: 1 for bf16, 2 for f16, 3 for f32.
+__host__ __device__ constexpr int fp4_query_terms(int bytes, bool is_bf16) { return bytes == 4 ? 3 : is_bf16 ? 1 : 2; }
+// Wavefronts per SIMD that the decode kernels' registers allow without spilling a vector
+// register: 4 registers per group for each query term and each of two accumulators, and the tile's own.
+// More wavefronts hide more of the loads: 64 x 512-4096 tokens, 32 heads of 128, bf16 took 150 us at
+// two, 131 at three.
+__host__ __device__ constexpr int fp4_occupancy(int groups, int query_terms) {
+  return groups * (2 + query_terms) <= 8    ? 4
+         : groups * (2 + query_terms) <= 12 ? 3
+         : groups * (2 + query_terms) <= 32 ? 2
+                                            : 1;
+}
+// Wavefronts of a workgroup of the one-launch form, at most.
+__host__ __device__ constexpr int fp4_one_waves(int groups, int query_terms) {
+  return fp4_occupancy(groups, query_terms) > 1 ? 8 : 4;
+}
+
 // Decode attention over the pool (paged_fp4.h).
 struct Fp4DecodeArgs {
   void* out;
@@ -80,8 +97,7 @@ struct Fp4DecodeArgs {
   uint32_t s_mul;          // division by S (magic_of)
   int s_shift;
   int one_launch;          // a workgroup of `waves` wavefronts per (sequence, KV head)
-  int waves;               // otherwise: wavefronts of the whole launch, at most, a multiple of 4
-  int cus;
+  int waves;               // otherwise: wavefronts of the whole launch, a multiple of 4
   float* ws_acc;           // [2 * waves][min(G, 16)][groups * 32]
   float2* ws_ml;           // [2 * waves][16]  (max, before the scale, and sum)
   int* ws_cum;             // [B + 1] exclusive prefix sums of tiles per sequence

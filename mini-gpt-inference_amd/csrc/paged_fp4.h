@@ -64,30 +64,15 @@ template <int NG> struct Pieces {
 };
 
 template <typename T> struct Terms;  // bf16 terms of a query element and of a softmax weight
-template <> struct Terms<bf16_t> { static constexpr int q = 1, p = 2; };
-template <> struct Terms<f16_t> { static constexpr int q = 2, p = 2; };
-template <> struct Terms<float> { static constexpr int q = 3, p = 3; };
+template <> struct Terms<bf16_t> { static constexpr int q = fp4_query_terms(2, true), p = 2; };
+template <> struct Terms<f16_t> { static constexpr int q = fp4_query_terms(2, false), p = 2; };
+template <> struct Terms<float> { static constexpr int q = fp4_query_terms(4, false), p = 3; };
 
 // A stride whose products the compiler does not compute ahead of the loop over (sequence,
 // head) pairs, where they would take a hundred registers.
 __device__ __forceinline__ int64_t unhoisted(int64_t x) {
   asm volatile("" : "+s"(x));
   return x;
-}
-
-// Wavefronts per SIMD that the registers allow without spilling a vector register: 4 registers
-// per group for each query term and each of two accumulators, and the tile's own. More
-// wavefronts hide more of the loads: 64 x 512-4096 tokens, 32 heads of 128, bf16 took 150 us at
-// two, 131 at three.
-template <typename T, int NG>
-constexpr int occupancy() {
-  constexpr int held = NG * (2 + Terms<T>::q);
-  return held <= 8 ? 4 : held <= 12 ? 3 : held <= 32 ? 2 : 1;
-}
-// Wavefronts of a workgroup of paged_fp4_one.
-template <typename T, int NG>
-constexpr int one_waves() {
-  return occupancy<T, NG>() > 1 ? 8 : 4;
 }
 
 template <int I> using Int = std::integral_constant<int, I>;
@@ -488,7 +473,7 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 // The whole call in one launch: a workgroup per (sequence, KV head, query tile), whose
 // wavefronts take its tiles in turn and meet in LDS.
 template <typename T, int NG, bool ANY>
-__global__ void __launch_bounds__((64 * one_waves<T, NG>())) paged_fp4_one(const Fp4DecodeArgs a) {
+__global__ void __launch_bounds__((64 * fp4_one_waves(NG, Terms<T>::q))) paged_fp4_one(const Fp4DecodeArgs a) {
   extern __shared__ float lds[];
   const int waves = (int)(blockDim.x >> 6), wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = a.Hk * a.q_tiles, b = (int)blockIdx.x / heads, r = (int)blockIdx.x - b * heads;
@@ -549,7 +534,7 @@ struct Runs {
 };
 
 template <typename T, int NG, bool ANY>
-__global__ void __launch_bounds__(256, (occupancy<T, NG>())) paged_fp4_split(const Fp4DecodeArgs a) {
+__global__ void __launch_bounds__(256, (fp4_occupancy(NG, Terms<T>::q))) paged_fp4_split(const Fp4DecodeArgs a) {
   const int wave = (int)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
   const int lane = (int)(threadIdx.x & 63), heads = a.Hk * a.q_tiles;
   // All tiles of one head, and from them this wavefront's run.
@@ -686,12 +671,10 @@ template <typename T, int NG, bool ANY>
 hipError_t launch_ng(Fp4DecodeArgs a, hipStream_t stream) {
   void* args[] = {&a, nullptr};
   if (a.one_launch) {
-    if (a.waves > one_waves<T, NG>()) a.waves = one_waves<T, NG>();
     const size_t lds = (size_t)a.waves * (a.G < 16 ? a.G : 16) * (NG * 32 + 4) * 4;
     return hipLaunchKernel(reinterpret_cast<const void*>(&paged_fp4_one<T, NG, ANY>),
                            dim3((unsigned)(a.B * a.Hk * a.q_tiles)), dim3(a.waves * 64), args, lds, stream);
   }
-  if (a.waves > 4 * occupancy<T, NG>() * a.cus) a.waves = 4 * occupancy<T, NG>() * a.cus;
   hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&paged_fp4_split<T, NG, ANY>),
                                  dim3((unsigned)(a.waves / 4)), dim3(256), args, 0, stream);
   if (e != hipSuccess) return e;

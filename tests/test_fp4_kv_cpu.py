@@ -168,3 +168,20 @@ def test_a_scale_whose_exponent_overflows_is_refused(scale):
     lib = _native.lib()
     assert lib.mgi_paged_decode_fp4(*{**DECODE, "scale": scale}.values()) == _native.MGI_EUNSUPPORTED
     assert "2^127" in lib.mgi_last_error().decode()
+
+
+def test_one_launch_or_two_by_the_wavefronts_a_call_has(monkeypatch):
+    """At most 8 tiles of 32 tokens for a wavefront in one launch; f32 heads of more than 192
+    dims have 4 wavefronts to a workgroup, other calls 8."""
+    lib = _native.lib()
+    monkeypatch.delenv("MINIVLLM_HIP_FP4_SPLIT", raising=False)
+    size = lib.mgi_paged_decode_fp4_workspace_bytes
+    for D in (193, 256):  # 1024 tokens, and 1040
+        slab = lib.mgi_fp4_slab_bytes(16, D)
+        call = {**DECODE, "D": D, "dt": 0, "Hq": 2, "ps": _st(4 * 2 * slab, 2 * slab, slab), "M": 65}
+        assert lib.mgi_paged_decode_fp4(*call.values()) == _native.MGI_EWORKSPACE
+        assert size(2, 2, 2, D, 16, 64) == 0 and size(2, 2, 2, D, 16, 65) > 0
+    for D in (64, 192):
+        assert size(2, 2, 2, D, 16, 128) == 0 and size(2, 2, 2, D, 16, 129) > 0
+    # Partials of the wavefronts that are resident: two for each of 2 per SIMD, 256 dims, 16 rows.
+    assert size(64, 128, 8, 256, 16, 8192) <= 1.05 * 2 * (8 * 256) * 16 * (256 + 2) * 4
