@@ -495,7 +495,8 @@ int mgi_kv_gather_fp4(void* k_out, void* v_out,
  * are clamped to [0, M*S], a table entry outside [0, N) masks its block, a row without keys
  * gives 0, and only the tokens of a row's context enter its result. Sums are f32; the
  * products take q and the softmax weights as sums of bf16 terms (q exactly, but for what
- * an f32 element has below 2^-133; weights to 2^-17, 2^-26 for f32). One launch or two, by sizes alone. Same inputs, same bits.
+ * an f32 element has below 2^-133; weights to 2^-17, 2^-26 for f32). Finite scores may have
+ * any size. One launch or two, by sizes alone. Same inputs, same bits.
  * B and Hq <= 65535, B*Hq < 2^25, M*S < 2^30, B*M*S < 2^35, |scale| < 2^127.
  *
  * workspace: mgi_paged_decode_fp4_workspace_bytes(...) bytes for the same sizes, 16-byte
@@ -530,7 +531,8 @@ size_t mgi_paged_decode_fp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, i
  * are left as they were, or become 0 with zero_rest. A row's result depends on the rows
  * it sees alone, to the bit, whatever the others hold (infinities and NaN too). Sums are f32; 2-byte
  * types round the softmax weights to their type for the second product, as
- * mgi_paged_prefill; f32 products are f32. Same inputs, same bits. No workspace.
+ * mgi_paged_prefill; f32 products are f32. Finite scores may have any size. Same inputs,
+ * same bits. No workspace.
  * D <= 256, T and B < 2^28, (T / 32 + B + 1) * Hq < 2^31, |scale| < 2^127.
  */
 int mgi_prompt_attention(void* out, const int64_t* out_strides, /* [3] */

@@ -1,6 +1,7 @@
 // lds_tiles.h -- key and value tiles in LDS: 16-byte copies from global memory
 // straight into LDS, the waits that go with them, the swizzles of the rows and the
-// transposed reads (2-byte types). Used by paged_prefill.hip and paged_shared.h.
+// transposed reads (2-byte types). Used by paged_prefill.hip and paged_shared.h,
+// and by prompt_attention.h, which has swizzles of its own.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -17,9 +17,9 @@
 // lane's codes are the dims that are its row of V^T, for its 8 tokens.
 //
 // Measured on MI355X, D = 128, bf16, where a large copy reaches 5.05 TB/s: 64 sequences of 512-4096
-// tokens, 32 heads, 131 us (5.2 TB/s); 8 of 32k-128k, 32 heads on 8, 174 us (5.4 TB/s); 13 of
-// 100-1000, 16 heads, 11 us; 256 of 128-2048, 32 heads of 64 on 8, f16, 56 us (2.6 TB/s: 17
-// tiles a wavefront at most, whose chains of table entry, codes and products nothing hides).
+// tokens, 32 heads, 132 us (5.2 TB/s); 8 of 32k-128k, 32 heads on 8, 174 us (5.4 TB/s); 13 of
+// 100-1000, 16 heads, 11 us; 256 of 128-2048, 32 heads of 64 on 8, f16, 57 us (2.5 TB/s: up to 8
+// tiles a wavefront, whose chains of table entry, codes and products nothing hides).
 // Of a large call's wavefront cycles half are waits, 42 % have a vector instruction in work.
 //
 // Numerics: q is cut into bf16 terms that add up to it (1 for bf16, 2 for f16, 3 for f32; what an
