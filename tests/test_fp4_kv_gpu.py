@@ -564,3 +564,19 @@ def test_tiny_queries_and_large_keys(route, dtype):
     lost = 2.0 ** -133 * float(k.abs().amax())
     tol = (2 * 68 * U * X + 8 * U + 2 * (n + 32) * U + 2.0 ** -26 + 2 * lost) * A + U * out.abs()
     assert ((got.double() - out).abs() <= tol).all()
+
+
+@ROUTES
+@pytest.mark.parametrize("scale", [1e-45, -1e-38, 1e20, -1.7e38])
+def test_scales_at_the_ends_of_the_range(scale, route):
+    """Down to scales that make every weight equal, up to ones that leave the largest score alone."""
+    q, pool, tables, ctx, layer = make(3, 4, 2, 64, 16, [300, 1, 77], F32, seed=15)
+    scale = torch.tensor(scale, dtype=F32).item()
+    if abs(scale) > 1:  # scores without an error: one dim of the keys
+        q = torch.zeros_like(q)
+        q[..., 5] = 1
+    got = entry(q, pool, tables, ctx, layer, scale, torch.empty_like(q))
+    out, A, _, n = reference(q, pool, tables, ctx, layer, scale)
+    tol = (16 * U + 2 * (n + 32) * U + 2.0 ** -26) * A + U * out.abs()
+    assert not torch.isnan(got).any()
+    assert ((got.double() - out).abs() <= tol).all()

@@ -388,3 +388,17 @@ def test_values_near_the_largest_number(dtype):
     v[:] = 6e4 if dtype == F16 else 2.0 ** 127
     v[..., ::2] *= -1
     check(hpd.prompt_attention_hip(q, k, v, torch.tensor([0, n], device=DEV)), q, k, v, torch.tensor([0, n], device=DEV))
+
+
+@DTYPES
+@pytest.mark.parametrize("scale", [1e-45, -1e-38, 1e20, -1.7e38])
+def test_scales_at_the_ends_of_the_range(scale, dtype):
+    """Down to scales that make every weight equal, up to ones that leave the largest score alone."""
+    scale = torch.tensor(scale, dtype=F32).item()
+    q, k, v, cu = make([70, 1, 200], 4, 2, 64, dtype, seed=14)
+    if abs(scale) > 1:  # scores without an error
+        q, k = q.clone().zero_(), k.clone().zero_()
+        q[..., 5], k[..., 5] = 1, torch.arange(len(k), device=DEV)[:, None].remainder(37).to(dtype)
+    got = torch.empty(q.shape, dtype=dtype, device=DEV)
+    entry(q, k, v, cu, got, scale, 1)
+    check_exact_scores(got, q, k, v, cu, scale)
